@@ -15,8 +15,8 @@
 //     without MKL it is SLEEF's Sleef_acosf*_u10.  The rule pinned here is SLEEF u10 -- the open routine torch
 //     itself ships, ISA-stable -- and srf_acosf_u10 equals torch's own build of it on every float in [-1, 1] (exhaustive check).  Against
 //     a reference run whose acos was MKL's AVX-512 kernel, 4-6 samples per million land on the neighbouring row (never column).
-// The two SLEEF sequences were written from the published algorithm (sleefsimdsp.c, Boost licence) and compared instruction by instruction
-// with the routines in torch's libtorch_cpu.so (tools/sleef_check/sleef_dis.py).  Every multiply-add below is explicit: a translation
+// The two SLEEF sequences follow SLEEF's published source (sleefsimdsp.c, Boost licence) and are held to the results of the routines that
+// torch exports, by calling them (tests/test_sphere_exact.py).  Every multiply-add below is explicit: a translation
 // unit that includes this header must be compiled with -ffp-contract=off (rays.hip is; so is the host-side check).
 //
 // One source, two compilers: hipcc (device, used by rays.hip) and gcc (host, used ONLY by tests/ to compare this sequence with torch,
