@@ -20,7 +20,9 @@ SOURCES = ["runtime.hip", "rays.hip", "gemm.hip", "wgrad.hip", "fused.hip", "wid
 # (a spill then shows up as scratch usage, which tools/asmcheck.sh and the build's resource check refuse)
 EXTRA = {"wide.hip": ["-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"]}
 HEADERS = ["common.h", "gemm.h", "fused.h", "sphere_exact.h", os.path.join("..", "..", "include", "scenerf_hip.h")]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics",
+# no packed fp32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this chip now and then, without an error
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics"] + NO_PACKED_F32 + [
          "-Wall", "-Wno-unused-function"] + os.environ.get("SRF_EXTRA_FLAGS", "").split()
 
 
