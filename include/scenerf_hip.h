@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define SCENERF_HIP_ABI_VERSION 10
+#define SCENERF_HIP_ABI_VERSION 11
 #define SCENERF_N_SCALES 5          /* feature maps "1_1","1_2","1_4","1_8","1_16" */
 #define SCENERF_D_LATENT 2480       /* 80+160+320+640+1280 (resnetfc d_latent, scenerf.py:100-114) */
 #define SCENERF_D_HIDDEN 512
@@ -565,6 +565,74 @@ int scenerf_hip_sphere_resample_forward_nhwc(const float* x, int64_t planes, int
                                              float* out, scenerf_stream_t stream);
 int scenerf_hip_sphere_resample_backward_nhwc(const float* dout, int64_t planes, int C, int H, int W, const int32_t* row_ptr,
                                               const int32_t* cells, int out_w, int out_h, float* dx, scenerf_stream_t stream);
+
+/* ---- row operators: a linear layer with its epilogue, its 8-bit form, the RMS norm and rows in 8 bits ------------------------
+ * What a ResnetFC (reference scenerf/models/resnetfc.py:20-64, 133-164) of any width is made of, one entry per operator.  Rows are
+ * independent; sums, norms and statistics are held in 32 bits, every output is rounded once to its type.  Matrices are row-major
+ * with unit stride inside a row; a leading dimension counts ELEMENTS and may be 0 (one row read by all) or larger than the row. */
+#define SCENERF_T_F32  0
+#define SCENERF_T_BF16 1
+#define SCENERF_T_F16  2
+#define SCENERF_T_E4M3 3            /* OCP e4m3 (no infinities, largest value 448) */
+#define SCENERF_ACT_NONE 0
+#define SCENERF_ACT_RELU 1
+#define SCENERF_ACT_GELU 2          /* z/2 (1 + erf(z / sqrt 2)) */
+#define SCENERF_ACT_SILU 3          /* z / (1 + exp(-z)) */
+
+/* y = act(z) + residual,  z = x w^T + bias       (x: [rows][k], w: [n][k], y: [rows][n])
+ * in_type E4M3: z = (x w^T) x_scale[row] w_scale[col] + bias, forward only.
+ * backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = the column sums of dz (the residual's gradient is dy itself). */
+typedef struct scenerf_linear {
+    int32_t in_type;                /* x, w (and dx, dw) */
+    int32_t out_type;               /* bias, residual, y, z, dy, db: equal to in_type unless that is E4M3 */
+    int32_t activation;
+    int32_t n, k;                   /* >= 1 */
+    int64_t rows;                   /* >= 0, < 2^31 - 1024 */
+    const void* x; int64_t ldx;
+    const void* w; int64_t ldw;
+    const float* x_scale;           /* [rows], E4M3 only */
+    const float* w_scale;           /* [n], E4M3 only */
+    const void* bias;               /* [n] or NULL */
+    const void* residual; int64_t ld_residual;   /* [rows][n] or NULL */
+    void* y;                        /* [rows][n], dense (forward) */
+    void* z;                        /* [rows][n], dense: written by forward unless NULL, read by backward where activation != NONE */
+    const void* dy; int64_t ld_dy;  /* backward */
+    void* dx;                       /* [rows][k], dense, or NULL */
+    void* dw;                       /* [n][k], dense, or NULL */
+    void* db;                       /* [n], or NULL */
+    void* workspace;                /* scenerf_hip_linear_workspace bytes, 16-byte aligned; contents are left undefined */
+    int64_t workspace_bytes;
+} scenerf_linear;
+/* bytes of workspace the call needs (the pointers of *p are looked at for NULL and alignment only), or -1 */
+int64_t scenerf_hip_linear_workspace(const scenerf_linear* p, int backward);
+int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream);
+int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream);
+
+/* h = x + residual (x where residual is NULL);  rstd = 1 / sqrt(mean(h^2) + eps);  v = h rstd weight  (v = h where weight is NULL)
+ * y: v rounded to `type`;  q, scale: the row in 8 bits, scale = max(max|v| / 448, 2^-126), q = e4m3(v / scale) -- a row that holds a NaN
+ * or an infinity gets a scale that is not finite.  Any of h_out, y, q + scale, rstd_out may be NULL (not written). */
+typedef struct scenerf_rms {
+    int32_t type;                   /* x, residual, weight, h, y (and the gradients): F32, BF16, F16 */
+    int32_t width;                  /* >= 1 */
+    int64_t rows;                   /* >= 0, < 2^31 - 1024 */
+    float eps;
+    const void* x; int64_t ldx;
+    const void* residual; int64_t ld_residual;
+    const void* weight;             /* [width] */
+    void* h; void* y;               /* [rows][width], dense */
+    uint8_t* q; float* scale;       /* [rows][width] e4m3, [rows] */
+    float* rstd;                    /* [rows]: written by forward, read by backward */
+    /* backward: x holds h as the forward stored it (its x where there was no residual);
+     * dx = rstd (dy weight - xhat mean(dy weight xhat)) + dh, xhat = x rstd;  dweight = sum over rows of dy xhat */
+    const void* dy; int64_t ld_dy;
+    const void* dh; int64_t ld_dh;  /* gradient of h, or NULL */
+    void* dx;                       /* [rows][width], dense: the gradient of x and of residual */
+    void* dweight;                  /* [width], or NULL */
+    void* workspace; int64_t workspace_bytes;
+} scenerf_rms;
+int64_t scenerf_hip_rms_workspace(const scenerf_rms* p, int backward);
+int scenerf_hip_rms_forward(const scenerf_rms* p, scenerf_stream_t stream);
+int scenerf_hip_rms_backward(const scenerf_rms* p, scenerf_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -23,7 +23,7 @@ D_HIDDEN = 512
 D_XENC = 48
 TILE_ROWS = 128
 W_STREAM_BLOCKS = (3 * D_XENC + D_LATENT) // 16 + 2 * ((512 + D_LATENT) // 16) + 10 * (512 // 16)   # scenerf_hip.h
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 vp = C.c_void_p
 
@@ -111,6 +111,26 @@ class AdamWTensor(C.Structure):
                 ("step", C.c_int64)]
 
 
+class Linear(C.Structure):
+    """scenerf_linear (scenerf_hip.h)."""
+    _fields_ = [("in_type", C.c_int32), ("out_type", C.c_int32), ("activation", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("rows", C.c_int64),
+                ("x", vp), ("ldx", C.c_int64), ("w", vp), ("ldw", C.c_int64), ("x_scale", vp), ("w_scale", vp), ("bias", vp),
+                ("residual", vp), ("ld_residual", C.c_int64), ("y", vp), ("z", vp), ("dy", vp), ("ld_dy", C.c_int64),
+                ("dx", vp), ("dw", vp), ("db", vp), ("workspace", vp), ("workspace_bytes", C.c_int64)]
+
+
+class Rms(C.Structure):
+    """scenerf_rms (scenerf_hip.h)."""
+    _fields_ = [("type", C.c_int32), ("width", C.c_int32), ("rows", C.c_int64), ("eps", C.c_float),
+                ("x", vp), ("ldx", C.c_int64), ("residual", vp), ("ld_residual", C.c_int64), ("weight", vp), ("h", vp), ("y", vp),
+                ("q", vp), ("scale", vp), ("rstd", vp), ("dy", vp), ("ld_dy", C.c_int64), ("dh", vp), ("ld_dh", C.c_int64),
+                ("dx", vp), ("dweight", vp), ("workspace", vp), ("workspace_bytes", C.c_int64)]
+
+
+T_F32, T_BF16, T_F16, T_E4M3 = 0, 1, 2, 3                        # SCENERF_T_*
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}       # SCENERF_ACT_*
+
+
 class ProfRec(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("launches", C.c_int32), ("total_ms", C.c_float),
                 ("flops", C.c_double), ("bytes", C.c_double)]
@@ -169,6 +189,12 @@ _PROTOS = {
     "scenerf_hip_test_chunk_table": (C.c_int, [C.POINTER(Cfg), i32, vp, i32]),
     "scenerf_hip_test_set_tuning": (C.c_int, [i32, i32]),
     "scenerf_hip_test_gemm_tn": (C.c_int, [i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]),
+    "scenerf_hip_linear_workspace": (C.c_int64, [C.POINTER(Linear), i32]),
+    "scenerf_hip_linear_forward": (C.c_int, [C.POINTER(Linear), vp]),
+    "scenerf_hip_linear_backward": (C.c_int, [C.POINTER(Linear), vp]),
+    "scenerf_hip_rms_workspace": (C.c_int64, [C.POINTER(Rms), i32]),
+    "scenerf_hip_rms_forward": (C.c_int, [C.POINTER(Rms), vp]),
+    "scenerf_hip_rms_backward": (C.c_int, [C.POINTER(Rms), vp]),
     "scenerf_hip_profile_enable": (C.c_int, [i32]),
     "scenerf_hip_profile_collect": (C.c_int, [C.POINTER(ProfRec), i32]),
 }

@@ -1,0 +1,93 @@
+// The product behind scenerf_hip_linear_*: C[i][j] = sum_k A(i, k) B(j, k), with the layer's epilogue.
+#pragma once
+#include "rowops.h"
+
+struct LinArgs {
+    const void* A; const void* B;        // A(i, k) = A[i * a_i + k * a_k], B(j, k) = B[j * b_j + k * b_k]; one of each pair is 1
+    long a_i, a_k, b_j, b_k;
+    int M, N, K;
+    // epilogue: v = acc * row_scale[i] * col_scale[j] + bias[j]; z = v; out = act(v) + residual
+    const float* row_scale; const float* col_scale;
+    const void* bias; const void* residual; long ld_residual;
+    void* out; void* z;                  // dense [M][N]
+    float* part;                         // not NULL: the raw sums of split s go to part[s][M][N] instead
+    int act, tiles_i, tiles_j, splits, k_split;     // k_split: contraction elements per split
+    int vec;                             // the epilogue may move 16 bytes at a time
+};
+
+__device__ static inline float act_any(int act, float v) {
+    if (act == SCENERF_ACT_RELU) return act_fwd<SCENERF_ACT_RELU>(v);
+    if (act == SCENERF_ACT_GELU) return act_fwd<SCENERF_ACT_GELU>(v);
+    if (act == SCENERF_ACT_SILU) return act_fwd<SCENERF_ACT_SILU>(v);
+    return v;
+}
+__device__ static inline float slope_any(int act, float v) {
+    if (act == SCENERF_ACT_RELU) return act_slope<SCENERF_ACT_RELU>(v);
+    if (act == SCENERF_ACT_GELU) return act_slope<SCENERF_ACT_GELU>(v);
+    if (act == SCENERF_ACT_SILU) return act_slope<SCENERF_ACT_SILU>(v);
+    return 1.f;
+}
+// z as it is kept for the backward pass, in O.  A positive z that rounds to zero (fp16) is kept as the smallest positive value: relu's
+// slope there is 1, and the other slopes do not notice.
+template <typename O> __device__ static inline float keep_z(float v) {
+    if constexpr (O::code == SCENERF_T_F16) return v > 0.f && v < 5.9604645e-8f ? 5.9604645e-8f : v;
+    return v;
+}
+template <typename O> __device__ static inline void epilogue_one(const LinArgs& p, long i, int j, float v) {
+    typedef typename O::raw raw;
+    if (p.row_scale) v = v * p.row_scale[i] * p.col_scale[j];
+    if (p.bias) v += O::to_f32(((const raw*)p.bias)[j]);
+    if (p.z) ((raw*)p.z)[i * p.N + j] = O::from_f32(keep_z<O>(v));
+    v = act_any(p.act, v);
+    if (p.residual) v += O::to_f32(((const raw*)p.residual)[i * p.ld_residual + j]);
+    ((raw*)p.out)[i * p.N + j] = O::from_f32(v);
+}
+// W = 16 / sizeof(O::raw) neighbouring elements, all inside the row, every address aligned to 16 bytes
+template <typename O, int W> __device__ static inline void epilogue_vec(const LinArgs& p, long i, int j, float (&v)[W]) {
+    typedef typename O::raw raw;
+    if (p.row_scale) {
+        const float s = p.row_scale[i];
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] = v[e] * s * p.col_scale[j + e];
+    }
+    float t[W];
+    if (p.bias) {
+        load_vec<O, W>((const raw*)p.bias + j, t);
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] += t[e];
+    }
+    if (p.z) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) t[e] = keep_z<O>(v[e]);
+        store_vec<O, W>((raw*)p.z + i * p.N + j, t);
+    }
+    if (p.act != SCENERF_ACT_NONE) {
+        if (p.act == SCENERF_ACT_RELU) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] = act_fwd<SCENERF_ACT_RELU>(v[e]);
+        } else if (p.act == SCENERF_ACT_GELU) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] = act_fwd<SCENERF_ACT_GELU>(v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] = act_fwd<SCENERF_ACT_SILU>(v[e]);
+        }
+    }
+    if (p.residual) {
+        load_vec<O, W>((const raw*)p.residual + i * p.ld_residual + j, t);
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] += t[e];
+    }
+    store_vec<O, W>((raw*)p.out + i * p.N + j, v);
+}
+
+// Tile shapes of the staged kernel (linear_tile.h): rows x columns of the result per workgroup
+enum LinTile { LIN_256x256, LIN_256x128, LIN_128x128, LIN_128x32, LIN_32x128, LIN_TILES };
+static const int kLinTileRows[LIN_TILES] = {256, 256, 128, 128, 32}, kLinTileCols[LIN_TILES] = {256, 128, 128, 32, 128};
+#define LIN_CHUNK_BYTES 64              // of the contraction per step: 16 fp32, 32 16-bit, 64 8-bit elements
+
+// a_k == 1 / b_k == 1: read along the contraction, else across
+int linear_tile_f32(const LinArgs& a, LinTile tile, hipStream_t s);
+int linear_tile_bf16(const LinArgs& a, LinTile tile, hipStream_t s);
+int linear_tile_f16(const LinArgs& a, LinTile tile, hipStream_t s);
+int linear_tile_e4m3(const LinArgs& a, LinTile tile, int out_type, hipStream_t s);

@@ -1,0 +1,498 @@
+// RMS norm of rows with the residual's addition, rows in 8 bits with scales, and the norm's gradients (gfx950).
+//
+//   h = x + r;  rstd = (mean h^2 + eps)^-1/2;  v = h rstd w;  y = v;  scale = max(max|v| / 448, 2^-126), q = e4m3(v / scale)
+//   dx = rstd (dy w - xhat mean(dy w xhat)) + dh,  xhat = h rstd;  dw = sum over rows of dy xhat
+//
+// All of it is bound by HBM: each input is read once and each output written once, everything in between lives in registers.  One
+// wave owns a row (the two row sums are one 6-step exchange, no barrier), holds it in registers up to ROW_REGS elements a lane, and
+// walks the rows in a grid stride, so that the weight is loaded once per wave.  Wider rows go through a workgroup that reads the row
+// twice (the second time from L2).  The weight's gradient is summed per lane over the wave's rows, then over the workgroup's waves in
+// LDS, then over the workgroups by a second kernel in a fixed order: no atomics, the same bits every time.
+#include "rowops.h"
+
+#define ROW_WAVES 4
+#define ROW_REGS 64                 // elements of a row a lane holds at most: 4096 columns
+#define WIDE_THREADS 1024
+
+// the largest |v| as bits: NaN is above infinity, so a row's NaN survives the maximum
+__device__ static inline uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ static inline uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t t = (uint32_t)__shfl_xor((int)v, o, WAVE);
+        v = t > v ? t : v;
+    }
+    return v;
+}
+__device__ static inline float row_scale(uint32_t max_bits) {
+    const float m = __uint_as_float(max_bits) / 448.f;
+    return m < 1.1754943508222875e-38f ? 1.1754943508222875e-38f : m;   // NaN stays
+}
+
+struct RmsArgs {
+    const void* x; const void* residual; const void* weight;
+    void* h; void* y; uint8_t* q; float* scale; float* rstd;
+    const void* dy; const void* dh; void* dx;
+    float* partial;
+    long ldx, ld_residual, ld_dy, ld_dh;
+    int rows, width;
+    float eps, inv_width;
+};
+
+// C chunks of 64 * VW columns: lane l holds columns c * 64 * VW + l * VW ..+ VW
+template <typename E, int VW, int C>
+__global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
+    typedef typename E::raw raw;
+    const int lane = threadIdx.x & 63;
+    const int D = p.width;
+    float w[C][VW];
+    bool in[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int col = (c * 64 + lane) * VW;
+        in[c] = col < D;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) w[c][e] = 0.f;
+        if (in[c] && p.weight) load_vec<E, VW>((const raw*)p.weight + col, w[c]);
+    }
+    const int waves = gridDim.x * ROW_WAVES;
+    for (long row = (long)blockIdx.x * ROW_WAVES + (threadIdx.x >> 6); row < p.rows; row += waves) {
+        float h[C][VW];
+        float ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = (c * 64 + lane) * VW;
+#pragma unroll
+            for (int e = 0; e < VW; ++e) h[c][e] = 0.f;
+            if (in[c]) load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h[c]);
+        }
+        if (p.residual) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int col = (c * 64 + lane) * VW;
+                if (in[c]) {
+                    float r[VW];
+                    load_vec<E, VW>((const raw*)p.residual + row * p.ld_residual + col, r);
+#pragma unroll
+                    for (int e = 0; e < VW; ++e) h[c][e] += r[e];
+                    if (p.h) store_vec<E, VW>((raw*)p.h + row * D + col, h[c]);
+                }
+            }
+        }
+        if (p.weight) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < VW; ++e) ss = fmaf(h[c][e], h[c][e], ss);
+            ss = wave_sum(ss);
+            const float rstd = 1.f / sqrtf(fmaf(ss, p.inv_width, p.eps));
+            if (p.rstd && lane == 0) p.rstd[row] = rstd;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < VW; ++e) h[c][e] = h[c][e] * rstd * w[c][e];
+        }
+        if (p.y) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (in[c]) store_vec<E, VW>((raw*)p.y + row * D + (c * 64 + lane) * VW, h[c]);
+        }
+        if (p.q) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < VW; ++e) {
+                    const uint32_t b = in[c] ? abs_bits(h[c][e]) : 0u;      // (columns past the row hold 0 * rstd: NaN in a NaN row only)
+                    m = b > m ? b : m;
+                }
+            const float s = row_scale(wave_max_u32(m)), inv = 1.f / s;
+            if (lane == 0) p.scale[row] = s;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (in[c]) {
+                    float v[VW];
+#pragma unroll
+                    for (int e = 0; e < VW; ++e) v[e] = h[c][e] * inv;
+                    store_vec<TypeE4M3, VW>(p.q + row * D + (c * 64 + lane) * VW, v);
+                }
+        }
+    }
+}
+
+// rows wider than a wave's registers: one workgroup a row, two reads
+__device__ static inline float block_sum(float v, float* red) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int i = 0; i < WIDE_THREADS / 64; ++i) v += red[i];
+    return v;
+}
+__device__ static inline uint32_t block_max_u32(uint32_t v, uint32_t* red) {
+    v = wave_max_u32(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+    for (int i = 0; i < WIDE_THREADS / 64; ++i) v = red[i] > v ? red[i] : v;
+    return v;
+}
+template <typename E, int VW>
+__global__ __launch_bounds__(WIDE_THREADS) void rms_rows_wide_kernel(RmsArgs p) {
+    typedef typename E::raw raw;
+    __shared__ float red[WIDE_THREADS / 64];
+    const long D = p.width;
+    for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        float ss = 0.f;
+        uint32_t m = 0;
+        for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
+            float h[VW];
+            load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h);
+            if (p.residual) {
+                float r[VW];
+                load_vec<E, VW>((const raw*)p.residual + row * p.ld_residual + col, r);
+#pragma unroll
+                for (int e = 0; e < VW; ++e) h[e] += r[e];
+                if (p.h) store_vec<E, VW>((raw*)p.h + row * D + col, h);
+            }
+            float w[VW];
+#pragma unroll
+            for (int e = 0; e < VW; ++e) w[e] = 1.f;
+            if (p.weight) load_vec<E, VW>((const raw*)p.weight + col, w);
+#pragma unroll
+            for (int e = 0; e < VW; ++e) {
+                ss = fmaf(h[e], h[e], ss);
+                const uint32_t b = abs_bits(h[e] * w[e]);
+                m = b > m ? b : m;
+            }
+        }
+        float rstd = 1.f;
+        if (p.weight) {
+            rstd = 1.f / sqrtf(fmaf(block_sum(ss, red), p.inv_width, p.eps));
+            if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
+        }
+        float s = 1.f, inv = 1.f;
+        if (p.q) {
+            // max |h rstd w| = rstd max |h w|: the last bit may differ from the largest value's own, the scale's rounding
+            s = row_scale(abs_bits(__uint_as_float(block_max_u32(m, (uint32_t*)red)) * rstd));
+            inv = 1.f / s;
+            if (threadIdx.x == 0) p.scale[row] = s;
+        }
+        for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
+            float h[VW];
+            load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h);
+            if (p.residual) {
+                float r[VW];
+                load_vec<E, VW>((const raw*)p.residual + row * p.ld_residual + col, r);
+#pragma unroll
+                for (int e = 0; e < VW; ++e) h[e] += r[e];
+            }
+            if (p.weight) {
+                float w[VW];
+                load_vec<E, VW>((const raw*)p.weight + col, w);
+#pragma unroll
+                for (int e = 0; e < VW; ++e) h[e] = h[e] * rstd * w[e];
+            }
+            if (p.y) store_vec<E, VW>((raw*)p.y + row * D + col, h);
+            if (p.q) {
+#pragma unroll
+                for (int e = 0; e < VW; ++e) h[e] *= inv;
+                store_vec<TypeE4M3, VW>(p.q + row * D + col, h);
+            }
+        }
+    }
+}
+
+// gradients: dx, and this workgroup's part of dweight in partial[blockIdx.x][width]
+template <typename E, int VW, int C>
+__global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
+    typedef typename E::raw raw;
+    __shared__ float red[ROW_WAVES][64 * VW];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int D = p.width;
+    float w[C][VW], dw[C][VW];
+    bool in[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int col = (c * 64 + lane) * VW;
+        in[c] = col < D;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) w[c][e] = dw[c][e] = 0.f;
+        if (in[c]) load_vec<E, VW>((const raw*)p.weight + col, w[c]);
+    }
+    const int waves = gridDim.x * ROW_WAVES;
+    for (long row = (long)blockIdx.x * ROW_WAVES + wv; row < p.rows; row += waves) {
+        float h[C][VW], g[C][VW];
+        const float rstd = p.rstd[row];
+        float dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = (c * 64 + lane) * VW;
+#pragma unroll
+            for (int e = 0; e < VW; ++e) h[c][e] = g[c][e] = 0.f;
+            if (in[c]) {
+                load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h[c]);
+                load_vec<E, VW>((const raw*)p.dy + row * p.ld_dy + col, g[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) {
+                h[c][e] *= rstd;
+                dw[c][e] = fmaf(g[c][e], h[c][e], dw[c][e]);
+                g[c][e] *= w[c][e];
+                dot = fmaf(g[c][e], h[c][e], dot);
+            }
+        if (!p.dx) continue;
+        dot = wave_sum(dot) * p.inv_width;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (in[c]) {
+                const int col = (c * 64 + lane) * VW;
+                float d[VW];
+#pragma unroll
+                for (int e = 0; e < VW; ++e) d[e] = 0.f;
+                if (p.dh) load_vec<E, VW>((const raw*)p.dh + row * p.ld_dh + col, d);
+#pragma unroll
+                for (int e = 0; e < VW; ++e) d[e] = fmaf(rstd, fmaf(-dot, h[c][e], g[c][e]), d[e]);
+                store_vec<E, VW>((raw*)p.dx + row * D + col, d);
+            }
+    }
+    if (!p.partial) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < VW; ++e) red[wv][lane * VW + e] = dw[c][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 64 * VW; i += 64 * ROW_WAVES) {
+            const int col = c * 64 * VW + i;
+            if (col < D) {
+                float s = 0.f;
+#pragma unroll
+                for (int k = 0; k < ROW_WAVES; ++k) s += red[k][i];
+                p.partial[(size_t)blockIdx.x * D + col] = s;
+            }
+        }
+    }
+}
+template <typename E, int VW>
+__global__ __launch_bounds__(WIDE_THREADS) void rms_grad_wide_kernel(RmsArgs p) {
+    typedef typename E::raw raw;
+    __shared__ float red[WIDE_THREADS / 64];
+    const long D = p.width;
+    for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const float rstd = p.rstd[row];
+        float dot = 0.f;
+        for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
+            float h[VW], g[VW], w[VW];
+            load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h);
+            load_vec<E, VW>((const raw*)p.dy + row * p.ld_dy + col, g);
+            load_vec<E, VW>((const raw*)p.weight + col, w);
+#pragma unroll
+            for (int e = 0; e < VW; ++e) dot = fmaf(g[e] * w[e], h[e] * rstd, dot);
+        }
+        dot = block_sum(dot, red) * p.inv_width;
+        for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
+            float h[VW], g[VW], w[VW], d[VW];
+            load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h);
+            load_vec<E, VW>((const raw*)p.dy + row * p.ld_dy + col, g);
+            load_vec<E, VW>((const raw*)p.weight + col, w);
+#pragma unroll
+            for (int e = 0; e < VW; ++e) d[e] = 0.f;
+            if (p.dh) load_vec<E, VW>((const raw*)p.dh + row * p.ld_dh + col, d);
+#pragma unroll
+            for (int e = 0; e < VW; ++e) d[e] = fmaf(rstd, fmaf(-dot, h[e] * rstd, g[e] * w[e]), d[e]);
+            store_vec<E, VW>((raw*)p.dx + row * D + col, d);
+        }
+    }
+}
+// the weight's gradient of wide rows, by columns: workgroup (x: 64 columns, y: a strip of rows)
+template <typename E>
+__global__ __launch_bounds__(256) void rms_dweight_cols_kernel(RmsArgs p, int strip) {
+    typedef typename E::raw raw;
+    __shared__ float red[4][64];
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), ty = threadIdx.x >> 6;
+    const long r0 = (long)blockIdx.y * strip, r1 = min((long)p.rows, r0 + strip);
+    float s = 0.f;
+    if (col < p.width)
+        for (long r = r0 + ty; r < r1; r += 4)
+            s = fmaf(E::to_f32(((const raw*)p.dy)[r * p.ld_dy + col]), E::to_f32(((const raw*)p.x)[r * p.ldx + col]) * p.rstd[r], s);
+    red[ty][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (ty == 0 && col < p.width)
+        p.partial[(size_t)blockIdx.y * p.width + col] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+}
+
+// out[col] = the sum of part[0..count)[col], in a fixed order: 8 interleaved chains, then their sum
+template <typename E>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ part, int count, int width, typename E::raw* __restrict__ out) {
+    __shared__ float red[8][32];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31), ty = threadIdx.x >> 5;
+    float s = 0.f;
+    if (col < width)
+        for (int i = ty; i < count; i += 8) s += part[(size_t)i * width + col];
+    red[ty][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (ty == 0 && col < width) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
+        out[col] = E::from_f32(s);
+    }
+}
+int launch_sum_parts(int type, const float* part, int count, int width, void* out, hipStream_t s) {
+    const int blocks = cdiv(width, 32);
+    if (type == SCENERF_T_F32) sum_parts_kernel<TypeF32><<<blocks, 256, 0, s>>>(part, count, width, (float*)out);
+    else if (type == SCENERF_T_BF16) sum_parts_kernel<TypeBF16><<<blocks, 256, 0, s>>>(part, count, width, (uint16_t*)out);
+    else sum_parts_kernel<TypeF16><<<blocks, 256, 0, s>>>(part, count, width, (uint16_t*)out);
+    SRF_LAUNCH_CHECK("sum_parts_kernel");
+    return 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host side
+static int rms_es(int type) { return type == SCENERF_T_F32 ? 4 : 2; }
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// 16-byte accesses need the row's length and every pitch in whole pieces, and aligned bases
+static bool rms_vector_ok(const scenerf_rms* p, bool backward) {
+    const int vw = 16 / rms_es(p->type);
+    if (p->width % vw || p->ldx % vw || !aligned16(p->x) || (p->weight && !aligned16(p->weight))) return false;
+    if (backward) {
+        if (p->ld_dy % vw || !aligned16(p->dy) || (p->dx && !aligned16(p->dx))) return false;
+        return !p->dh || (p->ld_dh % vw == 0 && aligned16(p->dh));
+    }
+    if (p->residual && (p->ld_residual % vw || !aligned16(p->residual))) return false;
+    return (!p->h || aligned16(p->h)) && (!p->y || aligned16(p->y)) && (!p->q || aligned16(p->q));
+}
+static bool rms_in_registers(const scenerf_rms* p) { return p->width <= 64 * ROW_REGS; }
+#define RMS_GRAD_BLOCKS 512         // workgroups (and parts of dweight) of the gradient kernel: two per CU
+#define RMS_STRIP 512
+static int rms_grad_parts(const scenerf_rms* p) {
+    if (!rms_in_registers(p)) return (int)((p->rows + RMS_STRIP - 1) / RMS_STRIP);
+    const long want = (p->rows + ROW_WAVES - 1) / ROW_WAVES;
+    return (int)(want < RMS_GRAD_BLOCKS ? want : RMS_GRAD_BLOCKS);
+}
+static int rms_check(const scenerf_rms* p, const char* what, bool backward) {
+    SRF_CHECK(p, "%s: NULL argument", what);
+    SRF_CHECK(p->type >= SCENERF_T_F32 && p->type <= SCENERF_T_F16, "%s: type must be F32, BF16 or F16", what);
+    SRF_CHECK(p->width >= 1 && p->rows >= 0 && p->rows < ROWOPS_GRID_MAX - 1024, "%s: width >= 1 and 0 <= rows < 2^31 - 1024", what);
+    SRF_CHECK(p->eps >= 0.f, "%s: eps must not be negative", what);
+    SRF_CHECK(p->ldx >= 0 && p->ld_residual >= 0 && p->ld_dy >= 0 && p->ld_dh >= 0, "%s: negative leading dimension", what);
+    if (p->rows == 0 && !(backward && p->dweight)) return 0;
+    if (backward) {
+        SRF_CHECK(p->rows == 0 || (p->x && p->weight && p->rstd && p->dy), "%s: NULL x, weight, rstd or dy", what);
+        SRF_CHECK(p->dx || p->dweight, "%s: nothing to compute", what);
+    } else {
+        SRF_CHECK(p->x, "%s: x is NULL", what);
+        SRF_CHECK(p->y || p->q || p->h, "%s: nothing to compute", what);
+        SRF_CHECK(!p->h || p->residual, "%s: h is written only where a residual is added", what);
+        SRF_CHECK(!p->q == !p->scale, "%s: q and scale go together", what);
+        SRF_CHECK(p->weight || !p->rstd, "%s: rstd without weight", what);
+    }
+    return 0;
+}
+static RmsArgs rms_args(const scenerf_rms* p) {
+    RmsArgs a = {};
+    a.x = p->x; a.residual = p->residual; a.weight = p->weight; a.h = p->h; a.y = p->y; a.q = p->q; a.scale = p->scale; a.rstd = p->rstd;
+    a.dy = p->dy; a.dh = p->dh; a.dx = p->dx;
+    a.ldx = p->ldx; a.ld_residual = p->ld_residual; a.ld_dy = p->ld_dy; a.ld_dh = p->ld_dh;
+    a.rows = (int)p->rows; a.width = p->width; a.eps = p->eps; a.inv_width = 1.f / (float)p->width;
+    return a;
+}
+
+template <typename E, int VW, int C> static void rms_launch(const RmsArgs& a, bool backward, int blocks, hipStream_t s) {
+    if (backward) rms_grad_kernel<E, VW, C><<<blocks, 64 * ROW_WAVES, 0, s>>>(a);
+    else rms_rows_kernel<E, VW, C><<<blocks, 64 * ROW_WAVES, 0, s>>>(a);
+}
+// the smallest number of chunks that holds the row
+template <typename E, int VW> static void rms_launch_chunks(const RmsArgs& a, bool backward, int blocks, hipStream_t s) {
+    const int chunks = cdiv(a.width, 64 * VW);
+    if (chunks <= 1) return rms_launch<E, VW, 1>(a, backward, blocks, s);
+    if (chunks <= 2) return rms_launch<E, VW, 2>(a, backward, blocks, s);
+    if (chunks <= 4) return rms_launch<E, VW, 4>(a, backward, blocks, s);
+    if (chunks <= 8) return rms_launch<E, VW, 8>(a, backward, blocks, s);
+    if constexpr (VW <= 4) {
+        if (chunks <= 16) return rms_launch<E, VW, 16>(a, backward, blocks, s);
+    }
+    if constexpr (VW == 1) {
+        if (chunks <= 32) return rms_launch<E, VW, 32>(a, backward, blocks, s);
+        rms_launch<E, VW, 64>(a, backward, blocks, s);
+    }
+}
+template <typename E> static int rms_dispatch(const scenerf_rms* p, bool backward, hipStream_t s) {
+    constexpr int VW = 16 / sizeof(typename E::raw);
+    RmsArgs a = rms_args(p);
+    const bool vec = rms_vector_ok(p, backward);
+    if (backward) {
+        const int parts = rms_grad_parts(p);
+        a.partial = p->dweight ? (float*)p->workspace : nullptr;
+        if (p->rows > 0 && rms_in_registers(p)) {
+            if (vec) rms_launch_chunks<E, VW>(a, true, parts, s);
+            else rms_launch_chunks<E, 1>(a, true, parts, s);
+            SRF_LAUNCH_CHECK("rms_grad_kernel");
+        } else if (p->rows > 0) {
+            if (p->dx) {
+                const int blocks = p->rows < 4096 ? (int)p->rows : 4096;
+                if (vec) rms_grad_wide_kernel<E, VW><<<blocks, WIDE_THREADS, 0, s>>>(a);
+                else rms_grad_wide_kernel<E, 1><<<blocks, WIDE_THREADS, 0, s>>>(a);
+                SRF_LAUNCH_CHECK("rms_grad_wide_kernel");
+            }
+            if (p->dweight) {
+                SRF_CHECK(parts <= 65535, "rms_backward: rows of more than %d columns are limited to %d rows", 64 * ROW_REGS, 65535 * RMS_STRIP);
+                rms_dweight_cols_kernel<E><<<dim3(cdiv(p->width, 64), parts), 256, 0, s>>>(a, RMS_STRIP);
+                SRF_LAUNCH_CHECK("rms_dweight_cols_kernel");
+            }
+        }
+        if (p->dweight) return launch_sum_parts(E::code, a.partial, parts, p->width, p->dweight, s);
+        return 0;
+    }
+    if (rms_in_registers(p)) {
+        const long want = (p->rows + ROW_WAVES - 1) / ROW_WAVES;
+        const int blocks = (int)(want < 8192 ? want : 8192);
+        if (vec) rms_launch_chunks<E, VW>(a, false, blocks, s);
+        else rms_launch_chunks<E, 1>(a, false, blocks, s);
+        SRF_LAUNCH_CHECK("rms_rows_kernel");
+    } else {
+        const int blocks = p->rows < 4096 ? (int)p->rows : 4096;
+        if (vec) rms_rows_wide_kernel<E, VW><<<blocks, WIDE_THREADS, 0, s>>>(a);
+        else rms_rows_wide_kernel<E, 1><<<blocks, WIDE_THREADS, 0, s>>>(a);
+        SRF_LAUNCH_CHECK("rms_rows_wide_kernel");
+    }
+    return 0;
+}
+static int rms_run(const scenerf_rms* p, bool backward, hipStream_t s) {
+    if (p->type == SCENERF_T_F32) return rms_dispatch<TypeF32>(p, backward, s);
+    if (p->type == SCENERF_T_BF16) return rms_dispatch<TypeBF16>(p, backward, s);
+    return rms_dispatch<TypeF16>(p, backward, s);
+}
+
+extern "C" {
+
+int64_t scenerf_hip_rms_workspace(const scenerf_rms* p, int backward) {
+    if (rms_check(p, "rms_workspace", backward != 0)) return -1;
+    return backward && p->dweight ? (int64_t)rms_grad_parts(p) * p->width * 4 : 0;
+}
+
+int scenerf_hip_rms_forward(const scenerf_rms* p, scenerf_stream_t stream) {
+    if (int e = rms_check(p, "rms_forward", false)) return e;
+    if (p->rows == 0) return 0;
+    const double es = rms_es(p->type), e = (double)p->rows * p->width;
+    SrfLaunchScope ps(as_stream(stream), "rms_forward", 5 * e, e * (es * (1 + !!p->residual + !!p->h + !!p->y) + !!p->q));
+    return rms_run(p, false, as_stream(stream));
+}
+
+int scenerf_hip_rms_backward(const scenerf_rms* p, scenerf_stream_t stream) {
+    if (int e = rms_check(p, "rms_backward", true)) return e;
+    if (p->rows == 0 && !p->dweight) return 0;
+    const int64_t need = scenerf_hip_rms_workspace(p, 1);
+    SRF_CHECK(need == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= need), "rms_backward: workspace of %lld bytes needed",
+              (long long)need);
+    const double es = rms_es(p->type), e = (double)p->rows * p->width;
+    SrfLaunchScope ps(as_stream(stream), "rms_backward", 10 * e, e * es * (2 + !!p->dh + !!p->dx));
+    return rms_run(p, true, as_stream(stream));
+}
+
+}  // extern "C"

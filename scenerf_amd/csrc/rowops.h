@@ -1,0 +1,101 @@
+// Element types, conversions and activations shared by the row operators (linear.hip, norm.hip).
+#pragma once
+#include "common.h"
+
+#define ROWOPS_GRID_MAX 0x7fffffffLL
+
+typedef __attribute__((ext_vector_type(2))) _Float16 srf_f16x2;
+
+// Storage of one element and its conversions.  Every store to 16 bits rounds to nearest even ONCE, from a 32-bit value.
+struct TypeF32 {
+    typedef float raw;
+    static constexpr int code = SCENERF_T_F32;
+    __device__ static inline float to_f32(raw v) { return v; }
+    __device__ static inline raw from_f32(float v) { return v; }
+};
+struct TypeBF16 {
+    typedef uint16_t raw;
+    static constexpr int code = SCENERF_T_BF16;
+    __device__ static inline float to_f32(raw v) { return __uint_as_float((uint32_t)v << 16); }
+    __device__ static inline raw from_f32(float v) { return (raw)pack_bf16x2(v, 0.f); }
+};
+struct TypeF16 {
+    typedef uint16_t raw;
+    static constexpr int code = SCENERF_T_F16;
+    __device__ static inline float to_f32(raw v) { return (float)__builtin_bit_cast(_Float16, v); }
+    __device__ static inline raw from_f32(float v) { return __builtin_bit_cast(raw, (_Float16)v); }
+};
+struct TypeE4M3 {
+    typedef uint8_t raw;
+    static constexpr int code = SCENERF_T_E4M3;
+    __device__ static inline float to_f32(raw v) { return __builtin_amdgcn_cvt_f32_fp8((int)v, 0); }
+    __device__ static inline raw from_f32(float v) { return (raw)__builtin_amdgcn_cvt_pk_fp8_f32(v, 0.f, 0, false); }
+};
+
+// W consecutive elements as floats.  W * sizeof(raw) is 4, 8 or 16 bytes (or 32: two loads) and the address is aligned to that, up to 16.
+template <typename E, int W> __device__ static inline void load_vec(const typename E::raw* p, float (&v)[W]) {
+    if constexpr (W == 1) {
+        v[0] = E::to_f32(p[0]);
+    } else if constexpr (sizeof(typename E::raw) == 4) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const float4 t = *(const float4*)(p + i);
+            v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
+        }
+    } else {
+        static_assert(sizeof(typename E::raw) == 2 && W == 8, "16-bit types move 8 elements");
+        const uint4 t = *(const uint4*)p;
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = E::to_f32((uint16_t)(w[i] & 0xffffu));
+            v[2 * i + 1] = E::to_f32((uint16_t)(w[i] >> 16));
+        }
+    }
+}
+template <typename E> __device__ static inline uint32_t pack2(float a, float b) {
+    if constexpr (E::code == SCENERF_T_BF16) {
+        return pack_bf16x2(a, b);
+    } else {
+        srf_f32x2 v = {a, b};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, srf_f16x2));
+    }
+}
+template <typename E, int W> __device__ static inline void store_vec(typename E::raw* p, const float (&v)[W]) {
+    if constexpr (W == 1) {
+        p[0] = E::from_f32(v[0]);
+    } else if constexpr (sizeof(typename E::raw) == 4) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) *(float4*)(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else if constexpr (sizeof(typename E::raw) == 2) {
+        static_assert(W == 8, "16-bit types move 8 elements");
+        *(uint4*)p = make_uint4(pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7]));
+    } else {
+        uint32_t w[W / 4];
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[i], v[i + 1], 0, false);
+            w[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[i + 2], v[i + 3], t, true);
+        }
+        if constexpr (W == 8) *(uint2*)p = make_uint2(w[0], w[1]);
+        else *(uint32_t*)p = w[0];
+    }
+}
+
+// Activations and their slopes.  relu keeps NaN (a comparison, not fmaxf, which would drop it) and its slope at 0 is 0.
+template <int ACT> __device__ static inline float act_fwd(float z) {
+    if constexpr (ACT == SCENERF_ACT_RELU) return z < 0.f ? 0.f : z;
+    if constexpr (ACT == SCENERF_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if constexpr (ACT == SCENERF_ACT_SILU) return z / (1.f + expf(-z));
+    return z;
+}
+template <int ACT> __device__ static inline float act_slope(float z) {
+    if constexpr (ACT == SCENERF_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if constexpr (ACT == SCENERF_ACT_GELU)
+        return fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+    if constexpr (ACT == SCENERF_ACT_SILU) {
+        const float p = 1.f / (1.f + expf(-z));
+        return p * fmaf(z, 1.f - p, 1.f);
+    }
+    return 1.f;
+}

@@ -1,0 +1,256 @@
+"""linear / linear_8bit / quantize_rows (scenerf_amd.linear) against their definitions in 64 bits (rowops_util: bounds per element)."""
+import pytest
+import torch
+
+from rowops_util import hold, linear64
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+ACTS = ["none", "relu", "gelu", "silu"]
+
+
+def normal(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+def gen(*key):
+    return torch.Generator(device=DEV).manual_seed(sum(ord(c) * (i + 1) for i, c in enumerate(repr(key))))
+
+
+def whole(g, *shape, dtype, top=2):
+    return torch.randint(-top, top + 1, shape, generator=g, device=DEV).to(dtype)
+
+
+# rows x k x n: one element, one row, odd everything, tile edges (63 .. 65, 127 .. 129, 255 .. 257), short and long sums
+SIZES = [(1, 1, 1), (1, 2480, 1536), (2, 42, 515), (7, 48, 4), (33, 130, 2), (63, 64, 65), (64, 63, 64), (65, 257, 63), (129, 128, 127),
+         (255, 42, 512), (257, 512, 256), (300, 1000, 24), (513, 31, 130), (1024, 512, 512), (4801, 96, 130)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_forward(m, k, n, dtype):
+    from scenerf_amd.linear import linear
+    g = gen("fwd", m, k, n, dtype)
+    x, w, b, r = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5), normal(g, n, dtype=dtype), normal(g, m, n, dtype=dtype)
+    for act in ACTS:
+        hold(linear(x, w, b, activation=act, residual=r), linear64(x, w, b, act, r)["y"], act)
+    hold(linear(x, w), linear64(x, w)["y"], "bare")
+    hold(linear(x, w, b), linear64(x, w, b)["y"], "bias")
+    hold(linear(x, w, residual=r, activation="gelu"), linear64(x, w, None, "gelu", r)["y"], "residual")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_gradients_against_the_formula(m, k, n, dtype):
+    from scenerf_amd.linear import linear
+    g = gen("bwd", m, k, n, dtype)
+    for act in ("none", "gelu", "silu"):
+        x, w, b, r = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5), normal(g, n, dtype=dtype), normal(g, m, n, dtype=dtype)
+        leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+        dy = normal(g, m, n, dtype=dtype)
+        y = linear(x, w, b, activation=act, residual=r)
+        grads = torch.autograd.grad(y, leaves, dy)
+        want = linear64(x.detach(), w.detach(), b.detach(), act, r.detach(), dy)
+        hold(y.detach(), want["y"], act + " y")
+        for name, got in zip(("dx", "dw", "db", "dr"), grads):
+            hold(got, want[name], "%s %s" % (act, name))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(1, 5, 3), (65, 42, 130), (300, 64, 257)])
+def test_relu_gradients_on_whole_numbers(m, k, n, dtype):
+    """Whole x and w and a bias of halves: every sum is exact and none is 0, so relu's slope is decided and only the results' own rounding is left."""
+    from scenerf_amd.linear import linear
+    g = gen("relu", m, k, n, dtype)
+    x, w, dy = whole(g, m, k, dtype=dtype), whole(g, n, k, dtype=dtype), whole(g, m, n, dtype=dtype)
+    b = whole(g, n, dtype=dtype) + 0.5
+    x, w, b = (t.requires_grad_(True) for t in (x, w, b))
+    y = linear(x, w, b, activation="relu")
+    grads = torch.autograd.grad(y, (x, w, b), dy)
+    want = linear64(x.detach(), w.detach(), b.detach(), "relu", None, dy)
+    for name, got in zip(("y", "dx", "dw", "db"), (y.detach(),) + grads):
+        value, exact = want[name][0], want[name][0].to(dtype)
+        assert torch.equal(got, exact), (name, float((got.double() - value).abs().max()))
+
+
+def test_gradients_against_differences():
+    """fp32, 64-bit oracle: (L(p + e d) - L(p - e d)) / 2 e of the definition equals <gradient, d> of the kernels."""
+    from scenerf_amd.linear import linear
+    g = gen("diff")
+    for act in ("gelu", "silu"):
+        x, w, b, r = normal(g, 37, 19), normal(g, 23, 19), normal(g, 23), normal(g, 37, 23)
+        c = normal(g, 37, 23)
+        leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+        grads = torch.autograd.grad((linear(x, w, b, activation=act, residual=r) * c).sum(), leaves)
+        for i, name in enumerate("xwbr"):
+            d = normal(g, *leaves[i].shape).double()
+            e = 1e-4
+            ends = []
+            for s in (e, -e):
+                v = [t.detach().double() for t in leaves]
+                v[i] = v[i] + s * d
+                ends.append(float((linear64(v[0], v[1], v[2], act, v[3])["y"][0] * c.double()).sum()))
+            want = (ends[0] - ends[1]) / (2 * e)
+            got = float((grads[i].double() * d).sum())
+            # differences: e^2 / 6 of the third derivative (under 10 per element); the kernels: 2^-20 of the terms' magnitudes
+            room = 2.0 ** -18 * float((grads[i].double() * d).abs().sum()) + 1e-6 * float(c.abs().sum())
+            assert abs(got - want) <= room, (act, name, got, want, room)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_layouts(dtype):
+    """Columns of wider tensors (aligned and not), transposed operands, a residual and a dy that one row stands for, more than two dimensions."""
+    from scenerf_amd.linear import linear
+    g = gen("layout", dtype)
+    for off, wide in ((8, 96), (3, 91), (1, 72)):
+        big, wbig = normal(g, 70, wide, dtype=dtype), normal(g, 40, wide, dtype=dtype)
+        x, w = big[:, off:off + 64], wbig[:, off:off + 64]
+        r = normal(g, 70, 40 + off, dtype=dtype)[:, off:]
+        x.requires_grad_(True)
+        y = linear(x, w, residual=r)
+        hold(y.detach(), linear64(x.detach(), w, None, "none", r)["y"], "sliced")
+        dy = normal(g, 70, 40 + off, dtype=dtype)[:, off:]
+        hold(torch.autograd.grad(y, x, dy)[0], linear64(x.detach(), w, None, "none", r, dy)["dx"], "sliced dx")
+    x, w = normal(g, 64, 70, dtype=dtype).t(), normal(g, 64, 40, dtype=dtype).t()
+    hold(linear(x, w), linear64(x, w)["y"], "transposed")
+    x3, r1 = normal(g, 3, 5, 64, dtype=dtype), normal(g, 40, dtype=dtype).expand(3, 5, 40)
+    hold(linear(x3, w.contiguous(), residual=r1), linear64(x3, w, None, "none", r1)["y"], "three dimensions, one residual row")
+    x3.requires_grad_(True)
+    got = torch.autograd.grad(linear(x3, w.contiguous(), activation="silu").sum(), x3)[0]
+    hold(got, linear64(x3.detach(), w, None, "silu", None, torch.ones(3, 5, 40, dtype=dtype, device=DEV))["dx"], "dy of ones, expanded")
+    v = normal(g, 64, dtype=dtype)
+    hold(linear(v, w.contiguous()), linear64(v, w)["y"], "a single vector")
+    few = normal(g, 1, 64, dtype=dtype).expand(70, 64)
+    hold(linear(few, w.contiguous()), linear64(few, w)["y"], "x of one row, expanded")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_no_rows_and_partial_gradients(dtype):
+    from scenerf_amd.linear import linear
+    g = gen("none", dtype)
+    x, w, b = normal(g, 0, 12, dtype=dtype), normal(g, 9, 12, dtype=dtype), normal(g, 9, dtype=dtype)
+    assert linear(x, w, b, activation="gelu").shape == (0, 9)
+    x, w, b = (t.requires_grad_(True) for t in (x, w, b))
+    dx, dw, db = torch.autograd.grad(linear(x, w, b, activation="gelu").sum(), (x, w, b))
+    assert dx.shape == (0, 12) and not dw.any() and not db.any() and dw.shape == (9, 12) and db.shape == (9,)
+    x, r = normal(g, 50, 12, dtype=dtype), normal(g, 50, 9, dtype=dtype)
+    dy = normal(g, 50, 9, dtype=dtype)
+    want = linear64(x, w.detach(), b.detach(), "gelu", r, dy)
+    for only, names in (((w,), ["dw"]), ((b,), ["db"]), ((w, b), ["dw", "db"])):
+        for t in (w, b):
+            t.requires_grad_(any(t is o for o in only))
+        for name, got in zip(names, torch.autograd.grad(linear(x, w, b, activation="gelu", residual=r), only, dy)):
+            hold(got, want[name], name)
+    w.requires_grad_(False), b.requires_grad_(False)
+    r.requires_grad_(True)
+    hold(torch.autograd.grad(linear(x, w, b, activation="gelu", residual=r), r, dy)[0], want["dr"], "dr alone")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_values_that_are_not_numbers_stay_in_their_rows(dtype):
+    from scenerf_amd.linear import linear
+    g = gen("nan", dtype)
+    x, w = normal(g, 70, 72, dtype=dtype), normal(g, 40, 72, dtype=dtype)
+    x[3, 5], x[66, 0], x[69, 71] = float("nan"), float("inf"), float("-inf")
+    r = normal(g, 70, 40, dtype=dtype)
+    r[10, 7] = float("nan")
+    for act in ACTS:
+        y = linear(x, w, activation=act, residual=r)
+        bad = torch.zeros(70, 40, dtype=torch.bool, device=DEV)
+        bad[3], bad[66], bad[69], bad[10, 7] = True, True, True, True
+        assert bool(torch.isfinite(y[~bad]).all()) and bool(torch.isnan(y[3]).all()) and bool(torch.isnan(y[10, 7]))
+        ok = [i for i in range(70) if i not in (3, 10, 66, 69)]
+        hold(y[ok], linear64(x[ok], w, None, act, r[ok])["y"], act)
+
+
+@pytest.mark.parametrize("out", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_8bit(m, k, n, out):
+    from scenerf_amd.linear import linear_8bit, quantize_rows
+    g = gen("8bit", m, k, n, out)
+    q, s = quantize_rows(normal(g, m, k))
+    wq, ws = quantize_rows(normal(g, n, k, scale=k ** -0.5))
+    b, r = normal(g, n, dtype=out), normal(g, m, n, dtype=out)
+    for act in ACTS:
+        hold(linear_8bit(q, s, wq, ws, b, activation=act, residual=r, out_dtype=out),
+             linear64(q.float(), wq.float(), b, act, r, scales=(s, ws), out_dtype=out)["y"], act)
+    hold(linear_8bit(q, s, wq, ws, out_dtype=out), linear64(q.float(), wq.float(), scales=(s, ws), out_dtype=out)["y"], "bare")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,d", [(1, 1), (3, 7), (5, 512), (17, 515), (9, 2480), (4, 4096), (3, 4100), (2, 9000), (3, 4099)])
+def test_quantize_rows(m, d, dtype):
+    from scenerf_amd.linear import quantize_rows
+    g = gen("q", m, d, dtype)
+    x = normal(g, m, d, dtype=dtype, scale=3.0)
+    x[m - 1] = 0
+    q, s = quantize_rows(x)
+    scale = (x.double().abs().amax(1) / 448).clamp(min=2.0 ** -126)
+    assert bool(((s.double() - scale).abs() <= 2.0 ** -23 * scale).all()) and not q[m - 1].float().any()
+    # half a step of e4m3 is 2^-4 of the value, or half its smallest subnormal 2^-9; the quotient is off by 2^-22
+    v = x.double() / s.double()[:, None]
+    assert bool(((q.double() - v).abs() <= (2.0 ** -4 + 2.0 ** -20) * v.abs() + 2.0 ** -10 * (1 + 2.0 ** -20)).all())
+    assert float(q.float().abs().max()) <= 448
+
+
+def test_quantize_rows_of_values_that_are_not_numbers():
+    from scenerf_amd.linear import quantize_rows
+    x = torch.ones(4, 600, device=DEV)
+    x[1, 599], x[2, 3] = float("nan"), float("-inf")
+    x[3] = 1e-44
+    q, s = quantize_rows(x)
+    assert float(s[0]) == torch.tensor(1.0).div(448).item() and not bool(torch.isfinite(s[1:3]).any())
+    assert bool(torch.isnan(q.float() * s[:, None])[1:3].all()) and float(s[3]) == 2.0 ** -126 and not bool(torch.isnan(q[3].float()).any())
+
+
+def test_another_stream_and_a_replayed_graph():
+    """Captured twice, replayed in turn between eager calls: each replay equals the eager result bit for bit."""
+    from scenerf_amd.linear import linear
+    g = gen("graph")
+    sets, graphs = [], []
+    for m, k, n in ((300, 128, 64), (1, 2480, 1536)):
+        x, w, b = normal(g, m, k, dtype=torch.bfloat16), normal(g, n, k, dtype=torch.bfloat16, scale=k ** -0.5), normal(g, n, dtype=torch.bfloat16)
+        x, w, b = (t.requires_grad_(True) for t in (x, w, b))
+        dy = normal(g, m, n, dtype=torch.bfloat16)
+
+        def step(x=x, w=w, b=b, dy=dy):
+            y = linear(x, w, b, activation="gelu")
+            return (y,) + torch.autograd.grad(y, (x, w, b), dy)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            first = step()
+        torch.cuda.current_stream().wait_stream(side)
+        eager = [t.detach().clone() for t in step()]
+        assert all(torch.equal(a.detach(), e) for a, e in zip(first, eager))
+        del first
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = [t.detach() for t in step()]
+        sets.append((x, step, out))
+        graphs.append(gr)
+    for rep in range(4):
+        for (x, step, out), gr in zip(sets, graphs):
+            with torch.no_grad():
+                x.copy_(normal(g, *x.shape, dtype=x.dtype))
+            gr.replay()
+        for x, step, out in sets:
+            eager = [t.detach() for t in step()]
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, e) for a, e in zip(out, eager)), rep
+
+
+def test_rows_past_32_bit_offsets():
+    """x and y of more than 2^31 elements: the last rows equal the same rows on their own."""
+    from scenerf_amd.linear import linear
+    g = gen("large")
+    m, k, n = 1_100_000, 2048, 16
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    w = normal(g, n, k, dtype=torch.bfloat16, scale=k ** -0.5)
+    y = linear(x, w)
+    hold(y[-300:], linear64(x[-300:], w)["y"], "last rows")
+    del y
+    wt = normal(g, 2048, 16, dtype=torch.bfloat16)
+    y = linear(x[:, :16], wt, activation="relu")
+    hold(y[-300:], linear64(x[-300:, :16], wt, None, "relu")["y"], "last rows of a large result")

@@ -1,0 +1,90 @@
+"""What the row operators refuse, without a GPU: the C entries' own checks and the Python entries' (no kernel runs)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from scenerf_amd import _capi
+from scenerf_amd.linear import linear, linear_8bit, quantize_rows
+from scenerf_amd.norm import rms_norm, rms_norm_8bit
+
+
+def test_there_is_no_cpu_path():
+    x, w = torch.ones(3, 4), torch.ones(5, 4)
+    q, s = x.to(torch.float8_e4m3fn), torch.ones(3)
+    for call in (lambda: linear(x, w), lambda: linear_8bit(q, s, w.to(torch.float8_e4m3fn), torch.ones(5)), lambda: quantize_rows(x),
+                 lambda: rms_norm(x, torch.ones(4)), lambda: rms_norm_8bit(x, torch.ones(4))):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+    with pytest.raises(ValueError, match="activation"):
+        linear(x, w, activation="tanh")
+
+
+def _linear(**kw):
+    p = _capi.Linear(in_type=0, out_type=0, activation=0, n=4, k=8, rows=3)
+    p.x = p.w = p.y = 4096
+    p.ldx = p.ldw = 8
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def _said(rc):
+    assert rc != 0
+    return _capi.load().scenerf_hip_last_error().decode()
+
+
+def test_linear_entry_refuses():
+    lib = _capi.load()
+    assert "NULL argument" in _said(lib.scenerf_hip_linear_forward(None, None))
+    assert "types must be" in _said(lib.scenerf_hip_linear_forward(C.byref(_linear(in_type=7)), None))
+    assert "types must be" in _said(lib.scenerf_hip_linear_forward(C.byref(_linear(out_type=3)), None))
+    assert "differ" in _said(lib.scenerf_hip_linear_forward(C.byref(_linear(in_type=1)), None))
+    assert "activation" in _said(lib.scenerf_hip_linear_forward(C.byref(_linear(activation=4)), None))
+    for bad in (dict(n=0), dict(k=0), dict(n=-1), dict(rows=-1), dict(rows=2 ** 31), dict(ldx=-8)):
+        assert lib.scenerf_hip_linear_forward(C.byref(_linear(**bad)), None) != 0
+        assert lib.scenerf_hip_linear_workspace(C.byref(_linear(**bad)), 0) == -1
+    assert "NULL x" in _said(lib.scenerf_hip_linear_forward(C.byref(_linear(x=None)), None))
+    assert "x_scale" in _said(lib.scenerf_hip_linear_forward(C.byref(_linear(in_type=3)), None))
+    assert "nothing to compute" in _said(lib.scenerf_hip_linear_backward(C.byref(_linear(dy=4096)), None))
+    assert "NULL dy" in _said(lib.scenerf_hip_linear_backward(C.byref(_linear(dx=4096)), None))
+    assert "z is NULL" in _said(lib.scenerf_hip_linear_backward(C.byref(_linear(dx=4096, dy=4096, activation=2)), None))
+    assert "no gradients" in _said(lib.scenerf_hip_linear_backward(C.byref(_linear(in_type=3, dx=4096, dy=4096)), None))
+    p = _linear(dx=4096, db=4096, dy=4096, z=4096, activation=2, ld_dy=4)
+    need = lib.scenerf_hip_linear_workspace(C.byref(p), 1)
+    assert need > 0
+    assert "workspace" in _said(lib.scenerf_hip_linear_backward(C.byref(p), None))
+    p.workspace, p.workspace_bytes = 4096, need - 1
+    assert "workspace" in _said(lib.scenerf_hip_linear_backward(C.byref(p), None))
+    p.workspace, p.workspace_bytes = 4096 + 8, need
+    assert "workspace" in _said(lib.scenerf_hip_linear_backward(C.byref(p), None))
+
+
+def test_linear_entry_with_no_rows_does_nothing():
+    lib = _capi.load()
+    assert lib.scenerf_hip_linear_forward(C.byref(_linear(rows=0, x=None, y=None)), None) == 0
+    assert lib.scenerf_hip_linear_workspace(C.byref(_linear(rows=0)), 0) == 0
+    assert lib.scenerf_hip_linear_workspace(C.byref(_linear(rows=0, dx=4096, dw=4096, db=4096)), 1) >= 0
+
+
+def _rms(**kw):
+    p = _capi.Rms(type=0, width=8, rows=3, eps=1e-6)
+    p.x = p.weight = p.y = 4096
+    p.ldx = 8
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def test_rms_entry_refuses():
+    lib = _capi.load()
+    assert "NULL argument" in _said(lib.scenerf_hip_rms_forward(None, None))
+    for bad in (dict(type=3), dict(width=0), dict(rows=-1), dict(rows=2 ** 31), dict(eps=-1.0), dict(eps=float("nan")), dict(ldx=-1), dict(x=None), dict(y=None),
+                dict(h=4096), dict(q=4096), dict(scale=4096), dict(weight=None, rstd=4096)):
+        assert lib.scenerf_hip_rms_forward(C.byref(_rms(**bad)), None) != 0, bad
+    assert "nothing to compute" in _said(lib.scenerf_hip_rms_backward(C.byref(_rms(dy=4096, rstd=4096)), None))
+    assert "NULL" in _said(lib.scenerf_hip_rms_backward(C.byref(_rms(dx=4096, rstd=4096)), None))
+    p = _rms(dx=4096, dweight=4096, dy=4096, rstd=4096)
+    need = lib.scenerf_hip_rms_workspace(C.byref(p), 1)
+    assert need >= 32 and "workspace" in _said(lib.scenerf_hip_rms_backward(C.byref(p), None))
+    assert lib.scenerf_hip_rms_forward(C.byref(_rms(rows=0, x=None, y=None)), None) == 0
