@@ -16,11 +16,11 @@ CSRC = os.path.join(HERE, "csrc")
 _TAG = os.environ.get("SRF_LIB_TAG", "")
 LIB = os.path.join(CSRC, "libscenerf_hip%s.so" % ("_" + _TAG if _TAG else ""))
 SOURCES = ["runtime.hip", "rays.hip", "gemm.hip", "wgrad.hip", "fused.hip", "wide.hip", "dfeat.hip", "mlp.hip", "loss.hip", "tsdf.hip", "sphere.hip", "optim.hip",
-           "linear.hip", "norm.hip"]
+           "linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip", "linear_e4m3.hip", "norm.hip"]
 # wide.hip owns the whole accumulator file (a[0:255] by name in inline-asm MFMAs): the compiler must not park spilled VGPRs there
 # (a spill then shows up as scratch usage, which tools/asmcheck.sh and the build's resource check refuse)
 EXTRA = {"wide.hip": ["-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"]}
-HEADERS = ["common.h", "gemm.h", "fused.h", "sphere_exact.h", "rowops.h", "linear.h", os.path.join("..", "..", "include", "scenerf_hip.h")]
+HEADERS = ["common.h", "gemm.h", "fused.h", "sphere_exact.h", "rowops.h", "linear.h", "linear_tile.h", os.path.join("..", "..", "include", "scenerf_hip.h")]
 # no packed fp32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this chip now and then, without an error
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics"] + NO_PACKED_F32 + [

@@ -6,6 +6,7 @@ struct LinArgs {
     const void* A; const void* B;        // A(i, k) = A[i * a_i + k * a_k], B(j, k) = B[j * b_j + k * b_k]; one of each pair is 1
     long a_i, a_k, b_j, b_k;
     int M, N, K;
+    int a_ext, b_ext;                    // staged kernel, operand read across: i (j) may be read up to here, a whole number of 16-byte pieces
     // epilogue: v = acc * row_scale[i] * col_scale[j] + bias[j]; z = v; out = act(v) + residual
     const float* row_scale; const float* col_scale;
     const void* bias; const void* residual; long ld_residual;

@@ -46,11 +46,11 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const long i0 = (long)(blockIdx.x / p.tiles_j) * ANY_TILE;
     const int j0 = (blockIdx.x % p.tiles_j) * ANY_TILE;
-    const int kb = blockIdx.y * p.k_split, ke = min(p.K, kb + p.k_split);
+    const long kb = (long)blockIdx.y * p.k_split, ke = min((long)p.K, kb + p.k_split);
     lin_f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-    for (int k0 = kb; k0 < ke; k0 += ANY_K) {
+    for (long k0 = kb; k0 < ke; k0 += ANY_K) {
         __syncthreads();
         // consecutive threads along the operand's unit stride
         for (int t = tid; t < ANY_TILE * ANY_K; t += 256) {
@@ -89,25 +89,108 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
         else epilogue_one<O>(p, i, j, acc[e]);
     }
 }
-// the splits' sums, added in order, then the epilogue
-template <typename O> __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs p, int splits) {
+// the splits' sums, added in order, then the epilogue; W elements a thread
+template <typename O, bool VEC> __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs p) {
+    constexpr int W = VEC ? 16 / (int)sizeof(typename O::raw) : 1;
     const size_t total = (size_t)p.M * p.N;
-    for (size_t t = (size_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (size_t)gridDim.x * 256) {
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += p.part[s * total + t];
-        epilogue_one<O>(p, (long)(t / p.N), (int)(t % p.N), v);
+    for (size_t t = ((size_t)blockIdx.x * 256 + threadIdx.x) * W; t < total; t += (size_t)gridDim.x * 256 * W) {
+        float v[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) {
+            float u[W];
+            load_vec<TypeF32, W>(p.part + s * total + t, u);
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] += u[e];
+        }
+        if constexpr (VEC) epilogue_vec<O, W>(p, (long)(t / p.N), (int)(t % p.N), v);
+        else epilogue_one<O>(p, (long)(t / p.N), (int)(t % p.N), v[0]);
+    }
+}
+
+// ---- a few rows: every weight read once, straight into registers ------------------------------------------------------------------
+// A workgroup owns COLS columns (per wave where KW == 1: its four waves take four groups of them; KW == 4: the four waves split the
+// contraction of one group), a lane every 64th (256th) 16 bytes of their rows of w and of up to MR rows of x; products and sums in fp32 on the vector
+// units, which idle otherwise: the call is bound by the latency of one round of loads and by w's bytes.
+#define FEW_COLS 4
+template <typename T, typename O, int MR, int KW>
+__global__ __launch_bounds__(256) void linear_few_kernel(LinArgs p) {
+    typedef typename T::raw raw;
+    constexpr int W = 16 / (int)sizeof(raw);
+    __shared__ float red[4][FEW_COLS * MR];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int j0 = (KW == 1 ? blockIdx.x * 4 + wv : blockIdx.x) * FEW_COLS;
+    const int pieces = p.K / W;
+    float acc[FEW_COLS][MR];
+#pragma unroll
+    for (int c = 0; c < FEW_COLS; ++c)
+#pragma unroll
+        for (int m = 0; m < MR; ++m) acc[c][m] = 0.f;
+    const raw* wrow[FEW_COLS];
+#pragma unroll
+    for (int c = 0; c < FEW_COLS; ++c) wrow[c] = (const raw*)p.B + (long)min(j0 + c, p.N - 1) * p.b_j;
+    for (int t = KW == 1 ? lane : (int)threadIdx.x; t < pieces; t += 64 * KW) {
+        uint4 w[FEW_COLS], x[MR];
+#pragma unroll
+        for (int c = 0; c < FEW_COLS; ++c) w[c] = *(const uint4*)(wrow[c] + t * W);
+#pragma unroll
+        for (int m = 0; m < MR; ++m) x[m] = *(const uint4*)((const raw*)p.A + (long)min(m, p.M - 1) * p.a_i + t * W);
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            float xv[W];
+            unpack16<T>(x[m], xv);
+#pragma unroll
+            for (int c = 0; c < FEW_COLS; ++c) {
+                float wf[W];
+                unpack16<T>(w[c], wf);
+#pragma unroll
+                for (int e = 0; e < W; ++e) acc[c][m] = fmaf(xv[e], wf[e], acc[c][m]);
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < FEW_COLS; ++c)
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            acc[c][m] = wave_sum(acc[c][m]);
+            if (lane == 0) red[wv][c * MR + m] = acc[c][m];
+        }
+    if constexpr (KW == 4) __syncthreads();
+    else wave_sync();
+    const int o = KW == 4 ? (int)threadIdx.x : lane;
+    if (o < FEW_COLS * MR) {
+        const int m = o % MR, j = j0 + o / MR;
+        float v = red[KW == 4 ? 0 : wv][o];
+        if constexpr (KW == 4) v = (v + red[1][o]) + (red[2][o] + red[3][o]);
+        if (m < p.M && j < p.N) epilogue_one<O>(p, m, j, v);
+    }
+}
+
+// ---- rows laid out anew: pitch a whole number of 16-byte pieces, zeros behind the row's end -----------------------------------------
+template <typename R>
+__global__ __launch_bounds__(256) void linear_pad_kernel(const R* __restrict__ src, long ld, int rows, int cols, R* __restrict__ dst, int pitch) {
+    constexpr int W = 16 / sizeof(R);
+    const long pieces = (long)rows * (pitch / W);
+    for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < pieces; t += (long)gridDim.x * 256) {
+        const long r = t / (pitch / W);
+        const int c = (int)(t - r * (pitch / W)) * W;
+        union { R e[W]; uint4 v; } u;
+#pragma unroll
+        for (int e = 0; e < W; ++e) u.e[e] = c + e < cols ? src[r * ld + c + e] : (R)0;
+        *(uint4*)(dst + r * pitch + c) = u.v;
     }
 }
 
 // ---- dz = dy act'(z), and the column sums of dz by strips of rows ------------------------------------------------------------------
 // thread: 8 neighbouring columns, every 8th row of the strip
 template <typename O, bool VEC>
-__global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld_dy, const void* z_, void* dz_, float* part, int M, int N, int act,
-                                                        int strip) {
+__global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld_dy, const void* z_, void* dz_, int pitch, float* part, int M, int N,
+                                                        int act, int strip) {
     typedef typename O::raw raw;
     __shared__ float red[8][32][9];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int j0 = blockIdx.y * 256 + tx * 8;
+    const int j0 = blockIdx.y * 256 + tx * 8;           // (a pitch above N: zeros in the columns between)
     const long r0 = (long)blockIdx.x * strip, r1 = min((long)M, r0 + strip);
     float sum[8];
 #pragma unroll
@@ -131,18 +214,9 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld
                     for (int e = 0; e < 8; ++e) z[e] = j0 + e < N ? O::to_f32(zp[e]) : 0.f;
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= slope_any(act, z[e]);
-                if (dz_) {
-                    raw* out = (raw*)dz_ + r * N + j0;
-                    if constexpr (VEC) {
-                        store_vec<O, 8>(out, g);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (j0 + e < N) out[e] = O::from_f32(g[e]);
-                    }
-                }
+                for (int e = 0; e < 8; ++e) g[e] = j0 + e < N ? g[e] * slope_any(act, z[e]) : 0.f;
             }
+            if (dz_) store_vec<O, 8>((raw*)dz_ + r * pitch + j0, g);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] += g[e];
         }
@@ -164,48 +238,139 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld
 static int lin_es(int type) { return type == SCENERF_T_F32 ? 4 : type == SCENERF_T_E4M3 ? 1 : 2; }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 static int64_t align256(int64_t v) { return (v + 255) & ~255LL; }
+static int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
-// the contraction is split where the tiles alone leave CUs idle; a split keeps at least 256 elements
-static int lin_splits(long M, int N, long K) {
-    if (M < 1) return 1;
-    const long tiles = ((M + ANY_TILE - 1) / ANY_TILE) * ((N + ANY_TILE - 1) / ANY_TILE);
-    long s = 1024 / tiles;
-    if (s > K / 256) s = K / 256;
-    return s < 1 ? 1 : s > 256 ? 256 : (int)s;
+// How a product runs.  kind 0: element loads (any strides), 1: a few rows, 2: staged tiles
+struct LinPlan {
+    int kind, splits, k_split;
+    LinTile tile;
+};
+// `staged`: both operands are in 16-byte pieces (lin_staged)
+static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, long K) {
+    LinPlan r = {0, 1, 0, LIN_128x128};
+    const int bk = staged ? LIN_CHUNK_BYTES / lin_es(type) : ANY_K;
+    if (staged && !ax && !bx && M <= 8) {
+        r.kind = 1;
+        return r;
+    }
+    long rows = ANY_TILE, cols = ANY_TILE, want = 512;
+    if (staged) {
+        r.kind = 2;
+        auto tiles = [&](LinTile t) { return ((M + kLinTileRows[t] - 1) / kLinTileRows[t]) * ((N + kLinTileCols[t] - 1) / kLinTileCols[t]); };
+        if (N <= 32) r.tile = LIN_128x32;
+        else if (M <= 32) r.tile = LIN_32x128;
+        else if (type != SCENERF_T_F32) {
+            if (tiles(LIN_256x256) >= 256) { r.tile = LIN_256x256; want = 256; }
+            else if (tiles(LIN_256x128) >= 256 || K >= 16384) { r.tile = LIN_256x128; want = 256; }
+        }
+        rows = kLinTileRows[r.tile];
+        cols = kLinTileCols[r.tile];
+    }
+    // the contraction is split where the tiles alone leave CUs idle; a split keeps at least 8 chunks
+    const long n_tiles = ((M + rows - 1) / rows) * ((N + cols - 1) / cols);
+    long s = n_tiles > 0 ? want / n_tiles : 1;
+    if (s > K / (8 * bk)) s = K / (8 * bk);
+    r.splits = s < 1 ? 1 : s > 256 ? 256 : (int)s;
+    r.k_split = (int)(((K + r.splits - 1) / r.splits + bk - 1) / bk * bk);
+    return r;
 }
-static int64_t lin_part_bytes(long M, int N, long K) {
-    const int s = lin_splits(M, N, K);
-    return s > 1 ? align256((int64_t)s * M * N * 4) : 0;
+static int64_t lin_part_bytes(const LinPlan& p, long M, int N) { return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0; }
+
+template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, hipStream_t s) {
+    // K over one wave up to 128 pieces a row, over four beyond: measured at one row of bf16 (see DESIGN.md's table)
+    if (a.K / (16 / (int)sizeof(typename T::raw)) <= 128) linear_few_kernel<T, O, MR, 1><<<cdiv(a.N, 4 * FEW_COLS), 256, 0, s>>>(a);
+    else linear_few_kernel<T, O, MR, 4><<<cdiv(a.N, FEW_COLS), 256, 0, s>>>(a);
 }
-template <typename T, typename O> static int lin_launch(LinArgs a, void* ws, hipStream_t s) {
-    const int splits = lin_splits(a.M, a.N, a.K);
-    a.tiles_j = cdiv(a.N, ANY_TILE);
-    a.part = splits > 1 ? (float*)ws : nullptr;
-    a.k_split = cdiv(cdiv(a.K, splits), ANY_K) * ANY_K;
-    const long blocks = (long)((a.M + ANY_TILE - 1L) / ANY_TILE) * a.tiles_j;
-    SRF_CHECK(blocks <= ROWOPS_GRID_MAX, "linear: %ld tiles are more than one launch holds", blocks);
-    linear_any_kernel<T, O><<<dim3((unsigned)blocks, splits), 256, 0, s>>>(a);
-    SRF_LAUNCH_CHECK("linear_any_kernel");
-    if (splits > 1) {
-        const long total = (long)a.M * a.N;
-        linear_join_kernel<O><<<(unsigned)((total + 255) / 256 < 8192 ? (total + 255) / 256 : 8192), 256, 0, s>>>(a, splits);
+template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& plan, void* ws, hipStream_t s) {
+    a.splits = plan.splits;
+    a.k_split = plan.k_split;
+    a.part = plan.splits > 1 ? (float*)ws : nullptr;
+    constexpr int W = 16 / (int)sizeof(typename O::raw);
+    a.vec = a.N % W == 0 && aligned16(a.out) && (!a.z || aligned16(a.z)) && (!a.bias || aligned16(a.bias)) &&
+            (!a.residual || (aligned16(a.residual) && a.ld_residual % W == 0));
+    if (plan.kind == 1) {
+        if (a.M == 1) lin_few<T, O, 1>(a, s);
+        else if (a.M == 2) lin_few<T, O, 2>(a, s);
+        else if (a.M <= 4) lin_few<T, O, 4>(a, s);
+        else lin_few<T, O, 8>(a, s);
+        SRF_LAUNCH_CHECK("linear_few_kernel");
+        return 0;
+    }
+    if (plan.kind == 2) {
+        a.tiles_i = (int)((a.M + (long)kLinTileRows[plan.tile] - 1) / kLinTileRows[plan.tile]);
+        a.tiles_j = (int)((a.N + (long)kLinTileCols[plan.tile] - 1) / kLinTileCols[plan.tile]);
+        int e;
+        if constexpr (T::code == SCENERF_T_F32) e = linear_tile_f32(a, plan.tile, s);
+        else if constexpr (T::code == SCENERF_T_BF16) e = linear_tile_bf16(a, plan.tile, s);
+        else if constexpr (T::code == SCENERF_T_F16) e = linear_tile_f16(a, plan.tile, s);
+        else e = linear_tile_e4m3(a, plan.tile, O::code, s);
+        if (e) return e;
+    } else {
+        a.tiles_j = cdiv(a.N, ANY_TILE);
+        const long blocks = (long)((a.M + ANY_TILE - 1L) / ANY_TILE) * a.tiles_j;
+        SRF_CHECK(blocks <= ROWOPS_GRID_MAX, "linear: %ld tiles are more than one launch holds", blocks);
+        linear_any_kernel<T, O><<<dim3((unsigned)blocks, plan.splits), 256, 0, s>>>(a);
+        SRF_LAUNCH_CHECK("linear_any_kernel");
+    }
+    if (plan.splits > 1) {
+        const size_t work = ((size_t)a.M * a.N / (a.vec ? W : 1) + 255) / 256;
+        const unsigned blocks = work < 1 ? 1 : work < 8192 ? (unsigned)work : 8192;
+        if (a.vec) linear_join_kernel<O, true><<<blocks, 256, 0, s>>>(a);
+        else linear_join_kernel<O, false><<<blocks, 256, 0, s>>>(a);
         SRF_LAUNCH_CHECK("linear_join_kernel");
     }
     return 0;
 }
-template <typename T> static int lin_launch_out(int out_type, const LinArgs& a, void* ws, hipStream_t s) {
-    if constexpr (T::code != SCENERF_T_E4M3) return lin_launch<T, T>(a, ws, s);
-    else if (out_type == SCENERF_T_F32) return lin_launch<T, TypeF32>(a, ws, s);
-    else if (out_type == SCENERF_T_BF16) return lin_launch<T, TypeBF16>(a, ws, s);
-    else return lin_launch<T, TypeF16>(a, ws, s);
-}
-static int lin_product(int in_type, int out_type, const LinArgs& a, void* ws, hipStream_t s) {
+static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPlan& plan, void* ws, hipStream_t s) {
     switch (in_type) {
-        case SCENERF_T_F32: return lin_launch_out<TypeF32>(out_type, a, ws, s);
-        case SCENERF_T_BF16: return lin_launch_out<TypeBF16>(out_type, a, ws, s);
-        case SCENERF_T_F16: return lin_launch_out<TypeF16>(out_type, a, ws, s);
-        default: return lin_launch_out<TypeE4M3>(out_type, a, ws, s);
+        case SCENERF_T_F32: return lin_run<TypeF32, TypeF32>(a, plan, ws, s);
+        case SCENERF_T_BF16: return lin_run<TypeBF16, TypeBF16>(a, plan, ws, s);
+        case SCENERF_T_F16: return lin_run<TypeF16, TypeF16>(a, plan, ws, s);
+        default:
+            if (out_type == SCENERF_T_F32) return lin_run<TypeE4M3, TypeF32>(a, plan, ws, s);
+            if (out_type == SCENERF_T_BF16) return lin_run<TypeE4M3, TypeBF16>(a, plan, ws, s);
+            return lin_run<TypeE4M3, TypeF16>(a, plan, ws, s);
     }
+}
+
+// A matrix whose rows the staged kernel can read in 16-byte pieces: aligned base, pitch and length, and a pitch whose 256 rows stay
+// inside a 32-bit offset.  What is not gets a copy in the workspace with a padded pitch, zeros behind each row's end.
+#define LIN_MAX_PITCH_BYTES (1 << 22)
+static bool lin_pieces(const void* p, int64_t ld, int cols, int es) {
+    return aligned16(p) && (ld * es) % 16 == 0 && (cols * (int64_t)es) % 16 == 0 && ld * es <= LIN_MAX_PITCH_BYTES;
+}
+static bool lin_can_pad(int cols, int es) { return cols * (int64_t)es <= LIN_MAX_PITCH_BYTES - 16; }
+static int lin_pitch(int cols, int es) { return round_up(cols, 16 / es); }
+static int lin_pad(const void* src, int64_t ld, int64_t rows, int cols, int es, void* dst, hipStream_t s) {
+    const int pitch = lin_pitch(cols, es);
+    const long pieces = (long)rows * (pitch / (16 / es));
+    const unsigned blocks = (unsigned)(pieces < 8192L * 256 ? (pieces + 255) / 256 : 8192);
+    if (es == 4) linear_pad_kernel<uint32_t><<<blocks, 256, 0, s>>>((const uint32_t*)src, ld, (int)rows, cols, (uint32_t*)dst, pitch);
+    else if (es == 2) linear_pad_kernel<uint16_t><<<blocks, 256, 0, s>>>((const uint16_t*)src, ld, (int)rows, cols, (uint16_t*)dst, pitch);
+    else linear_pad_kernel<uint8_t><<<blocks, 256, 0, s>>>((const uint8_t*)src, ld, (int)rows, cols, (uint8_t*)dst, pitch);
+    SRF_LAUNCH_CHECK("linear_pad_kernel");
+    return 0;
+}
+
+struct ForwardPlan {
+    bool pad_x, pad_w;
+    int64_t x, w, sums, bytes;      // offsets in the workspace
+    LinPlan product;
+};
+static ForwardPlan lin_forward_plan(const scenerf_linear* p) {
+    ForwardPlan f = {};
+    const int es = lin_es(p->in_type);
+    const bool can = lin_can_pad(p->k, es) && p->rows > 0;
+    // (a length that is no whole number of pieces needs both padded: the other operand's piece would reach into its next row)
+    f.pad_x = can && !lin_pieces(p->x, p->ldx, p->k, es);
+    f.pad_w = can && !lin_pieces(p->w, p->ldw, p->k, es);
+    f.product = lin_plan(p->in_type, false, false, can, p->rows, p->n, p->k);
+    int64_t at = 0;
+    if (f.pad_x) { f.x = at; at += align256(p->rows * lin_pitch(p->k, es) * es); }
+    if (f.pad_w) { f.w = at; at += align256((int64_t)p->n * lin_pitch(p->k, es) * es); }
+    f.sums = at;
+    f.bytes = at + lin_part_bytes(f.product, p->rows, p->n);
+    return f;
 }
 
 #define DZ_STRIPS 512
@@ -214,21 +379,32 @@ static int dz_strip(int64_t rows) {
     return per < 8 ? 8 : (int)((per + 7) / 8 * 8);
 }
 struct BackwardPlan {
-    bool need_dz;                   // dz is not dy itself
-    int strip, strips;
-    int64_t part, dz, sums;         // offsets of the column sums' parts, of dz and of the split sums
+    bool make_dz, pad_x, pad_w;     // dz is not dy itself; operands to lay out anew
+    int strip, strips, dz_pitch;
+    int64_t part, dz, x, w, sums;   // offsets of the column sums' parts, of dz, x, w and of the split sums
     int64_t bytes;
+    LinPlan dx, dw;
 };
 static BackwardPlan lin_backward_plan(const scenerf_linear* p) {
     BackwardPlan b = {};
-    b.need_dz = p->activation != SCENERF_ACT_NONE;
+    const int es = lin_es(p->in_type);
+    const bool products = (p->dx || p->dw) && p->rows > 0;
+    const bool can = lin_can_pad(p->n, es) && lin_can_pad(p->k, es);
+    b.make_dz = products && (p->activation != SCENERF_ACT_NONE || (can && !lin_pieces(p->dy, p->ld_dy, p->n, es)));
+    b.pad_x = can && products && p->dw && !lin_pieces(p->x, p->ldx, p->k, es);
+    b.pad_w = can && products && p->dx && !lin_pieces(p->w, p->ldw, p->k, es);
+    b.dz_pitch = round_up(p->n, 8);
     b.strip = dz_strip(p->rows);
     b.strips = (int)((p->rows + b.strip - 1) / b.strip);
+    b.dx = lin_plan(p->in_type, false, true, can, p->rows, p->k, p->n);
+    b.dw = lin_plan(p->in_type, true, true, can, p->n, p->k, p->rows);
     int64_t at = 0;
     if (p->db) { b.part = at; at += align256((int64_t)b.strips * p->n * 4); }
-    if (b.need_dz && (p->dx || p->dw)) { b.dz = at; at += align256(p->rows * p->n * lin_es(p->out_type)); }
+    if (b.make_dz) { b.dz = at; at += align256(p->rows * b.dz_pitch * es); }
+    if (b.pad_x) { b.x = at; at += align256(p->rows * lin_pitch(p->k, es) * es); }
+    if (b.pad_w) { b.w = at; at += align256((int64_t)p->n * lin_pitch(p->k, es) * es); }
     b.sums = at;
-    const int64_t sx = p->dx ? lin_part_bytes(p->rows, p->k, p->n) : 0, sw = p->dw ? lin_part_bytes(p->n, p->k, p->rows) : 0;
+    const int64_t sx = p->dx ? lin_part_bytes(b.dx, p->rows, p->k) : 0, sw = p->dw ? lin_part_bytes(b.dw, p->n, p->k) : 0;
     b.bytes = at + (sx > sw ? sx : sw);
     return b;
 }
@@ -254,11 +430,11 @@ static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
     return 0;
 }
 template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardPlan& b, void* dz, float* part, hipStream_t s) {
-    const bool vec = p->n % 8 == 0 && p->ld_dy % 8 == 0 && aligned16(p->dy) && (!b.need_dz || aligned16(p->z));
+    const bool vec = p->n % 8 == 0 && p->ld_dy % 8 == 0 && aligned16(p->dy) && (p->activation == SCENERF_ACT_NONE || aligned16(p->z));
     const dim3 grid(b.strips, cdiv(p->n, 256));
     SRF_CHECK(grid.y <= 65535, "linear_backward: n is too large");
-    if (vec) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, part, (int)p->rows, p->n, p->activation, b.strip);
-    else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, part, (int)p->rows, p->n, p->activation, b.strip);
+    if (vec) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip);
+    else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip);
     SRF_LAUNCH_CHECK("linear_dz_kernel");
     return 0;
 }
@@ -267,25 +443,37 @@ extern "C" {
 
 int64_t scenerf_hip_linear_workspace(const scenerf_linear* p, int backward) {
     if (lin_check(p, "linear_workspace", backward != 0)) return -1;
-    return backward ? lin_backward_plan(p).bytes : lin_part_bytes(p->rows, p->n, p->k);
+    return backward ? lin_backward_plan(p).bytes : lin_forward_plan(p).bytes;
 }
 
 int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream) {
     if (int e = lin_check(p, "linear_forward", false)) return e;
     if (p->rows == 0) return 0;
-    const int64_t need = lin_part_bytes(p->rows, p->n, p->k);
-    SRF_CHECK(need == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= need), "linear_forward: workspace of %lld bytes needed",
-              (long long)need);
+    const ForwardPlan f = lin_forward_plan(p);
+    SRF_CHECK(f.bytes == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= f.bytes), "linear_forward: workspace of %lld bytes needed",
+              (long long)f.bytes);
     const double m = (double)p->rows, es = lin_es(p->in_type), eo = lin_es(p->out_type);
-    SrfLaunchScope ps(as_stream(stream), "linear_forward", 2 * m * p->n * p->k, es * (m * p->k + (double)p->n * p->k) + eo * m * p->n);
+    hipStream_t s = as_stream(stream);
+    SrfLaunchScope ps(s, "linear_forward", 2 * m * p->n * p->k, es * (m * p->k + (double)p->n * p->k) + eo * m * p->n);
+    char* ws = (char*)p->workspace;
     LinArgs a = {};
     a.A = p->x; a.a_i = p->ldx; a.a_k = 1;
     a.B = p->w; a.b_j = p->ldw; a.b_k = 1;
     a.M = (int)p->rows; a.N = p->n; a.K = p->k;
+    const int pitch = lin_pitch(p->k, (int)es);
+    if (f.pad_x) {
+        if (int e = lin_pad(p->x, p->ldx, p->rows, p->k, (int)es, ws + f.x, s)) return e;
+        a.A = ws + f.x; a.a_i = pitch;
+    }
+    if (f.pad_w) {
+        if (int e = lin_pad(p->w, p->ldw, p->n, p->k, (int)es, ws + f.w, s)) return e;
+        a.B = ws + f.w; a.b_j = pitch;
+    }
+    if (f.pad_x && f.pad_w) a.K = pitch;
     if (p->in_type == SCENERF_T_E4M3) { a.row_scale = p->x_scale; a.col_scale = p->w_scale; }
     a.bias = p->bias; a.residual = p->residual; a.ld_residual = p->ld_residual;
     a.out = p->y; a.z = p->z; a.act = p->activation;
-    return lin_product(p->in_type, p->out_type, a, p->workspace, as_stream(stream));
+    return lin_product(p->in_type, p->out_type, a, f.product, ws + f.sums, s);
 }
 
 int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream) {
@@ -298,11 +486,11 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
     SrfLaunchScope ps(s, "linear_backward", 2 * m * p->n * p->k * (!!p->dx + !!p->dw), es * m * (p->n + 2. * p->k));
     char* ws = (char*)p->workspace;
     float* part = (float*)(ws + b.part);
-    const void* dz = b.need_dz ? ws + b.dz : p->dy;
-    const long ld_dz = b.need_dz ? p->n : p->ld_dy;
-    if (p->rows > 0 && (b.need_dz || p->db)) {
+    const void* dz = b.make_dz ? ws + b.dz : p->dy;
+    const long ld_dz = b.make_dz ? b.dz_pitch : p->ld_dy;
+    if (p->rows > 0 && (b.make_dz || p->db)) {
         float* sums = p->db ? part : nullptr;
-        void* to = b.need_dz && (p->dx || p->dw) ? (void*)dz : nullptr;
+        void* to = b.make_dz ? (void*)dz : nullptr;
         int e = p->out_type == SCENERF_T_F32 ? lin_dz<TypeF32>(p, b, to, sums, s)
                 : p->out_type == SCENERF_T_BF16 ? lin_dz<TypeBF16>(p, b, to, sums, s) : lin_dz<TypeF16>(p, b, to, sums, s);
         if (e) return e;
@@ -310,21 +498,35 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
     if (p->db) {
         if (int e = launch_sum_parts(p->out_type, part, b.strips, p->n, p->db, s)) return e;
     }
+    const int pitch = lin_pitch(p->k, (int)es);
+    const void* x = p->x;
+    const void* w = p->w;
+    long ldx = p->ldx, ldw = p->ldw;
+    if (b.pad_w) {
+        if (int e = lin_pad(p->w, p->ldw, p->n, p->k, (int)es, ws + b.w, s)) return e;
+        w = ws + b.w; ldw = pitch;
+    }
+    if (b.pad_x) {
+        if (int e = lin_pad(p->x, p->ldx, p->rows, p->k, (int)es, ws + b.x, s)) return e;
+        x = ws + b.x; ldx = pitch;
+    }
     if (p->dx && p->rows > 0) {
         LinArgs a = {};
         a.A = dz; a.a_i = ld_dz; a.a_k = 1;
-        a.B = p->w; a.b_j = 1; a.b_k = p->ldw;
+        a.B = w; a.b_j = 1; a.b_k = ldw;
         a.M = (int)p->rows; a.N = p->k; a.K = p->n;
+        a.b_ext = pitch;
         a.out = p->dx;
-        if (int e = lin_product(p->in_type, p->out_type, a, ws + b.sums, s)) return e;
+        if (int e = lin_product(p->in_type, p->out_type, a, b.dx, ws + b.sums, s)) return e;
     }
     if (p->dw) {     // rows == 0: an empty sum, zeros
         LinArgs a = {};
         a.A = dz; a.a_i = 1; a.a_k = ld_dz;
-        a.B = p->x; a.b_j = 1; a.b_k = p->ldx;
+        a.B = x; a.b_j = 1; a.b_k = ldx;
         a.M = p->n; a.N = p->k; a.K = (int)p->rows;
+        a.a_ext = b.make_dz ? b.dz_pitch : p->n; a.b_ext = pitch;
         a.out = p->dw;
-        if (int e = lin_product(p->in_type, p->out_type, a, ws + b.sums, s)) return e;
+        if (int e = lin_product(p->in_type, p->out_type, a, b.dw, ws + b.sums, s)) return e;
     }
     return 0;
 }

@@ -1,0 +1,4 @@
+// The staged product (linear_tile.h) of f16 operands.
+#include "linear_tile.h"
+
+int linear_tile_f16(const LinArgs& a, LinTile tile, hipStream_t s) { return lin_tile_layout<TypeF16>(a, tile, s); }

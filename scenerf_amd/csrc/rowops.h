@@ -4,6 +4,13 @@
 
 #define ROWOPS_GRID_MAX 0x7fffffffLL
 
+// what one lane of a wave wrote to LDS, another may read behind this (LDS executes a wave's accesses in order: nothing is waited for)
+__device__ static inline void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 typedef __attribute__((ext_vector_type(2))) _Float16 srf_f16x2;
 
 // Storage of one element and its conversions.  Every store to 16 bits rounds to nearest even ONCE, from a 32-bit value.
@@ -32,6 +39,24 @@ struct TypeE4M3 {
     __device__ static inline raw from_f32(float v) { return (raw)__builtin_amdgcn_cvt_pk_fp8_f32(v, 0.f, 0, false); }
 };
 
+// 16 bytes in hand as floats
+template <typename E> __device__ static inline void unpack16(uint4 t, float (&v)[16 / sizeof(typename E::raw)]) {
+    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(typename E::raw) == 4) {
+            v[i] = __uint_as_float(w[i]);
+        } else if constexpr (sizeof(typename E::raw) == 2) {
+            v[2 * i] = E::to_f32((uint16_t)(w[i] & 0xffffu));
+            v[2 * i + 1] = E::to_f32((uint16_t)(w[i] >> 16));
+        } else {
+            v[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 0);
+            v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 1);
+            v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 2);
+            v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 3);
+        }
+    }
+}
 // W consecutive elements as floats.  W * sizeof(raw) is 4, 8 or 16 bytes (or 32: two loads) and the address is aligned to that, up to 16.
 template <typename E, int W> __device__ static inline void load_vec(const typename E::raw* p, float (&v)[W]) {
     if constexpr (W == 1) {
@@ -44,13 +69,7 @@ template <typename E, int W> __device__ static inline void load_vec(const typena
         }
     } else {
         static_assert(sizeof(typename E::raw) == 2 && W == 8, "16-bit types move 8 elements");
-        const uint4 t = *(const uint4*)p;
-        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = E::to_f32((uint16_t)(w[i] & 0xffffu));
-            v[2 * i + 1] = E::to_f32((uint16_t)(w[i] >> 16));
-        }
+        unpack16<E>(*(const uint4*)p, v);
     }
 }
 template <typename E> __device__ static inline uint32_t pack2(float a, float b) {
