@@ -327,28 +327,29 @@ __global__ __launch_bounds__(256) void rms_dweight_cols_kernel(RmsArgs p, int st
         p.partial[(size_t)blockIdx.y * p.width + col] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
 }
 
-// out[col] = the sum of part[0..count)[col], in a fixed order: 8 interleaved chains, then their sum
+// out[col] = the sum of part[0..count)[col], in a fixed order: 32 interleaved chains per column, then their sum.  A workgroup owns 32 columns,
+// so that each of its loads is a line; bound by the latency of count / 32 loads in a row, which the unrolling overlaps
 template <typename E>
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ part, int count, int width, typename E::raw* __restrict__ out) {
-    __shared__ float red[8][32];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), ty = threadIdx.x >> 5;
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict__ part, int count, int width, typename E::raw* __restrict__ out) {
+    __shared__ float red[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.x * 32 + tx;
     float s = 0.f;
-    if (col < width)
-        for (int i = ty; i < count; i += 8) s += part[(size_t)i * width + col];
-    red[ty][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (ty == 0 && col < width) {
-        s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
-        out[col] = E::from_f32(s);
+    if (col < width) {
+#pragma unroll 8
+        for (int i = ty; i < count; i += 32) s += part[(size_t)i * width + col];
     }
+    red[ty][tx] = s;
+    __syncthreads();
+    s = red[tx][ty];              // column ty of the 32, chain tx: the halves of a wave add one column each
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor(s, o, WAVE);
+    if (tx == 0 && blockIdx.x * 32 + ty < width) out[blockIdx.x * 32 + ty] = E::from_f32(s);
 }
 int launch_sum_parts(int type, const float* part, int count, int width, void* out, hipStream_t s) {
     const int blocks = cdiv(width, 32);
-    if (type == SCENERF_T_F32) sum_parts_kernel<TypeF32><<<blocks, 256, 0, s>>>(part, count, width, (float*)out);
-    else if (type == SCENERF_T_BF16) sum_parts_kernel<TypeBF16><<<blocks, 256, 0, s>>>(part, count, width, (uint16_t*)out);
-    else sum_parts_kernel<TypeF16><<<blocks, 256, 0, s>>>(part, count, width, (uint16_t*)out);
+    if (type == SCENERF_T_F32) sum_parts_kernel<TypeF32><<<blocks, 1024, 0, s>>>(part, count, width, (float*)out);
+    else if (type == SCENERF_T_BF16) sum_parts_kernel<TypeBF16><<<blocks, 1024, 0, s>>>(part, count, width, (uint16_t*)out);
+    else sum_parts_kernel<TypeF16><<<blocks, 1024, 0, s>>>(part, count, width, (uint16_t*)out);
     SRF_LAUNCH_CHECK("sum_parts_kernel");
     return 0;
 }
