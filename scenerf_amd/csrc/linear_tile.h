@@ -5,7 +5,7 @@
 // by asynchronous global -> LDS loads (16 bytes a lane, 1 KiB a wave and instruction) that run NST - 1 chunks ahead: one barrier a chunk,
 // in front of which each wave waits for its own loads of that chunk by count.
 //
-// LDS image of an operand read ALONG the contraction: row r is 64 bytes, its 16-byte slots XORed with (r >> 1) & 3, so that the 8 lanes
+// LDS image of an operand read ALONG the contraction: row r is 64 bytes, its 16-byte slots XORed with (r >> 2) & 3, so that the 8 lanes
 // of a ds_read_b128 phase cover all banks.  The swizzle is applied on the source side of the load (LDS-bound loads place lanes in
 // sequence).  An operand read ACROSS (contraction along the rows in memory) keeps its rows: [k][tile columns]; 16-bit fragments come
 // out of it by the transposing read ds_read_b64_tr_b16 (within 16 lanes, lane 4r + c gives the address of 4 columns of row r, lane i
@@ -24,6 +24,8 @@ typedef __attribute__((ext_vector_type(8))) int lin_i32x8;
 typedef __attribute__((ext_vector_type(4))) short lin_s16x4;
 
 __device__ __attribute__((aligned(16))) const unsigned lin_zeros[4] = {0, 0, 0, 0};
+
+template <bool V> struct Bool { static constexpr bool value = V; };
 
 // 64 lanes x 16 bytes, global -> LDS at lds_base + lane * 16 (m0 is the base; saved around, the compiler owns it)
 __device__ static inline void lin_copy(const void* sbase, unsigned voff, unsigned lds_base) {
@@ -61,21 +63,21 @@ template <typename T, bool ACROSS, int TILE> struct LinSide {
             if constexpr (ES == 2) col = (((col >> 6) ^ (k & SWZ)) << 6) | (col & 63);
             across_idx = col / ES;
         } else {
-            const int r = q * 16 + (lane >> 2);
+            const int r = q * 8 + (lane >> 3);
             across_idx = r;
-            k = ((lane & 3) ^ ((r >> 1) & 3)) * (16 / ES);
+            k = ((lane & 7) ^ ((r >> 1) & 7)) * (16 / ES);
         }
     }
 };
 
-template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NST>
+template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     typedef typename T::raw raw;
     typedef LinSide<T, AX, BM> SA;
     typedef LinSide<T, BX, BN> SB;
     constexpr int ES = SA::ES, BK = SA::BK, WAVES = WM * WN;
-    constexpr int STAGE = SA::BYTES + SB::BYTES;
-    constexpr int PIECES = SA::PIECES + SB::PIECES, LOADS = (PIECES + WAVES - 1) / WAVES;
+    constexpr int LA = (SA::PIECES + WAVES - 1) / WAVES, LB = (SB::PIECES + WAVES - 1) / WAVES;     // loads per wave and chunk
+    static_assert(NSA >= 2 && (NSB == NSA || NSB == NSA - 1) && NSB >= 2, "the order of the loads and their counts");
     constexpr int I = BM / WM / 32, J = BN / WN / 32;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -90,45 +92,49 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     const int kb = (int)min((long)p.K, (long)split * p.k_split), ke = (int)min((long)p.K, (long)kb + p.k_split);
     const int chunks = ke > kb ? (ke - kb + BK - 1) / BK : 0;
 
-    // ---- loads: wave w moves pieces w, w + WAVES, ... (past the last one: the last one again, the same bytes to the same place)
+    // ---- loads: of each side wave w moves pieces w, w + WAVES, ... (past the last one: the last one again, the same bytes to the same
+    // place).  A's ring has NSA stages, B's behind it NSB.
     const char* baseA = (const char*)p.A + i0 * p.a_i * ES;
     const char* baseB = (const char*)p.B + (long)j0 * p.b_j * ES;
-    unsigned off[LOADS];
-    int kin[LOADS];
+    const unsigned ringB = lds0 + NSA * SA::BYTES;
+    unsigned offA[LA], offB[LB];
+    int kinA[LA], kinB[LB];
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
-        const int q = min(wv + u * WAVES, PIECES - 1);
-        int r, k;
-        if (q < SA::PIECES) {
-            SA::place(q, lane, r, k);
-            // rows past the last: the last again (their results are dropped); ACROSS: the last whole 16 bytes
-            r = (int)min((long)r, (AX ? (long)p.a_ext - 16 / ES : (long)p.M - 1) - i0);
-            off[u] = (unsigned)((long)r * p.a_i + (long)k * p.a_k) * ES;
-        } else {
-            SB::place(q - SA::PIECES, lane, r, k);
-            r = min(r, (BX ? p.b_ext - 16 / ES : p.N - 1) - j0);
-            off[u] = (unsigned)((long)r * p.b_j + (long)k * p.b_k) * ES;
-        }
-        kin[u] = k;
+    for (int u = 0; u < LA; ++u) {
+        int r;
+        SA::place(min(wv + u * WAVES, SA::PIECES - 1), lane, r, kinA[u]);
+        // rows past the last: the last again (their results are dropped); ACROSS: the last whole 16 bytes
+        r = (int)min((long)r, (AX ? (long)p.a_ext - 16 / ES : (long)p.M - 1) - i0);
+        offA[u] = (unsigned)((long)r * p.a_i + (long)kinA[u] * p.a_k) * ES;
     }
-    auto issue = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < LB; ++u) {
+        int r;
+        SB::place(min(wv + u * WAVES, SB::PIECES - 1), lane, r, kinB[u]);
+        r = min(r, (BX ? p.b_ext - 16 / ES : p.N - 1) - j0);
+        offB[u] = (unsigned)((long)r * p.b_j + (long)kinB[u] * p.b_k) * ES;
+    }
+    // what lies past the contraction's end, in the last chunk, comes from a zero
+    auto issueA = [&](int c) {
         const long k0 = kb + (long)c * BK;
         const char* a = baseA + k0 * p.a_k * ES;
+        const unsigned stage = lds0 + (c % NSA) * SA::BYTES;
+#pragma unroll
+        for (int u = 0; u < LA; ++u) {
+            const int q = min(wv + u * WAVES, SA::PIECES - 1);
+            if (k0 + BK <= p.K) lin_copy(a, offA[u], stage + q * 1024);
+            else lin_copy_v(k0 + kinA[u] < p.K ? a + offA[u] : (const char*)lin_zeros, stage + q * 1024);
+        }
+    };
+    auto issueB = [&](int c) {
+        const long k0 = kb + (long)c * BK;
         const char* b = baseB + k0 * p.b_k * ES;
-        const unsigned stage = lds0 + (c % NST) * STAGE;
-        if (k0 + BK <= p.K) {
+        const unsigned stage = ringB + (c % NSB) * SB::BYTES;
 #pragma unroll
-            for (int u = 0; u < LOADS; ++u) {
-                const int q = min(wv + u * WAVES, PIECES - 1);
-                lin_copy(q < SA::PIECES ? a : b, off[u], stage + q * 1024);
-            }
-        } else {      // the last chunk: what lies past the contraction's end comes from a zero
-#pragma unroll
-            for (int u = 0; u < LOADS; ++u) {
-                const int q = min(wv + u * WAVES, PIECES - 1);
-                const char* src = (q < SA::PIECES ? a : b) + off[u];
-                lin_copy_v(k0 + kin[u] < p.K ? src : (const char*)lin_zeros, stage + q * 1024);
-            }
+        for (int u = 0; u < LB; ++u) {
+            const int q = min(wv + u * WAVES, SB::PIECES - 1);
+            if (k0 + BK <= p.K) lin_copy(b, offB[u], stage + q * 1024);
+            else lin_copy_v(k0 + kinB[u] < p.K ? b + offB[u] : (const char*)lin_zeros, stage + q * 1024);
         }
     };
 
@@ -145,10 +151,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
 
     // 16 bytes of the lane's row for slot `slot` of a side read along k
     auto along = [&](const char* side, int row, int slot) -> uint4 {
-        return *(const uint4*)(side + row * LIN_CHUNK_BYTES + ((slot ^ ((row >> 1) & 3)) << 4));
+        return *(const uint4*)(side + row * LIN_CHUNK_BYTES + ((slot ^ ((row >> 1) & 7)) << 4));
     };
     const int tg = lane >> 4, tr = (lane >> 2) & 3, tc = lane & 3;
-    // 8 consecutive k of column `first + lane % 32` (16-bit, a side read across), k-step s
+    // 8 consecutive k of column `first + lane % 32` (16-bit, a side read across), from 16 s on
     auto across16 = [&](const char* side, int line, int swz, int first, int s) -> uint4 {
         const int k = 16 * s + 8 * (tg >> 1) + tr;
         const char* at = side + k * line + ((((first >> 5) ^ (k & swz)) << 6)) + (16 * (tg & 1) + 4 * tc) * 2;
@@ -162,122 +168,121 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
         return __builtin_bit_cast(unsigned, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true)
                                                  : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
     };
-    auto multiply = [&](int c) {
-        const char* sa = lds + (c % NST) * STAGE;
-        const char* sb = sa + SA::BYTES;
+    // the fragments of half a chunk: 8 registers a lane per 32 rows
+    constexpr bool WIDEN = ES == 1 && O::code == SCENERF_T_F32;
+    constexpr int FR = 8;
+    struct Frag { unsigned a[I][FR], b[J][FR]; };
+    auto fetch = [&](int c, int half, Frag& f) {
+        const char* sa = lds + (c % NSA) * SA::BYTES;
+        const char* sb = lds + NSA * SA::BYTES + (c % NSB) * SB::BYTES;
+        auto side = [&](auto across, const char* base, int first, int line, int swz, unsigned (&o)[FR]) {
+            if constexpr (decltype(across)::value && ES == 4) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[4 * s + e] = *(const unsigned*)(base + (16 * half + 8 * s + 4 * h + e) * line + (first + l31) * 4);
+            } else {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    uint4 v;
+                    if constexpr (decltype(across)::value) v = across16(base, line, swz, first, 2 * half + s);
+                    else v = along(base, first + l31, 4 * half + 2 * s + h);       // 8-bit: the lane's half takes 16-byte slots h and h + 2
+                    o[4 * s] = v.x; o[4 * s + 1] = v.y; o[4 * s + 2] = v.z; o[4 * s + 3] = v.w;
+                }
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < I; ++i) side(Bool<AX>(), sa, wi + i * 32, SA::LINE, SA::SWZ, f.a[i]);
+#pragma unroll
+        for (int j = 0; j < J; ++j) side(Bool<BX>(), sb, wj + j * 32, SB::LINE, SB::SWZ, f.b[j]);
+    };
+    auto four = [](const unsigned (&r)[FR], int s) { return make_uint4(r[4 * s], r[4 * s + 1], r[4 * s + 2], r[4 * s + 3]); };
+    auto multiply = [&](const Frag& f) {
         if constexpr (ES == 2) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                uint4 a[I], b[J];
-#pragma unroll
-                for (int i = 0; i < I; ++i) {
-                    if constexpr (AX) a[i] = across16(sa, SA::LINE, SA::SWZ, wi + i * 32, s);
-                    else a[i] = along(sa, wi + i * 32 + l31, 2 * s + h);
-                }
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    if constexpr (BX) b[j] = across16(sb, SB::LINE, SB::SWZ, wj + j * 32, s);
-                    else b[j] = along(sb, wj + j * 32 + l31, 2 * s + h);
-                }
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < I; ++i)
 #pragma unroll
                     for (int j = 0; j < J; ++j) {
                         if constexpr (T::code == SCENERF_T_BF16)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lin_bf16x8, b[j]), __builtin_bit_cast(lin_bf16x8, a[i]),
-                                                                                acc[i][j], 0, 0, 0);
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lin_bf16x8, four(f.b[j], s)),
+                                                                                __builtin_bit_cast(lin_bf16x8, four(f.a[i], s)), acc[i][j], 0, 0, 0);
                         else
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lin_f16x8, b[j]), __builtin_bit_cast(lin_f16x8, a[i]),
-                                                                               acc[i][j], 0, 0, 0);
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lin_f16x8, four(f.b[j], s)),
+                                                                               __builtin_bit_cast(lin_f16x8, four(f.a[i], s)), acc[i][j], 0, 0, 0);
                     }
-            }
-        } else if constexpr (ES == 1 && O::code == SCENERF_T_F32) {
+        } else if constexpr (WIDEN) {
             // the 8-bit matrix instruction adds 8 neighbouring products to 2^-13 of the largest of them (measured: linear.hip): not enough
             // for a result in 32 bits.  e4m3 is exact in bf16: widened here, at half the rate
-            uint4 a[I][4], b[J][4];
-            auto widen = [&](const char* side, int row, uint4 (&f)[4]) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const uint4 v = along(side, row, h + 2 * t);
-                    f[2 * t] = make_uint4(widen2(v.x, false), widen2(v.x, true), widen2(v.y, false), widen2(v.y, true));
-                    f[2 * t + 1] = make_uint4(widen2(v.z, false), widen2(v.z, true), widen2(v.w, false), widen2(v.w, true));
-                }
+            auto wide = [&](const unsigned (&r)[FR], int s) {
+                return __builtin_bit_cast(lin_bf16x8, make_uint4(widen2(r[2 * s], false), widen2(r[2 * s], true), widen2(r[2 * s + 1], false),
+                                                                 widen2(r[2 * s + 1], true)));
             };
-#pragma unroll
-            for (int i = 0; i < I; ++i) widen(sa, wi + i * 32 + l31, a[i]);
-#pragma unroll
-            for (int j = 0; j < J; ++j) widen(sb, wj + j * 32 + l31, b[j]);
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int i = 0; i < I; ++i)
 #pragma unroll
-                    for (int j = 0; j < J; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lin_bf16x8, b[j][s]), __builtin_bit_cast(lin_bf16x8, a[i][s]),
-                                                                            acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wide(f.b[j], s), wide(f.a[i], s), acc[i][j], 0, 0, 0);
         } else if constexpr (ES == 1) {
-            // 64 k in one instruction: the lane's half takes slots h and h + 2; every scale is 1 (127 as an exponent)
-            lin_i32x8 a[I], b[J];
-            auto two = [&](const char* side, int row) -> lin_i32x8 {
-                const uint4 x = along(side, row, h), y = along(side, row, h + 2);
-                return lin_i32x8{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+            // 64 k in one instruction; every scale is 1 (127 as an exponent)
+            auto eight = [](const unsigned (&r)[FR]) {
+                return lin_i32x8{(int)r[0], (int)r[1], (int)r[2], (int)r[3], (int)r[4], (int)r[5], (int)r[6], (int)r[7]};
             };
-#pragma unroll
-            for (int i = 0; i < I; ++i) a[i] = two(sa, wi + i * 32 + l31);
-#pragma unroll
-            for (int j = 0; j < J; ++j) b[j] = two(sb, wj + j * 32 + l31);
 #pragma unroll
             for (int i = 0; i < I; ++i)
 #pragma unroll
                 for (int j = 0; j < J; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(eight(f.b[j]), eight(f.a[i]), acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
         } else {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {           // the lane's half holds k = 8 s + 4 h + e
-                float a[I][4], b[J][4];
+            for (int e = 0; e < 8; ++e)             // the lane's half holds k = 8 (e / 4) + 4 h + e % 4
 #pragma unroll
-                for (int i = 0; i < I; ++i) {
-                    if constexpr (AX) {
+                for (int i = 0; i < I; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) a[i][e] = *(const float*)(sa + (8 * s + 4 * h + e) * SA::LINE + (wi + i * 32 + l31) * 4);
-                    } else {
-                        const uint4 v = along(sa, wi + i * 32 + l31, 2 * s + h);
-                        a[i][0] = __uint_as_float(v.x); a[i][1] = __uint_as_float(v.y); a[i][2] = __uint_as_float(v.z); a[i][3] = __uint_as_float(v.w);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    if constexpr (BX) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) b[j][e] = *(const float*)(sb + (8 * s + 4 * h + e) * SB::LINE + (wj + j * 32 + l31) * 4);
-                    } else {
-                        const uint4 v = along(sb, wj + j * 32 + l31, 2 * s + h);
-                        b[j][0] = __uint_as_float(v.x); b[j][1] = __uint_as_float(v.y); b[j][2] = __uint_as_float(v.z); b[j][3] = __uint_as_float(v.w);
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int i = 0; i < I; ++i)
-#pragma unroll
-                        for (int j = 0; j < J; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[j][e], a[i][e], acc[i][j], 0, 0, 0);
-            }
+                    for (int j = 0; j < J; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f.b[j][e]), __uint_as_float(f.a[i][e]), acc[i][j], 0, 0, 0);
         }
     };
 
-#pragma unroll 1
-    for (int c = 0; c < NST - 1 && c < chunks; ++c) issue(c);
-#pragma unroll 1
-    for (int c = 0; c < chunks; ++c) {
-        // this wave's loads of chunk c have landed (at most those of the NST - 2 chunks behind it are outstanding), its reads of
-        // chunk c - 1 are done: behind the barrier that holds for every wave, and the stage of chunk c - 1 may be overwritten
-        if (c + NST - 2 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * LOADS) : "memory");
+    // ---- the loop: while one half of a chunk is multiplied from registers, the next half is read from LDS, and further chunks are under
+    // way, in the order A(0) B(0) A(1) B(1) ..: up to A(c + NSA - 1) and B(c + NSB - 1).  Between the halves: this wave's loads of chunk
+    // c + 1 have landed (what was issued behind them may be outstanding) and its reads of chunk c are done; behind the barrier that holds
+    // for every wave, and the stages of chunk c are free.
+    // (No branch stands between a fetch and the products behind it: behind a join the compiler waits for every read in flight.)
+    auto next_stage = [&](int c) {
+        if (c + NSA - 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NSA - 2) * LA + (NSB - 2) * LB) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (c + NST - 1 < chunks) issue(c + NST - 1);
-        multiply(c);
+        if (NSA == NSB && c + NSA < chunks) issueA(c + NSA);
+        if (c + NSB < chunks) issueB(c + NSB);
+        if (NSA != NSB && c + NSA < chunks) issueA(c + NSA);
+    };
+    Frag f0, f1;
+#pragma unroll 1
+    for (int c = 0; c < NSA && c < chunks; ++c) {
+        issueA(c);
+        if (c < NSB) issueB(c);
+    }
+    if (chunks > 0) {
+        if (chunks >= NSA) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NSA - 1) * LA + (NSB - 1) * LB) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        fetch(0, 0, f0);
+#pragma unroll 1
+        for (int c = 0; c + 1 < chunks; ++c) {
+            fetch(c, 1, f1);
+            multiply(f0);
+            next_stage(c);
+            fetch(c + 1, 0, f0);
+            multiply(f1);
+        }
+        fetch(chunks - 1, 1, f1);
+        multiply(f0);
+        multiply(f1);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();       // the ring is free: it becomes the waves' store slabs
@@ -285,7 +290,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
 
     // ---- results: 32 rows of the wave at a time through a slab of [32][BN / WN] floats (rows 16 bytes apart in the banks)
     constexpr int WCOLS = BN / WN, PITCH = WCOLS + 4, W = 16 / (int)sizeof(typename O::raw), LANES_ROW = WCOLS / W, ROWS_PASS = 64 / LANES_ROW;
-    static_assert(WAVES * 32 * PITCH * 4 <= NST * STAGE, "the slabs fit the ring");
+    static_assert(WAVES * 32 * PITCH * 4 <= NSA * SA::BYTES + NSB * SB::BYTES, "the slabs fit the rings");
     float* slab = (float*)lds + wv * 32 * PITCH;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
@@ -323,9 +328,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     }
 }
 
-template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NST> static int lin_tile_launch(const LinArgs& a, hipStream_t s) {
-    constexpr int LDS = NST * (BM + BN) * LIN_CHUNK_BYTES;
-    auto kernel = linear_tile_kernel<T, O, AX, BX, BM, BN, WM, WN, NST>;
+template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB> static int lin_tile_launch(const LinArgs& a, hipStream_t s) {
+    constexpr int LDS = (NSA * BM + NSB * BN) * LIN_CHUNK_BYTES;
+    auto kernel = linear_tile_kernel<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB>;
     SRF_ONCE_PER_DEVICE(SRF_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS)));
     const long blocks = (long)a.tiles_i * a.tiles_j * a.splits;
     SRF_CHECK(blocks <= ROWOPS_GRID_MAX, "linear: %ld tiles are more than one launch holds", blocks);
@@ -336,14 +341,14 @@ template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int 
 template <typename T, typename O, bool AX, bool BX> static int lin_tile_pick(const LinArgs& a, LinTile tile, hipStream_t s) {
     switch (tile) {
         case LIN_256x256:
-            if constexpr (T::code != SCENERF_T_F32) return lin_tile_launch<T, O, AX, BX, 256, 256, 2, 4, 4>(a, s);
+            if constexpr (T::code != SCENERF_T_F32) return lin_tile_launch<T, O, AX, BX, 256, 256, 2, 4, 3, 2>(a, s);
             break;
         case LIN_256x128:
-            if constexpr (T::code != SCENERF_T_F32) return lin_tile_launch<T, O, AX, BX, 256, 128, 4, 2, 4>(a, s);
+            if constexpr (T::code != SCENERF_T_F32) return lin_tile_launch<T, O, AX, BX, 256, 128, 4, 2, 3, 3>(a, s);
             break;
-        case LIN_128x128: return lin_tile_launch<T, O, AX, BX, 128, 128, 2, 2, 3>(a, s);
-        case LIN_128x32: return lin_tile_launch<T, O, AX, BX, 128, 32, 4, 1, 4>(a, s);
-        case LIN_32x128: return lin_tile_launch<T, O, AX, BX, 32, 128, 1, 4, 4>(a, s);
+        case LIN_128x128: return lin_tile_launch<T, O, AX, BX, 128, 128, 2, 2, 3, 2>(a, s);
+        case LIN_128x32: return lin_tile_launch<T, O, AX, BX, 128, 32, 4, 1, 3, 3>(a, s);
+        case LIN_32x128: return lin_tile_launch<T, O, AX, BX, 32, 128, 1, 4, 3, 3>(a, s);
         default: break;
     }
     srf_set_error("linear: no such tile for this type");
