@@ -43,21 +43,31 @@ template <typename O> __device__ static inline void epilogue_one(const LinArgs& 
     if (p.residual) v += O::to_f32(((const raw*)p.residual)[i * p.ld_residual + j]);
     ((raw*)p.out)[i * p.N + j] = O::from_f32(v);
 }
-// W = 16 / sizeof(O::raw) neighbouring elements, all inside the row, every address aligned to 16 bytes
-template <typename O, int W> __device__ static inline void epilogue_vec(const LinArgs& p, long i, int j, float (&v)[W]) {
+// W = 16 / sizeof(O::raw) neighbouring elements, all inside the row, every address aligned to 16 bytes: what depends on the columns alone,
+// then one row's (its residual in hand)
+template <typename O, int W> struct EpilogueCols {
+    float bias[W], scale[W];
+    __device__ inline void load(const LinArgs& p, int j) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) bias[e] = 0.f;
+        if (p.bias) load_vec<O, W>((const typename O::raw*)p.bias + j, bias);
+        if (p.row_scale) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) scale[e] = p.col_scale[j + e];
+        }
+    }
+};
+template <typename O, int W> __device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<O, W>& ec, long i, int j, uint4 res, float (&v)[W]) {
     typedef typename O::raw raw;
     if (p.row_scale) {
         const float s = p.row_scale[i];
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] = v[e] * s * p.col_scale[j + e];
+        for (int e = 0; e < W; ++e) v[e] = v[e] * s * ec.scale[e];
     }
-    float t[W];
-    if (p.bias) {
-        load_vec<O, W>((const raw*)p.bias + j, t);
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] += t[e];
-    }
+    for (int e = 0; e < W; ++e) v[e] += ec.bias[e];
     if (p.z) {
+        float t[W];
 #pragma unroll
         for (int e = 0; e < W; ++e) t[e] = keep_z<O>(v[e]);
         store_vec<O, W>((raw*)p.z + i * p.N + j, t);
@@ -75,7 +85,8 @@ template <typename O, int W> __device__ static inline void epilogue_vec(const Li
         }
     }
     if (p.residual) {
-        load_vec<O, W>((const raw*)p.residual + i * p.ld_residual + j, t);
+        float t[W];
+        unpack16<O>(res, t);
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] += t[e];
     }
@@ -83,8 +94,8 @@ template <typename O, int W> __device__ static inline void epilogue_vec(const Li
 }
 
 // Tile shapes of the staged kernel (linear_tile.h): rows x columns of the result per workgroup
-enum LinTile { LIN_256x256, LIN_256x128, LIN_128x128, LIN_128x32, LIN_32x128, LIN_TILES };
-static const int kLinTileRows[LIN_TILES] = {256, 256, 128, 128, 32}, kLinTileCols[LIN_TILES] = {256, 128, 128, 32, 128};
+enum LinTile { LIN_256x256, LIN_128x128, LIN_128x32, LIN_32x128, LIN_TILES };
+static const int kLinTileRows[LIN_TILES] = {256, 128, 128, 32}, kLinTileCols[LIN_TILES] = {256, 128, 32, 128};
 #define LIN_CHUNK_BYTES 128             // of the contraction per step: 32 fp32, 64 16-bit, 128 8-bit elements
 
 // a_k == 1 / b_k == 1: read along the contraction, else across

@@ -104,8 +104,17 @@ template <typename O, bool VEC> __global__ __launch_bounds__(256) void linear_jo
 #pragma unroll
             for (int e = 0; e < W; ++e) v[e] += u[e];
         }
-        if constexpr (VEC) epilogue_vec<O, W>(p, (long)(t / p.N), (int)(t % p.N), v);
-        else epilogue_one<O>(p, (long)(t / p.N), (int)(t % p.N), v[0]);
+        const long i = (long)(t / p.N);
+        const int j = (int)(t % p.N);
+        if constexpr (VEC) {
+            EpilogueCols<O, W> ec;
+            ec.load(p, j);
+            uint4 res = make_uint4(0, 0, 0, 0);
+            if (p.residual) res = *(const uint4*)((const typename O::raw*)p.residual + i * p.ld_residual + j);
+            epilogue_vec<O, W>(p, ec, i, j, res, v);
+        } else {
+            epilogue_one<O>(p, i, j, v[0]);
+        }
     }
 }
 
@@ -260,8 +269,12 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
         if (N <= 32) r.tile = LIN_128x32;
         else if (M <= 32) r.tile = LIN_32x128;
         else if (type != SCENERF_T_F32) {
-            if (tiles(LIN_256x256) >= 256) { r.tile = LIN_256x256; want = 256; }
-            else if (tiles(LIN_256x128) >= 256 || K >= 16384) { r.tile = LIN_256x128; want = 256; }
+            // 256 x 256 (one workgroup a CU) against 128 x 128 (two): by rounds over the 256 CUs, a round of two small tiles counted as 2.5
+            // quarters of a large one -- they read twice the operand bytes per product (8,192^3 bf16: 878 against 1,182 us).  The small
+            // ones win where they fill the chip or the matrix better (4,800 x 512 x 512: 15 against 29 us; 153,600 x 128 x 128: 42 against
+            // 76).  A long contraction fills the chip either way, by splits.
+            const long big = (tiles(LIN_256x256) + 255) / 256 * 8, small = (tiles(LIN_128x128) + 511) / 512 * 5;
+            if (big <= small || (K >= 16384 && M > 128 && N > 128)) { r.tile = LIN_256x256; want = 256; }
         }
         rows = kLinTileRows[r.tile];
         cols = kLinTileCols[r.tile];

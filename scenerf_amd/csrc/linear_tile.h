@@ -27,16 +27,9 @@ __device__ __attribute__((aligned(16))) const unsigned lin_zeros[4] = {0, 0, 0, 
 
 template <bool V> struct Bool { static constexpr bool value = V; };
 
-// 64 lanes x 16 bytes, global -> LDS at lds_base + lane * 16 (m0 is the base; saved around, the compiler owns it)
-__device__ static inline void lin_copy(const void* sbase, unsigned voff, unsigned lds_base) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(voff), "s"(sbase), "s"(lds_base) : "memory");
-}
-__device__ static inline void lin_copy_v(const void* vaddr, unsigned lds_base) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(vaddr), "s"(lds_base) : "memory");
+// 64 lanes x 16 bytes, global -> LDS at lds_base + lane * 16 (m0 is the base)
+__device__ static inline void lin_copy(const void* src, unsigned lds_base) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_base) : "memory", "m0");
 }
 
 // contiguous ranges of work per XCD (blocks go round-robin over the 8 XCDs, each with its own L2); any count
@@ -76,7 +69,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     typedef LinSide<T, AX, BM> SA;
     typedef LinSide<T, BX, BN> SB;
     constexpr int ES = SA::ES, BK = SA::BK, WAVES = WM * WN;
-    constexpr int LA = (SA::PIECES + WAVES - 1) / WAVES, LB = (SB::PIECES + WAVES - 1) / WAVES;     // loads per wave and chunk
+    constexpr int LA = SA::PIECES / WAVES, LB = SB::PIECES / WAVES;     // loads per wave and chunk
     static_assert(NSA >= 2 && (NSB == NSA || NSB == NSA - 1) && NSB >= 2, "the order of the loads and their counts");
     constexpr int I = BM / WM / 32, J = BN / WN / 32;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -92,50 +85,42 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     const int kb = (int)min((long)p.K, (long)split * p.k_split), ke = (int)min((long)p.K, (long)kb + p.k_split);
     const int chunks = ke > kb ? (ke - kb + BK - 1) / BK : 0;
 
-    // ---- loads: of each side wave w moves pieces w, w + WAVES, ... (past the last one: the last one again, the same bytes to the same
-    // place).  A's ring has NSA stages, B's behind it NSB.
+    // ---- loads: of each side wave w moves pieces w, w + WAVES, ...  A's ring has NSA stages, B's behind it NSB.
     const char* baseA = (const char*)p.A + i0 * p.a_i * ES;
     const char* baseB = (const char*)p.B + (long)j0 * p.b_j * ES;
     const unsigned ringB = lds0 + NSA * SA::BYTES;
-    unsigned offA[LA], offB[LB];
-    int kinA[LA], kinB[LB];
+    // (the k of a wave's loads inside a chunk: the same for all of a side read along, equal steps apart for one read across)
+    constexpr int KA = AX ? WAVES * 1024 / SA::LINE : 0, KB = BX ? WAVES * 1024 / SB::LINE : 0;
+    static_assert((AX || WAVES % 2 == 0) && (BX || WAVES % 2 == 0) && (!AX || WAVES * 1024 % SA::LINE == 0) && (!BX || WAVES * 1024 % SB::LINE == 0) &&
+                  (AX ? KA % 4 == 0 : true) && (BX ? KB % 4 == 0 : true) && SA::PIECES % WAVES == 0 && SB::PIECES % WAVES == 0, "the steps of the loads");
+    unsigned offA[AX ? 1 : LA], offB[BX ? 1 : LB];
+    int kinA, kinB;
 #pragma unroll
-    for (int u = 0; u < LA; ++u) {
+    for (int u = 0; u < (AX ? 1 : LA); ++u) {
         int r;
-        SA::place(min(wv + u * WAVES, SA::PIECES - 1), lane, r, kinA[u]);
+        SA::place(wv + u * WAVES, lane, r, kinA);
         // rows past the last: the last again (their results are dropped); ACROSS: the last whole 16 bytes
         r = (int)min((long)r, (AX ? (long)p.a_ext - 16 / ES : (long)p.M - 1) - i0);
-        offA[u] = (unsigned)((long)r * p.a_i + (long)kinA[u] * p.a_k) * ES;
+        offA[u] = (unsigned)((long)r * p.a_i + (long)kinA * p.a_k) * ES;
     }
 #pragma unroll
-    for (int u = 0; u < LB; ++u) {
+    for (int u = 0; u < (BX ? 1 : LB); ++u) {
         int r;
-        SB::place(min(wv + u * WAVES, SB::PIECES - 1), lane, r, kinB[u]);
+        SB::place(wv + u * WAVES, lane, r, kinB);
         r = min(r, (BX ? p.b_ext - 16 / ES : p.N - 1) - j0);
-        offB[u] = (unsigned)((long)r * p.b_j + (long)kinB[u] * p.b_k) * ES;
+        offB[u] = (unsigned)((long)r * p.b_j + (long)kinB * p.b_k) * ES;
     }
-    // what lies past the contraction's end, in the last chunk, comes from a zero
-    auto issueA = [&](int c) {
+    // load u of chunk c of a side.  What lies past the end of the split comes from a zero, and so do chunks past the last (nobody reads
+    // them): every turn of the loop issues the same loads, without a branch.
+    auto loadA = [&](int c, int u) {
         const long k0 = kb + (long)c * BK;
-        const char* a = baseA + k0 * p.a_k * ES;
-        const unsigned stage = lds0 + (c % NSA) * SA::BYTES;
-#pragma unroll
-        for (int u = 0; u < LA; ++u) {
-            const int q = min(wv + u * WAVES, SA::PIECES - 1);
-            if (k0 + BK <= p.K) lin_copy(a, offA[u], stage + q * 1024);
-            else lin_copy_v(k0 + kinA[u] < p.K ? a + offA[u] : (const char*)lin_zeros, stage + q * 1024);
-        }
+        const char* src = baseA + (k0 + u * KA) * p.a_k * ES + offA[AX ? 0 : u];
+        lin_copy(kinA < ke - k0 - u * KA ? src : (const char*)lin_zeros, lds0 + (c % NSA) * SA::BYTES + (wv + u * WAVES) * 1024);
     };
-    auto issueB = [&](int c) {
+    auto loadB = [&](int c, int u) {
         const long k0 = kb + (long)c * BK;
-        const char* b = baseB + k0 * p.b_k * ES;
-        const unsigned stage = ringB + (c % NSB) * SB::BYTES;
-#pragma unroll
-        for (int u = 0; u < LB; ++u) {
-            const int q = min(wv + u * WAVES, SB::PIECES - 1);
-            if (k0 + BK <= p.K) lin_copy(b, offB[u], stage + q * 1024);
-            else lin_copy_v(k0 + kinB[u] < p.K ? b + offB[u] : (const char*)lin_zeros, stage + q * 1024);
-        }
+        const char* src = baseB + (k0 + u * KB) * p.b_k * ES + offB[BX ? 0 : u];
+        lin_copy(kinB < ke - k0 - u * KB ? src : (const char*)lin_zeros, ringB + (c % NSB) * SB::BYTES + (wv + u * WAVES) * 1024);
     };
 
     // ---- fragments
@@ -168,122 +153,105 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
         return __builtin_bit_cast(unsigned, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true)
                                                  : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
     };
-    // the fragments of half a chunk: 8 registers a lane per 32 rows
+    // a chunk's contraction in PARTS, each one fragment of FR registers a lane per 32 rows: 16 (16-bit), 64 (8-bit), 8 (fp32) of it
     constexpr bool WIDEN = ES == 1 && O::code == SCENERF_T_F32;
-    constexpr int FR = 8;
+    constexpr int PARTS = ES == 1 ? 2 : 4, FR = ES == 1 ? 8 : 4;
     struct Frag { unsigned a[I][FR], b[J][FR]; };
-    auto fetch = [&](int c, int half, Frag& f) {
-        const char* sa = lds + (c % NSA) * SA::BYTES;
-        const char* sb = lds + NSA * SA::BYTES + (c % NSB) * SB::BYTES;
+    // item t of the READS that fetch a part: 16 bytes of the lane's for 32 rows of one side
+    constexpr int READS = FR / 4 * (I + J);
+    auto fetch = [&](int c, int part, Frag& f, int t) {
+        const int s = t % (FR / 4), n = t / (FR / 4);
         auto side = [&](auto across, const char* base, int first, int line, int swz, unsigned (&o)[FR]) {
             if constexpr (decltype(across)::value && ES == 4) {
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[4 * s + e] = *(const unsigned*)(base + (16 * half + 8 * s + 4 * h + e) * line + (first + l31) * 4);
+                for (int e = 0; e < 4; ++e) o[e] = *(const unsigned*)(base + (8 * part + 4 * h + e) * line + (first + l31) * 4);
             } else {
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    uint4 v;
-                    if constexpr (decltype(across)::value) v = across16(base, line, swz, first, 2 * half + s);
-                    else v = along(base, first + l31, 4 * half + 2 * s + h);       // 8-bit: the lane's half takes 16-byte slots h and h + 2
-                    o[4 * s] = v.x; o[4 * s + 1] = v.y; o[4 * s + 2] = v.z; o[4 * s + 3] = v.w;
-                }
+                uint4 v;
+                if constexpr (decltype(across)::value) v = across16(base, line, swz, first, part);
+                else v = along(base, first + l31, (FR / 2) * part + 2 * s + h);    // 8-bit: the lane's half takes 16-byte slots h and h + 2
+                o[4 * s] = v.x; o[4 * s + 1] = v.y; o[4 * s + 2] = v.z; o[4 * s + 3] = v.w;
             }
         };
-#pragma unroll
-        for (int i = 0; i < I; ++i) side(Bool<AX>(), sa, wi + i * 32, SA::LINE, SA::SWZ, f.a[i]);
-#pragma unroll
-        for (int j = 0; j < J; ++j) side(Bool<BX>(), sb, wj + j * 32, SB::LINE, SB::SWZ, f.b[j]);
+        if (n < I) side(Bool<AX>(), lds + (c % NSA) * SA::BYTES, wi + n * 32, SA::LINE, SA::SWZ, f.a[n < I ? n : 0]);
+        else side(Bool<BX>(), lds + NSA * SA::BYTES + (c % NSB) * SB::BYTES, wj + (n - I) * 32, SB::LINE, SB::SWZ, f.b[n < I ? 0 : n - I]);
     };
     auto four = [](const unsigned (&r)[FR], int s) { return make_uint4(r[4 * s], r[4 * s + 1], r[4 * s + 2], r[4 * s + 3]); };
-    auto multiply = [&](const Frag& f) {
-        if constexpr (ES == 2) {
+    // group g of the STEPS * I groups of J matrix instructions that multiply a part
+    constexpr int STEPS = ES == 4 || WIDEN ? 4 : 1, GROUPS = STEPS * I;
+    auto multiply = [&](const Frag& f, int g) {
+        const int s = g / I, i = g % I;
+        auto eight = [](const unsigned (&r)[FR]) {
+            return lin_i32x8{(int)r[0], (int)r[1], (int)r[2], (int)r[3], (int)r[4], (int)r[5], (int)r[6], (int)r[7]};
+        };
+        // 8-bit operands of a result in 32 bits: the 8-bit matrix instruction adds 8 neighbouring products to 2^-13 of the largest of them
+        // (measured: linear.hip), not enough.  e4m3 is exact in bf16: widened here, at half the rate
+        auto wide = [&](const unsigned (&r)[FR]) {
+            return __builtin_bit_cast(lin_bf16x8, make_uint4(widen2(r[2 * s], false), widen2(r[2 * s], true), widen2(r[2 * s + 1], false),
+                                                             widen2(r[2 * s + 1], true)));
+        };
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < I; ++i)
-#pragma unroll
-                    for (int j = 0; j < J; ++j) {
-                        if constexpr (T::code == SCENERF_T_BF16)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lin_bf16x8, four(f.b[j], s)),
-                                                                                __builtin_bit_cast(lin_bf16x8, four(f.a[i], s)), acc[i][j], 0, 0, 0);
-                        else
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lin_f16x8, four(f.b[j], s)),
-                                                                               __builtin_bit_cast(lin_f16x8, four(f.a[i], s)), acc[i][j], 0, 0, 0);
-                    }
-        } else if constexpr (WIDEN) {
-            // the 8-bit matrix instruction adds 8 neighbouring products to 2^-13 of the largest of them (measured: linear.hip): not enough
-            // for a result in 32 bits.  e4m3 is exact in bf16: widened here, at half the rate
-            auto wide = [&](const unsigned (&r)[FR], int s) {
-                return __builtin_bit_cast(lin_bf16x8, make_uint4(widen2(r[2 * s], false), widen2(r[2 * s], true), widen2(r[2 * s + 1], false),
-                                                                 widen2(r[2 * s + 1], true)));
-            };
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int i = 0; i < I; ++i)
-#pragma unroll
-                    for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wide(f.b[j], s), wide(f.a[i], s), acc[i][j], 0, 0, 0);
-        } else if constexpr (ES == 1) {
-            // 64 k in one instruction; every scale is 1 (127 as an exponent)
-            auto eight = [](const unsigned (&r)[FR]) {
-                return lin_i32x8{(int)r[0], (int)r[1], (int)r[2], (int)r[3], (int)r[4], (int)r[5], (int)r[6], (int)r[7]};
-            };
-#pragma unroll
-            for (int i = 0; i < I; ++i)
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(eight(f.b[j]), eight(f.a[i]), acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)             // the lane's half holds k = 8 (e / 4) + 4 h + e % 4
-#pragma unroll
-                for (int i = 0; i < I; ++i)
-#pragma unroll
-                    for (int j = 0; j < J; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f.b[j][e]), __uint_as_float(f.a[i][e]), acc[i][j], 0, 0, 0);
+        for (int j = 0; j < J; ++j) {
+            if constexpr (T::code == SCENERF_T_BF16)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lin_bf16x8, four(f.b[j], s)),
+                                                                    __builtin_bit_cast(lin_bf16x8, four(f.a[i], s)), acc[i][j], 0, 0, 0);
+            else if constexpr (T::code == SCENERF_T_F16)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lin_f16x8, four(f.b[j], s)),
+                                                                   __builtin_bit_cast(lin_f16x8, four(f.a[i], s)), acc[i][j], 0, 0, 0);
+            else if constexpr (WIDEN)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wide(f.b[j]), wide(f.a[i]), acc[i][j], 0, 0, 0);
+            else if constexpr (ES == 1)         // 64 k in one instruction; every scale is 1 (127 as an exponent)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(eight(f.b[j]), eight(f.a[i]), acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+            else                                // the lane's half holds k = 4 h + s
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f.b[j][s]), __uint_as_float(f.a[i][s]), acc[i][j], 0, 0, 0);
         }
     };
 
-    // ---- the loop: while one half of a chunk is multiplied from registers, the next half is read from LDS, and further chunks are under
-    // way, in the order A(0) B(0) A(1) B(1) ..: up to A(c + NSA - 1) and B(c + NSB - 1).  Between the halves: this wave's loads of chunk
-    // c + 1 have landed (what was issued behind them may be outstanding) and its reads of chunk c are done; behind the barrier that holds
-    // for every wave, and the stages of chunk c are free.
-    // (No branch stands between a fetch and the products behind it: behind a join the compiler waits for every read in flight.)
-    auto next_stage = [&](int c) {
-        if (c + NSA - 1 < chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NSA - 2) * LA + (NSB - 2) * LB) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (NSA == NSB && c + NSA < chunks) issueA(c + NSA);
-        if (c + NSB < chunks) issueB(c + NSB);
-        if (NSA != NSB && c + NSA < chunks) issueA(c + NSA);
+    // ---- the loop.  A part is multiplied from registers while the next one is read from LDS and loads of further chunks are issued, a few of
+    // each between the groups of matrix instructions: in a burst, the loads kept both waves of a SIMD from their products.
+    // Loads run in the order A(0) B(0) .. , B(c + NSB) behind the barrier in front of chunk c's last part, A(c + NSA) behind the chunk.
+    auto turn = [&](const Frag& now, int c, int part, Frag& next, auto load, int first, int last) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+#pragma unroll
+            for (int t = g * READS / GROUPS; t < (g + 1) * READS / GROUPS; ++t) fetch(c, part, next, t);
+#pragma unroll
+            for (int u = first + g * (last - first) / GROUPS; u < first + (g + 1) * (last - first) / GROUPS; ++u) load(u);
+            multiply(now, g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     Frag f0, f1;
-#pragma unroll 1
-    for (int c = 0; c < NSA && c < chunks; ++c) {
-        issueA(c);
-        if (c < NSB) issueB(c);
-    }
     if (chunks > 0) {
-        if (chunks >= NSA) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NSA - 1) * LA + (NSB - 1) * LB) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < NSA; ++c) {
+#pragma unroll
+            for (int u = 0; u < LA; ++u)
+                if (c < NSA - 1) loadA(c, u);
+#pragma unroll
+            for (int u = 0; u < LB; ++u)
+                if (c < NSB) loadB(c, u);
+        }
+        // chunk 0 has landed: what was issued behind it may be outstanding
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NSA - 2) * LA + (NSB - 1) * LB) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        fetch(0, 0, f0);
+#pragma unroll
+        for (int t = 0; t < READS; ++t) fetch(0, 0, f0, t);
 #pragma unroll 1
-        for (int c = 0; c + 1 < chunks; ++c) {
-            fetch(c, 1, f1);
-            multiply(f0);
-            next_stage(c);
-            fetch(c + 1, 0, f0);
-            multiply(f1);
+        for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+            for (int part = 0; part < PARTS - 1; ++part)
+                turn(part % 2 ? f1 : f0, c, part + 1, part % 2 ? f0 : f1, [&](int u) { loadA(c + NSA - 1, u); }, part * LA / (PARTS - 1),
+                     (part + 1) * LA / (PARTS - 1));
+            // this wave's loads of chunk c + 1 have landed, its reads of chunk c are done; behind the barrier that holds for every wave:
+            // the stages of chunk c are free
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NSA - 2) * LA + (NSB - 2) * LB) : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            turn(f1, c + 1, 0, f0, [&](int u) { loadB(c + NSB, u); }, 0, LB);
         }
-        fetch(chunks - 1, 1, f1);
-        multiply(f0);
-        multiply(f1);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();       // the ring is free: it becomes the waves' store slabs
     asm volatile("" ::: "memory");
@@ -291,7 +259,26 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     // ---- results: 32 rows of the wave at a time through a slab of [32][BN / WN] floats (rows 16 bytes apart in the banks)
     constexpr int WCOLS = BN / WN, PITCH = WCOLS + 4, W = 16 / (int)sizeof(typename O::raw), LANES_ROW = WCOLS / W, ROWS_PASS = 64 / LANES_ROW;
     static_assert(WAVES * 32 * PITCH * 4 <= NSA * SA::BYTES + NSB * SB::BYTES, "the slabs fit the rings");
+    typedef typename O::raw oraw;
     float* slab = (float*)lds + wv * 32 * PITCH;
+    // (a lane's columns are the same in every row: their bias and scales are read once; the residual of the next 32 rows is under way
+    // while these leave, which a load per row and its wait cost 8 us a tile)
+    constexpr int PASSES = 32 / ROWS_PASS;
+    const int c = (lane % LANES_ROW) * W, col = j0 + wj + c, lrow = lane / LANES_ROW;
+    const bool vec = !p.part && p.vec, in_col = col < p.N;
+    EpilogueCols<O, W> ec;
+    uint4 res[PASSES];
+    auto residual = [&](int i) {
+#pragma unroll
+        for (int t = 0; t < PASSES; ++t) {
+            const long row = i0 + wi + i * 32 + lrow + t * ROWS_PASS;
+            if (row < p.M) res[t] = *(const uint4*)((const oraw*)p.residual + row * p.ld_residual + col);
+        }
+    };
+    if (vec && in_col) {
+        ec.load(p, col);
+        if (p.residual) residual(0);
+    }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
 #pragma unroll
@@ -302,27 +289,32 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
                     make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
         wave_sync();
         const long row0 = i0 + wi + i * 32;
-        if (p.part) {
-            float* part = p.part + (size_t)split * p.M * p.N;
-            for (int r = 0; r < 32; ++r)
-                for (int c = lane; c < WCOLS; c += 64)
-                    if (row0 + r < p.M && j0 + wj + c < p.N) part[(size_t)(row0 + r) * p.N + j0 + wj + c] = slab[r * PITCH + c];
-        } else if (p.vec) {
-            const int c = (lane % LANES_ROW) * W, col = j0 + wj + c;
+        if (vec) {
+            if (in_col) {
+                uint4 now[PASSES];
 #pragma unroll
-            for (int r = lane / LANES_ROW; r < 32; r += ROWS_PASS) {
-                float v[W];
+                for (int t = 0; t < PASSES; ++t) now[t] = res[t];
+                if (p.residual && i + 1 < I) residual(i + 1);
 #pragma unroll
-                for (int e = 0; e < W; e += 4) {
-                    const float4 t = *(const float4*)(slab + r * PITCH + c + e);
-                    v[e] = t.x; v[e + 1] = t.y; v[e + 2] = t.z; v[e + 3] = t.w;
+                for (int t = 0; t < PASSES; ++t) {
+                    const int r = lrow + t * ROWS_PASS;
+                    float v[W];
+#pragma unroll
+                    for (int e = 0; e < W; e += 4) {
+                        const float4 q = *(const float4*)(slab + r * PITCH + c + e);
+                        v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
+                    }
+                    if (row0 + r < p.M) epilogue_vec<O, W>(p, ec, row0 + r, col, now[t], v);
                 }
-                if (row0 + r < p.M && col < p.N) epilogue_vec<O, W>(p, row0 + r, col, v);
             }
         } else {
+            float* part = p.part ? p.part + (size_t)split * p.M * p.N : nullptr;
             for (int r = 0; r < 32; ++r)
-                for (int c = lane; c < WCOLS; c += 64)
-                    if (row0 + r < p.M && j0 + wj + c < p.N) epilogue_one<O>(p, row0 + r, j0 + wj + c, slab[r * PITCH + c]);
+                for (int k = lane; k < WCOLS; k += 64)
+                    if (row0 + r < p.M && j0 + wj + k < p.N) {
+                        if (part) part[(size_t)(row0 + r) * p.N + j0 + wj + k] = slab[r * PITCH + k];
+                        else epilogue_one<O>(p, row0 + r, j0 + wj + k, slab[r * PITCH + k]);
+                    }
         }
         wave_sync();
     }
@@ -342,9 +334,6 @@ template <typename T, typename O, bool AX, bool BX> static int lin_tile_pick(con
     switch (tile) {
         case LIN_256x256:
             if constexpr (T::code != SCENERF_T_F32) return lin_tile_launch<T, O, AX, BX, 256, 256, 2, 4, 3, 2>(a, s);
-            break;
-        case LIN_256x128:
-            if constexpr (T::code != SCENERF_T_F32) return lin_tile_launch<T, O, AX, BX, 256, 128, 4, 2, 3, 3>(a, s);
             break;
         case LIN_128x128: return lin_tile_launch<T, O, AX, BX, 128, 128, 2, 2, 3, 2>(a, s);
         case LIN_128x32: return lin_tile_launch<T, O, AX, BX, 128, 32, 4, 1, 3, 3>(a, s);
