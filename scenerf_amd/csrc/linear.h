@@ -22,12 +22,6 @@ __device__ static inline float act_any(int act, float v) {
     if (act == SCENERF_ACT_SILU) return act_fwd<SCENERF_ACT_SILU>(v);
     return v;
 }
-__device__ static inline float slope_any(int act, float v) {
-    if (act == SCENERF_ACT_RELU) return act_slope<SCENERF_ACT_RELU>(v);
-    if (act == SCENERF_ACT_GELU) return act_slope<SCENERF_ACT_GELU>(v);
-    if (act == SCENERF_ACT_SILU) return act_slope<SCENERF_ACT_SILU>(v);
-    return 1.f;
-}
 // z as it is kept for the backward pass, in O.  A positive z that rounds to zero (fp16) is kept as the smallest positive value: relu's
 // slope there is 1, and the other slopes do not notice.
 template <typename O> __device__ static inline float keep_z(float v) {

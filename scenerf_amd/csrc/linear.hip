@@ -192,53 +192,62 @@ __global__ __launch_bounds__(256) void linear_pad_kernel(const R* __restrict__ s
 }
 
 // ---- dz = dy act'(z), and the column sums of dz by strips of rows ------------------------------------------------------------------
-// thread: 8 neighbouring columns, every 8th row of the strip
+template <typename O, int ACT> __device__ static inline void slopes(float (&g)[8], const float (&z)[8], int valid) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = e < valid ? g[e] * act_slope<ACT>(z[e]) : 0.f;
+}
+// A workgroup's 256 threads stand as 2^lx columns of 8 by 256 / 2^lx rows (2^lx: 32, or what a narrower matrix needs: at 128 columns a
+// fixed 32 left half the threads idle, 150 us for 262,144 x 128 fp32); two rows a thread are in flight.
 template <typename O, bool VEC>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld_dy, const void* z_, void* dz_, int pitch, float* part, int M, int N,
-                                                        int act, int strip) {
+                                                        int act, int strip, int lx) {
     typedef typename O::raw raw;
-    __shared__ float red[8][32][9];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int j0 = blockIdx.y * 256 + tx * 8;           // (a pitch above N: zeros in the columns between)
+    __shared__ float red[256 * 9];
+    const int tx = threadIdx.x & ((1 << lx) - 1), ty = threadIdx.x >> lx, rows = 256 >> lx;
+    const int j0 = ((blockIdx.y << lx) + tx) * 8;           // (a pitch above N: zeros in the columns between)
     const long r0 = (long)blockIdx.x * strip, r1 = min((long)M, r0 + strip);
     float sum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+    auto get = [&](const raw* p, float (&v)[8]) {
+        if constexpr (VEC) {
+            load_vec<O, 8>(p, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = j0 + e < N ? O::to_f32(p[e]) : 0.f;
+        }
+    };
     if (j0 < N) {
-        for (long r = r0 + ty; r < r1; r += 8) {
-            float g[8], z[8];
-            const raw* dy = (const raw*)dy_ + r * ld_dy + j0;
-            if constexpr (VEC) {
-                load_vec<O, 8>(dy, g);
-            } else {
+        for (long r = r0 + ty; r < r1; r += 2 * rows) {
+            const bool two = r + rows < r1;
+            float g[2][8], z[2][8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] = j0 + e < N ? O::to_f32(dy[e]) : 0.f;
+            for (int q = 0; q < 2; ++q) {
+                const long at = q == 0 || two ? r + q * rows : r;
+                get((const raw*)dy_ + at * ld_dy + j0, g[q]);
+                if (act != SCENERF_ACT_NONE) get((const raw*)z_ + at * N + j0, z[q]);
             }
-            if (act != SCENERF_ACT_NONE) {
-                const raw* zp = (const raw*)z_ + r * N + j0;
-                if constexpr (VEC) {
-                    load_vec<O, 8>(zp, z);
-                } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] = j0 + e < N ? O::to_f32(zp[e]) : 0.f;
-                }
+            for (int q = 0; q < 2; ++q) {
+                if (q == 1 && !two) continue;
+                if (act == SCENERF_ACT_GELU) slopes<O, SCENERF_ACT_GELU>(g[q], z[q], N - j0);
+                else if (act == SCENERF_ACT_SILU) slopes<O, SCENERF_ACT_SILU>(g[q], z[q], N - j0);
+                else if (act == SCENERF_ACT_RELU) slopes<O, SCENERF_ACT_RELU>(g[q], z[q], N - j0);
+                if (dz_) store_vec<O, 8>((raw*)dz_ + (r + q * rows) * pitch + j0, g[q]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] = j0 + e < N ? g[e] * slope_any(act, z[e]) : 0.f;
+                for (int e = 0; e < 8; ++e) sum[e] += g[q][e];
             }
-            if (dz_) store_vec<O, 8>((raw*)dz_ + r * pitch + j0, g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += g[e];
         }
     }
     if (!part) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) red[ty][tx][e] = sum[e];
+    for (int e = 0; e < 8; ++e) red[threadIdx.x * 9 + e] = sum[e];
     __syncthreads();
-    const int c = threadIdx.x >> 3, e = threadIdx.x & 7, j = blockIdx.y * 256 + threadIdx.x;
-    if (j < N) {
+    for (int t = threadIdx.x; t < 8 << lx; t += 256) {
+        const int j = (blockIdx.y << lx) * 8 + t;
+        if (j >= N) continue;
         float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s += red[k][c][e];
+        for (int k = 0; k < rows; ++k) s += red[((k << lx) + (t >> 3)) * 9 + (t & 7)];
         part[(size_t)blockIdx.x * N + j] = s;
     }
 }
@@ -386,7 +395,7 @@ static ForwardPlan lin_forward_plan(const scenerf_linear* p) {
     return f;
 }
 
-#define DZ_STRIPS 512
+#define DZ_STRIPS 1024               // strips of rows: four workgroups a CU at 32 columns of 8
 static int dz_strip(int64_t rows) {
     const int64_t per = (rows + DZ_STRIPS - 1) / DZ_STRIPS;
     return per < 8 ? 8 : (int)((per + 7) / 8 * 8);
@@ -444,10 +453,12 @@ static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
 }
 template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardPlan& b, void* dz, float* part, hipStream_t s) {
     const bool vec = p->n % 8 == 0 && p->ld_dy % 8 == 0 && aligned16(p->dy) && (p->activation == SCENERF_ACT_NONE || aligned16(p->z));
-    const dim3 grid(b.strips, cdiv(p->n, 256));
+    int lx = 2;
+    while (lx < 5 && (8 << lx) < p->n) ++lx;
+    const dim3 grid(b.strips, cdiv(p->n, 8 << lx));
     SRF_CHECK(grid.y <= 65535, "linear_backward: n is too large");
-    if (vec) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip);
-    else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip);
+    if (vec) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
+    else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
     SRF_LAUNCH_CHECK("linear_dz_kernel");
     return 0;
 }

@@ -223,20 +223,43 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
         if (in[c]) load_vec<E, VW>((const raw*)p.weight + col, w[c]);
     }
     const int waves = gridDim.x * ROW_WAVES;
-    for (long row = (long)blockIdx.x * ROW_WAVES + wv; row < p.rows; row += waves) {
-        float h[C][VW], g[C][VW];
-        const float rstd = p.rstd[row];
-        float dot = 0.f;
+    // the next row's three loads are under way while this one is worked on (narrow rows: with one row at a time the 8 waves a CU had too
+    // few bytes in flight, 180 us for 153,600 x 512 bf16)
+    constexpr bool AHEAD = C * VW <= 16;
+    float nh[C][VW], ng[C][VW], nd[C][VW], nr = 0.f;
+    auto get = [&](long row, float (&h)[C][VW], float (&g)[C][VW], float (&d)[C][VW], float& rstd) {
+        rstd = p.rstd[row];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int col = (c * 64 + lane) * VW;
 #pragma unroll
-            for (int e = 0; e < VW; ++e) h[c][e] = g[c][e] = 0.f;
+            for (int e = 0; e < VW; ++e) h[c][e] = g[c][e] = d[c][e] = 0.f;
             if (in[c]) {
                 load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h[c]);
                 load_vec<E, VW>((const raw*)p.dy + row * p.ld_dy + col, g[c]);
+                if (AHEAD && p.dh) load_vec<E, VW>((const raw*)p.dh + row * p.ld_dh + col, d[c]);
             }
         }
+    };
+    const long first = (long)blockIdx.x * ROW_WAVES + wv;
+    if (AHEAD && first < p.rows) get(first, nh, ng, nd, nr);
+    for (long row = first; row < p.rows; row += waves) {
+        float h[C][VW], g[C][VW], d[C][VW], rstd;
+        if constexpr (AHEAD) {
+            rstd = nr;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < VW; ++e) {
+                    h[c][e] = nh[c][e];
+                    g[c][e] = ng[c][e];
+                    d[c][e] = nd[c][e];
+                }
+            if (row + waves < p.rows) get(row + waves, nh, ng, nd, nr);
+        } else {
+            get(row, h, g, d, rstd);
+        }
+        float dot = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -252,13 +275,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
         for (int c = 0; c < C; ++c)
             if (in[c]) {
                 const int col = (c * 64 + lane) * VW;
-                float d[VW];
+                if (!AHEAD && p.dh) load_vec<E, VW>((const raw*)p.dh + row * p.ld_dh + col, d[c]);
 #pragma unroll
-                for (int e = 0; e < VW; ++e) d[e] = 0.f;
-                if (p.dh) load_vec<E, VW>((const raw*)p.dh + row * p.ld_dh + col, d);
-#pragma unroll
-                for (int e = 0; e < VW; ++e) d[e] = fmaf(rstd, fmaf(-dot, h[c][e], g[c][e]), d[e]);
-                store_vec<E, VW>((raw*)p.dx + row * D + col, d);
+                for (int e = 0; e < VW; ++e) d[c][e] = fmaf(rstd, fmaf(-dot, h[c][e], g[c][e]), d[c][e]);
+                store_vec<E, VW>((raw*)p.dx + row * D + col, d[c]);
             }
     }
     if (!p.partial) return;
@@ -369,7 +389,7 @@ static bool rms_vector_ok(const scenerf_rms* p, bool backward) {
     return (!p->h || aligned16(p->h)) && (!p->y || aligned16(p->y)) && (!p->q || aligned16(p->q));
 }
 static bool rms_in_registers(const scenerf_rms* p) { return p->width <= 64 * ROW_REGS; }
-#define RMS_GRAD_BLOCKS 512         // workgroups (and parts of dweight) of the gradient kernel: two per CU
+#define RMS_GRAD_BLOCKS 1024        // workgroups (and parts of dweight) of the gradient kernel: four per CU
 #define RMS_STRIP 512
 static int rms_grad_parts(const scenerf_rms* p) {
     if (!rms_in_registers(p)) return (int)((p->rows + RMS_STRIP - 1) / RMS_STRIP);

@@ -18,65 +18,36 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .linear import MAX_ROWS, TYPE_CODES, give_workspace, no_gradient, require_cuda, require_type, rows_of, run_on
-
-
-def rows_forward(what, x, weight, residual, eps, *, quantize=False, keep_rstd=False) -> dict:
-    width, dev = x.shape[-1], x.device
-    x2 = rows_of(x, width)
-    rows = x2.shape[0]
-    p = _capi.Rms(TYPE_CODES[x.dtype], width, rows, eps)
-    p.x, p.ldx = x2.data_ptr(), x2.stride(0)
-    out = {"x2": x2}
-    if weight is not None:
-        weight = weight.contiguous()
-        p.weight = weight.data_ptr()
-    if residual is not None:
-        r2 = rows_of(residual, width)
-        out["h"] = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        p.residual, p.ld_residual, p.h = r2.data_ptr(), r2.stride(0), out["h"].data_ptr()
-    if quantize:
-        out["q"] = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-        out["scale"] = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-        p.q, p.scale = out["q"].data_ptr(), out["scale"].data_ptr()
-    else:
-        out["y"] = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        p.y = out["y"].data_ptr()
-    if keep_rstd:
-        out["rstd"] = torch.empty((rows,), dtype=torch.float32, device=dev)
-        p.rstd = out["rstd"].data_ptr()
-    run_on(dev, _capi.load().scenerf_hip_rms_forward, p, what)
-    return out
+from .rowops import MAX_ROWS, TYPE_CODES, check_float, check_tensors, give_workspace, no_gradient, rows_forward, rows_of, run_on
 
 
 def _check(what, x, weight, residual, eps) -> None:
-    require_cuda(what, x.device, weight=weight, residual=residual)
-    if x.dtype not in TYPE_CODES:
-        raise RuntimeError("%s: x must be float32, bfloat16 or float16 (got %s)" % (what, x.dtype))
-    require_type(what, x.dtype, weight=weight, residual=residual)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("%s: x must have at least one column (got %s)" % (what, tuple(x.shape)))
-    if tuple(weight.shape) != (x.shape[-1],):
-        raise ValueError("%s: weight must be (%d,) (got %s)" % (what, x.shape[-1], tuple(weight.shape)))
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError("%s: residual must be %s (got %s); expand it first if it is to be broadcast" % (what, tuple(x.shape), tuple(residual.shape)))
+    shape = x.shape
+    check_tensors(what, x.device, x.dtype, ("weight", weight), ("residual", residual))
+    check_float(what, "x", x.dtype)
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError("%s: x must have at least one column (got %s)" % (what, tuple(shape)))
+    if weight.shape != (shape[-1],):
+        raise ValueError("%s: weight must be (%d,) (got %s)" % (what, shape[-1], tuple(weight.shape)))
+    if residual is not None and residual.shape != shape:
+        raise ValueError("%s: residual must be %s (got %s); expand it first if it is to be broadcast" % (what, tuple(shape), tuple(residual.shape)))
     if not eps >= 0.0:
         raise ValueError("%s: eps must not be negative (got %r)" % (what, eps))
-    if x.numel() // x.shape[-1] > MAX_ROWS:
+    if x.numel() // shape[-1] > MAX_ROWS:
         raise ValueError("%s: more than 2^31 - 1025 rows" % what)
 
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        got = rows_forward("rms_norm", x, weight, residual, eps, keep_rstd=True)
+        y, _, h, rstd, x2 = rows_forward("rms_norm", x, weight, residual, eps, keep_rstd=True)
         ctx.eps, ctx.has_residual = eps, residual is not None
         ctx.set_materialize_grads(False)
         if residual is None:
-            ctx.save_for_backward(got["x2"], weight, got["rstd"])
-            return got["y"]
-        ctx.save_for_backward(got["h"], weight, got["rstd"])
-        return got["y"], got["h"]
+            ctx.save_for_backward(x2, weight, rstd)
+            return y
+        ctx.save_for_backward(h, weight, rstd)
+        return y, h
 
     @staticmethod
     @once_differentiable
@@ -89,19 +60,15 @@ class _RmsNorm(torch.autograd.Function):
                     dh if ctx.has_residual and ctx.needs_input_grad[2] else None, None)
         width, dev = h.shape[-1], h.device
         h2, dy2, w = rows_of(h, width), rows_of(dy, width), weight.contiguous()
+        dh2 = rows_of(dh, width) if dh is not None else None
         dx = torch.empty(dy.shape, dtype=h.dtype, device=dev) if need_x else None
         dw = torch.empty((width,), dtype=h.dtype, device=dev) if need_w else None
-        p = _capi.Rms(TYPE_CODES[h.dtype], width, h2.shape[0], ctx.eps)
-        p.x, p.ldx, p.weight, p.rstd = h2.data_ptr(), h2.stride(0), w.data_ptr(), rstd.data_ptr()
-        p.dy, p.ld_dy = dy2.data_ptr(), dy2.stride(0)
-        if dh is not None:
-            dh2 = rows_of(dh, width)
-            p.dh, p.ld_dh = dh2.data_ptr(), dh2.stride(0)
-        p.dx, p.dweight = _capi.ptr(dx), _capi.ptr(dw)
+        p = _capi.Rms(TYPE_CODES[h.dtype], width, h2.shape[0], ctx.eps, h2.data_ptr(), h2.stride(0), None, 0, w.data_ptr(), None, None, None, None,
+                      rstd.data_ptr(), dy2.data_ptr(), dy2.stride(0), None if dh2 is None else dh2.data_ptr(), 0 if dh2 is None else dh2.stride(0),
+                      None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr())
         lib = _capi.load()
-        ws = give_workspace(lib.scenerf_hip_rms_workspace, p, True, dev, "rms_norm backward")
+        ws = give_workspace(lib.scenerf_hip_rms_workspace, p, 1, dev, "rms_norm backward")  # noqa: F841 (alive up to the launch)
         run_on(dev, lib.scenerf_hip_rms_backward, p, "rms_norm backward")
-        del ws
         return (dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.has_residual and ctx.needs_input_grad[2] else None, None)
 
 
@@ -113,8 +80,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.
     _check("rms_norm", x, weight, residual, eps)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         return _RmsNorm.apply(x, weight, residual, float(eps))
-    got = rows_forward("rms_norm", x, weight, residual, float(eps))
-    return got["y"] if residual is None else (got["y"], got["h"])
+    y, _, h, _, _ = rows_forward("rms_norm", x, weight, residual, float(eps))
+    return y if residual is None else (y, h)
 
 
 def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
@@ -123,5 +90,5 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[t
     stand for).  Forward only."""
     _check("rms_norm_8bit", x, weight, residual, eps)
     no_gradient("rms_norm_8bit", x, weight, residual)
-    got = rows_forward("rms_norm_8bit", x, weight, residual, float(eps), quantize=True)
-    return (got["q"], got["scale"]) if residual is None else (got["q"], got["scale"], got["h"])
+    q, scale, h, _, _ = rows_forward("rms_norm_8bit", x, weight, residual, float(eps), quantize=True)
+    return (q, scale) if residual is None else (q, scale, h)
