@@ -89,31 +89,49 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
         else epilogue_one<O>(p, i, j, acc[e]);
     }
 }
-// the splits' sums, added in order, then the epilogue; W elements a thread
+// the splits' sums, added in a fixed order, then the epilogue: a workgroup owns 32 pieces of W results, 8 threads each, thread y of them
+// adds splits y, y + 8, ..
 template <typename O, bool VEC> __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs p) {
     constexpr int W = VEC ? 16 / (int)sizeof(typename O::raw) : 1;
+    __shared__ float red[8][32][W + 1];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const size_t total = (size_t)p.M * p.N;
-    for (size_t t = ((size_t)blockIdx.x * 256 + threadIdx.x) * W; t < total; t += (size_t)gridDim.x * 256 * W) {
+    for (size_t t0 = (size_t)blockIdx.x * 32 * W; t0 < total; t0 += (size_t)gridDim.x * 32 * W) {
+        const size_t t = t0 + tx * W;
         float v[W];
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] = 0.f;
+        if (t < total) {
 #pragma unroll 4
-        for (int s = 0; s < p.splits; ++s) {
-            float u[W];
-            load_vec<TypeF32, W>(p.part + s * total + t, u);
+            for (int s = ty; s < p.splits; s += 8) {
+                float u[W];
+                load_vec<TypeF32, W>(p.part + s * total + t, u);
 #pragma unroll
-            for (int e = 0; e < W; ++e) v[e] += u[e];
+                for (int e = 0; e < W; ++e) v[e] += u[e];
+            }
         }
-        const long i = (long)(t / p.N);
-        const int j = (int)(t % p.N);
-        if constexpr (VEC) {
-            EpilogueCols<O, W> ec;
-            ec.load(p, j);
-            uint4 res = make_uint4(0, 0, 0, 0);
-            if (p.residual) res = *(const uint4*)((const typename O::raw*)p.residual + i * p.ld_residual + j);
-            epilogue_vec<O, W>(p, ec, i, j, res, v);
-        } else {
-            epilogue_one<O>(p, i, j, v[0]);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < W; ++e) red[ty][tx][e] = v[e];
+        __syncthreads();
+        if (ty == 0 && t < total) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                v[e] = 0.f;
+#pragma unroll
+                for (int y = 0; y < 8; ++y) v[e] += red[y][tx][e];
+            }
+            const long i = (long)(t / p.N);
+            const int j = (int)(t % p.N);
+            if constexpr (VEC) {
+                EpilogueCols<O, W> ec;
+                ec.load(p, j);
+                uint4 res = make_uint4(0, 0, 0, 0);
+                if (p.residual) res = *(const uint4*)((const typename O::raw*)p.residual + i * p.ld_residual + j);
+                epilogue_vec<O, W>(p, ec, i, j, res, v);
+            } else {
+                epilogue_one<O>(p, i, j, v[0]);
+            }
         }
     }
 }
@@ -335,8 +353,8 @@ template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& p
         SRF_LAUNCH_CHECK("linear_any_kernel");
     }
     if (plan.splits > 1) {
-        const size_t work = ((size_t)a.M * a.N / (a.vec ? W : 1) + 255) / 256;
-        const unsigned blocks = work < 1 ? 1 : work < 8192 ? (unsigned)work : 8192;
+        const size_t work = ((size_t)a.M * a.N / (a.vec ? W : 1) + 31) / 32;
+        const unsigned blocks = work < 16384 ? (unsigned)work : 16384;
         if (a.vec) linear_join_kernel<O, true><<<blocks, 256, 0, s>>>(a);
         else linear_join_kernel<O, false><<<blocks, 256, 0, s>>>(a);
         SRF_LAUNCH_CHECK("linear_join_kernel");

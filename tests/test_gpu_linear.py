@@ -74,6 +74,24 @@ def test_relu_gradients_on_whole_numbers(m, k, n, dtype):
         assert torch.equal(got, exact), (name, float((got.double() - value).abs().max()))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(70001, 96, 264), (66003, 200, 136), (70001, 64, 129)])
+def test_more_tiles_than_workgroups(m, k, n, dtype):
+    """A workgroup goes through several tiles (results that leave in 16-byte pieces) or many workgroups queue (the odd width)."""
+    from scenerf_amd.linear import linear
+    g = gen("tiles", m, k, n, dtype)
+    x, w, b, r = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5), normal(g, n, dtype=dtype), normal(g, m, n, dtype=dtype)
+    for act in ACTS:
+        hold(linear(x, w, b, activation=act, residual=r), linear64(x, w, b, act, r)["y"], act)
+    hold(linear(x, w), linear64(x, w)["y"], "bare")
+    x, w, b = (t.requires_grad_(True) for t in (x, w, b))
+    dy = normal(g, m, n, dtype=dtype)
+    y = linear(x, w, b, activation="silu")
+    want = linear64(x.detach(), w.detach(), b.detach(), "silu", None, dy)
+    for name, got in zip(("y", "dx", "dw", "db"), (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy)):
+        hold(got, want[name], name)
+
+
 def test_gradients_against_differences():
     """fp32, 64-bit oracle: (L(p + e d) - L(p - e d)) / 2 e of the definition equals <gradient, d> of the kernels."""
     from scenerf_amd.linear import linear
