@@ -587,6 +587,7 @@ typedef struct scenerf_linear {
     int32_t out_type;               /* bias, residual, y, z, dy, db: equal to in_type unless that is E4M3 */
     int32_t activation;
     int32_t n, k;                   /* >= 1 */
+    int32_t padded;                 /* 1: x and w are scenerf_hip_linear_pad's copies, zeros behind each row up to a whole number of 16 bytes */
     int64_t rows;                   /* >= 0, < 2^31 - 1024 */
     const void* x; int64_t ldx;
     const void* w; int64_t ldw;
@@ -603,6 +604,11 @@ typedef struct scenerf_linear {
     void* workspace;                /* scenerf_hip_linear_workspace bytes, 16-byte aligned; contents are left undefined */
     int64_t workspace_bytes;
 } scenerf_linear;
+/* x and w laid out for 16-byte loads: copies with a row pitch of k rounded up to 16 bytes, zeros behind each row, in one launch (either may
+ * be NULL).  Rows that are 16-byte aligned, with a length and a pitch of whole 16 bytes, need none; others work without, element by element
+ * and many times slower. */
+int scenerf_hip_linear_pad(int type, int k, const void* x, int64_t ldx, int64_t rows, void* x_out, const void* w, int64_t ldw, int n, void* w_out,
+                           scenerf_stream_t stream);
 /* bytes of workspace the call needs (the pointers of *p are looked at for NULL and alignment only), or -1 */
 int64_t scenerf_hip_linear_workspace(const scenerf_linear* p, int backward);
 int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream);

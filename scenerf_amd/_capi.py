@@ -113,8 +113,8 @@ class AdamWTensor(C.Structure):
 
 class Linear(C.Structure):
     """scenerf_linear (scenerf_hip.h)."""
-    _fields_ = [("in_type", C.c_int32), ("out_type", C.c_int32), ("activation", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("rows", C.c_int64),
-                ("x", vp), ("ldx", C.c_int64), ("w", vp), ("ldw", C.c_int64), ("x_scale", vp), ("w_scale", vp), ("bias", vp),
+    _fields_ = [("in_type", C.c_int32), ("out_type", C.c_int32), ("activation", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("padded", C.c_int32),
+                ("rows", C.c_int64), ("x", vp), ("ldx", C.c_int64), ("w", vp), ("ldw", C.c_int64), ("x_scale", vp), ("w_scale", vp), ("bias", vp),
                 ("residual", vp), ("ld_residual", C.c_int64), ("y", vp), ("z", vp), ("dy", vp), ("ld_dy", C.c_int64),
                 ("dx", vp), ("dw", vp), ("db", vp), ("workspace", vp), ("workspace_bytes", C.c_int64)]
 
@@ -189,6 +189,7 @@ _PROTOS = {
     "scenerf_hip_test_chunk_table": (C.c_int, [C.POINTER(Cfg), i32, vp, i32]),
     "scenerf_hip_test_set_tuning": (C.c_int, [i32, i32]),
     "scenerf_hip_test_gemm_tn": (C.c_int, [i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]),
+    "scenerf_hip_linear_pad": (C.c_int, [i32, i32, vp, C.c_int64, C.c_int64, vp, vp, C.c_int64, i32, vp, vp]),
     "scenerf_hip_linear_workspace": (C.c_int64, [C.POINTER(Linear), i32]),
     "scenerf_hip_linear_forward": (C.c_int, [C.POINTER(Linear), vp]),
     "scenerf_hip_linear_backward": (C.c_int, [C.POINTER(Linear), vp]),

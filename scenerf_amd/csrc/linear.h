@@ -88,8 +88,8 @@ template <typename O, int W> __device__ static inline void epilogue_vec(const Li
 }
 
 // Tile shapes of the staged kernel (linear_tile.h): rows x columns of the result per workgroup
-enum LinTile { LIN_256x256, LIN_128x128, LIN_128x32, LIN_32x128, LIN_TILES };
-static const int kLinTileRows[LIN_TILES] = {256, 128, 128, 32}, kLinTileCols[LIN_TILES] = {256, 128, 32, 128};
+enum LinTile { LIN_256x256, LIN_128x128, LIN_64x64, LIN_128x32, LIN_TILES };
+static const int kLinTileRows[LIN_TILES] = {256, 128, 64, 128}, kLinTileCols[LIN_TILES] = {256, 128, 64, 32};
 #define LIN_CHUNK_BYTES 128             // of the contraction per step: 32 fp32, 64 16-bit, 128 8-bit elements
 
 // a_k == 1 / b_k == 1: read along the contraction, else across

@@ -195,17 +195,20 @@ __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs p) {
 }
 
 // ---- rows laid out anew: pitch a whole number of 16-byte pieces, zeros behind the row's end -----------------------------------------
+struct PadSide { const void* src; void* dst; long ld, rows; };
 template <typename R>
-__global__ __launch_bounds__(256) void linear_pad_kernel(const R* __restrict__ src, long ld, int rows, int cols, R* __restrict__ dst, int pitch) {
+__global__ __launch_bounds__(256) void linear_pad_kernel(PadSide x, PadSide w, int cols, int pitch) {
     constexpr int W = 16 / sizeof(R);
-    const long pieces = (long)rows * (pitch / W);
+    const int per = pitch / W;
+    const long first = x.rows * per, pieces = first + w.rows * per;
     for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < pieces; t += (long)gridDim.x * 256) {
-        const long r = t / (pitch / W);
-        const int c = (int)(t - r * (pitch / W)) * W;
-        union { R e[W]; uint4 v; } u;
+        const PadSide& s = t < first ? x : w;
+        const long u = t < first ? t : t - first, r = u / per;
+        const int c = (int)(u - r * per) * W;
+        union { R e[W]; uint4 v; } o;
 #pragma unroll
-        for (int e = 0; e < W; ++e) u.e[e] = c + e < cols ? src[r * ld + c + e] : (R)0;
-        *(uint4*)(dst + r * pitch + c) = u.v;
+        for (int e = 0; e < W; ++e) o.e[e] = c + e < cols ? ((const R*)s.src)[r * s.ld + c + e] : (R)0;
+        *(uint4*)((R*)s.dst + r * pitch + c) = o.v;
     }
 }
 
@@ -289,26 +292,28 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
         r.kind = 1;
         return r;
     }
-    long rows = ANY_TILE, cols = ANY_TILE, want = 512;
+    long rows = ANY_TILE, cols = ANY_TILE, slots = 512;
     if (staged) {
         r.kind = 2;
+        // Rounds over the chip's workgroup slots (1, 2, 3 a CU by their LDS), times what a round takes: measured at 4,800 to 153,600 rows and
+        // 48 to 2,480 features, 8 : 4.7 : 2.4 whatever the length (20,000 x 512 x 512 bf16: 1 round of 23 us, 2 of 13.5, 4 of 7).  The
+        // large tile reads half the operand bytes per product and wins where the matrix fills it (8,192^3: 878 against 1,182 us), the
+        // small one where rows are few (1,024 x 512 x 512: 6.1 us against 9.8 and 20) or the result is narrow.
         auto tiles = [&](LinTile t) { return ((M + kLinTileRows[t] - 1) / kLinTileRows[t]) * ((N + kLinTileCols[t] - 1) / kLinTileCols[t]); };
+        auto cost = [&](LinTile t, long per, double round) { return (tiles(t) + per - 1) / per * round; };
+        const double big = type == SCENERF_T_F32 ? 1e30 : cost(LIN_256x256, 256, 8.0), mid = cost(LIN_128x128, 512, 4.7), small = cost(LIN_64x64, 768, 2.4);
         if (N <= 32) r.tile = LIN_128x32;
-        else if (M <= 32) r.tile = LIN_32x128;
-        else if (type != SCENERF_T_F32) {
-            // 256 x 256 (one workgroup a CU) against 128 x 128 (two): by rounds over the 256 CUs, a round of two small tiles counted as 2.5
-            // quarters of a large one -- they read twice the operand bytes per product (8,192^3 bf16: 878 against 1,182 us).  The small
-            // ones win where they fill the chip or the matrix better (4,800 x 512 x 512: 15 against 29 us; 153,600 x 128 x 128: 42 against
-            // 76).  A long contraction fills the chip either way, by splits.
-            const long big = (tiles(LIN_256x256) + 255) / 256 * 8, small = (tiles(LIN_128x128) + 511) / 512 * 5;
-            if (big <= small || (K >= 16384 && M > 128 && N > 128)) { r.tile = LIN_256x256; want = 256; }
-        }
+        else if (K >= 16384 && M > 64 && N > 64) r.tile = type != SCENERF_T_F32 && M > 128 && N > 128 ? LIN_256x256 : LIN_128x128;    // (splits fill the chip)
+        else r.tile = big <= mid && big <= small ? LIN_256x256 : mid <= small ? LIN_128x128 : LIN_64x64;
         rows = kLinTileRows[r.tile];
         cols = kLinTileCols[r.tile];
+        // The contraction is split where the tiles leave CUs idle: one workgroup a CU for a short one (three splits of 152 tiles took
+        // 60 us against 42 unsplit), every slot for a long one; a split keeps at least 8 chunks (the
+        // join is a launch of its own: 1,024 x 512 x 512 bf16 took 13 us in two splits, 6 in one).
+        slots = K < 16384 ? 256 : r.tile == LIN_256x256 ? 256 : r.tile == LIN_128x128 ? 512 : 768;
     }
-    // the contraction is split where the tiles alone leave CUs idle; a split keeps at least 8 chunks
     const long n_tiles = ((M + rows - 1) / rows) * ((N + cols - 1) / cols);
-    long s = n_tiles > 0 ? want / n_tiles : 1;
+    long s = n_tiles > 0 ? slots / n_tiles : 1;
     if (s > K / (8 * bk)) s = K / (8 * bk);
     r.splits = s < 1 ? 1 : s > 256 ? 256 : (int)s;
     r.k_split = (int)(((K + r.splits - 1) / r.splits + bk - 1) / bk * bk);
@@ -373,44 +378,17 @@ static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPla
     }
 }
 
-// A matrix whose rows the staged kernel can read in 16-byte pieces: aligned base, pitch and length, and a pitch whose 256 rows stay
-// inside a 32-bit offset.  What is not gets a copy in the workspace with a padded pitch, zeros behind each row's end.
+// A matrix whose rows the staged kernel can read in 16-byte pieces: aligned base and pitch, a length of whole pieces (or zeros up to one),
+// and a pitch whose 256 rows stay inside a 32-bit offset
 #define LIN_MAX_PITCH_BYTES (1 << 22)
-static bool lin_pieces(const void* p, int64_t ld, int cols, int es) {
-    return aligned16(p) && (ld * es) % 16 == 0 && (cols * (int64_t)es) % 16 == 0 && ld * es <= LIN_MAX_PITCH_BYTES;
-}
-static bool lin_can_pad(int cols, int es) { return cols * (int64_t)es <= LIN_MAX_PITCH_BYTES - 16; }
 static int lin_pitch(int cols, int es) { return round_up(cols, 16 / es); }
-static int lin_pad(const void* src, int64_t ld, int64_t rows, int cols, int es, void* dst, hipStream_t s) {
-    const int pitch = lin_pitch(cols, es);
-    const long pieces = (long)rows * (pitch / (16 / es));
-    const unsigned blocks = (unsigned)(pieces < 8192L * 256 ? (pieces + 255) / 256 : 8192);
-    if (es == 4) linear_pad_kernel<uint32_t><<<blocks, 256, 0, s>>>((const uint32_t*)src, ld, (int)rows, cols, (uint32_t*)dst, pitch);
-    else if (es == 2) linear_pad_kernel<uint16_t><<<blocks, 256, 0, s>>>((const uint16_t*)src, ld, (int)rows, cols, (uint16_t*)dst, pitch);
-    else linear_pad_kernel<uint8_t><<<blocks, 256, 0, s>>>((const uint8_t*)src, ld, (int)rows, cols, (uint8_t*)dst, pitch);
-    SRF_LAUNCH_CHECK("linear_pad_kernel");
-    return 0;
+static bool lin_pieces(const void* p, int64_t ld, int cols, int es, bool padded) {
+    return aligned16(p) && (ld * es) % 16 == 0 && ld * es <= LIN_MAX_PITCH_BYTES && (padded ? ld >= lin_pitch(cols, es) : (cols * (int64_t)es) % 16 == 0);
 }
-
-struct ForwardPlan {
-    bool pad_x, pad_w;
-    int64_t x, w, sums, bytes;      // offsets in the workspace
-    LinPlan product;
-};
-static ForwardPlan lin_forward_plan(const scenerf_linear* p) {
-    ForwardPlan f = {};
+static LinPlan lin_forward_plan(const scenerf_linear* p) {
     const int es = lin_es(p->in_type);
-    const bool can = lin_can_pad(p->k, es) && p->rows > 0;
-    // (a length that is no whole number of pieces needs both padded: the other operand's piece would reach into its next row)
-    f.pad_x = can && !lin_pieces(p->x, p->ldx, p->k, es);
-    f.pad_w = can && !lin_pieces(p->w, p->ldw, p->k, es);
-    f.product = lin_plan(p->in_type, false, false, can, p->rows, p->n, p->k);
-    int64_t at = 0;
-    if (f.pad_x) { f.x = at; at += align256(p->rows * lin_pitch(p->k, es) * es); }
-    if (f.pad_w) { f.w = at; at += align256((int64_t)p->n * lin_pitch(p->k, es) * es); }
-    f.sums = at;
-    f.bytes = at + lin_part_bytes(f.product, p->rows, p->n);
-    return f;
+    const bool staged = lin_pieces(p->x, p->ldx, p->k, es, p->padded) && lin_pieces(p->w, p->ldw, p->k, es, p->padded);
+    return lin_plan(p->in_type, false, false, staged, p->rows, p->n, p->k);
 }
 
 #define DZ_STRIPS 1024               // strips of rows: four workgroups a CU at 32 columns of 8
@@ -419,9 +397,9 @@ static int dz_strip(int64_t rows) {
     return per < 8 ? 8 : (int)((per + 7) / 8 * 8);
 }
 struct BackwardPlan {
-    bool make_dz, pad_x, pad_w;     // dz is not dy itself; operands to lay out anew
+    bool make_dz;                   // dz is not dy itself
     int strip, strips, dz_pitch;
-    int64_t part, dz, x, w, sums;   // offsets of the column sums' parts, of dz, x, w and of the split sums
+    int64_t part, dz, sums;         // offsets of the column sums' parts, of dz and of the split sums
     int64_t bytes;
     LinPlan dx, dw;
 };
@@ -429,20 +407,17 @@ static BackwardPlan lin_backward_plan(const scenerf_linear* p) {
     BackwardPlan b = {};
     const int es = lin_es(p->in_type);
     const bool products = (p->dx || p->dw) && p->rows > 0;
-    const bool can = lin_can_pad(p->n, es) && lin_can_pad(p->k, es);
-    b.make_dz = products && (p->activation != SCENERF_ACT_NONE || (can && !lin_pieces(p->dy, p->ld_dy, p->n, es)));
-    b.pad_x = can && products && p->dw && !lin_pieces(p->x, p->ldx, p->k, es);
-    b.pad_w = can && products && p->dx && !lin_pieces(p->w, p->ldw, p->k, es);
     b.dz_pitch = round_up(p->n, 8);
+    const bool dz_fits = (int64_t)b.dz_pitch * es <= LIN_MAX_PITCH_BYTES;
+    // (a dy that cannot be read in pieces becomes a dz that can, with zeros behind its rows)
+    b.make_dz = products && (p->activation != SCENERF_ACT_NONE || (dz_fits && !lin_pieces(p->dy, p->ld_dy, p->n, es, false)));
     b.strip = dz_strip(p->rows);
     b.strips = (int)((p->rows + b.strip - 1) / b.strip);
-    b.dx = lin_plan(p->in_type, false, true, can, p->rows, p->k, p->n);
-    b.dw = lin_plan(p->in_type, true, true, can, p->n, p->k, p->rows);
+    b.dx = lin_plan(p->in_type, false, true, dz_fits && lin_pieces(p->w, p->ldw, p->k, es, p->padded), p->rows, p->k, p->n);
+    b.dw = lin_plan(p->in_type, true, true, dz_fits && lin_pieces(p->x, p->ldx, p->k, es, p->padded), p->n, p->k, p->rows);
     int64_t at = 0;
     if (p->db) { b.part = at; at += align256((int64_t)b.strips * p->n * 4); }
     if (b.make_dz) { b.dz = at; at += align256(p->rows * b.dz_pitch * es); }
-    if (b.pad_x) { b.x = at; at += align256(p->rows * lin_pitch(p->k, es) * es); }
-    if (b.pad_w) { b.w = at; at += align256((int64_t)p->n * lin_pitch(p->k, es) * es); }
     b.sums = at;
     const int64_t sx = p->dx ? lin_part_bytes(b.dx, p->rows, p->k) : 0, sw = p->dw ? lin_part_bytes(b.dw, p->n, p->k) : 0;
     b.bytes = at + (sx > sw ? sx : sw);
@@ -483,39 +458,49 @@ template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardP
 
 extern "C" {
 
+int scenerf_hip_linear_pad(int type, int k, const void* x, int64_t ldx, int64_t rows, void* x_out, const void* w, int64_t ldw, int n, void* w_out,
+                           scenerf_stream_t stream) {
+    SRF_CHECK(type >= SCENERF_T_F32 && type <= SCENERF_T_E4M3, "linear_pad: unknown type %d", type);
+    SRF_CHECK(k >= 1 && k < ROWOPS_GRID_MAX - 1024 && rows >= 0 && rows < ROWOPS_GRID_MAX - 1024 && n >= 0 && ldx >= 0 && ldw >= 0, "linear_pad: bad sizes");
+    SRF_CHECK(!x == !x_out && !w == !w_out, "linear_pad: a matrix and its copy go together");
+    SRF_CHECK(aligned16(x_out) && aligned16(w_out), "linear_pad: the copies must be aligned to 16 bytes");
+    const int es = lin_es(type), pitch = lin_pitch(k, es);
+    const PadSide sx = {x, x_out, ldx, x ? rows : 0}, sw = {w, w_out, ldw, w ? n : 0};
+    const long pieces = (sx.rows + sw.rows) * (pitch / (16 / es));
+    if (pieces == 0) return 0;
+    const unsigned blocks = (unsigned)(pieces < 8192L * 256 ? (pieces + 255) / 256 : 8192);
+    hipStream_t s = as_stream(stream);
+    SrfLaunchScope ps(s, "linear_pad", 0, 2. * pieces * 16);
+    if (es == 4) linear_pad_kernel<uint32_t><<<blocks, 256, 0, s>>>(sx, sw, k, pitch);
+    else if (es == 2) linear_pad_kernel<uint16_t><<<blocks, 256, 0, s>>>(sx, sw, k, pitch);
+    else linear_pad_kernel<uint8_t><<<blocks, 256, 0, s>>>(sx, sw, k, pitch);
+    SRF_LAUNCH_CHECK("linear_pad_kernel");
+    return 0;
+}
+
 int64_t scenerf_hip_linear_workspace(const scenerf_linear* p, int backward) {
     if (lin_check(p, "linear_workspace", backward != 0)) return -1;
-    return backward ? lin_backward_plan(p).bytes : lin_forward_plan(p).bytes;
+    return backward ? lin_backward_plan(p).bytes : lin_part_bytes(lin_forward_plan(p), p->rows, p->n);
 }
 
 int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream) {
     if (int e = lin_check(p, "linear_forward", false)) return e;
     if (p->rows == 0) return 0;
-    const ForwardPlan f = lin_forward_plan(p);
-    SRF_CHECK(f.bytes == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= f.bytes), "linear_forward: workspace of %lld bytes needed",
-              (long long)f.bytes);
+    const LinPlan plan = lin_forward_plan(p);
+    const int64_t need = lin_part_bytes(plan, p->rows, p->n);
+    SRF_CHECK(need == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= need), "linear_forward: workspace of %lld bytes needed",
+              (long long)need);
     const double m = (double)p->rows, es = lin_es(p->in_type), eo = lin_es(p->out_type);
     hipStream_t s = as_stream(stream);
     SrfLaunchScope ps(s, "linear_forward", 2 * m * p->n * p->k, es * (m * p->k + (double)p->n * p->k) + eo * m * p->n);
-    char* ws = (char*)p->workspace;
     LinArgs a = {};
     a.A = p->x; a.a_i = p->ldx; a.a_k = 1;
     a.B = p->w; a.b_j = p->ldw; a.b_k = 1;
-    a.M = (int)p->rows; a.N = p->n; a.K = p->k;
-    const int pitch = lin_pitch(p->k, (int)es);
-    if (f.pad_x) {
-        if (int e = lin_pad(p->x, p->ldx, p->rows, p->k, (int)es, ws + f.x, s)) return e;
-        a.A = ws + f.x; a.a_i = pitch;
-    }
-    if (f.pad_w) {
-        if (int e = lin_pad(p->w, p->ldw, p->n, p->k, (int)es, ws + f.w, s)) return e;
-        a.B = ws + f.w; a.b_j = pitch;
-    }
-    if (f.pad_x && f.pad_w) a.K = pitch;
+    a.M = (int)p->rows; a.N = p->n; a.K = plan.kind && p->padded ? lin_pitch(p->k, (int)es) : p->k;
     if (p->in_type == SCENERF_T_E4M3) { a.row_scale = p->x_scale; a.col_scale = p->w_scale; }
     a.bias = p->bias; a.residual = p->residual; a.ld_residual = p->ld_residual;
     a.out = p->y; a.z = p->z; a.act = p->activation;
-    return lin_product(p->in_type, p->out_type, a, f.product, ws + f.sums, s);
+    return lin_product(p->in_type, p->out_type, a, plan, p->workspace, s);
 }
 
 int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream) {
@@ -541,21 +526,10 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         if (int e = launch_sum_parts(p->out_type, part, b.strips, p->n, p->db, s)) return e;
     }
     const int pitch = lin_pitch(p->k, (int)es);
-    const void* x = p->x;
-    const void* w = p->w;
-    long ldx = p->ldx, ldw = p->ldw;
-    if (b.pad_w) {
-        if (int e = lin_pad(p->w, p->ldw, p->n, p->k, (int)es, ws + b.w, s)) return e;
-        w = ws + b.w; ldw = pitch;
-    }
-    if (b.pad_x) {
-        if (int e = lin_pad(p->x, p->ldx, p->rows, p->k, (int)es, ws + b.x, s)) return e;
-        x = ws + b.x; ldx = pitch;
-    }
     if (p->dx && p->rows > 0) {
         LinArgs a = {};
         a.A = dz; a.a_i = ld_dz; a.a_k = 1;
-        a.B = w; a.b_j = 1; a.b_k = ldw;
+        a.B = p->w; a.b_j = 1; a.b_k = p->ldw;
         a.M = (int)p->rows; a.N = p->k; a.K = p->n;
         a.b_ext = pitch;
         a.out = p->dx;
@@ -564,7 +538,7 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
     if (p->dw) {     // rows == 0: an empty sum, zeros
         LinArgs a = {};
         a.A = dz; a.a_i = 1; a.a_k = ld_dz;
-        a.B = x; a.b_j = 1; a.b_k = ldx;
+        a.B = p->x; a.b_j = 1; a.b_k = p->ldx;
         a.M = p->n; a.N = p->k; a.K = (int)p->rows;
         a.a_ext = b.make_dz ? b.dz_pitch : p->n; a.b_ext = pitch;
         a.out = p->dw;

@@ -336,8 +336,8 @@ template <typename T, typename O, bool AX, bool BX> static int lin_tile_pick(con
             if constexpr (T::code != SCENERF_T_F32) return lin_tile_launch<T, O, AX, BX, 256, 256, 2, 4, 3, 2>(a, s);
             break;
         case LIN_128x128: return lin_tile_launch<T, O, AX, BX, 128, 128, 2, 2, 3, 2>(a, s);
+        case LIN_64x64: return lin_tile_launch<T, O, AX, BX, 64, 64, 2, 2, 3, 3>(a, s);
         case LIN_128x32: return lin_tile_launch<T, O, AX, BX, 128, 32, 4, 1, 3, 3>(a, s);
-        case LIN_32x128: return lin_tile_launch<T, O, AX, BX, 32, 128, 1, 4, 3, 3>(a, s);
         default: break;
     }
     srf_set_error("linear: no such tile for this type");

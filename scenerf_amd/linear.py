@@ -13,6 +13,7 @@ free.  CUDA tensors only: anything else raises, there is no fallback.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import Optional, Tuple
 
 import torch
@@ -45,31 +46,45 @@ def _check_shapes(what, x, weight, bias, residual):
     return shape
 
 
-def _forward(what, x2, w2, bias, residual, shape, in_type, out_dtype, act, keep_z, scales=None):
-    (n, k), rows, dev = w2.shape, x2.shape[0], x2.device
+def _in_pieces(x2: torch.Tensor, w2: torch.Tensor):
+    """(x, w, padded): the two as the kernels read them fast, 16 bytes at a time -- as they are, or both copied with zeros behind each row."""
+    es = x2.element_size()
+    if not (w2.shape[1] * es % 16 or x2.stride(0) * es % 16 or w2.stride(0) * es % 16 or x2.data_ptr() % 16 or w2.data_ptr() % 16):
+        return x2, w2, 0
+    (n, k), rows, dev, dtype = w2.shape, x2.shape[0], x2.device, x2.dtype
+    pitch = -(-k * es // 16) * 16 // es
+    xp, wp = torch.empty((rows, pitch), dtype=dtype, device=dev), torch.empty((n, pitch), dtype=dtype, device=dev)
+    run_on(dev, _capi.load().scenerf_hip_linear_pad, (_capi.T_E4M3 if es == 1 else TYPE_CODES[dtype], k, x2.data_ptr() or None, x2.stride(0), rows,
+                                                      xp.data_ptr() or None, w2.data_ptr(), w2.stride(0), n, wp.data_ptr()), "linear (padding)")
+    return xp, wp, 1
+
+
+def _forward(what, x2, w2, padded, n, k, bias, residual, shape, in_type, out_dtype, act, keep_z, scales=None):
+    rows, dev = x2.shape[0], x2.device
     y = torch.empty(shape, dtype=out_dtype, device=dev)
     z = torch.empty((rows, n), dtype=out_dtype, device=dev) if keep_z else None
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     r = rows_of(residual, n) if residual is not None else None
-    p = _capi.Linear(in_type, TYPE_CODES[out_dtype], act, n, k, rows, x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0),
+    p = _capi.Linear(in_type, TYPE_CODES[out_dtype], act, n, k, padded, rows, x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0),
                      None if scales is None else scales[0].data_ptr(), None if scales is None else scales[1].data_ptr(),
                      None if bias is None else bias.data_ptr(), None if r is None else r.data_ptr(), 0 if r is None else r.stride(0),
                      y.data_ptr(), None if z is None else z.data_ptr())
     lib = _capi.load()
     ws = give_workspace(lib.scenerf_hip_linear_workspace, p, 0, dev, what)  # noqa: F841 (alive up to the launch)
-    run_on(dev, lib.scenerf_hip_linear_forward, p, what)
+    run_on(dev, lib.scenerf_hip_linear_forward, (C.byref(p),), what)
     return y, z
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, shape):
-        x2, w2 = rows_of(x, weight.shape[1]), rows_of(weight, weight.shape[1])
+        n, k = weight.shape
+        x2, w2, padded = _in_pieces(rows_of(x, k), rows_of(weight, k))
         keep_z = act != _capi.ACTIVATIONS["none"] and any(ctx.needs_input_grad[:3])
-        y, z = _forward("linear", x2, w2, bias, residual, shape, TYPE_CODES[x.dtype], x.dtype, act, keep_z)
+        y, z = _forward("linear", x2, w2, padded, n, k, bias, residual, shape, TYPE_CODES[x.dtype], x.dtype, act, keep_z)
         ctx.save_for_backward(x2, w2, z)
-        ctx.act, ctx.x_shape = act, x.shape
+        ctx.act, ctx.padded, ctx.x_shape, ctx.w_shape = act, padded, x.shape, (n, k)
         return y
 
     @staticmethod
@@ -77,18 +92,18 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         x2, w2, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dev, (n, k) = dy.device, w2.shape
+        dev, (n, k) = dy.device, ctx.w_shape
         dx = torch.empty(ctx.x_shape, dtype=x2.dtype, device=dev) if need_x else None
         dw = torch.empty((n, k), dtype=x2.dtype, device=dev) if need_w else None
         db = torch.empty((n,), dtype=x2.dtype, device=dev) if need_b else None
         if need_x or need_w or need_b:
             dy2 = rows_of(dy, n)
             code, lib = TYPE_CODES[x2.dtype], _capi.load()
-            p = _capi.Linear(code, code, ctx.act, n, k, x2.shape[0], x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), None, None, None,
+            p = _capi.Linear(code, code, ctx.act, n, k, ctx.padded, x2.shape[0], x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), None, None, None,
                              None, 0, None, None if z is None else z.data_ptr(), dy2.data_ptr(), dy2.stride(0), None if dx is None else dx.data_ptr(),
                              None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr())
             ws = give_workspace(lib.scenerf_hip_linear_workspace, p, 1, dev, "linear backward")  # noqa: F841
-            run_on(dev, lib.scenerf_hip_linear_backward, p, "linear backward")
+            run_on(dev, lib.scenerf_hip_linear_backward, (C.byref(p),), "linear backward")
         return dx, dw, db, (dy if need_r else None), None, None
 
 
@@ -107,8 +122,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act, shape)
-    k = weight.shape[1]
-    return _forward("linear", rows_of(x, k), rows_of(weight, k), bias, residual, shape, code, dtype, act, False)[0]
+    n, k = weight.shape
+    return _forward("linear", *_in_pieces(rows_of(x, k), rows_of(weight, k)), n, k, bias, residual, shape, code, dtype, act, False)[0]
 
 
 def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -127,8 +142,8 @@ def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
         raise ValueError("linear_8bit: x_scale must be %s and weight_scale (%d,) (got %s, %s)" % (
             tuple(x.shape[:-1]), weight.shape[0], tuple(x_scale.shape), tuple(weight_scale.shape)))
     no_gradient("linear_8bit", x_scale, weight_scale, bias, residual)
-    k = weight.shape[1]
-    return _forward("linear_8bit", rows_of(x, k), rows_of(weight, k), bias, residual, shape, _capi.T_E4M3, out_dtype, act, False,
+    n, k = weight.shape
+    return _forward("linear_8bit", *_in_pieces(rows_of(x, k), rows_of(weight, k)), n, k, bias, residual, shape, _capi.T_E4M3, out_dtype, act, False,
                     (x_scale.contiguous(), weight_scale.contiguous()))[0]
 
 

@@ -12,6 +12,7 @@ unrounded h).  CUDA tensors only: anything else raises, there is no fallback.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import Optional, Tuple, Union
 
 import torch
@@ -68,7 +69,7 @@ class _RmsNorm(torch.autograd.Function):
                       None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr())
         lib = _capi.load()
         ws = give_workspace(lib.scenerf_hip_rms_workspace, p, 1, dev, "rms_norm backward")  # noqa: F841 (alive up to the launch)
-        run_on(dev, lib.scenerf_hip_rms_backward, p, "rms_norm backward")
+        run_on(dev, lib.scenerf_hip_rms_backward, (C.byref(p),), "rms_norm backward")
         return (dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.has_residual and ctx.needs_input_grad[2] else None, None)
 
 

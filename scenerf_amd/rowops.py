@@ -38,15 +38,15 @@ def check_float(what: str, name: str, dtype: torch.dtype) -> int:
     return code
 
 
-def run_on(dev: torch.device, fn, args, what: str) -> None:
-    """``fn(args, stream)`` on ``dev``'s current stream, with ``dev`` current."""
+def run_on(dev: torch.device, fn, args: tuple, what: str) -> None:
+    """``fn(*args, stream)`` on ``dev``'s current stream, with ``dev`` current."""
     index = dev.index
     if index == torch.cuda.current_device():
         # (torch.cuda.current_stream(dev).cuda_stream without the Stream object: a fifth of a small call's host time)
-        rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _capi.check(rc, what)
 
@@ -87,5 +87,5 @@ def rows_forward(what, x, weight, residual, eps, *, quantize=False, keep_rstd=Fa
                   0 if r2 is None else r2.stride(0), None if weight is None else weight.data_ptr(), None if h is None else h.data_ptr(),
                   None if quantize else out.data_ptr(), out.data_ptr() if quantize else None, None if scale is None else scale.data_ptr(),
                   None if rstd is None else rstd.data_ptr())
-    run_on(dev, _capi.load().scenerf_hip_rms_forward, p, what)
+    run_on(dev, _capi.load().scenerf_hip_rms_forward, (C.byref(p),), what)
     return out, scale, h, rstd, x2
