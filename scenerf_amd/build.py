@@ -20,6 +20,8 @@ SOURCES = ["runtime.hip", "rays.hip", "gemm.hip", "wgrad.hip", "fused.hip", "wid
 # wide.hip owns the whole accumulator file (a[0:255] by name in inline-asm MFMAs): the compiler must not park spilled VGPRs there
 # (a spill then shows up as scratch usage, which tools/asmcheck.sh and the build's resource check refuse)
 EXTRA = {"wide.hip": ["-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"]}
+# linear_tile.h's loads into LDS name m0 as clobbered, which the compiler calls a reserved register and warns about
+EXTRA.update({"linear_%s.hip" % t: ["-Wno-inline-asm"] for t in ("f32", "bf16", "f16", "e4m3")})
 HEADERS = ["common.h", "gemm.h", "fused.h", "sphere_exact.h", "rowops.h", "linear.h", "linear_tile.h", os.path.join("..", "..", "include", "scenerf_hip.h")]
 # no packed fp32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this chip now and then, without an error
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

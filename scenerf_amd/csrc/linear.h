@@ -13,7 +13,6 @@ struct LinArgs {
     void* out; void* z;                  // dense [M][N]
     float* part;                         // not NULL: the raw sums of split s go to part[s][M][N] instead
     int act, tiles_i, tiles_j, splits, k_split;     // k_split: contraction elements per split
-    int vec;                             // the epilogue may move 16 bytes at a time
 };
 
 __device__ static inline float act_any(int act, float v) {
@@ -37,21 +36,28 @@ template <typename O> __device__ static inline void epilogue_one(const LinArgs& 
     if (p.residual) v += O::to_f32(((const raw*)p.residual)[i * p.ld_residual + j]);
     ((raw*)p.out)[i * p.N + j] = O::from_f32(v);
 }
-// W = 16 / sizeof(O::raw) neighbouring elements, all inside the row, every address aligned to 16 bytes: what depends on the columns alone,
-// then one row's (its residual in hand)
-template <typename O, int W> struct EpilogueCols {
+// W = 16 / sizeof(O::raw) neighbouring elements, of which n are inside the row: what depends on the columns alone, then one row's (its
+// residual in hand)
+template <typename O, int W, bool WHOLE> struct EpilogueCols {
     float bias[W], scale[W];
-    __device__ inline void load(const LinArgs& p, int j) {
+    __device__ inline void load(const LinArgs& p, int j, int n) {
 #pragma unroll
         for (int e = 0; e < W; ++e) bias[e] = 0.f;
-        if (p.bias) load_vec<O, W>((const typename O::raw*)p.bias + j, bias);
-        if (p.row_scale) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) scale[e] = p.col_scale[j + e];
-        }
+        if (p.bias) load_some<O, W, WHOLE>((const typename O::raw*)p.bias + j, n, bias);
+        if (p.row_scale) load_some<TypeF32, W, WHOLE>(p.col_scale + j, n, scale);
     }
 };
-template <typename O, int W> __device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<O, W>& ec, long i, int j, uint4 res, float (&v)[W]) {
+template <typename O, int W, bool WHOLE> __device__ static inline uint4 residual_piece(const LinArgs& p, long i, int j, int n) {
+    typedef typename O::raw raw;
+    const raw* at = (const raw*)p.residual + i * p.ld_residual + j;
+    if (WHOLE || n >= W) return load16(at);
+    union { raw e[W]; uint4 v; } u;
+#pragma unroll
+    for (int e = 0; e < W; ++e) u.e[e] = e < n ? at[e] : (raw)0;
+    return u.v;
+}
+template <typename O, int W, bool WHOLE>
+__device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<O, W, WHOLE>& ec, long i, int j, int n, uint4 res, float (&v)[W]) {
     typedef typename O::raw raw;
     if (p.row_scale) {
         const float s = p.row_scale[i];
@@ -64,7 +70,7 @@ template <typename O, int W> __device__ static inline void epilogue_vec(const Li
         float t[W];
 #pragma unroll
         for (int e = 0; e < W; ++e) t[e] = keep_z<O>(v[e]);
-        store_vec<O, W>((raw*)p.z + i * p.N + j, t);
+        store_some<O, W, WHOLE>((raw*)p.z + i * p.N + j, n, t);
     }
     if (p.act != SCENERF_ACT_NONE) {
         if (p.act == SCENERF_ACT_RELU) {
@@ -84,7 +90,7 @@ template <typename O, int W> __device__ static inline void epilogue_vec(const Li
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] += t[e];
     }
-    store_vec<O, W>((raw*)p.out + i * p.N + j, v);
+    store_some<O, W, WHOLE>((raw*)p.out + i * p.N + j, n, v);
 }
 
 // Tile shapes of the staged kernel (linear_tile.h): rows x columns of the result per workgroup

@@ -91,21 +91,23 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
 }
 // the splits' sums, added in a fixed order, then the epilogue: a workgroup owns 32 pieces of W results, 8 threads each, thread y of them
 // adds splits y, y + 8, ..
-template <typename O, bool VEC> __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs p) {
-    constexpr int W = VEC ? 16 / (int)sizeof(typename O::raw) : 1;
+template <typename O> __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs p) {
+    constexpr int W = 16 / (int)sizeof(typename O::raw);
     __shared__ float red[8][32][W + 1];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const size_t total = (size_t)p.M * p.N;
-    for (size_t t0 = (size_t)blockIdx.x * 32 * W; t0 < total; t0 += (size_t)gridDim.x * 32 * W) {
-        const size_t t = t0 + tx * W;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, per = (p.N + W - 1) / W;
+    const long pieces = (long)p.M * per;
+    for (long t0 = (long)blockIdx.x * 32; t0 < pieces; t0 += (long)gridDim.x * 32) {
+        const long i = (t0 + tx) / per;
+        const int j = (int)((t0 + tx) - i * per) * W;
+        const bool ok = t0 + tx < pieces;
         float v[W];
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] = 0.f;
-        if (t < total) {
+        if (ok) {
 #pragma unroll 4
             for (int s = ty; s < p.splits; s += 8) {
                 float u[W];
-                load_vec<TypeF32, W>(p.part + s * total + t, u);
+                load_some<TypeF32, W>(p.part + ((size_t)s * p.M + i) * p.N + j, p.N - j, u);
 #pragma unroll
                 for (int e = 0; e < W; ++e) v[e] += u[e];
             }
@@ -114,24 +116,18 @@ template <typename O, bool VEC> __global__ __launch_bounds__(256) void linear_jo
 #pragma unroll
         for (int e = 0; e < W; ++e) red[ty][tx][e] = v[e];
         __syncthreads();
-        if (ty == 0 && t < total) {
+        if (ty == 0 && ok) {
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 v[e] = 0.f;
 #pragma unroll
                 for (int y = 0; y < 8; ++y) v[e] += red[y][tx][e];
             }
-            const long i = (long)(t / p.N);
-            const int j = (int)(t % p.N);
-            if constexpr (VEC) {
-                EpilogueCols<O, W> ec;
-                ec.load(p, j);
-                uint4 res = make_uint4(0, 0, 0, 0);
-                if (p.residual) res = *(const uint4*)((const typename O::raw*)p.residual + i * p.ld_residual + j);
-                epilogue_vec<O, W>(p, ec, i, j, res, v);
-            } else {
-                epilogue_one<O>(p, i, j, v[0]);
-            }
+            EpilogueCols<O, W, false> ec;
+            ec.load(p, j, p.N - j);
+            uint4 res = make_uint4(0, 0, 0, 0);
+            if (p.residual) res = residual_piece<O, W, false>(p, i, j, p.N - j);
+            epilogue_vec<O, W, false>(p, ec, i, j, p.N - j, res, v);
         }
     }
 }
@@ -148,7 +144,7 @@ __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs p) {
     __shared__ float red[4][FEW_COLS * MR];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int j0 = (KW == 1 ? blockIdx.x * 4 + wv : blockIdx.x) * FEW_COLS;
-    const int pieces = p.K / W;
+    const int pieces = (p.K + W - 1) / W;
     float acc[FEW_COLS][MR];
 #pragma unroll
     for (int c = 0; c < FEW_COLS; ++c)
@@ -159,10 +155,18 @@ __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs p) {
     for (int c = 0; c < FEW_COLS; ++c) wrow[c] = (const raw*)p.B + (long)min(j0 + c, p.N - 1) * p.b_j;
     for (int t = KW == 1 ? lane : (int)threadIdx.x; t < pieces; t += 64 * KW) {
         uint4 w[FEW_COLS], x[MR];
+        const bool whole = t * W + W <= p.K;
+        auto piece = [&](const raw* at) -> uint4 {
+            if (whole) return load16(at);
+            union { raw e[W]; uint4 v; } u;          // the row's last elements, zeros behind them
 #pragma unroll
-        for (int c = 0; c < FEW_COLS; ++c) w[c] = *(const uint4*)(wrow[c] + t * W);
+            for (int e = 0; e < W; ++e) u.e[e] = t * W + e < p.K ? at[e] : (raw)0;
+            return u.v;
+        };
 #pragma unroll
-        for (int m = 0; m < MR; ++m) x[m] = *(const uint4*)((const raw*)p.A + (long)min(m, p.M - 1) * p.a_i + t * W);
+        for (int c = 0; c < FEW_COLS; ++c) w[c] = piece(wrow[c] + t * W);
+#pragma unroll
+        for (int m = 0; m < MR; ++m) x[m] = piece((const raw*)p.A + (long)min(m, p.M - 1) * p.a_i + t * W);
 #pragma unroll
         for (int m = 0; m < MR; ++m) {
             float xv[W];
@@ -219,7 +223,7 @@ template <typename O, int ACT> __device__ static inline void slopes(float (&g)[8
 }
 // A workgroup's 256 threads stand as 2^lx columns of 8 by 256 / 2^lx rows (2^lx: 32, or what a narrower matrix needs: at 128 columns a
 // fixed 32 left half the threads idle, 150 us for 262,144 x 128 fp32); two rows a thread are in flight.
-template <typename O, bool VEC>
+template <typename O, bool WHOLE>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld_dy, const void* z_, void* dz_, int pitch, float* part, int M, int N,
                                                         int act, int strip, int lx) {
     typedef typename O::raw raw;
@@ -230,14 +234,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld
     float sum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-    auto get = [&](const raw* p, float (&v)[8]) {
-        if constexpr (VEC) {
-            load_vec<O, 8>(p, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = j0 + e < N ? O::to_f32(p[e]) : 0.f;
-        }
-    };
+    auto get = [&](const raw* p, float (&v)[8]) { load_some<O, 8, WHOLE>(p, N - j0, v); };
     if (j0 < N) {
         for (long r = r0 + ty; r < r1; r += 2 * rows) {
             const bool two = r + rows < r1;
@@ -288,7 +285,7 @@ struct LinPlan {
 static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, long K) {
     LinPlan r = {0, 1, 0, LIN_128x128};
     const int bk = staged ? LIN_CHUNK_BYTES / lin_es(type) : ANY_K;
-    if (staged && !ax && !bx && M <= 8) {
+    if (!ax && !bx && M <= 8) {
         r.kind = 1;
         return r;
     }
@@ -323,7 +320,7 @@ static int64_t lin_part_bytes(const LinPlan& p, long M, int N) { return p.splits
 
 template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, hipStream_t s) {
     // K over one wave up to 128 pieces a row, over four beyond: measured at one row of bf16 (see DESIGN.md's table)
-    if (a.K / (16 / (int)sizeof(typename T::raw)) <= 128) linear_few_kernel<T, O, MR, 1><<<cdiv(a.N, 4 * FEW_COLS), 256, 0, s>>>(a);
+    if (a.K <= 128 * (16 / (int)sizeof(typename T::raw))) linear_few_kernel<T, O, MR, 1><<<cdiv(a.N, 4 * FEW_COLS), 256, 0, s>>>(a);
     else linear_few_kernel<T, O, MR, 4><<<cdiv(a.N, FEW_COLS), 256, 0, s>>>(a);
 }
 template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& plan, void* ws, hipStream_t s) {
@@ -331,8 +328,6 @@ template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& p
     a.k_split = plan.k_split;
     a.part = plan.splits > 1 ? (float*)ws : nullptr;
     constexpr int W = 16 / (int)sizeof(typename O::raw);
-    a.vec = a.N % W == 0 && aligned16(a.out) && (!a.z || aligned16(a.z)) && (!a.bias || aligned16(a.bias)) &&
-            (!a.residual || (aligned16(a.residual) && a.ld_residual % W == 0));
     if (plan.kind == 1) {
         if (a.M == 1) lin_few<T, O, 1>(a, s);
         else if (a.M == 2) lin_few<T, O, 2>(a, s);
@@ -358,10 +353,8 @@ template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& p
         SRF_LAUNCH_CHECK("linear_any_kernel");
     }
     if (plan.splits > 1) {
-        const size_t work = ((size_t)a.M * a.N / (a.vec ? W : 1) + 31) / 32;
-        const unsigned blocks = work < 16384 ? (unsigned)work : 16384;
-        if (a.vec) linear_join_kernel<O, true><<<blocks, 256, 0, s>>>(a);
-        else linear_join_kernel<O, false><<<blocks, 256, 0, s>>>(a);
+        const long work = ((long)a.M * ((a.N + W - 1) / W) + 31) / 32;
+        linear_join_kernel<O><<<(unsigned)(work < 16384 ? work : 16384), 256, 0, s>>>(a);
         SRF_LAUNCH_CHECK("linear_join_kernel");
     }
     return 0;
@@ -445,12 +438,11 @@ static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
     return 0;
 }
 template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardPlan& b, void* dz, float* part, hipStream_t s) {
-    const bool vec = p->n % 8 == 0 && p->ld_dy % 8 == 0 && aligned16(p->dy) && (p->activation == SCENERF_ACT_NONE || aligned16(p->z));
     int lx = 2;
     while (lx < 5 && (8 << lx) < p->n) ++lx;
     const dim3 grid(b.strips, cdiv(p->n, 8 << lx));
     SRF_CHECK(grid.y <= 65535, "linear_backward: n is too large");
-    if (vec) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
+    if (p->n % 8 == 0) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
     else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
     SRF_LAUNCH_CHECK("linear_dz_kernel");
     return 0;
@@ -496,7 +488,7 @@ int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream)
     LinArgs a = {};
     a.A = p->x; a.a_i = p->ldx; a.a_k = 1;
     a.B = p->w; a.b_j = p->ldw; a.b_k = 1;
-    a.M = (int)p->rows; a.N = p->n; a.K = plan.kind && p->padded ? lin_pitch(p->k, (int)es) : p->k;
+    a.M = (int)p->rows; a.N = p->n; a.K = plan.kind == 2 && p->padded ? lin_pitch(p->k, (int)es) : p->k;
     if (p->in_type == SCENERF_T_E4M3) { a.row_scale = p->x_scale; a.col_scale = p->w_scale; }
     a.bias = p->bias; a.residual = p->residual; a.ld_residual = p->ld_residual;
     a.out = p->y; a.z = p->z; a.act = p->activation;

@@ -27,7 +27,8 @@ __device__ __attribute__((aligned(16))) const unsigned lin_zeros[4] = {0, 0, 0, 
 
 template <bool V> struct Bool { static constexpr bool value = V; };
 
-// 64 lanes x 16 bytes, global -> LDS at lds_base + lane * 16 (m0 is the base)
+// 64 lanes x 16 bytes, global -> LDS at lds_base + lane * 16.  (m0 is the base.  Nothing else in these kernels reads it; saving and
+// restoring it around every load cost 5 to 10 percent of a call.)
 __device__ static inline void lin_copy(const void* src, unsigned lds_base) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_base) : "memory", "m0");
 }
@@ -63,9 +64,8 @@ template <typename T, bool ACROSS, int TILE> struct LinSide {
     }
 };
 
-template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB>
+template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB, bool WHOLE>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
-    typedef typename T::raw raw;
     typedef LinSide<T, AX, BM> SA;
     typedef LinSide<T, BX, BN> SB;
     constexpr int ES = SA::ES, BK = SA::BK, WAVES = WM * WN;
@@ -259,38 +259,44 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     // ---- results: 32 rows of the wave at a time through a slab of [32][BN / WN] floats (rows 16 bytes apart in the banks)
     constexpr int WCOLS = BN / WN, PITCH = WCOLS + 4, W = 16 / (int)sizeof(typename O::raw), LANES_ROW = WCOLS / W, ROWS_PASS = 64 / LANES_ROW;
     static_assert(WAVES * 32 * PITCH * 4 <= NSA * SA::BYTES + NSB * SB::BYTES, "the slabs fit the rings");
-    typedef typename O::raw oraw;
     float* slab = (float*)lds + wv * 32 * PITCH;
     // (a lane's columns are the same in every row: their bias and scales are read once; the residual of the next 32 rows is under way
     // while these leave, which a load per row and its wait cost 8 us a tile)
     constexpr int PASSES = 32 / ROWS_PASS;
     const int c = (lane % LANES_ROW) * W, col = j0 + wj + c, lrow = lane / LANES_ROW;
-    const bool vec = !p.part && p.vec, in_col = col < p.N;
-    EpilogueCols<O, W> ec;
-    uint4 res[PASSES];
-    auto residual = [&](int i) {
+    const int in = p.N - col;
+    // (WHOLE: no lane's piece reaches over the row's end)
+    {
+        EpilogueCols<O, W, WHOLE> ec;
+        uint4 res[PASSES];
+        auto residual = [&](int i) {
 #pragma unroll
-        for (int t = 0; t < PASSES; ++t) {
-            const long row = i0 + wi + i * 32 + lrow + t * ROWS_PASS;
-            if (row < p.M) res[t] = *(const uint4*)((const oraw*)p.residual + row * p.ld_residual + col);
+            for (int t = 0; t < PASSES; ++t) {
+                const long row = i0 + wi + i * 32 + lrow + t * ROWS_PASS;
+                if (row < p.M) res[t] = residual_piece<O, W, WHOLE>(p, row, col, in);
+            }
+        };
+        if (!p.part && in > 0) {
+            ec.load(p, col, in);
+            if (p.residual) residual(0);
         }
-    };
-    if (vec && in_col) {
-        ec.load(p, col);
-        if (p.residual) residual(0);
-    }
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
+        for (int i = 0; i < I; ++i) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+            for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                *(float4*)(slab + l31 * PITCH + j * 32 + 8 * e + 4 * h) =
-                    make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
-        wave_sync();
-        const long row0 = i0 + wi + i * 32;
-        if (vec) {
-            if (in_col) {
+                for (int e = 0; e < 4; ++e)
+                    *(float4*)(slab + l31 * PITCH + j * 32 + 8 * e + 4 * h) =
+                        make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
+            wave_sync();
+            const long row0 = i0 + wi + i * 32;
+            if (p.part) {
+                float* part = p.part + (size_t)split * p.M * p.N;
+#pragma unroll 4
+                for (int r = 0; r < 32; ++r)
+                    for (int k = lane; k < WCOLS; k += 64)
+                        if (row0 + r < p.M && j0 + wj + k < p.N) part[(size_t)(row0 + r) * p.N + j0 + wj + k] = slab[r * PITCH + k];
+            } else if (in > 0) {
                 uint4 now[PASSES];
 #pragma unroll
                 for (int t = 0; t < PASSES; ++t) now[t] = res[t];
@@ -304,31 +310,28 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
                         const float4 q = *(const float4*)(slab + r * PITCH + c + e);
                         v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
                     }
-                    if (row0 + r < p.M) epilogue_vec<O, W>(p, ec, row0 + r, col, now[t], v);
+                    if (row0 + r < p.M) epilogue_vec<O, W, WHOLE>(p, ec, row0 + r, col, in, now[t], v);
                 }
             }
-        } else {
-            float* part = p.part ? p.part + (size_t)split * p.M * p.N : nullptr;
-            for (int r = 0; r < 32; ++r)
-                for (int k = lane; k < WCOLS; k += 64)
-                    if (row0 + r < p.M && j0 + wj + k < p.N) {
-                        if (part) part[(size_t)(row0 + r) * p.N + j0 + wj + k] = slab[r * PITCH + k];
-                        else epilogue_one<O>(p, row0 + r, j0 + wj + k, slab[r * PITCH + k]);
-                    }
+            wave_sync();
         }
-        wave_sync();
     }
 }
 
-template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB> static int lin_tile_launch(const LinArgs& a, hipStream_t s) {
+template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB, bool WHOLE>
+static int lin_tile_start(const LinArgs& a, hipStream_t s) {
     constexpr int LDS = (NSA * BM + NSB * BN) * LIN_CHUNK_BYTES;
-    auto kernel = linear_tile_kernel<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB>;
+    auto kernel = linear_tile_kernel<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB, WHOLE>;
     SRF_ONCE_PER_DEVICE(SRF_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS)));
     const long blocks = (long)a.tiles_i * a.tiles_j * a.splits;
     SRF_CHECK(blocks <= ROWOPS_GRID_MAX, "linear: %ld tiles are more than one launch holds", blocks);
     kernel<<<(unsigned)blocks, 64 * WM * WN, LDS, s>>>(a);
     SRF_LAUNCH_CHECK("linear_tile_kernel");
     return 0;
+}
+template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB> static int lin_tile_launch(const LinArgs& a, hipStream_t s) {
+    if (a.N % (16 / (int)sizeof(typename O::raw)) == 0) return lin_tile_start<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB, true>(a, s);
+    return lin_tile_start<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB, false>(a, s);
 }
 template <typename T, typename O, bool AX, bool BX> static int lin_tile_pick(const LinArgs& a, LinTile tile, hipStream_t s) {
     switch (tile) {

@@ -7,7 +7,8 @@
 // wave owns a row (the two row sums are one 6-step exchange, no barrier), holds it in registers up to ROW_REGS elements a lane, and
 // walks the rows in a grid stride, so that the weight is loaded once per wave.  Wider rows go through a workgroup that reads the row
 // twice (the second time from L2).  The weight's gradient is summed per lane over the wave's rows, then over the workgroup's waves in
-// LDS, then over the workgroups by a second kernel in a fixed order: no atomics, the same bits every time.
+// LDS, then over the workgroups by a second kernel in a fixed order: no atomics, the same bits every time.  Rows of any length and
+// alignment move 16 bytes at a time, but for a last piece that the row does not fill.
 #include "rowops.h"
 
 #define ROW_WAVES 4
@@ -40,20 +41,20 @@ struct RmsArgs {
 };
 
 // C chunks of 64 * VW columns: lane l holds columns c * 64 * VW + l * VW ..+ VW
-template <typename E, int VW, int C>
+template <typename E, int VW, int C, bool WHOLE>
 __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
     typedef typename E::raw raw;
     const int lane = threadIdx.x & 63;
     const int D = p.width;
     float w[C][VW];
-    bool in[C];
+    int in[C];          // elements of the lane's pieces that are inside the row
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int col = (c * 64 + lane) * VW;
-        in[c] = col < D;
+        in[c] = D - col;
 #pragma unroll
         for (int e = 0; e < VW; ++e) w[c][e] = 0.f;
-        if (in[c] && p.weight) load_vec<E, VW>((const raw*)p.weight + col, w[c]);
+        if (in[c] > 0 && p.weight) load_some<E, VW, WHOLE>((const raw*)p.weight + col, in[c], w[c]);
     }
     const int waves = gridDim.x * ROW_WAVES;
     for (long row = (long)blockIdx.x * ROW_WAVES + (threadIdx.x >> 6); row < p.rows; row += waves) {
@@ -64,18 +65,18 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
             const int col = (c * 64 + lane) * VW;
 #pragma unroll
             for (int e = 0; e < VW; ++e) h[c][e] = 0.f;
-            if (in[c]) load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h[c]);
+            if (in[c] > 0) load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, in[c], h[c]);
         }
         if (p.residual) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int col = (c * 64 + lane) * VW;
-                if (in[c]) {
+                if (in[c] > 0) {
                     float r[VW];
-                    load_vec<E, VW>((const raw*)p.residual + row * p.ld_residual + col, r);
+                    load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, in[c], r);
 #pragma unroll
                     for (int e = 0; e < VW; ++e) h[c][e] += r[e];
-                    if (p.h) store_vec<E, VW>((raw*)p.h + row * D + col, h[c]);
+                    if (p.h) store_some<E, VW, WHOLE>((raw*)p.h + row * D + col, in[c], h[c]);
                 }
             }
         }
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
         if (p.y) {
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                if (in[c]) store_vec<E, VW>((raw*)p.y + row * D + (c * 64 + lane) * VW, h[c]);
+                if (in[c] > 0) store_some<E, VW, WHOLE>((raw*)p.y + row * D + (c * 64 + lane) * VW, in[c], h[c]);
         }
         if (p.q) {
             uint32_t m = 0;
@@ -103,18 +104,18 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int e = 0; e < VW; ++e) {
-                    const uint32_t b = in[c] ? abs_bits(h[c][e]) : 0u;      // (columns past the row hold 0 * rstd: NaN in a NaN row only)
+                    const uint32_t b = (WHOLE ? in[c] > 0 : e < in[c]) ? abs_bits(h[c][e]) : 0u;
                     m = b > m ? b : m;
                 }
             const float s = row_scale(wave_max_u32(m)), inv = 1.f / s;
             if (lane == 0) p.scale[row] = s;
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                if (in[c]) {
+                if (in[c] > 0) {
                     float v[VW];
 #pragma unroll
                     for (int e = 0; e < VW; ++e) v[e] = h[c][e] * inv;
-                    store_vec<TypeE4M3, VW>(p.q + row * D + (c * 64 + lane) * VW, v);
+                    store_some<TypeE4M3, VW, WHOLE>(p.q + row * D + (c * 64 + lane) * VW, in[c], v);
                 }
         }
     }
@@ -139,7 +140,7 @@ __device__ static inline uint32_t block_max_u32(uint32_t v, uint32_t* red) {
     for (int i = 0; i < WIDE_THREADS / 64; ++i) v = red[i] > v ? red[i] : v;
     return v;
 }
-template <typename E, int VW>
+template <typename E, int VW, bool WHOLE>
 __global__ __launch_bounds__(WIDE_THREADS) void rms_rows_wide_kernel(RmsArgs p) {
     typedef typename E::raw raw;
     __shared__ float red[WIDE_THREADS / 64];
@@ -149,18 +150,18 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_rows_wide_kernel(RmsArgs p) 
         uint32_t m = 0;
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW];
-            load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h);
+            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), h);
             if (p.residual) {
                 float r[VW];
-                load_vec<E, VW>((const raw*)p.residual + row * p.ld_residual + col, r);
+                load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, (int)min(D - col, (long)VW), r);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) h[e] += r[e];
-                if (p.h) store_vec<E, VW>((raw*)p.h + row * D + col, h);
+                if (p.h) store_some<E, VW, WHOLE>((raw*)p.h + row * D + col, (int)min(D - col, (long)VW), h);
             }
             float w[VW];
 #pragma unroll
             for (int e = 0; e < VW; ++e) w[e] = 1.f;
-            if (p.weight) load_vec<E, VW>((const raw*)p.weight + col, w);
+            if (p.weight) load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), w);
 #pragma unroll
             for (int e = 0; e < VW; ++e) {
                 ss = fmaf(h[e], h[e], ss);
@@ -182,45 +183,45 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_rows_wide_kernel(RmsArgs p) 
         }
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW];
-            load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h);
+            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), h);
             if (p.residual) {
                 float r[VW];
-                load_vec<E, VW>((const raw*)p.residual + row * p.ld_residual + col, r);
+                load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, (int)min(D - col, (long)VW), r);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) h[e] += r[e];
             }
             if (p.weight) {
                 float w[VW];
-                load_vec<E, VW>((const raw*)p.weight + col, w);
+                load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), w);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) h[e] = h[e] * rstd * w[e];
             }
-            if (p.y) store_vec<E, VW>((raw*)p.y + row * D + col, h);
+            if (p.y) store_some<E, VW, WHOLE>((raw*)p.y + row * D + col, (int)min(D - col, (long)VW), h);
             if (p.q) {
 #pragma unroll
                 for (int e = 0; e < VW; ++e) h[e] *= inv;
-                store_vec<TypeE4M3, VW>(p.q + row * D + col, h);
+                store_some<TypeE4M3, VW, WHOLE>(p.q + row * D + col, (int)min(D - col, (long)VW), h);
             }
         }
     }
 }
 
 // gradients: dx, and this workgroup's part of dweight in partial[blockIdx.x][width]
-template <typename E, int VW, int C>
+template <typename E, int VW, int C, bool WHOLE>
 __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
     typedef typename E::raw raw;
     __shared__ float red[ROW_WAVES][64 * VW];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int D = p.width;
     float w[C][VW], dw[C][VW];
-    bool in[C];
+    int in[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int col = (c * 64 + lane) * VW;
-        in[c] = col < D;
+        in[c] = D - col;
 #pragma unroll
         for (int e = 0; e < VW; ++e) w[c][e] = dw[c][e] = 0.f;
-        if (in[c]) load_vec<E, VW>((const raw*)p.weight + col, w[c]);
+        if (in[c] > 0) load_some<E, VW, WHOLE>((const raw*)p.weight + col, in[c], w[c]);
     }
     const int waves = gridDim.x * ROW_WAVES;
     // the next row's three loads are under way while this one is worked on (narrow rows: with one row at a time the 8 waves a CU had too
@@ -234,10 +235,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
             const int col = (c * 64 + lane) * VW;
 #pragma unroll
             for (int e = 0; e < VW; ++e) h[c][e] = g[c][e] = d[c][e] = 0.f;
-            if (in[c]) {
-                load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h[c]);
-                load_vec<E, VW>((const raw*)p.dy + row * p.ld_dy + col, g[c]);
-                if (AHEAD && p.dh) load_vec<E, VW>((const raw*)p.dh + row * p.ld_dh + col, d[c]);
+            if (in[c] > 0) {
+                load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, in[c], h[c]);
+                load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, in[c], g[c]);
+                if (AHEAD && p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, in[c], d[c]);
             }
         }
     };
@@ -273,12 +274,12 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
         dot = wave_sum(dot) * p.inv_width;
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (in[c]) {
+            if (in[c] > 0) {
                 const int col = (c * 64 + lane) * VW;
-                if (!AHEAD && p.dh) load_vec<E, VW>((const raw*)p.dh + row * p.ld_dh + col, d[c]);
+                if (!AHEAD && p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, in[c], d[c]);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) d[c][e] = fmaf(rstd, fmaf(-dot, h[c][e], g[c][e]), d[c][e]);
-                store_vec<E, VW>((raw*)p.dx + row * D + col, d[c]);
+                store_some<E, VW, WHOLE>((raw*)p.dx + row * D + col, in[c], d[c]);
             }
     }
     if (!p.partial) return;
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
         }
     }
 }
-template <typename E, int VW>
+template <typename E, int VW, bool WHOLE>
 __global__ __launch_bounds__(WIDE_THREADS) void rms_grad_wide_kernel(RmsArgs p) {
     typedef typename E::raw raw;
     __shared__ float red[WIDE_THREADS / 64];
@@ -309,24 +310,24 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_grad_wide_kernel(RmsArgs p) 
         float dot = 0.f;
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW], g[VW], w[VW];
-            load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h);
-            load_vec<E, VW>((const raw*)p.dy + row * p.ld_dy + col, g);
-            load_vec<E, VW>((const raw*)p.weight + col, w);
+            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), h);
+            load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, (int)min(D - col, (long)VW), g);
+            load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), w);
 #pragma unroll
             for (int e = 0; e < VW; ++e) dot = fmaf(g[e] * w[e], h[e] * rstd, dot);
         }
         dot = block_sum(dot, red) * p.inv_width;
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW], g[VW], w[VW], d[VW];
-            load_vec<E, VW>((const raw*)p.x + row * p.ldx + col, h);
-            load_vec<E, VW>((const raw*)p.dy + row * p.ld_dy + col, g);
-            load_vec<E, VW>((const raw*)p.weight + col, w);
+            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), h);
+            load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, (int)min(D - col, (long)VW), g);
+            load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), w);
 #pragma unroll
             for (int e = 0; e < VW; ++e) d[e] = 0.f;
-            if (p.dh) load_vec<E, VW>((const raw*)p.dh + row * p.ld_dh + col, d);
+            if (p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, (int)min(D - col, (long)VW), d);
 #pragma unroll
             for (int e = 0; e < VW; ++e) d[e] = fmaf(rstd, fmaf(-dot, h[e] * rstd, g[e] * w[e]), d[e]);
-            store_vec<E, VW>((raw*)p.dx + row * D + col, d);
+            store_some<E, VW, WHOLE>((raw*)p.dx + row * D + col, (int)min(D - col, (long)VW), d);
         }
     }
 }
@@ -377,17 +378,6 @@ int launch_sum_parts(int type, const float* part, int count, int width, void* ou
 // ---------------------------------------------------------------------------------------------------------------- host side
 static int rms_es(int type) { return type == SCENERF_T_F32 ? 4 : 2; }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-// 16-byte accesses need the row's length and every pitch in whole pieces, and aligned bases
-static bool rms_vector_ok(const scenerf_rms* p, bool backward) {
-    const int vw = 16 / rms_es(p->type);
-    if (p->width % vw || p->ldx % vw || !aligned16(p->x) || (p->weight && !aligned16(p->weight))) return false;
-    if (backward) {
-        if (p->ld_dy % vw || !aligned16(p->dy) || (p->dx && !aligned16(p->dx))) return false;
-        return !p->dh || (p->ld_dh % vw == 0 && aligned16(p->dh));
-    }
-    if (p->residual && (p->ld_residual % vw || !aligned16(p->residual))) return false;
-    return (!p->h || aligned16(p->h)) && (!p->y || aligned16(p->y)) && (!p->q || aligned16(p->q));
-}
 static bool rms_in_registers(const scenerf_rms* p) { return p->width <= 64 * ROW_REGS; }
 #define RMS_GRAD_BLOCKS 1024        // workgroups (and parts of dweight) of the gradient kernel: four per CU
 #define RMS_STRIP 512
@@ -424,41 +414,32 @@ static RmsArgs rms_args(const scenerf_rms* p) {
     return a;
 }
 
-template <typename E, int VW, int C> static void rms_launch(const RmsArgs& a, bool backward, int blocks, hipStream_t s) {
-    if (backward) rms_grad_kernel<E, VW, C><<<blocks, 64 * ROW_WAVES, 0, s>>>(a);
-    else rms_rows_kernel<E, VW, C><<<blocks, 64 * ROW_WAVES, 0, s>>>(a);
+template <typename E, int VW, int C, bool WHOLE> static void rms_launch(const RmsArgs& a, bool backward, int blocks, hipStream_t s) {
+    if (backward) rms_grad_kernel<E, VW, C, WHOLE><<<blocks, 64 * ROW_WAVES, 0, s>>>(a);
+    else rms_rows_kernel<E, VW, C, WHOLE><<<blocks, 64 * ROW_WAVES, 0, s>>>(a);
 }
 // the smallest number of chunks that holds the row
-template <typename E, int VW> static void rms_launch_chunks(const RmsArgs& a, bool backward, int blocks, hipStream_t s) {
+template <typename E, int VW, bool WHOLE> static void rms_launch_chunks(const RmsArgs& a, bool backward, int blocks, hipStream_t s) {
     const int chunks = cdiv(a.width, 64 * VW);
-    if (chunks <= 1) return rms_launch<E, VW, 1>(a, backward, blocks, s);
-    if (chunks <= 2) return rms_launch<E, VW, 2>(a, backward, blocks, s);
-    if (chunks <= 4) return rms_launch<E, VW, 4>(a, backward, blocks, s);
-    if (chunks <= 8) return rms_launch<E, VW, 8>(a, backward, blocks, s);
-    if constexpr (VW <= 4) {
-        if (chunks <= 16) return rms_launch<E, VW, 16>(a, backward, blocks, s);
-    }
-    if constexpr (VW == 1) {
-        if (chunks <= 32) return rms_launch<E, VW, 32>(a, backward, blocks, s);
-        rms_launch<E, VW, 64>(a, backward, blocks, s);
-    }
+    if (chunks <= 1) return rms_launch<E, VW, 1, WHOLE>(a, backward, blocks, s);
+    if (chunks <= 2) return rms_launch<E, VW, 2, WHOLE>(a, backward, blocks, s);
+    if (chunks <= 4) return rms_launch<E, VW, 4, WHOLE>(a, backward, blocks, s);
+    if (chunks <= 8) return rms_launch<E, VW, 8, WHOLE>(a, backward, blocks, s);
+    if constexpr (VW == 4) rms_launch<E, VW, 16, WHOLE>(a, backward, blocks, s);
 }
-template <typename E> static int rms_dispatch(const scenerf_rms* p, bool backward, hipStream_t s) {
+template <typename E, bool WHOLE> static int rms_dispatch(const scenerf_rms* p, bool backward, hipStream_t s) {
     constexpr int VW = 16 / sizeof(typename E::raw);
     RmsArgs a = rms_args(p);
-    const bool vec = rms_vector_ok(p, backward);
     if (backward) {
         const int parts = rms_grad_parts(p);
         a.partial = p->dweight ? (float*)p->workspace : nullptr;
         if (p->rows > 0 && rms_in_registers(p)) {
-            if (vec) rms_launch_chunks<E, VW>(a, true, parts, s);
-            else rms_launch_chunks<E, 1>(a, true, parts, s);
+            rms_launch_chunks<E, VW, WHOLE>(a, true, parts, s);
             SRF_LAUNCH_CHECK("rms_grad_kernel");
         } else if (p->rows > 0) {
             if (p->dx) {
                 const int blocks = p->rows < 4096 ? (int)p->rows : 4096;
-                if (vec) rms_grad_wide_kernel<E, VW><<<blocks, WIDE_THREADS, 0, s>>>(a);
-                else rms_grad_wide_kernel<E, 1><<<blocks, WIDE_THREADS, 0, s>>>(a);
+                rms_grad_wide_kernel<E, VW, WHOLE><<<blocks, WIDE_THREADS, 0, s>>>(a);
                 SRF_LAUNCH_CHECK("rms_grad_wide_kernel");
             }
             if (p->dweight) {
@@ -473,21 +454,22 @@ template <typename E> static int rms_dispatch(const scenerf_rms* p, bool backwar
     if (rms_in_registers(p)) {
         const long want = (p->rows + ROW_WAVES - 1) / ROW_WAVES;
         const int blocks = (int)(want < 8192 ? want : 8192);
-        if (vec) rms_launch_chunks<E, VW>(a, false, blocks, s);
-        else rms_launch_chunks<E, 1>(a, false, blocks, s);
+        rms_launch_chunks<E, VW, WHOLE>(a, false, blocks, s);
         SRF_LAUNCH_CHECK("rms_rows_kernel");
     } else {
         const int blocks = p->rows < 4096 ? (int)p->rows : 4096;
-        if (vec) rms_rows_wide_kernel<E, VW><<<blocks, WIDE_THREADS, 0, s>>>(a);
-        else rms_rows_wide_kernel<E, 1><<<blocks, WIDE_THREADS, 0, s>>>(a);
+        rms_rows_wide_kernel<E, VW, WHOLE><<<blocks, WIDE_THREADS, 0, s>>>(a);
         SRF_LAUNCH_CHECK("rms_rows_wide_kernel");
     }
     return 0;
 }
+template <typename E> static int rms_run_type(const scenerf_rms* p, bool backward, hipStream_t s) {
+    return p->width % (16 / (int)sizeof(typename E::raw)) == 0 ? rms_dispatch<E, true>(p, backward, s) : rms_dispatch<E, false>(p, backward, s);
+}
 static int rms_run(const scenerf_rms* p, bool backward, hipStream_t s) {
-    if (p->type == SCENERF_T_F32) return rms_dispatch<TypeF32>(p, backward, s);
-    if (p->type == SCENERF_T_BF16) return rms_dispatch<TypeBF16>(p, backward, s);
-    return rms_dispatch<TypeF16>(p, backward, s);
+    if (p->type == SCENERF_T_F32) return rms_run_type<TypeF32>(p, backward, s);
+    if (p->type == SCENERF_T_BF16) return rms_run_type<TypeBF16>(p, backward, s);
+    return rms_run_type<TypeF16>(p, backward, s);
 }
 
 extern "C" {

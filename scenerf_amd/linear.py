@@ -46,10 +46,11 @@ def _check_shapes(what, x, weight, bias, residual):
     return shape
 
 
-def _in_pieces(x2: torch.Tensor, w2: torch.Tensor):
-    """(x, w, padded): the two as the kernels read them fast, 16 bytes at a time -- as they are, or both copied with zeros behind each row."""
+def _in_pieces(x2: torch.Tensor, w2: torch.Tensor, back: bool = False):
+    """(x, w, padded): the two as the kernels read them fast, 16 bytes at a time -- as they are, or both copied with zeros behind each row.
+    Up to 8 rows are read from any address; the step ``back`` is not."""
     es = x2.element_size()
-    if not (w2.shape[1] * es % 16 or x2.stride(0) * es % 16 or w2.stride(0) * es % 16 or x2.data_ptr() % 16 or w2.data_ptr() % 16):
+    if (x2.shape[0] <= 8 and not back) or not (w2.shape[1] * es % 16 or x2.stride(0) * es % 16 or w2.stride(0) * es % 16 or x2.data_ptr() % 16 or w2.data_ptr() % 16):
         return x2, w2, 0
     (n, k), rows, dev, dtype = w2.shape, x2.shape[0], x2.device, x2.dtype
     pitch = -(-k * es // 16) * 16 // es
@@ -80,7 +81,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, shape):
         n, k = weight.shape
-        x2, w2, padded = _in_pieces(rows_of(x, k), rows_of(weight, k))
+        x2, w2, padded = _in_pieces(rows_of(x, k), rows_of(weight, k), True)
         keep_z = act != _capi.ACTIVATIONS["none"] and any(ctx.needs_input_grad[:3])
         y, z = _forward("linear", x2, w2, padded, n, k, bias, residual, shape, TYPE_CODES[x.dtype], x.dtype, act, keep_z)
         ctx.save_for_backward(x2, w2, z)
