@@ -43,18 +43,18 @@ template <typename O, int W, bool WHOLE> struct EpilogueCols {
     __device__ inline void load(const LinArgs& p, int j, int n) {
 #pragma unroll
         for (int e = 0; e < W; ++e) bias[e] = 0.f;
-        if (p.bias) load_some<O, W, WHOLE>((const typename O::raw*)p.bias + j, n, bias);
-        if (p.row_scale) load_some<TypeF32, W, WHOLE>(p.col_scale + j, n, scale);
+        if (p.bias) load_some<O, W, WHOLE>((const typename O::raw*)p.bias + j, n, p.N % W, bias);
+        if (p.row_scale) load_some<TypeF32, W, WHOLE>(p.col_scale + j, n, p.N % W, scale);
     }
 };
 template <typename O, int W, bool WHOLE> __device__ static inline uint4 residual_piece(const LinArgs& p, long i, int j, int n) {
     typedef typename O::raw raw;
     const raw* at = (const raw*)p.residual + i * p.ld_residual + j;
     if (WHOLE || n >= W) return load16(at);
-    union { raw e[W]; uint4 v; } u;
-#pragma unroll
-    for (int e = 0; e < W; ++e) u.e[e] = e < n ? at[e] : (raw)0;
-    return u.v;
+    float v[W];
+    load_some<O, W>(at, n, p.N % W, v);
+    if constexpr (sizeof(raw) == 4) return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    else return make_uint4(pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]), pack2<O>(v[4], v[5]), pack2<O>(v[6], v[7]));     // (exact)
 }
 template <typename O, int W, bool WHOLE>
 __device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<O, W, WHOLE>& ec, long i, int j, int n, uint4 res, float (&v)[W]) {
@@ -70,7 +70,7 @@ __device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<
         float t[W];
 #pragma unroll
         for (int e = 0; e < W; ++e) t[e] = keep_z<O>(v[e]);
-        store_some<O, W, WHOLE>((raw*)p.z + i * p.N + j, n, t);
+        store_some<O, W, WHOLE>((raw*)p.z + i * p.N + j, n, p.N % W, t);
     }
     if (p.act != SCENERF_ACT_NONE) {
         if (p.act == SCENERF_ACT_RELU) {
@@ -90,7 +90,7 @@ __device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] += t[e];
     }
-    store_some<O, W, WHOLE>((raw*)p.out + i * p.N + j, n, v);
+    store_some<O, W, WHOLE>((raw*)p.out + i * p.N + j, n, p.N % W, v);
 }
 
 // Tile shapes of the staged kernel (linear_tile.h): rows x columns of the result per workgroup

@@ -107,7 +107,7 @@ template <typename O> __global__ __launch_bounds__(256) void linear_join_kernel(
 #pragma unroll 4
             for (int s = ty; s < p.splits; s += 8) {
                 float u[W];
-                load_some<TypeF32, W>(p.part + ((size_t)s * p.M + i) * p.N + j, p.N - j, u);
+                load_some<TypeF32, W>(p.part + ((size_t)s * p.M + i) * p.N + j, p.N - j, p.N % W, u);
 #pragma unroll
                 for (int e = 0; e < W; ++e) v[e] += u[e];
             }
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld
     float sum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-    auto get = [&](const raw* p, float (&v)[8]) { load_some<O, 8, WHOLE>(p, N - j0, v); };
+    auto get = [&](const raw* p, float (&v)[8]) { load_some<O, 8, WHOLE>(p, N - j0, N % 8, v); };
     if (j0 < N) {
         for (long r = r0 + ty; r < r1; r += 2 * rows) {
             const bool two = r + rows < r1;

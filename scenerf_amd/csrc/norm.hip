@@ -54,7 +54,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
         in[c] = D - col;
 #pragma unroll
         for (int e = 0; e < VW; ++e) w[c][e] = 0.f;
-        if (in[c] > 0 && p.weight) load_some<E, VW, WHOLE>((const raw*)p.weight + col, in[c], w[c]);
+        if (in[c] > 0 && p.weight) load_some<E, VW, WHOLE>((const raw*)p.weight + col, in[c], D % VW, w[c]);
     }
     const int waves = gridDim.x * ROW_WAVES;
     for (long row = (long)blockIdx.x * ROW_WAVES + (threadIdx.x >> 6); row < p.rows; row += waves) {
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
             const int col = (c * 64 + lane) * VW;
 #pragma unroll
             for (int e = 0; e < VW; ++e) h[c][e] = 0.f;
-            if (in[c] > 0) load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, in[c], h[c]);
+            if (in[c] > 0) load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, in[c], D % VW, h[c]);
         }
         if (p.residual) {
 #pragma unroll
@@ -73,10 +73,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
                 const int col = (c * 64 + lane) * VW;
                 if (in[c] > 0) {
                     float r[VW];
-                    load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, in[c], r);
+                    load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, in[c], D % VW, r);
 #pragma unroll
                     for (int e = 0; e < VW; ++e) h[c][e] += r[e];
-                    if (p.h) store_some<E, VW, WHOLE>((raw*)p.h + row * D + col, in[c], h[c]);
+                    if (p.h) store_some<E, VW, WHOLE>((raw*)p.h + row * D + col, in[c], D % VW, h[c]);
                 }
             }
         }
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
         if (p.y) {
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                if (in[c] > 0) store_some<E, VW, WHOLE>((raw*)p.y + row * D + (c * 64 + lane) * VW, in[c], h[c]);
+                if (in[c] > 0) store_some<E, VW, WHOLE>((raw*)p.y + row * D + (c * 64 + lane) * VW, in[c], D % VW, h[c]);
         }
         if (p.q) {
             uint32_t m = 0;
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
                     float v[VW];
 #pragma unroll
                     for (int e = 0; e < VW; ++e) v[e] = h[c][e] * inv;
-                    store_some<TypeE4M3, VW, WHOLE>(p.q + row * D + (c * 64 + lane) * VW, in[c], v);
+                    store_some<TypeE4M3, VW, WHOLE>(p.q + row * D + (c * 64 + lane) * VW, in[c], D % VW, v);
                 }
         }
     }
@@ -150,18 +150,18 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_rows_wide_kernel(RmsArgs p) 
         uint32_t m = 0;
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW];
-            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), h);
+            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
             if (p.residual) {
                 float r[VW];
-                load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, (int)min(D - col, (long)VW), r);
+                load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, (int)min(D - col, (long)VW), (int)(D % VW), r);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) h[e] += r[e];
-                if (p.h) store_some<E, VW, WHOLE>((raw*)p.h + row * D + col, (int)min(D - col, (long)VW), h);
+                if (p.h) store_some<E, VW, WHOLE>((raw*)p.h + row * D + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
             }
             float w[VW];
 #pragma unroll
             for (int e = 0; e < VW; ++e) w[e] = 1.f;
-            if (p.weight) load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), w);
+            if (p.weight) load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), (int)(D % VW), w);
 #pragma unroll
             for (int e = 0; e < VW; ++e) {
                 ss = fmaf(h[e], h[e], ss);
@@ -183,24 +183,24 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_rows_wide_kernel(RmsArgs p) 
         }
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW];
-            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), h);
+            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
             if (p.residual) {
                 float r[VW];
-                load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, (int)min(D - col, (long)VW), r);
+                load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, (int)min(D - col, (long)VW), (int)(D % VW), r);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) h[e] += r[e];
             }
             if (p.weight) {
                 float w[VW];
-                load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), w);
+                load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), (int)(D % VW), w);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) h[e] = h[e] * rstd * w[e];
             }
-            if (p.y) store_some<E, VW, WHOLE>((raw*)p.y + row * D + col, (int)min(D - col, (long)VW), h);
+            if (p.y) store_some<E, VW, WHOLE>((raw*)p.y + row * D + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
             if (p.q) {
 #pragma unroll
                 for (int e = 0; e < VW; ++e) h[e] *= inv;
-                store_some<TypeE4M3, VW, WHOLE>(p.q + row * D + col, (int)min(D - col, (long)VW), h);
+                store_some<TypeE4M3, VW, WHOLE>(p.q + row * D + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
             }
         }
     }
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
         in[c] = D - col;
 #pragma unroll
         for (int e = 0; e < VW; ++e) w[c][e] = dw[c][e] = 0.f;
-        if (in[c] > 0) load_some<E, VW, WHOLE>((const raw*)p.weight + col, in[c], w[c]);
+        if (in[c] > 0) load_some<E, VW, WHOLE>((const raw*)p.weight + col, in[c], D % VW, w[c]);
     }
     const int waves = gridDim.x * ROW_WAVES;
     // the next row's three loads are under way while this one is worked on (narrow rows: with one row at a time the 8 waves a CU had too
@@ -236,9 +236,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
 #pragma unroll
             for (int e = 0; e < VW; ++e) h[c][e] = g[c][e] = d[c][e] = 0.f;
             if (in[c] > 0) {
-                load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, in[c], h[c]);
-                load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, in[c], g[c]);
-                if (AHEAD && p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, in[c], d[c]);
+                load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, in[c], D % VW, h[c]);
+                load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, in[c], D % VW, g[c]);
+                if (AHEAD && p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, in[c], D % VW, d[c]);
             }
         }
     };
@@ -276,10 +276,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
         for (int c = 0; c < C; ++c)
             if (in[c] > 0) {
                 const int col = (c * 64 + lane) * VW;
-                if (!AHEAD && p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, in[c], d[c]);
+                if (!AHEAD && p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, in[c], D % VW, d[c]);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) d[c][e] = fmaf(rstd, fmaf(-dot, h[c][e], g[c][e]), d[c][e]);
-                store_some<E, VW, WHOLE>((raw*)p.dx + row * D + col, in[c], d[c]);
+                store_some<E, VW, WHOLE>((raw*)p.dx + row * D + col, in[c], D % VW, d[c]);
             }
     }
     if (!p.partial) return;
@@ -310,24 +310,24 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_grad_wide_kernel(RmsArgs p) 
         float dot = 0.f;
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW], g[VW], w[VW];
-            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), h);
-            load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, (int)min(D - col, (long)VW), g);
-            load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), w);
+            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
+            load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, (int)min(D - col, (long)VW), (int)(D % VW), g);
+            load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), (int)(D % VW), w);
 #pragma unroll
             for (int e = 0; e < VW; ++e) dot = fmaf(g[e] * w[e], h[e] * rstd, dot);
         }
         dot = block_sum(dot, red) * p.inv_width;
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW], g[VW], w[VW], d[VW];
-            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), h);
-            load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, (int)min(D - col, (long)VW), g);
-            load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), w);
+            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
+            load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, (int)min(D - col, (long)VW), (int)(D % VW), g);
+            load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), (int)(D % VW), w);
 #pragma unroll
             for (int e = 0; e < VW; ++e) d[e] = 0.f;
-            if (p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, (int)min(D - col, (long)VW), d);
+            if (p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, (int)min(D - col, (long)VW), (int)(D % VW), d);
 #pragma unroll
             for (int e = 0; e < VW; ++e) d[e] = fmaf(rstd, fmaf(-dot, h[e] * rstd, g[e] * w[e]), d[e]);
-            store_some<E, VW, WHOLE>((raw*)p.dx + row * D + col, (int)min(D - col, (long)VW), d);
+            store_some<E, VW, WHOLE>((raw*)p.dx + row * D + col, (int)min(D - col, (long)VW), (int)(D % VW), d);
         }
     }
 }

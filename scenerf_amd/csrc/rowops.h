@@ -80,14 +80,63 @@ template <typename E, int W> __device__ static inline void load_vec(const typena
         for (int e = 0; e < S; ++e) v[i + e] = t[e];
     }
 }
-// the first n > 0 of them, zeros behind.  WHOLE: n is known to be W or more -- where a matrix's length is in whole pieces no lane has to
-// branch, and a row's loads go out together (with the branch, 40,001 x 2,480 rows to 8 bits took 97 us instead of 76)
-template <typename E, int W, bool WHOLE = false> __device__ static inline void load_some(const typename E::raw* p, int n, float (&v)[W]) {
+// The first n > 0 of them, zeros behind; tail: the row's length % W.  WHOLE: n is known to be W or more -- where a matrix's length is in
+// whole pieces no lane has to branch, and a row's loads go out together (with the branch, 40,001 x 2,480 rows to 8 bits took 97 us instead
+// of 76).  A row's last piece moves as 1 to 3 powers of two: element by element it cost a row of 511 twice the rest of it.
+template <typename E, int AT, int N, int W> __device__ static inline void load_part(const typename E::raw* p, float (&v)[W]) {
+    typedef typename E::raw raw;
+    union { raw e[N]; uint8_t b1; uint16_t b2; uint32_t b4; uint64_t b8; uint4 b16; } u;
+    typedef uint16_t u16_any __attribute__((aligned(1)));
+    typedef uint64_t u64_any __attribute__((aligned(1)));
+    constexpr int B = N * (int)sizeof(raw);
+    static_assert(B <= 16, "one access");
+    if constexpr (B == 1) u.b1 = *(const uint8_t*)(p + AT);
+    else if constexpr (B == 2) u.b2 = *(const u16_any*)(p + AT);
+    else if constexpr (B == 4) u.b4 = *(const srf_u32_any*)(p + AT);
+    else if constexpr (B == 8) u.b8 = *(const u64_any*)(p + AT);
+    else u.b16 = load16(p + AT);
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[AT + e] = E::to_f32(u.e[e]);
+}
+template <typename E, int AT, int N, int W> __device__ static inline void store_part(typename E::raw* p, const float (&v)[W]) {
+    typedef typename E::raw raw;
+    union { raw e[N]; uint8_t b1; uint16_t b2; uint32_t b4; uint64_t b8; uint4 b16; } u;
+    typedef uint16_t u16_any __attribute__((aligned(1)));
+    typedef uint64_t u64_any __attribute__((aligned(1)));
+    constexpr int B = N * (int)sizeof(raw);
+#pragma unroll
+    for (int e = 0; e < N; ++e) u.e[e] = E::from_f32(v[AT + e]);
+    if constexpr (B == 1) *(uint8_t*)(p + AT) = u.b1;
+    else if constexpr (B == 2) *(u16_any*)(p + AT) = u.b2;
+    else if constexpr (B == 4) *(srf_u32_any*)(p + AT) = u.b4;
+    else if constexpr (B == 8) *(u64_any*)(p + AT) = u.b8;
+    else store16(p + AT, u.b16);
+}
+template <typename E, int TAIL, int W> __device__ static inline void load_tail(const typename E::raw* p, float (&v)[W]) {
+    if constexpr (TAIL >= 4) load_part<E, 0, 4, W>(p, v);
+    if constexpr (TAIL & 2) load_part<E, TAIL & 4, 2, W>(p, v);
+    if constexpr (TAIL & 1) load_part<E, TAIL & 6, 1, W>(p, v);
+}
+template <typename E, int TAIL, int W> __device__ static inline void store_tail(typename E::raw* p, const float (&v)[W]) {
+    if constexpr (TAIL >= 4) store_part<E, 0, 4, W>(p, v);
+    if constexpr (TAIL & 2) store_part<E, TAIL & 4, 2, W>(p, v);
+    if constexpr (TAIL & 1) store_part<E, TAIL & 6, 1, W>(p, v);
+}
+template <typename E, int W, bool WHOLE = false> __device__ static inline void load_some(const typename E::raw* p, int n, int tail, float (&v)[W]) {
     if (WHOLE || n >= W) {
         load_vec<E, W>(p, v);
-    } else {
+        return;
+    }
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] = e < n ? E::to_f32(p[e]) : 0.f;
+    for (int e = 0; e < W; ++e) v[e] = 0.f;
+    if (tail == 1) load_tail<E, 1, W>(p, v);
+    else if (tail == 2) load_tail<E, 2, W>(p, v);
+    else if (tail == 3) load_tail<E, 3, W>(p, v);
+    if constexpr (W == 8) {
+        if (tail == 4) load_tail<E, 4, W>(p, v);
+        else if (tail == 5) load_tail<E, 5, W>(p, v);
+        else if (tail == 6) load_tail<E, 6, W>(p, v);
+        else if (tail == 7) load_tail<E, 7, W>(p, v);
     }
 }
 template <typename E> __device__ static inline uint32_t pack2(float a, float b) {
@@ -117,13 +166,19 @@ template <typename E, int W> __device__ static inline void store_vec(typename E:
         else *(srf_u32_any*)p = w[0];
     }
 }
-template <typename E, int W, bool WHOLE = false> __device__ static inline void store_some(typename E::raw* p, int n, const float (&v)[W]) {
+template <typename E, int W, bool WHOLE = false> __device__ static inline void store_some(typename E::raw* p, int n, int tail, const float (&v)[W]) {
     if (WHOLE || n >= W) {
         store_vec<E, W>(p, v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-            if (e < n) p[e] = E::from_f32(v[e]);
+        return;
+    }
+    if (tail == 1) store_tail<E, 1, W>(p, v);
+    else if (tail == 2) store_tail<E, 2, W>(p, v);
+    else if (tail == 3) store_tail<E, 3, W>(p, v);
+    if constexpr (W == 8) {
+        if (tail == 4) store_tail<E, 4, W>(p, v);
+        else if (tail == 5) store_tail<E, 5, W>(p, v);
+        else if (tail == 6) store_tail<E, 6, W>(p, v);
+        else if (tail == 7) store_tail<E, 7, W>(p, v);
     }
 }
 
