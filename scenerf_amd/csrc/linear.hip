@@ -210,8 +210,13 @@ __global__ __launch_bounds__(256) void linear_pad_kernel(PadSide x, PadSide w, i
         const long u = t < first ? t : t - first, r = u / per;
         const int c = (int)(u - r * per) * W;
         union { R e[W]; uint4 v; } o;
+        const R* at = (const R*)s.src + r * s.ld + c;
+        if (c + W <= cols) {
+            o.v = load16(at);
+        } else {
 #pragma unroll
-        for (int e = 0; e < W; ++e) o.e[e] = c + e < cols ? ((const R*)s.src)[r * s.ld + c + e] : (R)0;
+            for (int e = 0; e < W; ++e) o.e[e] = c + e < cols ? at[e] : (R)0;
+        }
         *(uint4*)((R*)s.dst + r * pitch + c) = o.v;
     }
 }
@@ -378,10 +383,33 @@ static int lin_pitch(int cols, int es) { return round_up(cols, 16 / es); }
 static bool lin_pieces(const void* p, int64_t ld, int cols, int es, bool padded) {
     return aligned16(p) && (ld * es) % 16 == 0 && ld * es <= LIN_MAX_PITCH_BYTES && (padded ? ld >= lin_pitch(cols, es) : (cols * (int64_t)es) % 16 == 0);
 }
+// Large tiles read w once per row of tiles: rows of w that start inside a line make every 128-byte chunk touch two (1,536 x 2,480 bf16
+// against 153,600 rows: 1,073 us, 1,043 with w's rows on lines, 8 bit 686 and 646), so w is copied to a pitch of whole lines where it is
+// small beside x.
+static int lin_line_pitch(int k, int es) { return round_up(k, 128 / es); }
+static bool lin_onto_lines(const scenerf_linear* p, const LinPlan& plan) {
+    const int es = lin_es(p->in_type);
+    return plan.kind == 2 && plan.tile == LIN_256x256 && ((p->ldw * es) % 128 || (uintptr_t)p->w % 128) && p->rows >= 16LL * p->n &&
+           (int64_t)lin_line_pitch(p->k, es) * es <= LIN_MAX_PITCH_BYTES;
+}
+static int64_t lin_onto_lines_bytes(const scenerf_linear* p, const LinPlan& plan) {
+    return lin_onto_lines(p, plan) ? align256((int64_t)p->n * lin_line_pitch(p->k, lin_es(p->in_type)) * lin_es(p->in_type)) : 0;
+}
 static LinPlan lin_forward_plan(const scenerf_linear* p) {
     const int es = lin_es(p->in_type);
     const bool staged = lin_pieces(p->x, p->ldx, p->k, es, p->padded) && lin_pieces(p->w, p->ldw, p->k, es, p->padded);
     return lin_plan(p->in_type, false, false, staged, p->rows, p->n, p->k);
+}
+
+static int lin_copy_rows(int es, int cols, int pitch, PadSide x, PadSide w, hipStream_t s) {
+    const long pieces = (x.rows + w.rows) * (pitch / (16 / es));
+    if (pieces == 0) return 0;
+    const unsigned blocks = (unsigned)(pieces < 8192L * 256 ? (pieces + 255) / 256 : 8192);
+    if (es == 4) linear_pad_kernel<uint32_t><<<blocks, 256, 0, s>>>(x, w, cols, pitch);
+    else if (es == 2) linear_pad_kernel<uint16_t><<<blocks, 256, 0, s>>>(x, w, cols, pitch);
+    else linear_pad_kernel<uint8_t><<<blocks, 256, 0, s>>>(x, w, cols, pitch);
+    SRF_LAUNCH_CHECK("linear_pad_kernel");
+    return 0;
 }
 
 #define DZ_STRIPS 1024               // strips of rows: four workgroups a CU at 32 columns of 8
@@ -456,30 +484,23 @@ int scenerf_hip_linear_pad(int type, int k, const void* x, int64_t ldx, int64_t 
     SRF_CHECK(k >= 1 && k < ROWOPS_GRID_MAX - 1024 && rows >= 0 && rows < ROWOPS_GRID_MAX - 1024 && n >= 0 && ldx >= 0 && ldw >= 0, "linear_pad: bad sizes");
     SRF_CHECK(!x == !x_out && !w == !w_out, "linear_pad: a matrix and its copy go together");
     SRF_CHECK(aligned16(x_out) && aligned16(w_out), "linear_pad: the copies must be aligned to 16 bytes");
-    const int es = lin_es(type), pitch = lin_pitch(k, es);
-    const PadSide sx = {x, x_out, ldx, x ? rows : 0}, sw = {w, w_out, ldw, w ? n : 0};
-    const long pieces = (sx.rows + sw.rows) * (pitch / (16 / es));
-    if (pieces == 0) return 0;
-    const unsigned blocks = (unsigned)(pieces < 8192L * 256 ? (pieces + 255) / 256 : 8192);
-    hipStream_t s = as_stream(stream);
-    SrfLaunchScope ps(s, "linear_pad", 0, 2. * pieces * 16);
-    if (es == 4) linear_pad_kernel<uint32_t><<<blocks, 256, 0, s>>>(sx, sw, k, pitch);
-    else if (es == 2) linear_pad_kernel<uint16_t><<<blocks, 256, 0, s>>>(sx, sw, k, pitch);
-    else linear_pad_kernel<uint8_t><<<blocks, 256, 0, s>>>(sx, sw, k, pitch);
-    SRF_LAUNCH_CHECK("linear_pad_kernel");
-    return 0;
+    const int es = lin_es(type);
+    SrfLaunchScope ps(as_stream(stream), "linear_pad", 0, 2. * (rows + n) * k * es);
+    return lin_copy_rows(es, k, lin_pitch(k, es), PadSide{x, x_out, ldx, x ? rows : 0}, PadSide{w, w_out, ldw, w ? n : 0}, as_stream(stream));
 }
 
 int64_t scenerf_hip_linear_workspace(const scenerf_linear* p, int backward) {
     if (lin_check(p, "linear_workspace", backward != 0)) return -1;
-    return backward ? lin_backward_plan(p).bytes : lin_part_bytes(lin_forward_plan(p), p->rows, p->n);
+    if (backward) return lin_backward_plan(p).bytes;
+    const LinPlan plan = lin_forward_plan(p);
+    return lin_onto_lines_bytes(p, plan) + lin_part_bytes(plan, p->rows, p->n);
 }
 
 int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream) {
     if (int e = lin_check(p, "linear_forward", false)) return e;
     if (p->rows == 0) return 0;
     const LinPlan plan = lin_forward_plan(p);
-    const int64_t need = lin_part_bytes(plan, p->rows, p->n);
+    const int64_t lines = lin_onto_lines_bytes(p, plan), need = lines + lin_part_bytes(plan, p->rows, p->n);
     SRF_CHECK(need == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= need), "linear_forward: workspace of %lld bytes needed",
               (long long)need);
     const double m = (double)p->rows, es = lin_es(p->in_type), eo = lin_es(p->out_type);
@@ -492,7 +513,13 @@ int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream)
     if (p->in_type == SCENERF_T_E4M3) { a.row_scale = p->x_scale; a.col_scale = p->w_scale; }
     a.bias = p->bias; a.residual = p->residual; a.ld_residual = p->ld_residual;
     a.out = p->y; a.z = p->z; a.act = p->activation;
-    return lin_product(p->in_type, p->out_type, a, plan, p->workspace, s);
+    if (lines) {
+        const int pitch = lin_line_pitch(p->k, (int)es), cols = p->padded ? lin_pitch(p->k, (int)es) : p->k;
+        if (int e = lin_copy_rows((int)es, cols, pitch, PadSide{nullptr, nullptr, 0, 0}, PadSide{p->w, p->workspace, p->ldw, p->n}, s)) return e;
+        a.B = p->workspace;
+        a.b_j = pitch;
+    }
+    return lin_product(p->in_type, p->out_type, a, plan, (char*)p->workspace + lines, s);
 }
 
 int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream) {

@@ -423,9 +423,16 @@ template <typename E, int VW, bool WHOLE> static void rms_launch_chunks(const Rm
     const int chunks = cdiv(a.width, 64 * VW);
     if (chunks <= 1) return rms_launch<E, VW, 1, WHOLE>(a, backward, blocks, s);
     if (chunks <= 2) return rms_launch<E, VW, 2, WHOLE>(a, backward, blocks, s);
+    if (chunks <= 3) return rms_launch<E, VW, 3, WHOLE>(a, backward, blocks, s);
     if (chunks <= 4) return rms_launch<E, VW, 4, WHOLE>(a, backward, blocks, s);
+    if (chunks <= 5) return rms_launch<E, VW, 5, WHOLE>(a, backward, blocks, s);
+    if (chunks <= 6) return rms_launch<E, VW, 6, WHOLE>(a, backward, blocks, s);
     if (chunks <= 8) return rms_launch<E, VW, 8, WHOLE>(a, backward, blocks, s);
-    if constexpr (VW == 4) rms_launch<E, VW, 16, WHOLE>(a, backward, blocks, s);
+    if constexpr (VW == 4) {
+        if (chunks <= 10) return rms_launch<E, VW, 10, WHOLE>(a, backward, blocks, s);
+        if (chunks <= 12) return rms_launch<E, VW, 12, WHOLE>(a, backward, blocks, s);
+        rms_launch<E, VW, 16, WHOLE>(a, backward, blocks, s);
+    }
 }
 template <typename E, bool WHOLE> static int rms_dispatch(const scenerf_rms* p, bool backward, hipStream_t s) {
     constexpr int VW = 16 / sizeof(typename E::raw);
