@@ -464,6 +464,11 @@ int scenerf_hip_resnetfc_backward(const scenerf_cfg* cfg, const scenerf_resnetfc
                                   const int32_t* tap_texel, const float* tap_weight, int M, const scenerf_resnetfc_acts* acts,
                                   const float* dlog16 /*[M][16]*/, float* dhz, float* dh, float* dn,
                                   float* const gmaps_hwc[SCENERF_N_SCALES] /*NULL: no map gradients*/, scenerf_stream_t stream);
+/* The last of those on its own, for a net whose other gradients come from elsewhere (a ResnetFC with norms): dhz [M][width], w_z_t[s]
+ * [map_C[s]][width], both fp32 or, at cfg->precision 1, bf16; the maps' gradients accumulate in fp32.  A level with no gmaps_hwc[s] is left out. */
+int scenerf_hip_resnetfc_feature_grads(const scenerf_cfg* cfg, const void* const w_z_t[SCENERF_N_SCALES], int width /*n_blocks * d_hidden*/,
+                                       const uint8_t* tile_mask, const int32_t* tap_texel, const float* tap_weight, int M, const void* dhz,
+                                       float* const gmaps_hwc[SCENERF_N_SCALES], scenerf_stream_t stream);
 
 /* ---- generic building blocks exported for unit tests ------------------------------------------------------- */
 /* C[M][N] = relu?(A[M][K]) @ W[N][K]^T (+bias); act operands per `precision`, fp32 output.

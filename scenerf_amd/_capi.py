@@ -185,6 +185,7 @@ _PROTOS = {
     "scenerf_hip_resnetfc_forward_train": (C.c_int, [C.POINTER(Cfg), C.POINTER(ResnetFCNet), vp, vp, vp, i32, C.POINTER(ResnetFCActs), vp, vp, vp]),
     "scenerf_hip_resnetfc_backward": (C.c_int, [C.POINTER(Cfg), C.POINTER(ResnetFCNet), C.POINTER(ResnetFCNetT), C.POINTER(ResnetFCGrads),
                                                 vp, vp, vp, vp, vp, i32, C.POINTER(ResnetFCActs), vp, vp, vp, vp, vp, vp]),
+    "scenerf_hip_resnetfc_feature_grads": (C.c_int, [C.POINTER(Cfg), C.POINTER(vp * N_SCALES), i32, vp, vp, vp, i32, vp, C.POINTER(vp * N_SCALES), vp]),
     "scenerf_hip_test_gemm_nt": (C.c_int, [i32, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp]),
     "scenerf_hip_test_chunk_table": (C.c_int, [C.POINTER(Cfg), i32, vp, i32]),
     "scenerf_hip_test_set_tuning": (C.c_int, [i32, i32]),

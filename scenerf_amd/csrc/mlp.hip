@@ -510,6 +510,37 @@ static int resnetfc_check(const scenerf_cfg* cfg, const scenerf_resnetfc* net, c
     return 0;
 }
 
+// dz = dhz Wz scattered through the forward's taps: one launch for all levels (the GEMM family's scatter epilogue)
+static int resnetfc_feature_grads(const scenerf_cfg* cfg, int prec, const void* const* w_z_t, int LD, const uint8_t* tile_mask,
+                                  const int32_t* tap_texel, const float* tap_weight, int M, const void* dhz, float* const* gmaps_hwc,
+                                  hipStream_t s) {
+    GemmNT g;
+    g.name = "gemm_generic_dfeat_scatter";
+    g.A1 = dhz; g.lda1 = LD; g.K1 = LD;
+    g.ldw = LD;
+    g.M = M;
+    g.tile_mask = tile_mask;
+    g.tap_texel = tap_texel; g.tap_weight = tap_weight;
+    bool any = false;
+    int t = 0;
+    for (int sc = 0; sc < 5; ++sc) {
+        SRF_CHECK(w_z_t[sc] || !gmaps_hwc[sc], "resnetfc_backward: w_z_t[%d] missing", sc);
+        g.ms_t0[sc] = t;
+        g.ms_C[sc] = cfg->map_C[sc];
+        g.ms_W[sc] = w_z_t[sc];
+        g.ms_gmap[sc] = gmaps_hwc[sc];
+        if (cfg->map_chw[sc] == 1) { g.ms_st[sc] = 1; g.ms_sc[sc] = (long)cfg->map_H[sc] * cfg->map_W[sc]; }
+        any = any || gmaps_hwc[sc];
+        t += cdiv(cfg->map_C[sc], 128);
+    }
+    if (!any) return 0;
+    g.ms_t0[5] = t;
+    g.ms_n = 5;
+    g.N = SCENERF_D_LATENT;
+    g.scatter_scale = 0;
+    return launch_gemm_nt(prec, g, s);
+}
+
 int scenerf_hip_resnetfc_forward_train(const scenerf_cfg* cfg, const scenerf_resnetfc* net, const float* xenc, const float* Z,
                                        const uint8_t* tile_mask, int M, const scenerf_resnetfc_acts* acts, float* h_scratch,
                                        float* logits, scenerf_stream_t stream) {
@@ -673,35 +704,16 @@ int scenerf_hip_resnetfc_backward(const scenerf_cfg* cfg, const scenerf_resnetfc
         t.allow_tr = 0;
         if (int e = launch_gemm_tn(0, t, s)) return e;
     }
-    if (gmaps_hwc) {   // dz = dhz Wz scattered through the forward's taps: one launch for all levels (the GEMM family's scatter epilogue)
-        GemmNT g;
-        g.name = "gemm_generic_dfeat_scatter";
-        g.A1 = dhz; g.lda1 = LD; g.K1 = LD;
-        g.ldw = LD;
-        g.M = M;
-        g.tile_mask = tile_mask;
-        g.tap_texel = tap_texel; g.tap_weight = tap_weight;
-        bool any = false;
-        int t = 0;
-        for (int sc = 0; sc < 5; ++sc) {
-            SRF_CHECK(nt->w_z_t[sc] || !gmaps_hwc[sc], "resnetfc_backward: w_z_t[%d] missing", sc);
-            g.ms_t0[sc] = t;
-            g.ms_C[sc] = cfg->map_C[sc];
-            g.ms_W[sc] = nt->w_z_t[sc];
-            g.ms_gmap[sc] = gmaps_hwc[sc];
-            if (cfg->map_chw[sc] == 1) { g.ms_st[sc] = 1; g.ms_sc[sc] = (long)cfg->map_H[sc] * cfg->map_W[sc]; }
-            any = any || gmaps_hwc[sc];
-            t += cdiv(cfg->map_C[sc], 128);
-        }
-        if (any) {
-            g.ms_t0[5] = t;
-            g.ms_n = 5;
-            g.N = SCENERF_D_LATENT;
-            g.scatter_scale = 0;
-            if (int e = launch_gemm_nt(0, g, s)) return e;
-        }
-    }
+    if (gmaps_hwc) return resnetfc_feature_grads(cfg, 0, (const void* const*)nt->w_z_t, LD, tile_mask, tap_texel, tap_weight, M, dhz, gmaps_hwc, s);
     return 0;
+}
+
+int scenerf_hip_resnetfc_feature_grads(const scenerf_cfg* cfg, const void* const w_z_t[SCENERF_N_SCALES], int width, const uint8_t* tile_mask,
+                                       const int32_t* tap_texel, const float* tap_weight, int M, const void* dhz,
+                                       float* const gmaps_hwc[SCENERF_N_SCALES], scenerf_stream_t stream) {
+    SRF_CHECK(cfg && w_z_t && tile_mask && tap_texel && tap_weight && dhz && gmaps_hwc && M > 0, "resnetfc_feature_grads: NULL argument");
+    SRF_CHECK(width >= 16 && width % 16 == 0, "resnetfc_feature_grads: width=%d must be a multiple of 16", width);
+    return resnetfc_feature_grads(cfg, cfg->precision, w_z_t, width, tile_mask, tap_texel, tap_weight, M, dhz, gmaps_hwc, as_stream(stream));
 }
 
 int scenerf_hip_mlp_backward(const scenerf_cfg* cfg, const scenerf_mlp_weights* w, const scenerf_mlp_grads* g_,

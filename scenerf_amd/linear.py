@@ -77,35 +77,47 @@ def _forward(what, x2, w2, padded, n, k, bias, residual, shape, in_type, out_dty
     return y, z
 
 
+def linear_step(x: torch.Tensor, weight: torch.Tensor, bias, residual, act: int, shape, keep_z: bool):
+    """(y, what ``linear_step_back`` needs) of a layer that will be differentiated; no checks, no autograd."""
+    n, k = weight.shape
+    x2, w2, padded = _in_pieces(rows_of(x, k), rows_of(weight, k), True)
+    y, z = _forward("linear", x2, w2, padded, n, k, bias, residual, shape, TYPE_CODES[x.dtype], x.dtype, act, keep_z)
+    return y, (x2, w2, z, n, k, padded, act)
+
+
+def linear_step_back(saved, dy: torch.Tensor, x_shape, need_x: bool, need_w: bool, need_b: bool):
+    """(dx, dweight, dbias), None where not needed."""
+    x2, w2, z, n, k, padded, act = saved
+    dev, dtype = dy.device, x2.dtype
+    dx = torch.empty(x_shape, dtype=dtype, device=dev) if need_x else None
+    dw = torch.empty((n, k), dtype=dtype, device=dev) if need_w else None
+    db = torch.empty((n,), dtype=dtype, device=dev) if need_b else None
+    dy2 = rows_of(dy, n)
+    code, lib = TYPE_CODES[dtype], _capi.load()
+    p = _capi.Linear(code, code, act, n, k, padded, x2.shape[0], x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), None, None, None, None, 0,
+                     None, None if z is None else z.data_ptr(), dy2.data_ptr(), dy2.stride(0), None if dx is None else dx.data_ptr(),
+                     None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr())
+    ws = give_workspace(lib.scenerf_hip_linear_workspace, p, 1, dev, "linear backward")  # noqa: F841 (alive up to the launch)
+    run_on(dev, lib.scenerf_hip_linear_backward, (C.byref(p),), "linear backward")
+    return dx, dw, db
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, shape):
-        n, k = weight.shape
-        x2, w2, padded = _in_pieces(rows_of(x, k), rows_of(weight, k), True)
-        keep_z = act != _capi.ACTIVATIONS["none"] and any(ctx.needs_input_grad[:3])
-        y, z = _forward("linear", x2, w2, padded, n, k, bias, residual, shape, TYPE_CODES[x.dtype], x.dtype, act, keep_z)
-        ctx.save_for_backward(x2, w2, z)
-        ctx.act, ctx.padded, ctx.x_shape, ctx.w_shape = act, padded, x.shape, (n, k)
+        y, saved = linear_step(x, weight, bias, residual, act, shape, act != _capi.ACTIVATIONS["none"] and any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(*saved[:3])
+        ctx.rest, ctx.x_shape = saved[3:], x.shape
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2, w2, z = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dev, (n, k) = dy.device, ctx.w_shape
-        dx = torch.empty(ctx.x_shape, dtype=x2.dtype, device=dev) if need_x else None
-        dw = torch.empty((n, k), dtype=x2.dtype, device=dev) if need_w else None
-        db = torch.empty((n,), dtype=x2.dtype, device=dev) if need_b else None
-        if need_x or need_w or need_b:
-            dy2 = rows_of(dy, n)
-            code, lib = TYPE_CODES[x2.dtype], _capi.load()
-            p = _capi.Linear(code, code, ctx.act, n, k, ctx.padded, x2.shape[0], x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), None, None, None,
-                             None, 0, None, None if z is None else z.data_ptr(), dy2.data_ptr(), dy2.stride(0), None if dx is None else dx.data_ptr(),
-                             None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr())
-            ws = give_workspace(lib.scenerf_hip_linear_workspace, p, 1, dev, "linear backward")  # noqa: F841
-            run_on(dev, lib.scenerf_hip_linear_backward, (C.byref(p),), "linear backward")
-        return dx, dw, db, (dy if need_r else None), None, None
+        need = ctx.needs_input_grad
+        grads = (None, None, None)
+        if any(need[:3]):
+            grads = linear_step_back(ctx.saved_tensors + ctx.rest, dy, ctx.x_shape, *need[:3])
+        return grads + (dy if need[3] else None, None, None)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: str = "none",

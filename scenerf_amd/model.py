@@ -24,7 +24,9 @@ import numpy as np
 import torch
 import torch.nn as nn
 
+from . import normed
 from .config import BF_FOV, KITTI_FOV, RenderConfig
+from .norm import RMSNorm
 from .renderer import MLP_PARAM_NAMES, OUTPUT_KEYS, RenderSession
 from .training import BundleFusionTrainingMixin, TrainingMixin
 
@@ -118,10 +120,12 @@ def _load_reference_state(model, state_dict, strict=True):
 
 
 class ResnetBlockFC(nn.Module):
-    """Parameter container for one block (resnetfc.py:20-52): fc_0, fc_1 with the reference initialisation."""
+    """Parameter container for one block (resnetfc.py:20-52): fc_0, fc_1 with the reference initialisation (and a norm in front)."""
 
-    def __init__(self, size: int):
+    def __init__(self, size: int, norm: bool = False, eps: float = 1e-6):
         super().__init__()
+        if norm:
+            self.norm = RMSNorm(size, eps)
         self.fc_0 = nn.Linear(size, size)
         self.fc_1 = nn.Linear(size, size)
         nn.init.constant_(self.fc_0.bias, 0.0)
@@ -135,26 +139,42 @@ class ResnetFC(nn.Module):
 
     It has no ``forward``: evaluation happens inside the HIP MLP pass.  The shape SceneRF instantiates (``n_blocks=3, d_hidden=512``,
     scenerf.py:100-114) runs on the fused kernels, forward and backward; every other block count / hidden width (the reference class is
-    generic: BASELINE.json configs[0] names 1 block x 128) runs in fp32 with one MFMA GEMM per ``nn.Linear`` -- and, since round 6, one per
+    generic: 1 block x 128, say) runs in fp32 with one MFMA GEMM per ``nn.Linear`` and one per
     gradient: ``scenerf_hip_resnetfc_forward`` under ``no_grad``, ``_forward_train`` / ``_backward`` otherwise.  Assign such a net to
     ``model.mlp`` / ``model.mlp_gaussian`` of a ``precision="fp32"`` model.
+
+    ``norm="rms"``: a variant the reference does not have, for nets that are deeper or typed more narrowly -- each block reads its
+    residual stream through an RMS norm (``h <- h + lin_z(z)``, ``h <- h + fc_1(act(fc_0(norm(h))))``, ``out = lin_out(norm_out(h))``;
+    ``activation`` "gelu" (the default), "silu" or "relu").  Any shape, fp32 and bf16, trained and rendered through ``render_rays_batch`` like the
+    others, on the row operators of ``scenerf_amd.linear`` / ``scenerf_amd.norm``; ``forward(zx)`` evaluates it on its own
+    (resnetfc.py:133-164: rows of latent and encoded point side by side).  ``eight_bit = True`` makes ``no_grad`` renders of it multiply
+    e4m3 rows by e4m3 weights in the hidden layers.
     """
 
-    def __init__(self, d_in: int = 42, d_out: int = 4, n_blocks: int = 3, d_latent: int = 2480, d_hidden: int = 512):
+    def __init__(self, d_in: int = 42, d_out: int = 4, n_blocks: int = 3, d_latent: int = 2480, d_hidden: int = 512, norm: str = "none",
+                 activation: Optional[str] = None, norm_eps: float = 1e-6):
         super().__init__()
+        activation = activation or ("gelu" if norm == "rms" else "relu")
+        if norm not in ("none", "rms") or activation not in ("relu", "gelu", "silu") or (norm == "none" and activation != "relu"):
+            raise ValueError("ResnetFC: norm is 'none' or 'rms', activation 'relu', 'gelu' or 'silu' (the net without a norm has relu)")
+        if not norm_eps > 0:
+            raise ValueError("ResnetFC: norm_eps must be positive")
         if (d_in, d_latent) != (42, 2480) or d_out not in (2, 4):
             raise ValueError("the HIP ray pipeline feeds a ResnetFC(d_in=42, d_latent=2480, d_out in {2,4}) (positional encoding + view direction, "
                              "the five feature maps' 2480 channels)")
         if not (1 <= n_blocks <= 8) or d_hidden < 16 or d_hidden % 16:
             raise ValueError("ResnetFC: n_blocks in 1..8 and d_hidden a multiple of 16 (the MFMA GEMM's K granularity)")
         self.d_in, self.d_out, self.n_blocks, self.d_latent, self.d_hidden = d_in, d_out, n_blocks, d_latent, d_hidden
+        self.norm, self.activation, self.norm_eps, self.eight_bit = norm, activation, norm_eps, False
         self.lin_in = nn.Linear(d_in, d_hidden)
         nn.init.constant_(self.lin_in.bias, 0.0)
         nn.init.kaiming_normal_(self.lin_in.weight, a=0, mode="fan_in")
         self.lin_out = nn.Linear(d_hidden, d_out)
         nn.init.constant_(self.lin_out.bias, 0.0)
         nn.init.kaiming_normal_(self.lin_out.weight, a=0, mode="fan_in")
-        self.blocks = nn.ModuleList([ResnetBlockFC(d_hidden) for _ in range(n_blocks)])
+        self.blocks = nn.ModuleList([ResnetBlockFC(d_hidden, norm == "rms", norm_eps) for _ in range(n_blocks)])
+        if norm == "rms":
+            self.norm_out = RMSNorm(d_hidden, norm_eps)
         self.lin_z = nn.ModuleList([nn.Linear(d_latent, d_hidden) for _ in range(n_blocks)])
         for i in range(n_blocks):
             nn.init.constant_(self.lin_z[i].bias, 0.0)
@@ -163,7 +183,7 @@ class ResnetFC(nn.Module):
     @property
     def is_standard(self) -> bool:
         """The trunk SceneRF instantiates: the shape the fused kernels (forward + backward) are built for."""
-        return self.n_blocks == 3 and self.d_hidden == 512
+        return self.n_blocks == 3 and self.d_hidden == 512 and self.norm == "none"
 
     def ordered_params(self):
         """Parameters in the order the renderer's pack expects: ``MLP_PARAM_NAMES`` for the standard shape; the same pattern over
@@ -175,9 +195,18 @@ class ResnetFC(nn.Module):
         for b in range(self.n_blocks):
             names += ["blocks.%d.fc_0.weight" % b, "blocks.%d.fc_0.bias" % b, "blocks.%d.fc_1.weight" % b, "blocks.%d.fc_1.bias" % b,
                       "lin_z.%d.weight" % b, "lin_z.%d.bias" % b]
+        if self.norm == "rms":          # behind those: the norms' weights, in the blocks' order, norm_out last
+            names += ["blocks.%d.norm.weight" % b for b in range(self.n_blocks)] + ["norm_out.weight"]
+            return normed.NetParams([p[n] for n in names], self.n_blocks, self.activation, self.norm_eps, self.eight_bit)
         return [p[n] for n in names]
 
-    def forward(self, *a, **k):
+    def forward(self, zx, *a, **k):
+        """resnetfc.py:133-164 for a net with ``norm="rms"``: zx (..., d_latent + d_in), latent first -> (..., d_out), differentiable.
+        The nets without a norm are evaluated inside the render pass only."""
+        if self.norm == "rms":
+            if a or k:
+                raise TypeError("ResnetFC.forward takes the rows alone")
+            return normed.evaluate(self.ordered_params(), zx[..., :self.d_latent], zx[..., self.d_latent:])
         raise RuntimeError("ResnetFC is evaluated by the HIP MLP pass; call SceneRF.render_rays_batch")
 
 

@@ -16,6 +16,7 @@ import ctypes as C
 from typing import Optional, Tuple, Union
 
 import torch
+import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -38,6 +39,23 @@ def _check(what, x, weight, residual, eps) -> None:
         raise ValueError("%s: more than 2^31 - 1025 rows" % what)
 
 
+def rms_step_back(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, eps: float, dy: torch.Tensor, dh: Optional[torch.Tensor],
+                  need_x: bool, need_w: bool):
+    """(gradient of h, gradient of weight), None where not needed; h as the forward stored it, ``dh`` what else flows into it."""
+    width, dev = h.shape[-1], h.device
+    h2, dy2, w = rows_of(h, width), rows_of(dy, width), weight.contiguous()
+    dh2 = rows_of(dh, width) if dh is not None else None
+    dx = torch.empty(dy.shape, dtype=h.dtype, device=dev) if need_x else None
+    dw = torch.empty((width,), dtype=h.dtype, device=dev) if need_w else None
+    p = _capi.Rms(TYPE_CODES[h.dtype], width, h2.shape[0], eps, h2.data_ptr(), h2.stride(0), None, 0, w.data_ptr(), None, None, None, None,
+                  rstd.data_ptr(), dy2.data_ptr(), dy2.stride(0), None if dh2 is None else dh2.data_ptr(), 0 if dh2 is None else dh2.stride(0),
+                  None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr())
+    lib = _capi.load()
+    ws = give_workspace(lib.scenerf_hip_rms_workspace, p, 1, dev, "rms_norm backward")  # noqa: F841 (alive up to the launch)
+    run_on(dev, lib.scenerf_hip_rms_backward, (C.byref(p),), "rms_norm backward")
+    return dx, dw
+
+
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
@@ -54,23 +72,12 @@ class _RmsNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dh=None):
         h, weight, rstd = ctx.saved_tensors
-        need_w = ctx.needs_input_grad[1]
-        need_x = ctx.needs_input_grad[0] or (ctx.has_residual and ctx.needs_input_grad[2])
+        need_h = ctx.needs_input_grad[0] or (ctx.has_residual and ctx.needs_input_grad[2])
         if dy is None:               # only h was used
-            return (dh if ctx.needs_input_grad[0] else None, torch.zeros_like(weight) if need_w and dh is not None else None,
-                    dh if ctx.has_residual and ctx.needs_input_grad[2] else None, None)
-        width, dev = h.shape[-1], h.device
-        h2, dy2, w = rows_of(h, width), rows_of(dy, width), weight.contiguous()
-        dh2 = rows_of(dh, width) if dh is not None else None
-        dx = torch.empty(dy.shape, dtype=h.dtype, device=dev) if need_x else None
-        dw = torch.empty((width,), dtype=h.dtype, device=dev) if need_w else None
-        p = _capi.Rms(TYPE_CODES[h.dtype], width, h2.shape[0], ctx.eps, h2.data_ptr(), h2.stride(0), None, 0, w.data_ptr(), None, None, None, None,
-                      rstd.data_ptr(), dy2.data_ptr(), dy2.stride(0), None if dh2 is None else dh2.data_ptr(), 0 if dh2 is None else dh2.stride(0),
-                      None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr())
-        lib = _capi.load()
-        ws = give_workspace(lib.scenerf_hip_rms_workspace, p, 1, dev, "rms_norm backward")  # noqa: F841 (alive up to the launch)
-        run_on(dev, lib.scenerf_hip_rms_backward, (C.byref(p),), "rms_norm backward")
-        return (dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.has_residual and ctx.needs_input_grad[2] else None, None)
+            dx, dw = dh, torch.zeros_like(weight) if ctx.needs_input_grad[1] and dh is not None else None
+        else:
+            dx, dw = rms_step_back(h, weight, rstd, ctx.eps, dy, dh, need_h, ctx.needs_input_grad[1])
+        return dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.has_residual and ctx.needs_input_grad[2] else None, None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
@@ -93,3 +100,14 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[t
     no_gradient("rms_norm_8bit", x, weight, residual)
     q, scale, h, _, _ = rows_forward("rms_norm_8bit", x, weight, residual, float(eps), quantize=True)
     return (q, scale) if residual is None else (q, scale, h)
+
+
+class RMSNorm(nn.Module):
+    """``rms_norm`` with its weight: ``forward(x)`` -> y, ``forward(x, residual)`` -> (y, h)."""
+
+    def __init__(self, width: int, eps: float = 1e-6):
+        super().__init__()
+        self.weight, self.eps = nn.Parameter(torch.ones(width)), eps
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        return rms_norm(x, self.weight, residual=residual, eps=self.eps)

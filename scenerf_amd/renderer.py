@@ -22,6 +22,7 @@ import torch
 
 from . import _capi
 from .config import FEAT_CHANNELS, RenderConfig
+from .normed import NetParams, PackedNormedMLP
 
 D_H = _capi.D_HIDDEN
 D_L = _capi.D_LATENT
@@ -752,6 +753,22 @@ class _GenericRun:
             self.h = [torch.empty((M, pk.d_hidden), **f32) for _ in range(3)]
 
 
+class _NormedRun:
+    """Buffers of one evaluation of a ResnetFC with norms: what the rest of the chunk reads of an ``_MlpRun`` (+ the saved activations)."""
+
+    def __init__(self, M: int, pk: PackedNormedMLP, dev):
+        self.M = M
+        self.Mpad = (M + _capi.TILE_ROWS - 1) // _capi.TILE_ROWS * _capi.TILE_ROWS
+        self.sphere_idx = torch.empty((M, 2), dtype=torch.int32, device=dev)
+        self.xenc = torch.empty((M, D_X), dtype=torch.float32, device=dev)
+        # (the gather leaves the columns of a level that a row tile does not touch unwritten: they stand for zeros)
+        self.Z = torch.zeros((self.Mpad, D_L), dtype=pk.dtype, device=dev)
+        self.tile_mask = torch.empty((self.Mpad // _capi.TILE_ROWS,), dtype=torch.uint8, device=dev)
+        self.tap_texel = torch.empty((M, 5, 4), dtype=torch.int32, device=dev)
+        self.tap_weight = torch.empty((M, 5, 4), dtype=torch.float32, device=dev)
+        self.logits = self.saved = self.sign_bits = self.h0pre = self.h = None
+
+
 class MlpHolder:
     def __init__(self, grad_sync=None, grad_sync_async=None):
         self.packed: Optional[PackedMLP] = None
@@ -763,6 +780,7 @@ class MlpHolder:
         self.defer_pack = False      # pack on the side stream (the radiance MLP: first used after the gaussian head's chain)
         self.split_pack = False      # ... in two calls, a forward's operands first (the gaussian head: its forward is the step's first GEMM)
         self.grad_mode = True        # torch.is_grad_enabled() where the session was opened (inside Function.forward it is always off)
+        self.net: Optional[NetParams] = None     # a ResnetFC with norms says here what it is
         self.pack_cache: Optional[dict] = None   # caller-owned, valid while the parameters cannot change (one trainer forward): see PackMLP
 
 
@@ -777,6 +795,11 @@ class PackMLP(torch.autograd.Function):
     def forward(ctx, holder: MlpHolder, d_out: int, cfg: RenderConfig, *params):
         # training sessions (a parameter gradient will be asked for): the radiance MLP is packed on the side stream
         side = _side_stream(params[0].device) if (holder.defer_pack and any(ctx.needs_input_grad[3:])) else None
+        if holder.net is not None:
+            # a ResnetFC with norms: the row operators, any shape and precision
+            holder.packed = PackedNormedMLP(list(params), holder.net, d_out, cfg, trainable=bool(holder.grad_mode))
+            ctx.holder = holder
+            return torch.empty(1, device=params[0].device)
         if len(params) != len(MLP_PARAM_NAMES) or params[0].shape[0] != D_H:
             # any other ResnetFC shape: the per-layer fp32 GEMM path (scenerf_hip_resnetfc_forward / _forward_train / _backward)
             # (needs_input_grad reports the parameters' requires_grad flags whatever the grad mode: the session recorded the mode)
@@ -884,6 +907,20 @@ def _mlp_eval(ccfg, cfg: RenderConfig, maps: MapHolder, pk: PackedMLP, dist, dis
               K, inv_K, T, M, keep_acts: bool = True, before_forward=None, before_wait=None) -> _MlpRun:
     lib = _capi.load()
     st = _stream(dist.device)
+    if getattr(pk, "normed", False):
+        run = _NormedRun(M, pk, dist.device)
+        _capi.check(lib.scenerf_hip_encode_points(C.byref(ccfg), dist.data_ptr(), dist_ray_stride, ppr, unit_dir.data_ptr(),
+                                                  viewdir.data_ptr(), K.data_ptr(), inv_K.data_ptr(), T.data_ptr(), M, None,
+                                                  run.sphere_idx.data_ptr(), run.xenc.data_ptr(), None, st), "encode_points")
+        _capi.check(lib.scenerf_hip_gather_features(C.byref(ccfg), C.byref(maps.map_ptr_array()), run.sphere_idx.data_ptr(), M,
+                                                    run.Z.data_ptr(), run.tile_mask.data_ptr(), run.tap_texel.data_ptr(),
+                                                    run.tap_weight.data_ptr(), st), "gather_features")
+        if before_wait is not None:
+            before_wait()
+        if before_forward is not None:
+            before_forward()
+        run.logits, run.saved = pk.forward(run.xenc, run.Z[:M], keep_acts and pk.trainable)
+        return run
     if getattr(pk, "generic", False):
         keep_acts = keep_acts and pk.trainable
         run = _GenericRun(M, pk, dist.device, keep_acts=keep_acts)
@@ -939,6 +976,13 @@ def _mlp_backward(ccfg, cfg: RenderConfig, maps: MapHolder, pk: PackedMLP, run: 
     does not wait for the map gradients' tail (GraphedStep)."""
     lib = _capi.load()
     pk.wait_ready(backward=True)
+    if getattr(pk, "normed", False):
+        if before_grads is not None:
+            before_grads()
+        dzs = pk.backward(run.saved, d_logits)
+        if want_map_grads:
+            pk.feature_grads(ccfg, run, dzs, C.byref(maps.gmap_ptr_array()), _stream(d_logits.device))
+        return sync_async(pk.gflat) if sync_async is not None else None
     if getattr(pk, "generic", False):
         # any other ResnetFC shape: one fp32 GEMM per gradient, all on the current stream (scenerf_hip_resnetfc_backward)
         if before_grads is not None:
@@ -1328,6 +1372,7 @@ class RenderSession:
         # (first read ~0.3 ms into the step).  The side stream runs them in this order: head, then radiance MLP.
         self.mlp.grad_mode = self.mlpg.grad_mode = torch.is_grad_enabled()
         self.mlp.pack_cache = self.mlpg.pack_cache = self._pack_cache
+        self.mlp.net, self.mlpg.net = (p if isinstance(p, NetParams) else None for p in (mlp_params, mlpg_params))
         self.mlp.defer_pack = True
         self.mlpg.defer_pack = DEFER_HEAD_PACK
         self.mlpg.split_pack = SPLIT_HEAD_PACK

@@ -88,3 +88,22 @@ def test_rms_entry_refuses():
     need = lib.scenerf_hip_rms_workspace(C.byref(p), 1)
     assert need >= 32 and "workspace" in _said(lib.scenerf_hip_rms_backward(C.byref(p), None))
     assert lib.scenerf_hip_rms_forward(C.byref(_rms(rows=0, x=None, y=None)), None) == 0
+
+
+def test_the_net_with_norms():
+    from scenerf_amd.model import ResnetFC, SceneRF
+    m = ResnetFC(n_blocks=2, d_hidden=32, norm="rms")
+    assert not m.is_standard and m.activation == "gelu" and not ResnetFC(norm="rms").is_standard and ResnetFC().activation == "relu"
+    p = m.ordered_params()
+    assert len(p) == 4 + 6 * 2 + 3 and {id(t) for t in p} == {id(t) for t in m.parameters()} and tuple(p[-1].shape) == (32,)
+    for bad in (dict(norm="layer"), dict(norm="rms", activation="tanh"), dict(activation="gelu"), dict(norm="rms", norm_eps=0.0)):
+        with pytest.raises(ValueError):
+            ResnetFC(**bad)
+    with pytest.raises(RuntimeError, match="render_rays_batch"):
+        ResnetFC()(torch.zeros(1, 2522))
+    with pytest.raises((RuntimeError, ValueError)):        # no CPU path
+        m(torch.zeros(1, 2522))
+    r = SceneRF(som_sigma=2.0, std=2.0, add_fov_hor=20, add_fov_ver=8, precision="bf16")
+    r.mlp = m
+    with pytest.raises(NotImplementedError):
+        r.render_image(None, None, {})
