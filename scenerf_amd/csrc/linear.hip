@@ -135,13 +135,14 @@ template <typename O> __global__ __launch_bounds__(256) void linear_join_kernel(
 // ---- a few rows: every weight read once, straight into registers ------------------------------------------------------------------
 // A workgroup owns COLS columns (per wave where KW == 1: its four waves take four groups of them; KW == 4: the four waves split the
 // contraction of one group), a lane every 64th (256th) 16 bytes of their rows of w and of up to MR rows of x; products and sums in fp32 on the vector
-// units, which idle otherwise: the call is bound by the latency of one round of loads and by w's bytes.
+// units, which idle otherwise: the call is bound by the latency of one round of loads and by w's bytes.  One row x 2,480 x 1,536 bf16: 3.0 us
+// replayed from a graph, 7.6 MB of w, of which an empty launch is about 2.
 #define FEW_COLS 4
 template <typename T, typename O, int MR, int KW>
 __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs p) {
     typedef typename T::raw raw;
     constexpr int W = 16 / (int)sizeof(raw);
-    __shared__ float red[4][FEW_COLS * MR];
+    __shared__ float red[KW][FEW_COLS * MR];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int j0 = (KW == 1 ? blockIdx.x * 4 + wv : blockIdx.x) * FEW_COLS;
     const int pieces = (p.K + W - 1) / W;
@@ -154,19 +155,20 @@ __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs p) {
 #pragma unroll
     for (int c = 0; c < FEW_COLS; ++c) wrow[c] = (const raw*)p.B + (long)min(j0 + c, p.N - 1) * p.b_j;
     for (int t = KW == 1 ? lane : (int)threadIdx.x; t < pieces; t += 64 * KW) {
-        uint4 w[FEW_COLS], x[MR];
-        const bool whole = t * W + W <= p.K;
-        auto piece = [&](const raw* at) -> uint4 {
-            if (whole) return load16(at);
-            union { raw e[W]; uint4 v; } u;          // the row's last elements, zeros behind them
+        // a last piece that the row does not fill: the row's last 16 bytes (K >= W), those that another piece has set to zero in both operands
+        const int at = min(t * W, p.K - W), seen = (t * W - at) * (int)sizeof(raw);
+        uint32_t fresh[4];
 #pragma unroll
-            for (int e = 0; e < W; ++e) u.e[e] = t * W + e < p.K ? at[e] : (raw)0;
-            return u.v;
+        for (int i = 0; i < 4; ++i) fresh[i] = seen >= 4 * i + 4 ? 0u : seen <= 4 * i ? ~0u : ~0u << (8 * (seen - 4 * i));
+        auto piece = [&](const raw* row) -> uint4 {
+            const uint4 v = load16(row + at);
+            return make_uint4(v.x & fresh[0], v.y & fresh[1], v.z & fresh[2], v.w & fresh[3]);
         };
+        uint4 w[FEW_COLS], x[MR];
 #pragma unroll
-        for (int c = 0; c < FEW_COLS; ++c) w[c] = piece(wrow[c] + t * W);
+        for (int c = 0; c < FEW_COLS; ++c) w[c] = piece(wrow[c]);
 #pragma unroll
-        for (int m = 0; m < MR; ++m) x[m] = piece((const raw*)p.A + (long)min(m, p.M - 1) * p.a_i + t * W);
+        for (int m = 0; m < MR; ++m) x[m] = piece((const raw*)p.A + (long)min(m, p.M - 1) * p.a_i);
 #pragma unroll
         for (int m = 0; m < MR; ++m) {
             float xv[W];
@@ -180,22 +182,36 @@ __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs p) {
             }
         }
     }
+    // The lanes' sums added: with every exchange a lane gives away half of its sums and keeps the other, so that SUMS of them take
+    // SUMS - 1 exchanges instead of 6 each (8 rows x 512 x 512 bf16: 9.1 us with 6 each, 3.7 so); in the end SPAN neighbouring lanes hold sum o
+    constexpr int SUMS = FEW_COLS * MR, SPAN = 64 / SUMS;
+    float v[SUMS];
 #pragma unroll
-    for (int c = 0; c < FEW_COLS; ++c)
+    for (int t = 0; t < SUMS; ++t) v[t] = acc[t / MR][t % MR];
 #pragma unroll
-        for (int m = 0; m < MR; ++m) {
-            acc[c][m] = wave_sum(acc[c][m]);
-            if (lane == 0) red[wv][c * MR + m] = acc[c][m];
-        }
-    if constexpr (KW == 4) __syncthreads();
-    else wave_sync();
-    const int o = KW == 4 ? (int)threadIdx.x : lane;
-    if (o < FEW_COLS * MR) {
-        const int m = o % MR, j = j0 + o / MR;
-        float v = red[KW == 4 ? 0 : wv][o];
-        if constexpr (KW == 4) v = (v + red[1][o]) + (red[2][o] + red[3][o]);
-        if (m < p.M && j < p.N) epilogue_one<O>(p, m, j, v);
+    for (int step = 0; step < 6; ++step) {
+        const int half = SUMS >> (step + 1), far = 32 >> step;
+        const bool up = lane & far;
+        if (half == 0) v[0] += __shfl_xor(v[0], far, WAVE);
+#pragma unroll
+        for (int t = 0; t < SUMS / 2; ++t)
+            if (t < half) {
+                const float low = v[t], high = v[t + half];        // (v[up ? .. : ..] becomes a search through the registers)
+                const float give = __shfl_xor(up ? low : high, far, WAVE);
+                v[t] = (up ? high : low) + give;
+            }
     }
+    int o = lane / SPAN;
+    bool mine = lane % SPAN == 0;
+    if constexpr (KW == 4) {
+        if (mine) red[wv][o] = v[0];
+        __syncthreads();
+        o = (int)threadIdx.x;
+        mine = o < SUMS;
+        if (mine) v[0] = (red[0][o] + red[1][o]) + (red[2][o] + red[3][o]);
+    }
+    const int m = o % MR, j = j0 + o / MR;
+    if (mine && m < p.M && j < p.N) epilogue_one<O>(p, m, j, v[0]);
 }
 
 // ---- rows laid out anew: pitch a whole number of 16-byte pieces, zeros behind the row's end -----------------------------------------
@@ -290,7 +306,9 @@ struct LinPlan {
 static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, long K) {
     LinPlan r = {0, 1, 0, LIN_128x128};
     const int bk = staged ? LIN_CHUNK_BYTES / lin_es(type) : ANY_K;
-    if (!ax && !bx && M <= 8) {
+    // (bf16, this kernel against staged tiles: 1 row x 512 x 512 2.2 against 4.9 us, 8 rows 3.7 against 4.9, 8 x 2,480 x 1,536 5.5 against 9.7;
+    // 16 rows 5.3 against 5.0.  It reads whole 16 bytes inside the row: a shorter row takes the element loads)
+    if (!ax && !bx && M <= 8 && K >= 16 / lin_es(type)) {
         r.kind = 1;
         return r;
     }
@@ -324,8 +342,9 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
 static int64_t lin_part_bytes(const LinPlan& p, long M, int N) { return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0; }
 
 template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, hipStream_t s) {
-    // K over one wave up to 128 pieces a row, over four beyond: measured at one row of bf16 (see DESIGN.md's table)
-    if (a.K <= 128 * (16 / (int)sizeof(typename T::raw))) linear_few_kernel<T, O, MR, 1><<<cdiv(a.N, 4 * FEW_COLS), 256, 0, s>>>(a);
+    // one piece a lane and row of w: one wave a group of columns; longer rows: four (bf16, 8 rows, 512 outputs, one wave against four: 512
+    // features 3.64 and 3.55 us, 1,024 4.47 and 3.66, 2,480 6.96 and 4.61; one row of 512: 2.22 and 2.44)
+    if (a.K <= 64 * (16 / (int)sizeof(typename T::raw))) linear_few_kernel<T, O, MR, 1><<<cdiv(a.N, 4 * FEW_COLS), 256, 0, s>>>(a);
     else linear_few_kernel<T, O, MR, 4><<<cdiv(a.N, FEW_COLS), 256, 0, s>>>(a);
 }
 template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& plan, void* ws, hipStream_t s) {

@@ -272,3 +272,20 @@ def test_rows_past_32_bit_offsets():
     wt = normal(g, 2048, 16, dtype=torch.bfloat16)
     y = linear(x[:, :16], wt, activation="relu")
     hold(y[-300:], linear64(x[-300:, :16], wt, None, "relu")["y"], "last rows of a large result")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("k", [1, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 257, 511, 513, 1023, 1030, 2049])
+def test_few_rows_of_any_length(k, dtype):
+    """1 to 9 rows whose last 16 bytes overlap the piece in front of them; starts that nothing is aligned to; 8 bits too."""
+    from scenerf_amd.linear import linear, linear_8bit, quantize_rows
+    g = gen("few", k, dtype)
+    for m in (1, 2, 3, 4, 5, 8, 9):
+        n = 2 * m + 5
+        x, w = normal(g, m, k + 3, dtype=dtype)[:, 1:k + 1], normal(g, n, k + 1, dtype=dtype, scale=k ** -0.5)[:, 1:]
+        b, r = normal(g, n, dtype=dtype), normal(g, m, n, dtype=dtype)
+        hold(linear(x, w, b, activation="silu", residual=r), linear64(x, w, b, "silu", r)["y"], "%d rows" % m)
+        q, s = quantize_rows(x)
+        wq, ws = quantize_rows(w)
+        hold(linear_8bit(q, s, wq, ws, b, residual=r, out_dtype=dtype), linear64(q.float(), wq.float(), b, "none", r, scales=(s, ws), out_dtype=dtype)["y"],
+             "%d rows in 8 bits" % m)

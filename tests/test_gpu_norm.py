@@ -186,3 +186,39 @@ def test_graph_replays():
         eager = [t.detach() for t in step()]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,d", [(257, 1030), (300, 1536), (260, 2047), (400, 2480), (257, 3000), (300, 4096), (256, 4096), (1, 1025), (520, 5000)])
+def test_wide_rows_few_and_many(m, d, dtype):
+    """A workgroup a row and a wave a row, either side of the choice between them."""
+    from scenerf_amd.norm import rms_norm, rms_norm_8bit
+    g = gen("wide", m, d, dtype)
+    x, r, w = normal(g, m, d, dtype=dtype), normal(g, m, d, dtype=dtype), (1 + 0.2 * normal(g, d)).to(dtype)
+    dy, dh = normal(g, m, d, dtype=dtype), normal(g, m, d, dtype=dtype)
+    leaves = [t.requires_grad_(True) for t in (x, r, w)]
+    y, h = rms_norm(x, w, residual=r)
+    dx, dr, dw = torch.autograd.grad((y, h), leaves, (dy, dh))
+    want = rms64(x.detach(), w.detach(), 1e-6, r.detach(), dy, dh)
+    for name, t in (("y", y), ("h", h), ("dx", dx), ("dx", dr), ("dw", dw)):
+        hold(t.detach(), want[name], name)
+    q, s, h8 = rms_norm_8bit(x.detach(), w.detach(), residual=r.detach())
+    assert torch.equal(h8, h.detach())
+    exact, bound = want["y"]
+    top = exact.abs().amax(1)
+    assert bool(((s.double() - top / 448).abs() <= (top / 448) * (d + 24) * 2.0 ** -23).all())
+    # half a step of e4m3 at the value, or of its smallest values, on top of the unrounded y's own error
+    room = 2.0 ** -4 * exact.abs() + s.double()[:, None] * 2.0 ** -10 + (d + 24) * 2.0 ** -22 * exact.abs()
+    assert bool(((q.double() * s.double()[:, None] - exact).abs() <= room * (1 + 2.0 ** -10)).all())
+
+
+def test_wide_8bit_rows_whose_weighted_values_overflow():
+    """h w beyond the largest fp32, h rstd w inside it: the scale comes from y."""
+    from scenerf_amd.norm import rms_norm_8bit
+    g = gen("overflow")
+    x, w = normal(g, 3, 5000) * 1e10, torch.ones(5000, device=DEV)
+    w[7] = 1e30
+    q, s = rms_norm_8bit(x, w)
+    y = rms64(x, w, 1e-6)["y"][0]
+    assert bool(torch.isfinite(s).all()) and bool(((s.double() / (y.abs().amax(1) / 448) - 1).abs() <= 2.0 ** -10).all())
+    assert bool(((q[:, 7].double() * s.double() - y[:, 7]).abs() <= 2.0 ** -4 * y[:, 7].abs()).all())
