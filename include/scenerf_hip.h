@@ -574,7 +574,9 @@ int scenerf_hip_sphere_resample_backward_nhwc(const float* dout, int64_t planes,
 /* ---- row operators: a linear layer with its epilogue, its 8-bit form, the RMS norm and rows in 8 bits ------------------------
  * What a ResnetFC (reference scenerf/models/resnetfc.py:20-64, 133-164) of any width is made of, one entry per operator.  Rows are
  * independent; sums, norms and statistics are held in 32 bits, every output is rounded once to its type.  Matrices are row-major
- * with unit stride inside a row; a leading dimension counts ELEMENTS and may be 0 (one row read by all) or larger than the row. */
+ * with unit stride inside a row; a leading dimension counts ELEMENTS and may be 0 (one row read by all) or larger than the row.  No output may
+ * overlap an input or another output: some kernels read their rows twice. */
+#define SCENERF_NEEDS_WORKSPACE 4   /* what a call returns, having done nothing, whose workspace is missing or too small */
 #define SCENERF_T_F32  0
 #define SCENERF_T_BF16 1
 #define SCENERF_T_F16  2

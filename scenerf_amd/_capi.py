@@ -127,6 +127,7 @@ class Rms(C.Structure):
                 ("dx", vp), ("dweight", vp), ("workspace", vp), ("workspace_bytes", C.c_int64)]
 
 
+NEEDS_WORKSPACE = 4                                              # SCENERF_NEEDS_WORKSPACE
 T_F32, T_BF16, T_F16, T_E4M3 = 0, 1, 2, 3                        # SCENERF_T_*
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}       # SCENERF_ACT_*
 

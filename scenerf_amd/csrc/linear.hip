@@ -307,8 +307,8 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
     LinPlan r = {0, 1, 0, LIN_128x128};
     const int bk = staged ? LIN_CHUNK_BYTES / lin_es(type) : ANY_K;
     // (bf16, this kernel against staged tiles: 1 row x 512 x 512 2.2 against 4.9 us, 8 rows 3.7 against 4.9, 8 x 2,480 x 1,536 5.5 against 9.7;
-    // 16 rows 5.3 against 5.0.  It reads whole 16 bytes inside the row: a shorter row takes the element loads)
-    if (!ax && !bx && M <= 8 && K >= 16 / lin_es(type)) {
+    // 16 rows 5.3 against 5.0.  It reads whole 16 bytes inside the row: a shorter row takes the element loads; a launch holds 2^32 threads)
+    if (!ax && !bx && M <= 8 && K >= 16 / lin_es(type) && N < 1 << 26) {
         r.kind = 1;
         return r;
     }
@@ -372,7 +372,7 @@ template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& p
     } else {
         a.tiles_j = cdiv(a.N, ANY_TILE);
         const long blocks = (long)((a.M + ANY_TILE - 1L) / ANY_TILE) * a.tiles_j;
-        SRF_CHECK(blocks <= ROWOPS_GRID_MAX, "linear: %ld tiles are more than one launch holds", blocks);
+        SRF_CHECK(blocks < (1L << 32) / 256, "linear: %ld tiles are more than one launch holds", blocks);
         linear_any_kernel<T, O><<<dim3((unsigned)blocks, plan.splits), 256, 0, s>>>(a);
         SRF_LAUNCH_CHECK("linear_any_kernel");
     }
@@ -520,8 +520,10 @@ int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream)
     if (p->rows == 0) return 0;
     const LinPlan plan = lin_forward_plan(p);
     const int64_t lines = lin_onto_lines_bytes(p, plan), need = lines + lin_part_bytes(plan, p->rows, p->n);
-    SRF_CHECK(need == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= need), "linear_forward: workspace of %lld bytes needed",
-              (long long)need);
+    if (need > 0 && !(p->workspace && aligned16(p->workspace) && p->workspace_bytes >= need)) {
+        srf_set_error("linear_forward: workspace of %lld bytes needed", (long long)need);
+        return SCENERF_NEEDS_WORKSPACE;
+    }
     const double m = (double)p->rows, es = lin_es(p->in_type), eo = lin_es(p->out_type);
     hipStream_t s = as_stream(stream);
     SrfLaunchScope ps(s, "linear_forward", 2 * m * p->n * p->k, es * (m * p->k + (double)p->n * p->k) + eo * m * p->n);
@@ -545,8 +547,10 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
     if (int e = lin_check(p, "linear_backward", true)) return e;
     hipStream_t s = as_stream(stream);
     const BackwardPlan b = lin_backward_plan(p);
-    SRF_CHECK(b.bytes == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= b.bytes),
-              "linear_backward: workspace of %lld bytes needed", (long long)b.bytes);
+    if (b.bytes > 0 && !(p->workspace && aligned16(p->workspace) && p->workspace_bytes >= b.bytes)) {
+        srf_set_error("linear_backward: workspace of %lld bytes needed", (long long)b.bytes);
+        return SCENERF_NEEDS_WORKSPACE;
+    }
     const double m = (double)p->rows, es = lin_es(p->in_type);
     SrfLaunchScope ps(s, "linear_backward", 2 * m * p->n * p->k * (!!p->dx + !!p->dw), es * m * (p->n + 2. * p->k));
     char* ws = (char*)p->workspace;

@@ -327,7 +327,7 @@ static int lin_tile_start(const LinArgs& a, hipStream_t s) {
     auto kernel = linear_tile_kernel<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB, WHOLE>;
     SRF_ONCE_PER_DEVICE(SRF_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS)));
     const long blocks = (long)a.tiles_i * a.tiles_j * a.splits;
-    SRF_CHECK(blocks <= ROWOPS_GRID_MAX, "linear: %ld tiles are more than one launch holds", blocks);
+    SRF_CHECK(blocks < (1L << 32) / (64 * WM * WN), "linear: %ld tiles are more than one launch holds", blocks);
     kernel<<<(unsigned)blocks, 64 * WM * WN, LDS, s>>>(a);
     SRF_LAUNCH_CHECK("linear_tile_kernel");
     return 0;

@@ -514,8 +514,10 @@ int scenerf_hip_rms_backward(const scenerf_rms* p, scenerf_stream_t stream) {
     if (int e = rms_check(p, "rms_backward", true)) return e;
     if (p->rows == 0 && !p->dweight) return 0;
     const int64_t need = scenerf_hip_rms_workspace(p, 1);
-    SRF_CHECK(need == 0 || (p->workspace && aligned16(p->workspace) && p->workspace_bytes >= need), "rms_backward: workspace of %lld bytes needed",
-              (long long)need);
+    if (need > 0 && !(p->workspace && aligned16(p->workspace) && p->workspace_bytes >= need)) {
+        srf_set_error("rms_backward: workspace of %lld bytes needed", (long long)need);
+        return SCENERF_NEEDS_WORKSPACE;
+    }
     const double es = rms_es(p->type), e = (double)p->rows * p->width;
     SrfLaunchScope ps(as_stream(stream), "rms_backward", 10 * e, e * es * (2 + !!p->dh + !!p->dx));
     return rms_run(p, true, as_stream(stream));

@@ -13,14 +13,14 @@ free.  CUDA tensors only: anything else raises, there is no fallback.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .rowops import MAX_ROWS, TYPE_CODES, check_float, check_tensors, give_workspace, no_gradient, rows_forward, rows_of, run_on
+from .rowops import LINEAR, MAX_ROWS, TYPE_CODES, check_float, check_tensors, no_gradient, rows_forward, rows_of, run_on, run_rows, together
+
 
 def _activation(name: str) -> int:
     code = _capi.ACTIVATIONS.get(name)
@@ -47,58 +47,63 @@ def _check_shapes(what, x, weight, bias, residual):
 
 
 def _in_pieces(x2: torch.Tensor, w2: torch.Tensor, back: bool = False):
-    """(x, w, padded): the two as the kernels read them fast, 16 bytes at a time -- as they are, or both copied with zeros behind each row.
-    Up to 8 rows are read from any address; the step ``back`` is not."""
-    es = x2.element_size()
-    if (x2.shape[0] <= 8 and not back) or not (w2.shape[1] * es % 16 or x2.stride(0) * es % 16 or w2.stride(0) * es % 16 or x2.data_ptr() % 16 or w2.data_ptr() % 16):
-        return x2, w2, 0
-    (n, k), rows, dev, dtype = w2.shape, x2.shape[0], x2.device, x2.dtype
+    """(x's pointer, its pitch, w's pointer, its pitch, padded, what holds them): the two as the kernels read them fast, 16 bytes at a time --
+    as they are, or both copied into one buffer with zeros behind each row.  Up to 8 rows are read from any address; the step ``back`` is not."""
+    es, rows = x2.element_size(), x2.shape[0]
+    xp, wp, ldx, ldw = x2.data_ptr(), w2.data_ptr(), x2.stride(0), w2.stride(0)
+    if (rows <= 8 and not back) or not (w2.shape[1] | ldx | ldw) * es & 15 | (xp | wp) & 15:
+        return xp, ldx, wp, ldw, 0, (x2, w2)
+    (n, k), dev, dtype = w2.shape, x2.device, x2.dtype
     pitch = -(-k * es // 16) * 16 // es
-    xp, wp = torch.empty((rows, pitch), dtype=dtype, device=dev), torch.empty((n, pitch), dtype=dtype, device=dev)
-    run_on(dev, _capi.load().scenerf_hip_linear_pad, (_capi.T_E4M3 if es == 1 else TYPE_CODES[dtype], k, x2.data_ptr() or None, x2.stride(0), rows,
-                                                      xp.data_ptr() or None, w2.data_ptr(), w2.stride(0), n, wp.data_ptr()), "linear (padding)")
-    return xp, wp, 1
+    both = torch.empty((rows + n) * pitch, dtype=dtype, device=dev)
+    to = both.data_ptr()
+    run_on(dev, _capi.load().scenerf_hip_linear_pad, (_capi.T_E4M3 if es == 1 else TYPE_CODES[dtype], k, xp if rows else None, ldx, rows,
+                                                      to if rows else None, wp, ldw, n, to + rows * pitch * es), "linear (padding)")
+    return to, pitch, to + rows * pitch * es, pitch, 1, (both, None)
 
 
-def _forward(what, x2, w2, padded, n, k, bias, residual, shape, in_type, out_dtype, act, keep_z, scales=None):
-    rows, dev = x2.shape[0], x2.device
+def _forward(what, pieces, rows, n, k, bias, residual, shape, in_type, out_dtype, dev, act, keep_z, scales=None):
     y = torch.empty(shape, dtype=out_dtype, device=dev)
-    z = torch.empty((rows, n), dtype=out_dtype, device=dev) if keep_z else None
+    z = y.new_empty((rows, n)) if keep_z else None
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     r = rows_of(residual, n) if residual is not None else None
-    p = _capi.Linear(in_type, TYPE_CODES[out_dtype], act, n, k, padded, rows, x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0),
-                     None if scales is None else scales[0].data_ptr(), None if scales is None else scales[1].data_ptr(),
-                     None if bias is None else bias.data_ptr(), None if r is None else r.data_ptr(), 0 if r is None else r.stride(0),
-                     y.data_ptr(), None if z is None else z.data_ptr())
-    lib = _capi.load()
-    ws = give_workspace(lib.scenerf_hip_linear_workspace, p, 0, dev, what)  # noqa: F841 (alive up to the launch)
-    run_on(dev, lib.scenerf_hip_linear_forward, (C.byref(p),), what)
+    xp, ldx, wp, ldw, padded, _ = pieces
+    run_rows("linear", False, LINEAR.pack(
+        in_type, TYPE_CODES[out_dtype], act, n, k, padded, rows, xp, ldx, wp, ldw, 0 if scales is None else scales[0].data_ptr(),
+        0 if scales is None else scales[1].data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if r is None else r.data_ptr(),
+        0 if r is None else r.stride(0), y.data_ptr(), 0 if z is None else z.data_ptr(), 0, 0, 0, 0, 0, 0, 0), dev, what)
     return y, z
 
 
 def linear_step(x: torch.Tensor, weight: torch.Tensor, bias, residual, act: int, shape, keep_z: bool):
     """(y, what ``linear_step_back`` needs) of a layer that will be differentiated; no checks, no autograd."""
     n, k = weight.shape
-    x2, w2, padded = _in_pieces(rows_of(x, k), rows_of(weight, k), True)
-    y, z = _forward("linear", x2, w2, padded, n, k, bias, residual, shape, TYPE_CODES[x.dtype], x.dtype, act, keep_z)
-    return y, (x2, w2, z, n, k, padded, act)
+    x2 = rows_of(x, k)
+    rows = x2.shape[0]
+    pieces = _in_pieces(x2, rows_of(weight, k), True)
+    y, z = _forward("linear", pieces, rows, n, k, bias, residual, shape, TYPE_CODES[x.dtype], x.dtype, x.device, act, keep_z)
+    # (x and w or the one copy of both, z; then numbers)
+    return y, (*pieces[5], z, rows, n, k, pieces[1], pieces[4], act)
 
 
 def linear_step_back(saved, dy: torch.Tensor, x_shape, need_x: bool, need_w: bool, need_b: bool):
     """(dx, dweight, dbias), None where not needed."""
-    x2, w2, z, n, k, padded, act = saved
-    dev, dtype = dy.device, x2.dtype
-    dx = torch.empty(x_shape, dtype=dtype, device=dev) if need_x else None
-    dw = torch.empty((n, k), dtype=dtype, device=dev) if need_w else None
-    db = torch.empty((n,), dtype=dtype, device=dev) if need_b else None
+    x2, w2, z, rows, n, k, pitch, padded, act = saved
+    dev = dy.device
+    # (dy is of x's type: autograd sees to it; new_empty takes less of the host's time than empty)
+    dx = dy.new_empty(x_shape) if need_x else None
+    dw = dy.new_empty((n, k)) if need_w else None
+    db = dy.new_empty(n) if need_b else None
     dy2 = rows_of(dy, n)
-    code, lib = TYPE_CODES[dtype], _capi.load()
-    p = _capi.Linear(code, code, act, n, k, padded, x2.shape[0], x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), None, None, None, None, 0,
-                     None, None if z is None else z.data_ptr(), dy2.data_ptr(), dy2.stride(0), None if dx is None else dx.data_ptr(),
-                     None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr())
-    ws = give_workspace(lib.scenerf_hip_linear_workspace, p, 1, dev, "linear backward")  # noqa: F841 (alive up to the launch)
-    run_on(dev, lib.scenerf_hip_linear_backward, (C.byref(p),), "linear backward")
+    code, xp = TYPE_CODES[x2.dtype], x2.data_ptr()
+    if padded:
+        ldx, wp, ldw = pitch, xp + rows * pitch * x2.element_size(), pitch
+    else:       # (where a hook on saved tensors has moved them, their pitch may be another)
+        ldx, wp, ldw = x2.stride(0), w2.data_ptr(), w2.stride(0)
+    run_rows("linear", True, LINEAR.pack(
+        code, code, act, n, k, padded, rows, xp, ldx, wp, ldw, 0, 0, 0, 0, 0, 0, 0 if z is None else z.data_ptr(), dy2.data_ptr(), dy2.stride(0),
+        0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), 0, 0), dev, "linear backward")
     return dx, dw, db
 
 
@@ -129,14 +134,16 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     be, the sums in front of it are kept in the operands' type."""
     act = _activation(activation)
     dtype = x.dtype
-    check_tensors("linear", x.device, dtype, ("weight", weight), ("bias", bias), ("residual", residual))
+    if not together(x, weight, bias, residual):
+        check_tensors("linear", x.device, dtype, ("weight", weight), ("bias", bias), ("residual", residual))
     code = check_float("linear", "x", dtype)
     shape = _check_shapes("linear", x, weight, bias, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act, shape)
     n, k = weight.shape
-    return _forward("linear", *_in_pieces(rows_of(x, k), rows_of(weight, k)), n, k, bias, residual, shape, code, dtype, act, False)[0]
+    x2 = rows_of(x, k)
+    return _forward("linear", _in_pieces(x2, rows_of(weight, k)), x2.shape[0], n, k, bias, residual, shape, code, dtype, x.device, act, False)[0]
 
 
 def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -156,8 +163,9 @@ def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
             tuple(x.shape[:-1]), weight.shape[0], tuple(x_scale.shape), tuple(weight_scale.shape)))
     no_gradient("linear_8bit", x_scale, weight_scale, bias, residual)
     n, k = weight.shape
-    return _forward("linear_8bit", *_in_pieces(rows_of(x, k), rows_of(weight, k)), n, k, bias, residual, shape, _capi.T_E4M3, out_dtype, act, False,
-                    (x_scale.contiguous(), weight_scale.contiguous()))[0]
+    x2 = rows_of(x, k)
+    return _forward("linear_8bit", _in_pieces(x2, rows_of(weight, k)), x2.shape[0], n, k, bias, residual, shape, _capi.T_E4M3, out_dtype, dev, act,
+                    False, (x_scale.contiguous(), weight_scale.contiguous()))[0]
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -12,20 +12,19 @@ unrounded h).  CUDA tensors only: anything else raises, there is no fallback.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from . import _capi
-from .rowops import MAX_ROWS, TYPE_CODES, check_float, check_tensors, give_workspace, no_gradient, rows_forward, rows_of, run_on
+from .rowops import MAX_ROWS, RMS, TYPE_CODES, check_float, check_tensors, no_gradient, rows_forward, rows_of, run_rows, together
 
 
 def _check(what, x, weight, residual, eps) -> None:
     shape = x.shape
-    check_tensors(what, x.device, x.dtype, ("weight", weight), ("residual", residual))
+    if not together(x, weight, residual):
+        check_tensors(what, x.device, x.dtype, ("weight", weight), ("residual", residual))
     check_float(what, "x", x.dtype)
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("%s: x must have at least one column (got %s)" % (what, tuple(shape)))
@@ -45,14 +44,12 @@ def rms_step_back(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, eps
     width, dev = h.shape[-1], h.device
     h2, dy2, w = rows_of(h, width), rows_of(dy, width), weight.contiguous()
     dh2 = rows_of(dh, width) if dh is not None else None
-    dx = torch.empty(dy.shape, dtype=h.dtype, device=dev) if need_x else None
-    dw = torch.empty((width,), dtype=h.dtype, device=dev) if need_w else None
-    p = _capi.Rms(TYPE_CODES[h.dtype], width, h2.shape[0], eps, h2.data_ptr(), h2.stride(0), None, 0, w.data_ptr(), None, None, None, None,
-                  rstd.data_ptr(), dy2.data_ptr(), dy2.stride(0), None if dh2 is None else dh2.data_ptr(), 0 if dh2 is None else dh2.stride(0),
-                  None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr())
-    lib = _capi.load()
-    ws = give_workspace(lib.scenerf_hip_rms_workspace, p, 1, dev, "rms_norm backward")  # noqa: F841 (alive up to the launch)
-    run_on(dev, lib.scenerf_hip_rms_backward, (C.byref(p),), "rms_norm backward")
+    dx = dy.new_empty(dy.shape) if need_x else None
+    dw = dy.new_empty(width) if need_w else None
+    run_rows("rms", True, RMS.pack(
+        TYPE_CODES[h.dtype], width, h2.shape[0], eps, h2.data_ptr(), h2.stride(0), 0, 0, w.data_ptr(), 0, 0, 0, 0, rstd.data_ptr(),
+        dy2.data_ptr(), dy2.stride(0), 0 if dh2 is None else dh2.data_ptr(), 0 if dh2 is None else dh2.stride(0),
+        0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0, 0), dev, "rms_norm backward")
     return dx, dw
 
 

@@ -2,7 +2,8 @@
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+import struct
+from typing import Any, Dict
 
 import torch
 
@@ -38,29 +39,65 @@ def check_float(what: str, name: str, dtype: torch.dtype) -> int:
     return code
 
 
+def together(x: torch.Tensor, *others) -> bool:
+    """All on x's GPU and of x's type: the usual call, without what ``check_tensors`` needs to say otherwise."""
+    dtype, dev = x.dtype, x.device
+    for t in others:
+        if t is not None and (t.dtype is not dtype or t.device != dev):
+            return False
+    return x.is_cuda
+
+
+# The arguments of one call, laid out as scenerf_linear / scenerf_rms: packed bytes cost a small call half of what the structures do
+# (tests/test_rowops_refusals.py holds them to the structures' offsets).  The last two fields are the workspace and its bytes.
+LINEAR = struct.Struct("@6i19q")
+RMS = struct.Struct("@2iqf18q")
+_WORKSPACE = struct.Struct("@2q")
+_entries: Dict[str, Any] = {}
+
+
+def _entry(name: str, backward: bool):
+    """(the call, its workspace query) of ``scenerf_hip_<name>_*`` on packed bytes."""
+    key = name + ("_backward" if backward else "_forward")
+    got = _entries.get(key)
+    if got is None:
+        lib = _capi.load()
+        run, query = lib["scenerf_hip_" + key], lib["scenerf_hip_%s_workspace" % name]
+        run.argtypes, run.restype = [C.c_char_p, C.c_void_p], C.c_int
+        query.argtypes, query.restype = [C.c_char_p, C.c_int], C.c_int64
+        got = _entries[key] = (run, query)
+    return got
+
+
 def run_on(dev: torch.device, fn, args: tuple, what: str) -> None:
     """``fn(*args, stream)`` on ``dev``'s current stream, with ``dev`` current."""
-    index = dev.index
-    if index == torch.cuda.current_device():
-        # (torch.cuda.current_stream(dev).cuda_stream without the Stream object: a fifth of a small call's host time)
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
+    if dev.index != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            return run_on(dev, fn, args, what)
+    _capi.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), what)
+
+
+def run_rows(name: str, backward: bool, args: bytes, dev: torch.device, what: str) -> None:
+    """One call on ``dev``'s current stream, with ``dev`` current and a workspace of the calling stream's own where the call needs one: two
+    captured graphs, or two streams, never share it."""
+    index = dev.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return run_rows(name, backward, args, dev, what)
+    run, query = _entry(name, backward)
+    # (torch.cuda.current_stream(dev).cuda_stream without the Stream object)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    rc = _capi.NEEDS_WORKSPACE if backward else run(args, stream)     # (few forward calls need one, nearly all backward calls do)
+    if rc == _capi.NEEDS_WORKSPACE:
+        need = query(args, 1 if backward else 0)
+        if need < 0:
+            _capi.check(1, what)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            args = args[:-_WORKSPACE.size] + _WORKSPACE.pack(ws.data_ptr(), need)
+        rc = run(args, stream)
     if rc:
         _capi.check(rc, what)
-
-
-def give_workspace(fn, args, backward: int, dev: torch.device, what: str) -> Optional[torch.Tensor]:
-    """A workspace of the calling stream's own, for one call: two captured graphs, or two streams, never share one."""
-    need = fn(C.byref(args), backward)
-    if need == 0:
-        return None
-    if need < 0:
-        _capi.check(1, what)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    return ws
 
 
 def no_gradient(what: str, *tensors) -> None:
@@ -79,13 +116,13 @@ def rows_forward(what, x, weight, residual, eps, *, quantize=False, keep_rstd=Fa
     if weight is not None and not weight.is_contiguous():
         weight = weight.contiguous()
     r2 = rows_of(residual, width) if residual is not None else None
-    h = torch.empty(shape, dtype=dtype, device=dev) if residual is not None else None
-    out = torch.empty(shape, dtype=torch.float8_e4m3fn if quantize else dtype, device=dev)
+    h = x.new_empty(shape) if residual is not None else None
+    out = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev) if quantize else x.new_empty(shape)
     scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if quantize else None
     rstd = torch.empty((rows,), dtype=torch.float32, device=dev) if keep_rstd else None
-    p = _capi.Rms(TYPE_CODES[dtype], width, rows, eps, x2.data_ptr(), x2.stride(0), None if r2 is None else r2.data_ptr(),
-                  0 if r2 is None else r2.stride(0), None if weight is None else weight.data_ptr(), None if h is None else h.data_ptr(),
-                  None if quantize else out.data_ptr(), out.data_ptr() if quantize else None, None if scale is None else scale.data_ptr(),
-                  None if rstd is None else rstd.data_ptr())
-    run_on(dev, _capi.load().scenerf_hip_rms_forward, (C.byref(p),), what)
+    run_rows("rms", False, RMS.pack(
+        TYPE_CODES[dtype], width, rows, eps, x2.data_ptr(), x2.stride(0), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0),
+        0 if weight is None else weight.data_ptr(), 0 if h is None else h.data_ptr(), 0 if quantize else out.data_ptr(),
+        out.data_ptr() if quantize else 0, 0 if scale is None else scale.data_ptr(), 0 if rstd is None else rstd.data_ptr(),
+        0, 0, 0, 0, 0, 0, 0, 0), dev, what)
     return out, scale, h, rstd, x2

@@ -289,3 +289,21 @@ def test_few_rows_of_any_length(k, dtype):
         wq, ws = quantize_rows(w)
         hold(linear_8bit(q, s, wq, ws, b, residual=r, out_dtype=dtype), linear64(q.float(), wq.float(), b, "none", r, scales=(s, ws), out_dtype=dtype)["y"],
              "%d rows in 8 bits" % m)
+
+
+@pytest.mark.parametrize("k,pitch", [(48, 48), (48, 64), (42, 42)])
+def test_saved_tensors_moved_by_hooks(k, pitch):
+    """torch.autograd.graph.save_on_cpu hands the backward pass other copies, with another pitch, of what the forward saved."""
+    from scenerf_amd.linear import linear
+    g = gen("hooks", k, pitch)
+    bf = torch.bfloat16
+    x, w, b = normal(g, 300, pitch, dtype=bf)[:, :k].requires_grad_(True), normal(g, 130, k, dtype=bf, scale=k ** -0.5).requires_grad_(True), None
+    dy = normal(g, 300, 130, dtype=bf)
+    want = torch.autograd.grad(linear(x, w, b, activation="gelu"), (x, w), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = linear(x, w, b, activation="gelu")
+    got = torch.autograd.grad(y, (x, w), dy)
+    full = linear64(x.detach(), w.detach(), b, "gelu", None, dy)
+    hold(got[0], full["dx"], "dx")
+    hold(got[1], full["dw"], "dw")
+    assert want[0].shape == got[0].shape

@@ -174,8 +174,8 @@ def test_render_and_its_gradients_against_the_oracle(R, precision, monkeypatch):
                            som_choices=(aux["bmu"].reshape(R, -1).long(), aux["kl_mask"].reshape(R, -1).bool()))
     loss_of(ref).backward()
     tol = dict(depth=1e-4, color=1e-5, grad=1e-2) if precision == "fp32" else dict(depth=2e-2, color=2e-2, grad=1.5e-1)
-    assert float(((out["depth"].cpu() - ref["depth"]).abs() / (1 + ref["depth"].abs())).max()) <= tol["depth"]
-    assert float((out["color"].cpu() - ref["color"]).abs().max()) <= tol["color"]
+    assert float(((out["depth"].detach().cpu() - ref["depth"].detach()).abs() / (1 + ref["depth"].detach().abs())).max()) <= tol["depth"]
+    assert float((out["color"].detach().cpu() - ref["color"].detach()).abs().max()) <= tol["color"]
     for mod, want in ((m.mlp, po), (m.mlp_gaussian, pg)):
         for k, v in mod.named_parameters():
             assert off(v.grad.cpu(), want[k].grad) <= tol["grad"], (k, off(v.grad.cpu(), want[k].grad))

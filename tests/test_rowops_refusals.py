@@ -107,3 +107,25 @@ def test_the_net_with_norms():
     r.mlp = m
     with pytest.raises(NotImplementedError):
         r.render_image(None, None, {})
+
+
+def test_packed_arguments_are_the_structures():
+    from scenerf_amd.rowops import LINEAR, RMS
+    for packer, kind in ((LINEAR, _capi.Linear), (RMS, _capi.Rms)):
+        assert packer.size == C.sizeof(kind)
+        values = [2.5 if t is C.c_float else i + 1 for i, (_, t) in enumerate(kind._fields_)]
+        got = kind.from_buffer_copy(packer.pack(*values))
+        assert [getattr(got, name) for name, _ in kind._fields_] == values
+
+
+def test_a_call_without_its_workspace_says_so():
+    lib = _capi.load()
+    p = _capi.Linear(in_type=0, out_type=0, activation=0, n=4, k=8, rows=3)
+    p.dy, p.x, p.w, p.db, p.ld_dy, p.ldx, p.ldw = 16, 16, 16, 16, 4, 8, 8
+    assert lib.scenerf_hip_linear_workspace(C.byref(p), 1) > 0
+    assert lib.scenerf_hip_linear_backward(C.byref(p), None) == _capi.NEEDS_WORKSPACE
+    p.workspace, p.workspace_bytes = 16, 1
+    assert lib.scenerf_hip_linear_backward(C.byref(p), None) == _capi.NEEDS_WORKSPACE
+    r = _capi.Rms(type=0, width=8, rows=3, eps=1e-6)
+    r.x, r.weight, r.rstd, r.dy, r.dweight = 16, 16, 16, 16, 16
+    assert lib.scenerf_hip_rms_backward(C.byref(r), None) == _capi.NEEDS_WORKSPACE
