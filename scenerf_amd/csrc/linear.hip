@@ -242,8 +242,9 @@ template <typename O, int ACT> __device__ static inline void slopes(float (&g)[8
 #pragma unroll
     for (int e = 0; e < 8; ++e) g[e] = e < valid ? g[e] * act_slope<ACT>(z[e]) : 0.f;
 }
-// A workgroup's 256 threads stand as 2^lx columns of 8 by 256 / 2^lx rows (2^lx: 32, or what a narrower matrix needs: at 128 columns a
-// fixed 32 left half the threads idle, 150 us for 262,144 x 128 fp32); two rows a thread are in flight.
+// A workgroup's 256 threads stand as 2^lx columns of 8 by 256 / 2^lx rows (2^lx: 64, a wave a row, or what a narrower matrix needs: at 128
+// columns a fixed 32 left half the threads idle, 150 us for 262,144 x 128 fp32 instead of 78; 32 at 512 columns took 111 us for 153,600 rows
+// of bf16, 64 100); two rows a thread are in flight.  Bound by HBM: 4.7 and 5.2 TB/s.
 template <typename O, bool WHOLE>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld_dy, const void* z_, void* dz_, int pitch, float* part, int M, int N,
                                                         int act, int strip, int lx) {
@@ -486,7 +487,7 @@ static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
 }
 template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardPlan& b, void* dz, float* part, hipStream_t s) {
     int lx = 2;
-    while (lx < 5 && (8 << lx) < p->n) ++lx;
+    while (lx < 6 && (8 << lx) < p->n) ++lx;
     const dim3 grid(b.strips, cdiv(p->n, 8 << lx));
     SRF_CHECK(grid.y <= 65535, "linear_backward: n is too large");
     if (p->n % 8 == 0) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
