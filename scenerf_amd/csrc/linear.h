@@ -15,11 +15,10 @@ struct LinArgs {
     int act, tiles_i, tiles_j, splits, k_split;     // k_split: contraction elements per split
 };
 
-__device__ static inline float act_any(int act, float v) {
-    if (act == SCENERF_ACT_RELU) return act_fwd<SCENERF_ACT_RELU>(v);
-    if (act == SCENERF_ACT_GELU) return act_fwd<SCENERF_ACT_GELU>(v);
-    if (act == SCENERF_ACT_SILU) return act_fwd<SCENERF_ACT_SILU>(v);
-    return v;
+template <int W> __device__ static inline void act_any(int act, float (&v)[W]) {
+    if (act == SCENERF_ACT_RELU) act_fwd<SCENERF_ACT_RELU, W>(v);
+    else if (act == SCENERF_ACT_GELU) act_fwd<SCENERF_ACT_GELU, W>(v);
+    else if (act == SCENERF_ACT_SILU) act_fwd<SCENERF_ACT_SILU, W>(v);
 }
 // z as it is kept for the backward pass, in O.  A positive z that rounds to zero (fp16) is kept as the smallest positive value: relu's
 // slope there is 1, and the other slopes do not notice.
@@ -32,7 +31,9 @@ template <typename O> __device__ static inline void epilogue_one(const LinArgs& 
     if (p.row_scale) v = v * p.row_scale[i] * p.col_scale[j];
     if (p.bias) v += O::to_f32(((const raw*)p.bias)[j]);
     if (p.z) ((raw*)p.z)[i * p.N + j] = O::from_f32(keep_z<O>(v));
-    v = act_any(p.act, v);
+    float one[1] = {v};
+    act_any<1>(p.act, one);
+    v = one[0];
     if (p.residual) v += O::to_f32(((const raw*)p.residual)[i * p.ld_residual + j]);
     ((raw*)p.out)[i * p.N + j] = O::from_f32(v);
 }
@@ -72,18 +73,7 @@ __device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<
         for (int e = 0; e < W; ++e) t[e] = keep_z<O>(v[e]);
         store_some<O, W, WHOLE>((raw*)p.z + i * p.N + j, n, p.N % W, t);
     }
-    if (p.act != SCENERF_ACT_NONE) {
-        if (p.act == SCENERF_ACT_RELU) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) v[e] = act_fwd<SCENERF_ACT_RELU>(v[e]);
-        } else if (p.act == SCENERF_ACT_GELU) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) v[e] = act_fwd<SCENERF_ACT_GELU>(v[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < W; ++e) v[e] = act_fwd<SCENERF_ACT_SILU>(v[e]);
-        }
-    }
+    act_any<W>(p.act, v);
     if (p.residual) {
         float t[W];
         unpack16<O>(res, t);

@@ -238,9 +238,10 @@ __global__ __launch_bounds__(256) void linear_pad_kernel(PadSide x, PadSide w, i
 }
 
 // ---- dz = dy act'(z), and the column sums of dz by strips of rows ------------------------------------------------------------------
-template <typename O, int ACT> __device__ static inline void slopes(float (&g)[8], const float (&z)[8], int valid) {
+template <int ACT> __device__ static inline void slopes(float (&g)[8], float (&z)[8], int valid) {
+    act_slope<ACT, 8>(z);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] = e < valid ? g[e] * act_slope<ACT>(z[e]) : 0.f;
+    for (int e = 0; e < 8; ++e) g[e] = e < valid ? g[e] * z[e] : 0.f;
 }
 // A workgroup's 256 threads stand as 2^lx columns of 8 by 256 / 2^lx rows (2^lx: 64, a wave a row, or what a narrower matrix needs: at 128
 // columns a fixed 32 left half the threads idle, 150 us for 262,144 x 128 fp32 instead of 78; 32 at 512 columns took 111 us for 153,600 rows
@@ -270,9 +271,9 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 if (q == 1 && !two) continue;
-                if (act == SCENERF_ACT_GELU) slopes<O, SCENERF_ACT_GELU>(g[q], z[q], N - j0);
-                else if (act == SCENERF_ACT_SILU) slopes<O, SCENERF_ACT_SILU>(g[q], z[q], N - j0);
-                else if (act == SCENERF_ACT_RELU) slopes<O, SCENERF_ACT_RELU>(g[q], z[q], N - j0);
+                if (act == SCENERF_ACT_GELU) slopes<SCENERF_ACT_GELU>(g[q], z[q], N - j0);
+                else if (act == SCENERF_ACT_SILU) slopes<SCENERF_ACT_SILU>(g[q], z[q], N - j0);
+                else if (act == SCENERF_ACT_RELU) slopes<SCENERF_ACT_RELU>(g[q], z[q], N - j0);
                 if (dz_) store_vec<O, 8>((raw*)dz_ + (r + q * rows) * pitch + j0, g[q]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum[e] += g[q][e];
