@@ -304,40 +304,66 @@ struct LinPlan {
     int kind, splits, k_split;
     LinTile tile;
 };
-// `staged`: both operands are in 16-byte pieces (lin_staged)
+// What a tile costs, in us: a workgroup's start and end, and a chunk of 128 bytes of the contraction with 1, 2, 3 workgroups on a CU (as many as
+// their LDS lets in).  Fitted to products of 1,024 to 153,600 rows by 48 to 2,480 features, forward and both gradients: on 364 of 366 of them
+// (bf16 and fp32) what the plan chooses took no more than 7 percent or 2 us above the fastest of all tiles and splits.  Where the tiles
+// differ most: 153,600 x 2,480 x 1,536 bf16 256^2 1,034 us and 128^2 1,521; 262,144 x 128 x 128 50 and 32; 1,024 x 512 x 512 20, 9.8 and 64^2
+// 6.1; dw of 12,288 rows x 512 x 2,480 54, 52 (6 splits) and 64^2 unsplit 108.
+struct LinTileCost { LinTile tile; int per_cu; double ends, chunk[3]; };
+static const LinTileCost kLinCost16[] = {{LIN_256x256, 1, 9.0, {1.7}}, {LIN_128x128, 2, 4.7, {0.61, 1.1}}, {LIN_64x64, 3, 1.8, {0.35, 0.55, 0.78}}};
+static const LinTileCost kLinCost32[] = {{LIN_128x128, 2, 4.7, {1.8, 3.6}}, {LIN_64x64, 3, 1.8, {0.5, 0.95, 1.55}}};
+#define LIN_BYTES_US 5.0e6          // of HBM
+#define LIN_PART_BYTES_US 7.0e6     // of splits' sums, written and read again from the last cache
+#define LIN_MIN_CHUNKS 8            // a split keeps at least so many: its ends cost as much
+
+// `staged`: both operands are in 16-byte pieces
 static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, long K) {
     LinPlan r = {0, 1, 0, LIN_128x128};
-    const int bk = staged ? LIN_CHUNK_BYTES / lin_es(type) : ANY_K;
     // (bf16, this kernel against staged tiles: 1 row x 512 x 512 2.2 against 4.9 us, 8 rows 3.7 against 4.9, 8 x 2,480 x 1,536 5.5 against 9.7;
     // 16 rows 5.3 against 5.0.  It reads whole 16 bytes inside the row: a shorter row takes the element loads; a launch holds 2^32 threads)
     if (!ax && !bx && M <= 8 && K >= 16 / lin_es(type) && N < 1 << 26) {
         r.kind = 1;
         return r;
     }
-    long rows = ANY_TILE, cols = ANY_TILE, slots = 512;
-    if (staged) {
+    const int bk = staged ? LIN_CHUNK_BYTES / lin_es(type) : ANY_K;
+    const long chunks = (K + bk - 1) / bk;
+    auto tiles_of = [&](long rows, long cols) { return ((M + rows - 1) / rows) * ((N + cols - 1) / cols); };
+    long splits = 1;
+    if (!staged) {
+        const long tiles = tiles_of(ANY_TILE, ANY_TILE);
+        splits = min(tiles > 0 ? 512 / tiles : 1, chunks / LIN_MIN_CHUNKS);
+    } else if (N <= 32) {
         r.kind = 2;
-        // Rounds over the chip's workgroup slots (1, 2, 3 a CU by their LDS), times what a round takes: measured at 4,800 to 153,600 rows and
-        // 48 to 2,480 features, 8 : 4.7 : 2.4 whatever the length (20,000 x 512 x 512 bf16: 1 round of 23 us, 2 of 13.5, 4 of 7).  The
-        // large tile reads half the operand bytes per product and wins where the matrix fills it (8,192^3: 878 against 1,182 us), the
-        // small one where rows are few (1,024 x 512 x 512: 6.1 us against 9.8 and 20) or the result is narrow.
-        auto tiles = [&](LinTile t) { return ((M + kLinTileRows[t] - 1) / kLinTileRows[t]) * ((N + kLinTileCols[t] - 1) / kLinTileCols[t]); };
-        auto cost = [&](LinTile t, long per, double round) { return (tiles(t) + per - 1) / per * round; };
-        const double big = type == SCENERF_T_F32 ? 1e30 : cost(LIN_256x256, 256, 8.0), mid = cost(LIN_128x128, 512, 4.7), small = cost(LIN_64x64, 768, 2.4);
-        if (N <= 32) r.tile = LIN_128x32;
-        else if (K >= 16384 && M > 64 && N > 64) r.tile = type != SCENERF_T_F32 && M > 128 && N > 128 ? LIN_256x256 : LIN_128x128;    // (splits fill the chip)
-        else r.tile = big <= mid && big <= small ? LIN_256x256 : mid <= small ? LIN_128x128 : LIN_64x64;
-        rows = kLinTileRows[r.tile];
-        cols = kLinTileCols[r.tile];
-        // The contraction is split where the tiles leave CUs idle: one workgroup a CU for a short one (three splits of 152 tiles took
-        // 60 us against 42 unsplit), every slot for a long one; a split keeps at least 8 chunks (the
-        // join is a launch of its own: 1,024 x 512 x 512 bf16 took 13 us in two splits, 6 in one).
-        slots = K < 16384 ? 256 : r.tile == LIN_256x256 ? 256 : r.tile == LIN_128x128 ? 512 : 768;
+        r.tile = LIN_128x32;
+        const long tiles = tiles_of(128, 32);
+        splits = min(tiles > 0 ? (chunks < 256 ? 256 : 768) / tiles : 1, chunks / LIN_MIN_CHUNKS);
+    } else {
+        r.kind = 2;
+        const LinTileCost* cost = type == SCENERF_T_F32 ? kLinCost32 : kLinCost16;
+        const int kinds = type == SCENERF_T_F32 ? 2 : 3;
+        const double bytes = ((double)M * K + (double)N * K + (double)M * N) * lin_es(type) / LIN_BYTES_US;
+        double best = 1e300;
+        for (int c = 0; c < kinds; ++c) {
+            const LinTileCost& t = cost[c];
+            const long tiles = tiles_of(kLinTileRows[t.tile], kLinTileCols[t.tile]), slots = 256L * t.per_cu;
+            const long most = max(1L, min(slots / max(1L, tiles), chunks / LIN_MIN_CHUNKS));
+            // 1, 2 or 3 workgroups a CU, or none of it split
+            for (int per_cu = 0; per_cu <= t.per_cu; ++per_cu) {
+                const long s = per_cu == 0 ? 1 : min(most, 256L * per_cu / max(1L, tiles));
+                if (s < 1) continue;
+                const long work = tiles * s, each = (chunks + s - 1) / s, full = work / slots, rest = work % slots;
+                double us = full * (each * t.chunk[t.per_cu - 1] + t.ends);
+                if (rest > 0) {         // (a CU gets along faster where others have nothing to do)
+                    const int on_cu = (int)((rest + 255) / 256);
+                    us += each * t.chunk[on_cu - 1] * (0.75 + 0.25 * rest / (256.0 * on_cu)) + t.ends;
+                }
+                us = max(us, bytes + 2.0);
+                if (s > 1) us += 5.0 + 8.0 * s * M * N / LIN_PART_BYTES_US;
+                if (us < best) { best = us; r.tile = t.tile; splits = s; }
+            }
+        }
     }
-    const long n_tiles = ((M + rows - 1) / rows) * ((N + cols - 1) / cols);
-    long s = n_tiles > 0 ? slots / n_tiles : 1;
-    if (s > K / (8 * bk)) s = K / (8 * bk);
-    r.splits = s < 1 ? 1 : s > 256 ? 256 : (int)s;
+    r.splits = (int)max(1L, min(splits, 256L));
     r.k_split = (int)(((K + r.splits - 1) / r.splits + bk - 1) / bk * bk);
     return r;
 }
