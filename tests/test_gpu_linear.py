@@ -307,3 +307,37 @@ def test_saved_tensors_moved_by_hooks(k, pitch):
     hold(got[0], full["dx"], "dx")
     hold(got[1], full["dw"], "dw")
     assert want[0].shape == got[0].shape
+
+
+# sizes from which the plan takes each of its tiles, whole and in splits, forward and for both gradients, rows and columns that end inside one
+TILES = [(9001, 42, 1541), (9001, 1541, 48), (16385, 4104, 130), (20011, 264, 48), (20011, 42, 263), (1001, 4104, 776), (20011, 199, 520),
+         (300, 16392, 520), (300, 2056, 1543), (5003, 16392, 130), (2049, 2056, 520), (1001, 1032, 1544), (33000, 2048, 264)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", TILES)
+def test_every_tile(m, k, n, dtype):
+    from scenerf_amd.linear import linear
+    g = gen("tile", m, k, n, dtype)
+    x, w, b, r = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5), normal(g, n, dtype=dtype), normal(g, m, n, dtype=dtype)
+    dy = normal(g, m, n, dtype=dtype)
+    want = linear64(x, w, b, "gelu", r, dy)
+    with torch.no_grad():
+        hold(linear(x, w, b, activation="gelu", residual=r), want["y"], "y")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = linear(*leaves, activation="gelu", residual=r)
+    hold(y.detach(), want["y"], "y")
+    for name, got in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves, dy)):
+        hold(got, want[name], name)
+
+
+@pytest.mark.parametrize("out", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(20011, 42, 263), (300, 16392, 1544), (9001, 42, 1541), (9001, 16392, 130), (20011, 1544, 520), (300, 4104, 48)])
+def test_every_tile_in_8_bits(m, k, n, out):
+    from scenerf_amd.linear import linear_8bit, quantize_rows
+    g = gen("tile8", m, k, n, out)
+    q, s = quantize_rows(normal(g, m, k))
+    wq, ws = quantize_rows(normal(g, n, k, scale=k ** -0.5))
+    b, r = normal(g, n, dtype=out), normal(g, m, n, dtype=out)
+    hold(linear_8bit(q, s, wq, ws, b, activation="silu", residual=r, out_dtype=out),
+         linear64(q.float(), wq.float(), b, "silu", r, scales=(s, ws), out_dtype=out)["y"])
