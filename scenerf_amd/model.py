@@ -150,6 +150,7 @@ class ResnetFC(nn.Module):
     (resnetfc.py:133-164: rows of latent and encoded point side by side).  ``eight_bit = True`` makes ``no_grad`` renders of it multiply
     e4m3 rows by e4m3 weights in the hidden layers.
     """
+    norm, activation, norm_eps, eight_bit = "none", "relu", 1e-6, False      # (what a net pickled before these existed is)
 
     def __init__(self, d_in: int = 42, d_out: int = 4, n_blocks: int = 3, d_latent: int = 2480, d_hidden: int = 512, norm: str = "none",
                  activation: Optional[str] = None, norm_eps: float = 1e-6):

@@ -58,7 +58,7 @@ def evaluate(params: NetParams, z: torch.Tensor, x: torch.Tensor) -> torch.Tenso
         t = linear(a, *net.fc0[b], activation=params.activation)
         h = linear(t, *net.fc1[b], residual=h)
     a = rms_norm(h, net.norm_out, eps=params.eps)
-    return linear(a.float(), net.w_out, net.b_out).view(*lead, -1).to(z.dtype)
+    return linear(a.float(), net.w_out, net.b_out).view(*lead, net.w_out.shape[0]).to(z.dtype)
 
 
 class PackedNormedMLP:

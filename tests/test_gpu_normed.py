@@ -81,6 +81,21 @@ def test_the_net_and_its_gradients_against_64_bits(rows, n_blocks, d_hidden, act
         assert lim is None or off(a, b) <= lim, (name, off(a, b), lim)
 
 
+def test_no_rows_one_row_and_more_dimensions():
+    m = net(5, 2, 2, 32)
+    zx = torch.randn(3, 4, 2522, device=DEV)
+    with torch.no_grad():
+        y = m(zx)
+        assert y.shape == (3, 4, 2) and m(zx[:0]).shape == (0, 4, 2) and m(zx[0, 0]).shape == (2,)
+        assert off(m(zx[1, 2]), y[1, 2]) <= room(torch.float32, 2, 1) and torch.equal(m(zx.view(12, 2522)).view(3, 4, 2), y)
+    got = torch.autograd.grad(m(zx[:0].requires_grad_(True)).sum(), list(m.parameters()))
+    assert all(float(t.abs().max()) == 0.0 for t in got)
+    with pytest.raises(ValueError):
+        m(zx[..., :2500])
+    with pytest.raises(TypeError):
+        m(zx, zx)
+
+
 def packed(m, precision, trainable):
     from scenerf_amd.normed import PackedNormedMLP
     cfg = SceneRF(som_sigma=2.0, std=2.0, add_fov_hor=20, add_fov_ver=8, precision=precision).render_cfg
