@@ -97,12 +97,30 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
 }
 // the splits' sums, added in a fixed order, then the epilogue: a workgroup owns 32 pieces of W results, 8 threads each, thread y of them
 // adds splits y, y + 8, ..  Bound by the sums' bytes: 64 splits of 512 x 512 13.7 us, 4.9 TB/s
-template <typename O> __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs p) {
+// db's column sums ride along in front of dw's join, a launch less: each of `sums.blocks` workgroups adds 16 columns in 16 chains
+struct ColumnSums { const float* part; void* out; int count, width, blocks; };
+template <typename O> __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs p, ColumnSums sums) {
     constexpr int W = 16 / (int)sizeof(typename O::raw);
     __shared__ float red[8][32][W + 1];
+    if ((int)blockIdx.x < sums.blocks) {
+        float (*chain)[17] = (float (*)[17])red;
+        const int cx = threadIdx.x & 15, cy = threadIdx.x >> 4, col = blockIdx.x * 16 + cx;
+        float s = 0.f;
+        if (col < sums.width) {
+#pragma unroll 8
+            for (int i = cy; i < sums.count; i += 16) s += sums.part[(size_t)i * sums.width + col];
+        }
+        chain[cy][cx] = s;
+        __syncthreads();
+        s = chain[cx][cy];            // column cy, chain cx
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, WAVE);
+        if (cx == 0 && (int)blockIdx.x * 16 + cy < sums.width) ((typename O::raw*)sums.out)[blockIdx.x * 16 + cy] = O::from_f32(s);
+        return;
+    }
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, per = (p.N + W - 1) / W;
     const long pieces = (long)p.M * per;
-    for (long t0 = (long)blockIdx.x * 32; t0 < pieces; t0 += (long)gridDim.x * 32) {
+    for (long t0 = (long)(blockIdx.x - sums.blocks) * 32; t0 < pieces; t0 += (long)(gridDim.x - sums.blocks) * 32) {
         const long i = (t0 + tx) / per;
         const int j = (int)((t0 + tx) - i * per) * W;
         const bool ok = t0 + tx < pieces;
@@ -382,11 +400,25 @@ template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, 
     if (a.K <= 64 * (16 / (int)sizeof(typename T::raw))) linear_few_kernel<T, O, MR, 1><<<cdiv(a.N, 4 * FEW_COLS), 256, 0, s>>>(a);
     else linear_few_kernel<T, O, MR, 4><<<cdiv(a.N, FEW_COLS), 256, 0, s>>>(a);
 }
-template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& plan, void* ws, hipStream_t s) {
+static void lin_fill(LinArgs& a, const LinPlan& plan, void* ws) {
     a.splits = plan.splits;
     a.k_split = plan.k_split;
     a.part = plan.splits > 1 ? (float*)ws : nullptr;
+    if (plan.kind == 2) {
+        a.tiles_i = (int)((a.M + (long)kLinTileRows[plan.tile] - 1) / kLinTileRows[plan.tile]);
+        a.tiles_j = (int)((a.N + (long)kLinTileCols[plan.tile] - 1) / kLinTileCols[plan.tile]);
+    }
+}
+template <typename O> static int lin_join(const LinArgs& a, const ColumnSums& sums, hipStream_t s) {
     constexpr int W = 16 / (int)sizeof(typename O::raw);
+    const long work = ((long)a.M * ((a.N + W - 1) / W) + 31) / 32;
+    linear_join_kernel<O><<<(unsigned)(work < 16384 ? work : 16384) + sums.blocks, 256, 0, s>>>(a, sums);
+    SRF_LAUNCH_CHECK("linear_join_kernel");
+    return 0;
+}
+// `sums`: column sums that ride along where the product is joined (plan.splits > 1)
+template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& plan, void* ws, const ColumnSums& sums, hipStream_t s) {
+    lin_fill(a, plan, ws);
     if (plan.kind == 1) {
         if (a.M == 1) lin_few<T, O, 1>(a, s);
         else if (a.M == 2) lin_few<T, O, 2>(a, s);
@@ -396,8 +428,6 @@ template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& p
         return 0;
     }
     if (plan.kind == 2) {
-        a.tiles_i = (int)((a.M + (long)kLinTileRows[plan.tile] - 1) / kLinTileRows[plan.tile]);
-        a.tiles_j = (int)((a.N + (long)kLinTileCols[plan.tile] - 1) / kLinTileCols[plan.tile]);
         int e;
         if constexpr (T::code == SCENERF_T_F32) e = linear_tile_f32(a, plan.tile, s);
         else if constexpr (T::code == SCENERF_T_BF16) e = linear_tile_bf16(a, plan.tile, s);
@@ -411,23 +441,26 @@ template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& p
         linear_any_kernel<T, O><<<dim3((unsigned)blocks, plan.splits), 256, 0, s>>>(a);
         SRF_LAUNCH_CHECK("linear_any_kernel");
     }
-    if (plan.splits > 1) {
-        const long work = ((long)a.M * ((a.N + W - 1) / W) + 31) / 32;
-        linear_join_kernel<O><<<(unsigned)(work < 16384 ? work : 16384), 256, 0, s>>>(a);
-        SRF_LAUNCH_CHECK("linear_join_kernel");
-    }
-    return 0;
+    return plan.splits > 1 ? lin_join<O>(a, sums, s) : 0;
 }
-static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPlan& plan, void* ws, hipStream_t s) {
+static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPlan& plan, void* ws, const ColumnSums& sums, hipStream_t s) {
     switch (in_type) {
-        case SCENERF_T_F32: return lin_run<TypeF32, TypeF32>(a, plan, ws, s);
-        case SCENERF_T_BF16: return lin_run<TypeBF16, TypeBF16>(a, plan, ws, s);
-        case SCENERF_T_F16: return lin_run<TypeF16, TypeF16>(a, plan, ws, s);
+        case SCENERF_T_F32: return lin_run<TypeF32, TypeF32>(a, plan, ws, sums, s);
+        case SCENERF_T_BF16: return lin_run<TypeBF16, TypeBF16>(a, plan, ws, sums, s);
+        case SCENERF_T_F16: return lin_run<TypeF16, TypeF16>(a, plan, ws, sums, s);
         default:
-            if (out_type == SCENERF_T_F32) return lin_run<TypeE4M3, TypeF32>(a, plan, ws, s);
-            if (out_type == SCENERF_T_BF16) return lin_run<TypeE4M3, TypeBF16>(a, plan, ws, s);
-            return lin_run<TypeE4M3, TypeF16>(a, plan, ws, s);
+            if (out_type == SCENERF_T_F32) return lin_run<TypeE4M3, TypeF32>(a, plan, ws, sums, s);
+            if (out_type == SCENERF_T_BF16) return lin_run<TypeE4M3, TypeBF16>(a, plan, ws, sums, s);
+            return lin_run<TypeE4M3, TypeF16>(a, plan, ws, sums, s);
     }
+}
+// dx and dw in one launch of 64 x 64 tiles, then dw's join
+static int lin_pair(int type, LinArgs dx, const LinPlan& plan_x, LinArgs dw, const LinPlan& plan_w, void* ws, const ColumnSums& sums, hipStream_t s) {
+    lin_fill(dx, plan_x, nullptr);
+    lin_fill(dw, plan_w, ws);
+    if (int e = type == SCENERF_T_F32 ? linear_pair_f32(dx, dw, s) : type == SCENERF_T_BF16 ? linear_pair_bf16(dx, dw, s) : linear_pair_f16(dx, dw, s)) return e;
+    if (plan_w.splits == 1) return 0;
+    return type == SCENERF_T_F32 ? lin_join<TypeF32>(dw, sums, s) : type == SCENERF_T_BF16 ? lin_join<TypeBF16>(dw, sums, s) : lin_join<TypeF16>(dw, sums, s);
 }
 
 // A matrix whose rows the staged kernel can read in 16-byte pieces: aligned base and pitch, a length of whole pieces (or zeros up to one),
@@ -575,7 +608,7 @@ int scenerf_hip_linear_forward(const scenerf_linear* p, scenerf_stream_t stream)
         a.B = p->workspace;
         a.b_j = pitch;
     }
-    return lin_product(p->in_type, p->out_type, a, plan, (char*)p->workspace + lines, s);
+    return lin_product(p->in_type, p->out_type, a, plan, (char*)p->workspace + lines, ColumnSums{}, s);
 }
 
 int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream) {
@@ -599,28 +632,35 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
                 : p->out_type == SCENERF_T_BF16 ? lin_dz<TypeBF16>(p, b, to, sums, s) : lin_dz<TypeF16>(p, b, to, sums, s);
         if (e) return e;
     }
-    if (p->db) {
+    ColumnSums sums = {};
+    if (p->db && p->dw && b.dw.splits > 1) sums = {part, p->db, b.strips, p->n, cdiv(p->n, 16)};
+    else if (p->db) {
         if (int e = launch_sum_parts(p->out_type, part, b.strips, p->n, p->db, s)) return e;
     }
     const int pitch = lin_pitch(p->k, (int)es);
+    LinArgs ax = {}, aw = {};
     if (p->dx && p->rows > 0) {
-        LinArgs a = {};
-        a.A = dz; a.a_i = ld_dz; a.a_k = 1;
-        a.B = p->w; a.b_j = 1; a.b_k = p->ldw;
-        a.M = (int)p->rows; a.N = p->k; a.K = p->n;
-        a.b_ext = pitch;
-        a.out = p->dx;
-        if (int e = lin_product(p->in_type, p->out_type, a, b.dx, ws + b.sums, s)) return e;
+        ax.A = dz; ax.a_i = ld_dz; ax.a_k = 1;
+        ax.B = p->w; ax.b_j = 1; ax.b_k = p->ldw;
+        ax.M = (int)p->rows; ax.N = p->k; ax.K = p->n;
+        ax.b_ext = pitch;
+        ax.out = p->dx;
     }
     if (p->dw) {     // rows == 0: an empty sum, zeros
-        LinArgs a = {};
-        a.A = dz; a.a_i = 1; a.a_k = ld_dz;
-        a.B = p->x; a.b_j = 1; a.b_k = p->ldx;
-        a.M = p->n; a.N = p->k; a.K = (int)p->rows;
-        a.a_ext = b.make_dz ? b.dz_pitch : p->n; a.b_ext = pitch;
-        a.out = p->dw;
-        if (int e = lin_product(p->in_type, p->out_type, a, b.dw, ws + b.sums, s)) return e;
+        aw.A = dz; aw.a_i = 1; aw.a_k = ld_dz;
+        aw.B = p->x; aw.b_j = 1; aw.b_k = p->ldx;
+        aw.M = p->n; aw.N = p->k; aw.K = (int)p->rows;
+        aw.a_ext = b.make_dz ? b.dz_pitch : p->n; aw.b_ext = pitch;
+        aw.out = p->dw;
     }
+    // Both on 64 x 64 tiles and two rounds of them at most: one launch, beside each other (64 x 512 x 512 bf16 14.3 -> 11.2 us with dz and all,
+    // 1,024 rows 21.0 -> 15.5, 4,800 36.7 -> 33.8; 2,020 tiles of 20,000 x 256 x 256 fp32 took 90 us instead of 83)
+    auto tiles = [](const LinPlan& plan, long m, long n) { return plan.kind == 2 && plan.tile == LIN_64x64 ? (m + 63) / 64 * ((n + 63) / 64) * plan.splits : 1 << 20; };
+    if (ax.out && aw.out && b.dx.splits == 1 && tiles(b.dx, ax.M, ax.N) + tiles(b.dw, aw.M, aw.N) <= 2 * 768) return lin_pair(p->in_type, ax, b.dx, aw, b.dw, ws + b.sums, sums, s);
+    if (ax.out)
+        if (int e = lin_product(p->in_type, p->out_type, ax, b.dx, ws + b.sums, ColumnSums{}, s)) return e;
+    if (aw.out)
+        if (int e = lin_product(p->in_type, p->out_type, aw, b.dw, ws + b.sums, sums, s)) return e;
     return 0;
 }
 

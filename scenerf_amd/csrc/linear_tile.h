@@ -67,8 +67,9 @@ template <typename T, bool ACROSS, int TILE> struct LinSide {
     }
 };
 
+// workgroup `block` of `blocks` of one product
 template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB, bool WHOLE>
-__global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
+__device__ static inline void linear_tile(const LinArgs& p, int block, int blocks) {
     typedef LinSide<T, AX, BM> SA;
     typedef LinSide<T, BX, BN> SB;
     constexpr int ES = SA::ES, BK = SA::BK, WAVES = WM * WN;
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     const unsigned lds0 = (unsigned)(uintptr_t)lds;
 
     const int tiles = p.tiles_i * p.tiles_j;
-    const int id = lin_xcd_order(blockIdx.x, gridDim.x);
+    const int id = lin_xcd_order(block, blocks);
     const int split = id / tiles, tile = id - split * tiles;
     const long i0 = (long)(tile / p.tiles_j) * BM;
     const int j0 = (tile % p.tiles_j) * BN;
@@ -322,6 +323,17 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
 }
 
 template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB, bool WHOLE>
+__global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
+    linear_tile<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB, WHOLE>(p, blockIdx.x, gridDim.x);
+}
+// dx and dw of a small layer in one launch, beside each other: workgroups before `first` make dx
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void linear_pair_kernel(LinArgs dx, LinArgs dw, int first) {
+    if ((int)blockIdx.x < first) linear_tile<T, T, false, true, 64, 64, 2, 2, 3, 3, WHOLE>(dx, blockIdx.x, first);
+    else linear_tile<T, T, true, true, 64, 64, 2, 2, 3, 3, WHOLE>(dw, blockIdx.x - first, gridDim.x - first);
+}
+
+template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB, bool WHOLE>
 static int lin_tile_start(const LinArgs& a, hipStream_t s) {
     constexpr int LDS = (NSA * BM + NSB * BN) * LIN_CHUNK_BYTES;
     auto kernel = linear_tile_kernel<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB, WHOLE>;
@@ -356,4 +368,16 @@ template <typename T> static int lin_tile_layout(const LinArgs& a, LinTile tile,
     if (ax && bx) return lin_tile_pick<T, T, true, true>(a, tile, s);
     srf_set_error("linear: no such operand layout");
     return 1;
+}
+template <typename T, bool WHOLE> static int lin_pair_start(const LinArgs& dx, const LinArgs& dw, hipStream_t s) {
+    constexpr int LDS = 6 * 64 * LIN_CHUNK_BYTES;
+    const long first = (long)dx.tiles_i * dx.tiles_j * dx.splits, blocks = first + (long)dw.tiles_i * dw.tiles_j * dw.splits;
+    SRF_CHECK(blocks < (1L << 32) / 256, "linear: %ld tiles are more than one launch holds", blocks);
+    linear_pair_kernel<T, WHOLE><<<(unsigned)blocks, 256, LDS, s>>>(dx, dw, (int)first);
+    SRF_LAUNCH_CHECK("linear_pair_kernel");
+    return 0;
+}
+template <typename T> static int lin_pair(const LinArgs& dx, const LinArgs& dw, hipStream_t s) {      // (both have k columns)
+    if (dx.N % (16 / (int)sizeof(typename T::raw)) == 0) return lin_pair_start<T, true>(dx, dw, s);
+    return lin_pair_start<T, false>(dx, dw, s);
 }
