@@ -92,7 +92,8 @@ static const int kLinTileRows[LIN_TILES] = {256, 128, 64, 128}, kLinTileCols[LIN
 int linear_tile_f32(const LinArgs& a, LinTile tile, hipStream_t s);
 int linear_tile_bf16(const LinArgs& a, LinTile tile, hipStream_t s);
 int linear_tile_f16(const LinArgs& a, LinTile tile, hipStream_t s);
-int linear_pair_f32(const LinArgs& dx, const LinArgs& dw, hipStream_t s);     // 64 x 64 tiles, tiles_i .. k_split filled in
-int linear_pair_bf16(const LinArgs& dx, const LinArgs& dw, hipStream_t s);
-int linear_pair_f16(const LinArgs& dx, const LinArgs& dw, hipStream_t s);
+// a layer's two gradients on tiles of one shape
+int linear_pair_f32(const LinArgs& dx, const LinArgs& dw, LinTile tile, hipStream_t s);
+int linear_pair_bf16(const LinArgs& dx, const LinArgs& dw, LinTile tile, hipStream_t s);
+int linear_pair_f16(const LinArgs& dx, const LinArgs& dw, LinTile tile, hipStream_t s);
 int linear_tile_e4m3(const LinArgs& a, LinTile tile, int out_type, hipStream_t s);

@@ -342,7 +342,8 @@ static const LinTileCost kLinCost32[] = {{LIN_128x128, 2, 4.7, {1.8, 3.6}}, {LIN
 #define LIN_MIN_CHUNKS 8            // a split keeps at least so many: its ends cost as much
 
 // `staged`: both operands are in 16-byte pieces
-static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, long K) {
+// `like`: a tile whose product could share another one's launch, worth a tenth
+static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, long K, LinTile like = LIN_TILES) {
     LinPlan r = {0, 1, 0, LIN_128x128};
     // (bf16, this kernel against staged tiles: 1 row x 512 x 512 2.2 against 4.9 us, 8 rows 3.7 against 4.9, 8 x 2,480 x 1,536 5.5 against 9.7;
     // 16 rows 5.3 against 5.0.  It reads whole 16 bytes inside the row: a shorter row takes the element loads; a launch holds 2^32 threads)
@@ -384,6 +385,7 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
                 }
                 us = max(us, bytes + 2.0);
                 if (s > 1) us += 5.0 + 8.0 * s * M * N / LIN_PART_BYTES_US;
+                if (t.tile == like) us *= 0.9;
                 if (us < best) { best = us; r.tile = t.tile; splits = s; }
             }
         }
@@ -454,11 +456,11 @@ static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPla
             return lin_run<TypeE4M3, TypeF16>(a, plan, ws, sums, s);
     }
 }
-// dx and dw in one launch of 64 x 64 tiles, then dw's join
+// dx and dw in one launch, then dw's join
 static int lin_pair(int type, LinArgs dx, const LinPlan& plan_x, LinArgs dw, const LinPlan& plan_w, void* ws, const ColumnSums& sums, hipStream_t s) {
     lin_fill(dx, plan_x, nullptr);
     lin_fill(dw, plan_w, ws);
-    if (int e = type == SCENERF_T_F32 ? linear_pair_f32(dx, dw, s) : type == SCENERF_T_BF16 ? linear_pair_bf16(dx, dw, s) : linear_pair_f16(dx, dw, s)) return e;
+    if (int e = type == SCENERF_T_F32 ? linear_pair_f32(dx, dw, plan_x.tile, s) : type == SCENERF_T_BF16 ? linear_pair_bf16(dx, dw, plan_x.tile, s) : linear_pair_f16(dx, dw, plan_x.tile, s)) return e;
     if (plan_w.splits == 1) return 0;
     return type == SCENERF_T_F32 ? lin_join<TypeF32>(dw, sums, s) : type == SCENERF_T_BF16 ? lin_join<TypeBF16>(dw, sums, s) : lin_join<TypeF16>(dw, sums, s);
 }
@@ -510,6 +512,10 @@ struct BackwardPlan {
     int64_t part, dz, sums;         // offsets of the column sums' parts, of dz and of the split sums
     int64_t bytes;
     LinPlan dx, dw;
+    // One launch for both where they are on tiles of one shape, two workgroups or more a CU: dw's start first, dx's fill the CUs behind them.
+    // With dz and all: 64 x 512 x 512 bf16 14.3 -> 11.2 us, 4,800 x 512 x 512 36 -> 30 and fp32 80 -> 71, 262,144 x 128 x 128 fp32 263 -> 248; with dx in
+    // front 20,000 x 256 x 256 fp32 took 90 us, not 74 (apart 83).  Tiles of 256, one a CU, gain nothing (153,600 x 512 x 512: 325 and 326).
+    bool pair;
 };
 static BackwardPlan lin_backward_plan(const scenerf_linear* p) {
     BackwardPlan b = {};
@@ -522,7 +528,9 @@ static BackwardPlan lin_backward_plan(const scenerf_linear* p) {
     b.strip = dz_strip(p->rows);
     b.strips = (int)((p->rows + b.strip - 1) / b.strip);
     b.dx = lin_plan(p->in_type, false, true, dz_fits && lin_pieces(p->w, p->ldw, p->k, es, p->padded), p->rows, p->k, p->n);
-    b.dw = lin_plan(p->in_type, true, true, dz_fits && lin_pieces(p->x, p->ldx, p->k, es, p->padded), p->n, p->k, p->rows);
+    b.dw = lin_plan(p->in_type, true, true, dz_fits && lin_pieces(p->x, p->ldx, p->k, es, p->padded), p->n, p->k, p->rows,
+                    p->dx && b.dx.kind == 2 && b.dx.splits == 1 && b.dx.tile != LIN_256x256 ? b.dx.tile : LIN_TILES);
+    b.pair = p->dx && p->dw && p->rows > 0 && b.dx.kind == 2 && b.dw.kind == 2 && b.dx.tile == b.dw.tile && b.dx.tile != LIN_256x256 && b.dx.splits == 1;
     int64_t at = 0;
     if (p->db) { b.part = at; at += align256((int64_t)b.strips * p->n * 4); }
     if (b.make_dz) { b.dz = at; at += align256(p->rows * b.dz_pitch * es); }
@@ -653,10 +661,7 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         aw.a_ext = b.make_dz ? b.dz_pitch : p->n; aw.b_ext = pitch;
         aw.out = p->dw;
     }
-    // Both on 64 x 64 tiles and two rounds of them at most: one launch, beside each other (64 x 512 x 512 bf16 14.3 -> 11.2 us with dz and all,
-    // 1,024 rows 21.0 -> 15.5, 4,800 36.7 -> 33.8; 2,020 tiles of 20,000 x 256 x 256 fp32 took 90 us instead of 83)
-    auto tiles = [](const LinPlan& plan, long m, long n) { return plan.kind == 2 && plan.tile == LIN_64x64 ? (m + 63) / 64 * ((n + 63) / 64) * plan.splits : 1 << 20; };
-    if (ax.out && aw.out && b.dx.splits == 1 && tiles(b.dx, ax.M, ax.N) + tiles(b.dw, aw.M, aw.N) <= 2 * 768) return lin_pair(p->in_type, ax, b.dx, aw, b.dw, ws + b.sums, sums, s);
+    if (b.pair) return lin_pair(p->in_type, ax, b.dx, aw, b.dw, ws + b.sums, sums, s);
     if (ax.out)
         if (int e = lin_product(p->in_type, p->out_type, ax, b.dx, ws + b.sums, ColumnSums{}, s)) return e;
     if (aw.out)

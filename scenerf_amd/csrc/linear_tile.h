@@ -326,11 +326,11 @@ template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int 
 __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinArgs p) {
     linear_tile<T, O, AX, BX, BM, BN, WM, WN, NSA, NSB, WHOLE>(p, blockIdx.x, gridDim.x);
 }
-// dx and dw of a small layer in one launch, beside each other: workgroups before `first` make dx
-template <typename T, bool WHOLE>
-__global__ __launch_bounds__(256) void linear_pair_kernel(LinArgs dx, LinArgs dw, int first) {
-    if ((int)blockIdx.x < first) linear_tile<T, T, false, true, 64, 64, 2, 2, 3, 3, WHOLE>(dx, blockIdx.x, first);
-    else linear_tile<T, T, true, true, 64, 64, 2, 2, 3, 3, WHOLE>(dw, blockIdx.x - first, gridDim.x - first);
+// dx and dw of a layer in one launch: workgroups before `first` make dw, whose contraction is the longer one
+template <typename T, int BM, int BN, int WM, int WN, int NSA, int NSB, bool WHOLE>
+__global__ __launch_bounds__(64 * WM * WN) void linear_pair_kernel(LinArgs dx, LinArgs dw, int first) {
+    if ((int)blockIdx.x < first) linear_tile<T, T, true, true, BM, BN, WM, WN, NSA, NSB, WHOLE>(dw, blockIdx.x, first);
+    else linear_tile<T, T, false, true, BM, BN, WM, WN, NSA, NSB, WHOLE>(dx, blockIdx.x - first, gridDim.x - first);
 }
 
 template <typename T, typename O, bool AX, bool BX, int BM, int BN, int WM, int WN, int NSA, int NSB, bool WHOLE>
@@ -369,15 +369,28 @@ template <typename T> static int lin_tile_layout(const LinArgs& a, LinTile tile,
     srf_set_error("linear: no such operand layout");
     return 1;
 }
-template <typename T, bool WHOLE> static int lin_pair_start(const LinArgs& dx, const LinArgs& dw, hipStream_t s) {
-    constexpr int LDS = 6 * 64 * LIN_CHUNK_BYTES;
-    const long first = (long)dx.tiles_i * dx.tiles_j * dx.splits, blocks = first + (long)dw.tiles_i * dw.tiles_j * dw.splits;
-    SRF_CHECK(blocks < (1L << 32) / 256, "linear: %ld tiles are more than one launch holds", blocks);
-    linear_pair_kernel<T, WHOLE><<<(unsigned)blocks, 256, LDS, s>>>(dx, dw, (int)first);
+template <typename T, int BM, int BN, int WM, int WN, int NSA, int NSB, bool WHOLE> static int lin_pair_start(const LinArgs& dx, const LinArgs& dw, hipStream_t s) {
+    constexpr int LDS = (NSA * BM + NSB * BN) * LIN_CHUNK_BYTES;
+    auto kernel = linear_pair_kernel<T, BM, BN, WM, WN, NSA, NSB, WHOLE>;
+    SRF_ONCE_PER_DEVICE(SRF_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS)));
+    const long first = (long)dw.tiles_i * dw.tiles_j * dw.splits, blocks = first + (long)dx.tiles_i * dx.tiles_j * dx.splits;
+    SRF_CHECK(blocks < (1L << 32) / (64 * WM * WN), "linear: %ld tiles are more than one launch holds", blocks);
+    kernel<<<(unsigned)blocks, 64 * WM * WN, LDS, s>>>(dx, dw, (int)first);
     SRF_LAUNCH_CHECK("linear_pair_kernel");
     return 0;
 }
-template <typename T> static int lin_pair(const LinArgs& dx, const LinArgs& dw, hipStream_t s) {      // (both have k columns)
-    if (dx.N % (16 / (int)sizeof(typename T::raw)) == 0) return lin_pair_start<T, true>(dx, dw, s);
-    return lin_pair_start<T, false>(dx, dw, s);
+template <typename T, int BM, int BN, int WM, int WN, int NSA, int NSB> static int lin_pair_launch(const LinArgs& dx, const LinArgs& dw, hipStream_t s) {
+    // (both have k columns)
+    if (dx.N % (16 / (int)sizeof(typename T::raw)) == 0) return lin_pair_start<T, BM, BN, WM, WN, NSA, NSB, true>(dx, dw, s);
+    return lin_pair_start<T, BM, BN, WM, WN, NSA, NSB, false>(dx, dw, s);
+}
+template <typename T> static int lin_pair(const LinArgs& dx, const LinArgs& dw, LinTile tile, hipStream_t s) {
+    switch (tile) {
+        case LIN_128x128: return lin_pair_launch<T, 128, 128, 2, 2, 3, 2>(dx, dw, s);
+        case LIN_64x64: return lin_pair_launch<T, 64, 64, 2, 2, 3, 3>(dx, dw, s);
+        case LIN_128x32: return lin_pair_launch<T, 128, 32, 4, 1, 3, 3>(dx, dw, s);
+        default: break;
+    }
+    srf_set_error("linear: no such tile for this type");
+    return 1;
 }
