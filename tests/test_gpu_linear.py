@@ -341,3 +341,136 @@ def test_every_tile_in_8_bits(m, k, n, out):
     b, r = normal(g, n, dtype=out), normal(g, m, n, dtype=out)
     hold(linear_8bit(q, s, wq, ws, b, activation="silu", residual=r, out_dtype=out),
          linear64(q.float(), wq.float(), b, "silu", r, scales=(s, ws), out_dtype=out)["y"])
+
+
+@pytest.mark.parametrize("k,n", [(2048, 16), (16, 2048)])
+def test_gradients_past_32_bit_offsets(k, n):
+    """x, dx (or y, z, dy and dz) of more than 2^31 elements; a gradient that reaches the last rows alone, so that their own call is the oracle."""
+    from scenerf_amd.linear import linear
+    g = gen("large back", k, n)
+    m, last, bf = 1_100_000, 300, torch.bfloat16
+    x = torch.empty(m, k, dtype=bf, device=DEV).normal_(generator=g).requires_grad_(True)
+    w, b = normal(g, n, k, dtype=bf, scale=k ** -0.5).requires_grad_(True), normal(g, n, dtype=bf).requires_grad_(True)
+    dy = torch.zeros(m, n, dtype=bf, device=DEV)
+    dy[-last:] = normal(g, last, n, dtype=bf)
+    dx, dw, db = torch.autograd.grad(linear(x, w, b, activation="silu"), (x, w, b), dy)
+    want = linear64(x.detach()[-last:], w.detach(), b.detach(), "silu", None, dy[-last:])
+    hold(dx[-last:], want["dx"], "dx")
+    hold(dw, want["dw"], "dw")
+    hold(db, want["db"], "db")
+    assert not bool(dx[:-last].any())
+
+
+@pytest.mark.parametrize("m", [5, 300])
+def test_8bit_rows_and_columns_that_are_not_numbers(m):
+    """A row of x, or of w, that quantize_rows could not hold spoils its own row, or column, of the result and no other."""
+    from scenerf_amd.linear import linear_8bit, quantize_rows
+    g = gen("nan8", m)
+    x, w = normal(g, m, 200), normal(g, 70, 200, scale=200 ** -0.5)
+    clean = linear_8bit(*quantize_rows(x), *quantize_rows(w), activation="gelu")
+    x[m - 2, 3], w[69, 199] = float("inf"), float("nan")
+    y = linear_8bit(*quantize_rows(x), *quantize_rows(w), activation="gelu")
+    assert not bool(torch.isfinite(y[m - 2]).any()) and not bool(torch.isfinite(y[:, 69]).any())
+    keep = [i for i in range(m) if i != m - 2]
+    assert torch.equal(y[keep][:, :69], clean[keep][:, :69])
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 520, 136), (5003, 1032, 130), (20011, 200, 520)])
+def test_the_same_bits_every_time(m, k, n):
+    from scenerf_amd.linear import linear
+    g = gen("bits", m, k, n)
+    bf = torch.bfloat16
+    x, w, b, dy = (t.requires_grad_(True) for t in (normal(g, m, k, dtype=bf), normal(g, n, k, dtype=bf), normal(g, n, dtype=bf), normal(g, m, n, dtype=bf)))
+
+    def once():
+        y = linear(x, w, b, activation="gelu")
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy.detach())
+    first = once()
+    for _ in range(5):
+        assert all(torch.equal(a, c) for a, c in zip(first, once()))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_rows_far_apart(dtype):
+    """A pitch of more than 4 MiB: beyond the tiles' 32-bit offsets."""
+    from scenerf_amd.linear import linear
+    g = gen("far", dtype)
+    big = torch.empty(40, 2_200_000, dtype=dtype, device=DEV)
+    x = big[:, 64:168]
+    x.copy_(normal(g, 40, 104, dtype=dtype))
+    w, b, dy = normal(g, 72, 104, dtype=dtype, scale=0.1).requires_grad_(True), normal(g, 72, dtype=dtype).requires_grad_(True), normal(g, 40, 72, dtype=dtype)
+    x.requires_grad_(True)
+    y = linear(x, w, b, activation="gelu")
+    want = linear64(x.detach(), w.detach(), b.detach(), "gelu", None, dy)
+    hold(y.detach(), want["y"], "y")
+    for name, t in zip(("dx", "dw", "db"), torch.autograd.grad(y, (x, w, b), dy)):
+        hold(t, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(1, 3, 5), (9, 42, 515), (200, 1001, 130), (5000, 42, 65)])
+def test_the_c_entries_on_rows_as_they_are(m, k, n, dtype):
+    """The entries without scenerf_hip_linear_pad's copies: rows of any length and start, element by element."""
+    import ctypes as C
+
+    from scenerf_amd import _capi
+    g = gen("c", m, k, n, dtype)
+    lib = _capi.load()
+    code = {torch.float32: _capi.T_F32, torch.bfloat16: _capi.T_BF16, torch.float16: _capi.T_F16}[dtype]
+    x, w = normal(g, m, k + 1, dtype=dtype)[:, 1:], normal(g, n, k + 3, dtype=dtype, scale=k ** -0.5)[:, 3:]
+    b, r, dy = normal(g, n, dtype=dtype), normal(g, m, n + 1, dtype=dtype)[:, :n], normal(g, m, n + 1, dtype=dtype)[:, 1:]
+    y, z, dx, dw, db = (torch.empty(*s, dtype=dtype, device=DEV) for s in ((m, n), (m, n), (m, k), (n, k), (n,)))
+    p = _capi.Linear(code, code, _capi.ACTIVATIONS["silu"], n, k, 0, m, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), None, None, b.data_ptr(),
+                     r.data_ptr(), r.stride(0), y.data_ptr(), z.data_ptr(), dy.data_ptr(), dy.stride(0), dx.data_ptr(), dw.data_ptr(), db.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    for backward, fn in ((0, lib.scenerf_hip_linear_forward), (1, lib.scenerf_hip_linear_backward)):
+        need = lib.scenerf_hip_linear_workspace(C.byref(p), backward)
+        assert need >= 0
+        ws = torch.empty(need + 16, dtype=torch.uint8, device=DEV)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        assert fn(C.byref(p), stream) == 0, lib.scenerf_hip_last_error()
+    want = linear64(x, w, b, "silu", r, dy)
+    for name, t in (("y", y), ("dx", dx), ("dw", dw), ("db", db)):
+        hold(t, want[name], name)
+
+
+def test_threads_on_their_own_streams():
+    """Four host threads, each with a stream, a shape and a graph of its own: what each gets is what it gets alone."""
+    import threading
+
+    from scenerf_amd.linear import linear, linear_8bit, quantize_rows
+    from scenerf_amd.norm import rms_norm
+    bf = torch.bfloat16
+    shapes = [(300, 520, 136), (5003, 72, 515), (4, 512, 512), (1001, 1032, 264)]
+
+    def work(i, reps, out):
+        m, k, n = shapes[i]
+        g = gen("threads", i)
+        x, w, dy = normal(g, m, k, dtype=bf).requires_grad_(True), normal(g, n, k, dtype=bf, scale=k ** -0.5).requires_grad_(True), normal(g, m, n, dtype=bf)
+        gain = torch.ones(k, device=DEV, dtype=bf)
+        for _ in range(reps):
+            y = linear(rms_norm(x, gain), w, activation="gelu")
+            grads = torch.autograd.grad(y, (x, w), dy)
+            with torch.no_grad():
+                y8 = linear_8bit(*quantize_rows(x), *quantize_rows(w))
+            out.append([t.detach().clone() for t in (y, *grads, y8)])
+    alone = []
+    for i in range(4):
+        work(i, 1, alone)
+    torch.cuda.synchronize()
+    together = [[] for _ in range(4)]
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            work(i, 10, together[i])
+            s.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(4):
+        assert len(together[i]) == 10
+        for got in together[i]:
+            assert all(torch.equal(a, b) for a, b in zip(got, alone[i]))

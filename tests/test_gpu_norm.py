@@ -222,3 +222,26 @@ def test_wide_8bit_rows_whose_weighted_values_overflow():
     y = rms64(x, w, 1e-6)["y"][0]
     assert bool(torch.isfinite(s).all()) and bool(((s.double() / (y.abs().amax(1) / 448) - 1).abs() <= 2.0 ** -10).all())
     assert bool(((q[:, 7].double() * s.double() - y[:, 7]).abs() <= 2.0 ** -4 * y[:, 7].abs()).all())
+
+
+def test_rows_past_32_bit_offsets():
+    """More than 2^31 elements, the gradient on the last rows alone: their own call is the oracle."""
+    from scenerf_amd.norm import rms_norm, rms_norm_8bit
+    g = gen("large rms")
+    m, d, last, bf = 4_200_000, 520, 300, torch.bfloat16
+    x = torch.empty(m, d, dtype=bf, device=DEV).normal_(generator=g).requires_grad_(True)
+    r = torch.empty(m, d, dtype=bf, device=DEV).normal_(generator=g)
+    w = (1 + 0.1 * normal(g, d)).to(bf).requires_grad_(True)
+    y, h = rms_norm(x, w, residual=r)
+    dy = torch.zeros(m, d, dtype=bf, device=DEV)
+    dy[-last:] = normal(g, last, d, dtype=bf)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    want = rms64(x.detach()[-last:], w.detach(), 1e-6, r[-last:], dy[-last:])
+    for name, t in (("y", y.detach()[-last:]), ("h", h.detach()[-last:]), ("dx", dx[-last:]), ("dw", dw)):
+        hold(t, want[name], name)
+    assert not bool(dx[:-last].any())
+    del dx, dy, y, h
+    with torch.no_grad():
+        q, s, _ = rms_norm_8bit(x, w, residual=r)
+        one = rms_norm_8bit(x[-last:], w, residual=r[-last:])
+    assert torch.equal(q[-last:].view(torch.uint8), one[0].view(torch.uint8)) and torch.equal(s[-last:], one[1])
