@@ -5,8 +5,8 @@
 // Three matrix products of one shape family, C[i][j] = sum_k A(i, k) B(j, k): the forward contracts the features (both operands are
 // read along k), dx contracts the outputs (w is read across), dw contracts the rows (both are read across).
 //
-// Products of many rows run on staged tiles (linear_tile.h): bound by the matrix instructions where the contraction is long (153,600 x 2,480
-// x 1,536 bf16 1,041 us = 1.12 PFLOP/s; the library's product of that shape without an epilogue 1,054; 8 bits 654 us), by the operands' and
+// Products of many rows run on staged tiles (linear_tile.h): bound by the chip's power where the contraction is long (153,600 x 2,480
+// x 1,536 bf16 1,044 us = 1.12 PFLOP/s; the library's product of that shape without an epilogue 1,054; 8 bits 635 us; 4,096 x 8,192 x 4,096 takes 256 us, and 162 if all of it is zeros), by the operands' and
 // results' bytes where it is short (153,600 x 512 x 512 bf16 with gelu, residual and kept sums 165 us for 629 MB).
 #include "linear.h"
 
