@@ -635,7 +635,8 @@ typedef struct scenerf_rms {
     void* h; void* y;               /* [rows][width], dense */
     uint8_t* q; float* scale;       /* [rows][width] e4m3, [rows] */
     float* rstd;                    /* [rows]: written by forward, read by backward */
-    /* backward: x holds h as the forward stored it (its x where there was no residual);
+    /* backward: x holds h as the forward stored it (its x where there was no residual), or x and residual are the forward's, h their
+     * unrounded sum;
      * dx = rstd (dy weight - xhat mean(dy weight xhat)) + dh, xhat = x rstd;  dweight = sum over rows of dy xhat */
     const void* dy; int64_t ld_dy;
     const void* dh; int64_t ld_dh;  /* gradient of h, or NULL */

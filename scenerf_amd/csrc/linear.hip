@@ -52,7 +52,9 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const long i0 = (long)(blockIdx.x / p.tiles_j) * ANY_TILE;
     const int j0 = (blockIdx.x % p.tiles_j) * ANY_TILE;
-    const long kb = (long)blockIdx.y * p.k_split, ke = min((long)p.K, kb + p.k_split);
+    const bool again = p.half && (int)blockIdx.y >= p.half;
+    const void* A = again ? p.A2 : p.A;
+    const long kb = (long)(again ? blockIdx.y - p.half : blockIdx.y) * p.k_split, ke = min((long)p.K, kb + p.k_split);
     lin_f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
@@ -62,7 +64,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
         for (int t = tid; t < ANY_TILE * ANY_K; t += 256) {
             const int r = p.a_k == 1 ? t / ANY_K : t % ANY_TILE, k = p.a_k == 1 ? t % ANY_K : t / ANY_TILE;
             const bool ok = i0 + r < p.M && k0 + k < ke;
-            ((staged*)(la + r * PITCH))[k] = ok ? stage(((const raw*)p.A)[(i0 + r) * p.a_i + (k0 + k) * p.a_k]) : (staged)0;
+            ((staged*)(la + r * PITCH))[k] = ok ? stage(((const raw*)A)[(i0 + r) * p.a_i + (k0 + k) * p.a_k]) : (staged)0;
         }
         for (int t = tid; t < ANY_TILE * ANY_K; t += 256) {
             const int r = p.b_k == 1 ? t / ANY_K : t % ANY_TILE, k = p.b_k == 1 ? t % ANY_K : t / ANY_TILE;
@@ -272,8 +274,8 @@ template <int ACT> __device__ static inline void slopes(float (&g)[8], float (&z
 // columns a fixed 32 left half the threads idle, 150 us for 262,144 x 128 fp32 instead of 78; 32 at 512 columns took 111 us for 153,600 rows
 // of bf16, 64 100); two rows a thread are in flight.  Bound by HBM: 4.7 and 5.2 TB/s.
 template <typename O, bool WHOLE>
-__global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld_dy, const void* z_, void* dz_, int pitch, float* part, int M, int N,
-                                                        int act, int strip, int lx) {
+__global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld_dy, const void* z_, void* dz_, void* rest_, int pitch, float* part,
+                                                        int M, int N, int act, int strip, int lx) {
     typedef typename O::raw raw;
     __shared__ float red[256 * 9];
     const int tx = threadIdx.x & ((1 << lx) - 1), ty = threadIdx.x >> lx, rows = 256 >> lx;
@@ -302,6 +304,14 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld
                 if (dz_) store_vec<O, 8>((raw*)dz_ + (r + q * rows) * pitch + j0, g[q]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum[e] += g[q][e];
+                if (rest_) {            // what dz's rounding left out
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float left = g[q][e] - O::to_f32(O::from_f32(g[q][e]));
+                        g[q][e] = fabsf(left) < 3.0e38f ? left : 0.f;            // (dz infinite or NaN: says it itself)
+                    }
+                    store_vec<O, 8>((raw*)rest_ + (r + q * rows) * pitch + j0, g[q]);
+                }
             }
         }
     }
@@ -394,7 +404,11 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
     r.k_split = (int)(((K + r.splits - 1) / r.splits + bk - 1) / bk * bk);
     return r;
 }
-static int64_t lin_part_bytes(const LinPlan& p, long M, int N) { return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0; }
+// `twice`: with a second A (LinArgs.A2)
+static int64_t lin_part_bytes(const LinPlan& p, long M, int N, bool twice = false) {
+    const int splits = p.splits * (twice ? 2 : 1);
+    return splits > 1 ? align256((int64_t)splits * M * N * 4) : 0;
+}
 
 template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, hipStream_t s) {
     // one piece a lane and row of w: one wave a group of columns; longer rows: four (bf16, 8 rows, 512 outputs, one wave against four: 512
@@ -403,9 +417,10 @@ template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, 
     else linear_few_kernel<T, O, MR, 4><<<cdiv(a.N, FEW_COLS), 256, 0, s>>>(a);
 }
 static void lin_fill(LinArgs& a, const LinPlan& plan, void* ws) {
-    a.splits = plan.splits;
+    a.half = a.A2 ? plan.splits : 0;
+    a.splits = plan.splits + a.half;
     a.k_split = plan.k_split;
-    a.part = plan.splits > 1 ? (float*)ws : nullptr;
+    a.part = a.splits > 1 ? (float*)ws : nullptr;
     if (plan.kind == 2) {
         a.tiles_i = (int)((a.M + (long)kLinTileRows[plan.tile] - 1) / kLinTileRows[plan.tile]);
         a.tiles_j = (int)((a.N + (long)kLinTileCols[plan.tile] - 1) / kLinTileCols[plan.tile]);
@@ -418,7 +433,7 @@ template <typename O> static int lin_join(const LinArgs& a, const ColumnSums& su
     SRF_LAUNCH_CHECK("linear_join_kernel");
     return 0;
 }
-// `sums`: column sums that ride along where the product is joined (plan.splits > 1)
+// `sums`: column sums that ride along where the product is joined
 template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& plan, void* ws, const ColumnSums& sums, hipStream_t s) {
     lin_fill(a, plan, ws);
     if (plan.kind == 1) {
@@ -440,10 +455,10 @@ template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& p
         a.tiles_j = cdiv(a.N, ANY_TILE);
         const long blocks = (long)((a.M + ANY_TILE - 1L) / ANY_TILE) * a.tiles_j;
         SRF_CHECK(blocks < (1L << 32) / 256, "linear: %ld tiles are more than one launch holds", blocks);
-        linear_any_kernel<T, O><<<dim3((unsigned)blocks, plan.splits), 256, 0, s>>>(a);
+        linear_any_kernel<T, O><<<dim3((unsigned)blocks, a.splits), 256, 0, s>>>(a);
         SRF_LAUNCH_CHECK("linear_any_kernel");
     }
-    return plan.splits > 1 ? lin_join<O>(a, sums, s) : 0;
+    return a.splits > 1 ? lin_join<O>(a, sums, s) : 0;
 }
 static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPlan& plan, void* ws, const ColumnSums& sums, hipStream_t s) {
     switch (in_type) {
@@ -456,13 +471,17 @@ static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPla
             return lin_run<TypeE4M3, TypeF16>(a, plan, ws, sums, s);
     }
 }
-// dx and dw in one launch, then dw's join
-static int lin_pair(int type, LinArgs dx, const LinPlan& plan_x, LinArgs dw, const LinPlan& plan_w, void* ws, const ColumnSums& sums, hipStream_t s) {
-    lin_fill(dx, plan_x, nullptr);
-    lin_fill(dw, plan_w, ws);
+static int lin_join_as(int type, const LinArgs& a, const ColumnSums& sums, hipStream_t s) {
+    return type == SCENERF_T_F32 ? lin_join<TypeF32>(a, sums, s) : type == SCENERF_T_BF16 ? lin_join<TypeBF16>(a, sums, s) : lin_join<TypeF16>(a, sums, s);
+}
+// dx and dw in one launch, then their joins
+static int lin_pair(int type, LinArgs dx, const LinPlan& plan_x, void* ws_x, LinArgs dw, const LinPlan& plan_w, void* ws_w, const ColumnSums& sums, hipStream_t s) {
+    lin_fill(dx, plan_x, ws_x);
+    lin_fill(dw, plan_w, ws_w);
     if (int e = type == SCENERF_T_F32 ? linear_pair_f32(dx, dw, plan_x.tile, s) : type == SCENERF_T_BF16 ? linear_pair_bf16(dx, dw, plan_x.tile, s) : linear_pair_f16(dx, dw, plan_x.tile, s)) return e;
-    if (plan_w.splits == 1) return 0;
-    return type == SCENERF_T_F32 ? lin_join<TypeF32>(dw, sums, s) : type == SCENERF_T_BF16 ? lin_join<TypeBF16>(dw, sums, s) : lin_join<TypeF16>(dw, sums, s);
+    if (dw.splits > 1)
+        if (int e = lin_join_as(type, dw, sums, s)) return e;
+    return dx.splits > 1 ? lin_join_as(type, dx, ColumnSums{}, s) : 0;
 }
 
 // A matrix whose rows the staged kernel can read in 16-byte pieces: aligned base and pitch, a length of whole pieces (or zeros up to one),
@@ -508,8 +527,12 @@ static int dz_strip(int64_t rows) {
 }
 struct BackwardPlan {
     bool make_dz;                   // dz is not dy itself
+    // Where few values share it, the rounding of dz to 16 bits is undone: its rest is a second operand of dx's (dw's) product, whose sums are
+    // joined.  With many values dx and dw are 1.45 times as far from exact as their own rounding makes them, whatever the inputs; of few, now
+    // and then twice as far, and the second product costs little.
+    bool rest_x, rest_w;
     int strip, strips, dz_pitch;
-    int64_t part, dz, sums;         // offsets of the column sums' parts, of dz and of the split sums
+    int64_t part, dz, rest, sums_x, sums_w;     // offsets of the column sums' parts, of dz, of its rest and of the split sums
     int64_t bytes;
     LinPlan dx, dw;
     // One launch for both where they are on tiles of one shape, two workgroups or more a CU: dw's start first, dx's fill the CUs behind them.
@@ -531,12 +554,18 @@ static BackwardPlan lin_backward_plan(const scenerf_linear* p) {
     b.dw = lin_plan(p->in_type, true, true, dz_fits && lin_pieces(p->x, p->ldx, p->k, es, p->padded), p->n, p->k, p->rows,
                     p->dx && b.dx.kind == 2 && b.dx.splits == 1 && b.dx.tile != LIN_256x256 ? b.dx.tile : LIN_TILES);
     b.pair = p->dx && p->dw && p->rows > 0 && b.dx.kind == 2 && b.dw.kind == 2 && b.dx.tile == b.dw.tile && b.dx.tile != LIN_256x256 && b.dx.splits == 1;
+    const bool few = (int64_t)p->rows * p->n < 32768, rounds = products && es == 2 && p->activation != SCENERF_ACT_NONE;
+    b.rest_x = rounds && p->dx && (few || (int64_t)p->rows * p->k < 16384);
+    b.rest_w = rounds && p->dw && (few || (int64_t)p->n * p->k < 16384);
     int64_t at = 0;
     if (p->db) { b.part = at; at += align256((int64_t)b.strips * p->n * 4); }
     if (b.make_dz) { b.dz = at; at += align256(p->rows * b.dz_pitch * es); }
-    b.sums = at;
-    const int64_t sx = p->dx ? lin_part_bytes(b.dx, p->rows, p->k) : 0, sw = p->dw ? lin_part_bytes(b.dw, p->n, p->k) : 0;
-    b.bytes = at + (sx > sw ? sx : sw);
+    if (b.rest_x || b.rest_w) { b.rest = at; at += align256(p->rows * b.dz_pitch * es); }
+    b.sums_x = at;
+    if (p->dx) at += lin_part_bytes(b.dx, p->rows, p->k, b.rest_x);
+    b.sums_w = at;
+    if (p->dw) at += lin_part_bytes(b.dw, p->n, p->k, b.rest_w);
+    b.bytes = at;
     return b;
 }
 static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
@@ -560,13 +589,13 @@ static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
     }
     return 0;
 }
-template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardPlan& b, void* dz, float* part, hipStream_t s) {
+template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardPlan& b, void* dz, void* rest, float* part, hipStream_t s) {
     int lx = 2;
     while (lx < 6 && (8 << lx) < p->n) ++lx;
     const dim3 grid(b.strips, cdiv(p->n, 8 << lx));
     SRF_CHECK(grid.y <= 65535, "linear_backward: n is too large");
-    if (p->n % 8 == 0) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
-    else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
+    if (p->n % 8 == 0) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, rest, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
+    else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, rest, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
     SRF_LAUNCH_CHECK("linear_dz_kernel");
     return 0;
 }
@@ -633,15 +662,16 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
     float* part = (float*)(ws + b.part);
     const void* dz = b.make_dz ? ws + b.dz : p->dy;
     const long ld_dz = b.make_dz ? b.dz_pitch : p->ld_dy;
+    void* rest = b.rest_x || b.rest_w ? ws + b.rest : nullptr;
     if (p->rows > 0 && (b.make_dz || p->db)) {
         float* sums = p->db ? part : nullptr;
         void* to = b.make_dz ? (void*)dz : nullptr;
-        int e = p->out_type == SCENERF_T_F32 ? lin_dz<TypeF32>(p, b, to, sums, s)
-                : p->out_type == SCENERF_T_BF16 ? lin_dz<TypeBF16>(p, b, to, sums, s) : lin_dz<TypeF16>(p, b, to, sums, s);
+        int e = p->out_type == SCENERF_T_F32 ? lin_dz<TypeF32>(p, b, to, nullptr, sums, s)
+                : p->out_type == SCENERF_T_BF16 ? lin_dz<TypeBF16>(p, b, to, rest, sums, s) : lin_dz<TypeF16>(p, b, to, rest, sums, s);
         if (e) return e;
     }
     ColumnSums sums = {};
-    if (p->db && p->dw && b.dw.splits > 1) sums = {part, p->db, b.strips, p->n, cdiv(p->n, 16)};
+    if (p->db && p->dw && (b.dw.splits > 1 || b.rest_w)) sums = {part, p->db, b.strips, p->n, cdiv(p->n, 16)};
     else if (p->db) {
         if (int e = launch_sum_parts(p->out_type, part, b.strips, p->n, p->db, s)) return e;
     }
@@ -653,6 +683,7 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         ax.M = (int)p->rows; ax.N = p->k; ax.K = p->n;
         ax.b_ext = pitch;
         ax.out = p->dx;
+        ax.A2 = b.rest_x ? rest : nullptr;
     }
     if (p->dw) {     // rows == 0: an empty sum, zeros
         aw.A = dz; aw.a_i = 1; aw.a_k = ld_dz;
@@ -660,12 +691,13 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         aw.M = p->n; aw.N = p->k; aw.K = (int)p->rows;
         aw.a_ext = b.make_dz ? b.dz_pitch : p->n; aw.b_ext = pitch;
         aw.out = p->dw;
+        aw.A2 = b.rest_w ? rest : nullptr;
     }
-    if (b.pair) return lin_pair(p->in_type, ax, b.dx, aw, b.dw, ws + b.sums, sums, s);
+    if (b.pair) return lin_pair(p->in_type, ax, b.dx, ws + b.sums_x, aw, b.dw, ws + b.sums_w, sums, s);
     if (ax.out)
-        if (int e = lin_product(p->in_type, p->out_type, ax, b.dx, ws + b.sums, ColumnSums{}, s)) return e;
+        if (int e = lin_product(p->in_type, p->out_type, ax, b.dx, ws + b.sums_x, ColumnSums{}, s)) return e;
     if (aw.out)
-        if (int e = lin_product(p->in_type, p->out_type, aw, b.dw, ws + b.sums, sums, s)) return e;
+        if (int e = lin_product(p->in_type, p->out_type, aw, b.dw, ws + b.sums_w, sums, s)) return e;
     return 0;
 }
 

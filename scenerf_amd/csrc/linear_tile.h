@@ -86,11 +86,12 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
     const int split = id / tiles, tile = id - split * tiles;
     const long i0 = (long)(tile / p.tiles_j) * BM;
     const int j0 = (tile % p.tiles_j) * BN;
-    const int kb = (int)min((long)p.K, (long)split * p.k_split), ke = (int)min((long)p.K, (long)kb + p.k_split);
+    const bool again = p.half && split >= p.half;
+    const int kb = (int)min((long)p.K, (long)(again ? split - p.half : split) * p.k_split), ke = (int)min((long)p.K, (long)kb + p.k_split);
     const int chunks = ke > kb ? (ke - kb + BK - 1) / BK : 0;
 
     // ---- loads: of each side wave w moves pieces w, w + WAVES, ...  A's ring has NSA stages, B's behind it NSB.
-    const char* baseA = (const char*)p.A + i0 * p.a_i * ES;
+    const char* baseA = (const char*)(again ? p.A2 : p.A) + i0 * p.a_i * ES;
     const char* baseB = (const char*)p.B + (long)j0 * p.b_j * ES;
     const unsigned ringB = lds0 + NSA * SA::BYTES;
     // (the k of a wave's loads inside a chunk: the same for all of a side read along, equal steps apart for one read across)

@@ -9,7 +9,7 @@
 // wide ones, go through a workgroup that reads the row twice (the second time from L2).  The weight's gradient is summed per lane over the wave's rows, then over the workgroup's waves in
 // LDS, then over the workgroups by a second kernel in a fixed order: no atomics, the same bits every time.  Rows of any length and
 // alignment move 16 bytes at a time, but for a last piece that the row does not fill.
-// 153,600 x 512 bf16: forward with residual 109 to 116 us for 629 MB (5.4 to 5.8 TB/s; a large copy reaches 5.2), gradients 96 to 135 for 629 MB, 8
+// 153,600 x 512 bf16: forward with residual 109 to 116 us for 629 MB (5.4 to 5.8 TB/s; a large copy reaches 5.2), gradients with residual 130 for 786 MB, 8
 // bits 102 us for 551 MB; 40,001 x 2,480 fp16 to 8 bits 60 us for 298 MB; 4,801 x 515 fp32 out of wider rows 9 us.
 #include "rowops.h"
 
@@ -252,6 +252,12 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_grad_kernel(RmsArgs p) {
             if (in[c] > 0) {
                 load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, in[c], D % VW, h[c]);
                 load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, in[c], D % VW, g[c]);
+                if (p.residual) {
+                    float r[VW];
+                    load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, in[c], D % VW, r);
+#pragma unroll
+                    for (int e = 0; e < VW; ++e) h[c][e] += r[e];
+                }
                 if (AHEAD && p.dh) load_some<E, VW, WHOLE>((const raw*)p.dh + row * p.ld_dh + col, in[c], D % VW, d[c]);
             }
         }
@@ -319,12 +325,21 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_grad_wide_kernel(RmsArgs p) 
     typedef typename E::raw raw;
     __shared__ float red[WIDE_THREADS / 64];
     const long D = p.width;
+    auto row_values = [&](long row, long col, float (&h)[VW]) {
+        load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
+        if (p.residual) {
+            float r[VW];
+            load_some<E, VW, WHOLE>((const raw*)p.residual + row * p.ld_residual + col, (int)min(D - col, (long)VW), (int)(D % VW), r);
+#pragma unroll
+            for (int e = 0; e < VW; ++e) h[e] += r[e];
+        }
+    };
     for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const float rstd = p.rstd[row];
         float dot = 0.f;
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW], g[VW], w[VW];
-            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
+            row_values(row, col, h);
             load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, (int)min(D - col, (long)VW), (int)(D % VW), g);
             load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), (int)(D % VW), w);
 #pragma unroll
@@ -333,7 +348,7 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_grad_wide_kernel(RmsArgs p) 
         dot = block_sum(dot, red) * p.inv_width;
         for (long col = (long)threadIdx.x * VW; col < D; col += WIDE_THREADS * VW) {
             float h[VW], g[VW], w[VW], d[VW];
-            load_some<E, VW, WHOLE>((const raw*)p.x + row * p.ldx + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
+            row_values(row, col, h);
             load_some<E, VW, WHOLE>((const raw*)p.dy + row * p.ld_dy + col, (int)min(D - col, (long)VW), (int)(D % VW), g);
             load_some<E, VW, WHOLE>((const raw*)p.weight + col, (int)min(D - col, (long)VW), (int)(D % VW), w);
 #pragma unroll
@@ -354,8 +369,11 @@ __global__ __launch_bounds__(256) void rms_dweight_cols_kernel(RmsArgs p, int st
     const long r0 = (long)blockIdx.y * strip, r1 = min((long)p.rows, r0 + strip);
     float s = 0.f;
     if (col < p.width)
-        for (long r = r0 + ty; r < r1; r += 4)
-            s = fmaf(E::to_f32(((const raw*)p.dy)[r * p.ld_dy + col]), E::to_f32(((const raw*)p.x)[r * p.ldx + col]) * p.rstd[r], s);
+        for (long r = r0 + ty; r < r1; r += 4) {
+            float h = E::to_f32(((const raw*)p.x)[r * p.ldx + col]);
+            if (p.residual) h += E::to_f32(((const raw*)p.residual)[r * p.ld_residual + col]);
+            s = fmaf(E::to_f32(((const raw*)p.dy)[r * p.ld_dy + col]), h * p.rstd[r], s);
+        }
     red[ty][threadIdx.x & 63] = s;
     __syncthreads();
     if (ty == 0 && col < p.width)

@@ -39,15 +39,18 @@ def _check(what, x, weight, residual, eps) -> None:
 
 
 def rms_step_back(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, eps: float, dy: torch.Tensor, dh: Optional[torch.Tensor],
-                  need_x: bool, need_w: bool):
-    """(gradient of h, gradient of weight), None where not needed; h as the forward stored it, ``dh`` what else flows into it."""
+                  need_x: bool, need_w: bool, residual: Optional[torch.Tensor] = None):
+    """(gradient of h, gradient of weight), None where not needed; h as the forward stored it (or its x, with its ``residual``), ``dh`` what
+    else flows into it."""
     width, dev = h.shape[-1], h.device
     h2, dy2, w = rows_of(h, width), rows_of(dy, width), weight.contiguous()
     dh2 = rows_of(dh, width) if dh is not None else None
+    r2 = rows_of(residual, width) if residual is not None else None
     dx = dy.new_empty(dy.shape) if need_x else None
     dw = dy.new_empty(width) if need_w else None
     run_rows("rms", True, RMS.pack(
-        TYPE_CODES[h.dtype], width, h2.shape[0], eps, h2.data_ptr(), h2.stride(0), 0, 0, w.data_ptr(), 0, 0, 0, 0, rstd.data_ptr(),
+        TYPE_CODES[h.dtype], width, h2.shape[0], eps, h2.data_ptr(), h2.stride(0), 0 if r2 is None else r2.data_ptr(),
+        0 if r2 is None else r2.stride(0), w.data_ptr(), 0, 0, 0, 0, rstd.data_ptr(),
         dy2.data_ptr(), dy2.stride(0), 0 if dh2 is None else dh2.data_ptr(), 0 if dh2 is None else dh2.stride(0),
         0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0, 0), dev, "rms_norm backward")
     return dx, dw
@@ -60,20 +63,25 @@ class _RmsNorm(torch.autograd.Function):
         ctx.eps, ctx.has_residual = eps, residual is not None
         ctx.set_materialize_grads(False)
         if residual is None:
-            ctx.save_for_backward(x2, weight, rstd)
+            ctx.save_for_backward(x2, weight, rstd, None)
             return y
-        ctx.save_for_backward(h, weight, rstd)
+        if x.dtype == torch.float32:
+            ctx.save_for_backward(h, weight, rstd, None)
+        else:
+            # 16 bits: the gradients are made from x + residual once more, not from h as it was stored, whose rounding made dweight half as
+            # inexact again as its own does (153,600 x 512 bf16: 96 us from h, 130 so)
+            ctx.save_for_backward(x2, weight, rstd, residual)
         return y, h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
+        h, weight, rstd, residual = ctx.saved_tensors
         need_h = ctx.needs_input_grad[0] or (ctx.has_residual and ctx.needs_input_grad[2])
         if dy is None:               # only h was used
             dx, dw = dh, torch.zeros_like(weight) if ctx.needs_input_grad[1] and dh is not None else None
         else:
-            dx, dw = rms_step_back(h, weight, rstd, ctx.eps, dy, dh, need_h, ctx.needs_input_grad[1])
+            dx, dw = rms_step_back(h, weight, rstd, ctx.eps, dy, dh, need_h, ctx.needs_input_grad[1], residual)
         return dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.has_residual and ctx.needs_input_grad[2] else None, None
 
 
@@ -81,7 +89,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.
              eps: float = 1e-6) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, h = x (+ residual): x and residual (..., width), weight
     (width,), all of one type.  Returns y, or ``(y, h)`` where a residual is added: h is the next residual stream.  Differentiable once in
-    x, weight and residual (one gradient serves x and residual)."""
+    x, weight and residual (one gradient serves x and residual); none of x, residual and h may change before the backward pass."""
     _check("rms_norm", x, weight, residual, eps)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         return _RmsNorm.apply(x, weight, residual, float(eps))

@@ -43,8 +43,9 @@ def slope64(z, name):
     return torch.ones_like(z)
 
 
-def linear64(x, w, b=None, act="none", r=None, dy=None, scales=None, out_dtype=None):
-    """{name: (value, bound)} of y and, with dy, of dx, dw, db, dr."""
+def linear64(x, w, b=None, act="none", r=None, dy=None, scales=None, out_dtype=None, whole_dz=False):
+    """{name: (value, bound)} of y and, with dy, of dx, dw, db, dr.  ``whole_dz``: dz with what its rounding leaves out as an operand of its own,
+    so that the rest's rounding alone is left."""
     t = out_dtype or x.dtype
     u, tiny = half(t), least(t)
     X, W = x.double(), w.double()
@@ -74,7 +75,7 @@ def linear64(x, w, b=None, act="none", r=None, dy=None, scales=None, out_dtype=N
     dz = g * slope64(z, act)
     # the slope at the kept z (rounded to t); dz itself is rounded to t where it is an operand
     esum = g.abs() * (BEND[act] * (ez + u * z.abs() + tiny) + (2.0 ** -20 if act in ("gelu", "silu") else 0.0))
-    edz = esum if act == "none" else esum + u * dz.abs() + tiny
+    edz = esum if act == "none" else esum + (u * u * dz.abs() if whole_dz else u * dz.abs()) + tiny
     m = X.shape[0]
     dx = dz @ W
     out["dx"] = (dx.reshape(*lead, k), (edz @ W.abs() + (n + 8) * 2.0 ** -23 * (dz.abs() @ W.abs()) + u * dx.abs() + tiny).reshape(*lead, k))

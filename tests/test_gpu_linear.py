@@ -474,3 +474,24 @@ def test_threads_on_their_own_streams():
         assert len(together[i]) == 10
         for got in together[i]:
             assert all(torch.equal(a, b) for a, b in zip(got, alone[i]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("m,k,n", [(1, 16, 16), (1, 300, 1000), (5, 43, 544), (33, 512, 130), (60, 2480, 130), (300, 12, 512), (4801, 64, 40), (20011, 42, 96), (1, 512, 3)])
+def test_few_gradients_are_made_from_the_whole_dz(m, k, n, dtype):
+    """Below 32,768 dz (16,384 dx, dw) their rounding to 16 bits is made good by a second operand: the bounds know no rounding of dz."""
+    from scenerf_amd.linear import linear
+    g = gen("whole dz", m, k, n, dtype)
+    leaves = [t.requires_grad_(True) for t in (normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5), normal(g, n, dtype=dtype))]
+    dy = normal(g, m, n, dtype=dtype)
+    for act in ("gelu", "silu"):
+        want = linear64(*(t.detach() for t in leaves), act, None, dy, whole_dz=True)
+        dx, dw, db = torch.autograd.grad(linear(*leaves, activation=act), leaves, dy)
+        hold(db, want["db"], "db")
+        if m * n < 32768 or m * k < 16384:
+            hold(dx, want["dx"], "dx")
+        if m * n < 32768 or n * k < 16384:
+            hold(dw, want["dw"], "dw")
+    dy[0, 0] = float("inf")
+    dx, dw, db = torch.autograd.grad(linear(*leaves, activation="silu"), leaves, dy)
+    assert not bool(torch.isfinite(db[0])) and bool(torch.isfinite(db[1:]).all()) and bool(torch.isfinite(dx[1:]).all()) and bool(torch.isfinite(dw[1:]).all())

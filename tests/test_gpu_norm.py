@@ -245,3 +245,28 @@ def test_rows_past_32_bit_offsets():
         q, s, _ = rms_norm_8bit(x, w, residual=r)
         one = rms_norm_8bit(x[-last:], w, residual=r[-last:])
     assert torch.equal(q[-last:].view(torch.uint8), one[0].view(torch.uint8)) and torch.equal(s[-last:], one[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("m,d", [(1, 16), (1, 5000), (3, 515), (32, 272), (120, 512), (4801, 515), (700, 4100)])
+def test_gradients_are_made_from_the_unrounded_sum(m, d, dtype):
+    """16 bits: the gradients against the formula at x + residual, with bounds that know no rounding of h."""
+    from scenerf_amd.norm import rms_norm
+    g = gen("unrounded", m, d, dtype)
+    x, r, dy, dh = (normal(g, m, d, dtype=dtype) for _ in range(4))
+    w = (1 + 0.2 * normal(g, d)).to(dtype)
+    leaves = [t.requires_grad_(True) for t in (x, r, w)]
+    dx, dr, dw = torch.autograd.grad(rms_norm(x, w, residual=r), leaves, (dy, dh))
+    # in 32 bits x + r is off by 2^-24 at most: the oracle without a residual, on that sum, rounded as the outputs are
+    want = rms64(x.detach().double() + r.detach().double(), w.detach().double(), 1e-6, None, dy.double(), dh.double())
+    u, tiny, e = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2, (d + 64) * 2.0 ** -22
+    for name, got in (("dx", dx), ("dx", dr), ("dw", dw)):
+        value, _ = want[name]
+        h64 = x.detach().double() + r.detach().double()
+        rstd = 1 / torch.sqrt((h64 * h64).mean(1, keepdim=True) + 1e-6)
+        if name == "dx":
+            a = (dy.double() * w.detach().double()).abs()
+            size = rstd * (a + (h64 * rstd).abs() * (a * (h64 * rstd).abs()).mean(1, keepdim=True)) + dh.double().abs()
+        else:
+            size = (dy.double() * h64 * rstd).abs().sum(0) * (1 + m)
+        hold(got, (value, u * value.abs() + e * size + tiny), name)
