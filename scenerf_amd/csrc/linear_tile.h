@@ -36,6 +36,11 @@ __device__ static inline void lin_copy(const void* src, unsigned lds_base) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_base) : "memory", "m0");
 }
 
+// the same from a base all lanes share and an offset of each: no vector instruction but the load itself
+__device__ static inline void lin_copy_from(const void* base, unsigned offset, unsigned lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds_base) : "memory", "m0");
+}
+
 // contiguous ranges of work per XCD (blocks go round-robin over the 8 XCDs, each with its own L2); any count
 __device__ static inline int lin_xcd_order(int id, int total) {
     const int q = total >> 3, r = total & 7, xcd = id & 7, slot = id >> 3;
@@ -117,15 +122,24 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
     }
     // load u of chunk c of a side.  What lies past the end of the split comes from a zero, and so do chunks past the last (nobody reads
     // them): every turn of the loop issues the same loads, without a branch.
-    auto loadA = [&](int c, int u) {
+    // (inside: the chunk is known to end before the split does)
+    auto loadA = [&](int c, int u, auto inside) {
         const long k0 = kb + (long)c * BK;
-        const char* src = baseA + (k0 + u * KA) * p.a_k * ES + offA[AX ? 0 : u];
-        lin_copy(kinA < ke - k0 - u * KA ? src : (const char*)lin_zeros, lds0 + (c % NSA) * SA::BYTES + (wv + u * WAVES) * 1024);
+        if constexpr (decltype(inside)::value) {
+            lin_copy_from(baseA + (k0 + u * KA) * p.a_k * ES, offA[AX ? 0 : u], lds0 + (c % NSA) * SA::BYTES + (wv + u * WAVES) * 1024);
+        } else {
+            const char* src = baseA + (k0 + u * KA) * p.a_k * ES + offA[AX ? 0 : u];
+            lin_copy(kinA < ke - k0 - u * KA ? src : (const char*)lin_zeros, lds0 + (c % NSA) * SA::BYTES + (wv + u * WAVES) * 1024);
+        }
     };
-    auto loadB = [&](int c, int u) {
+    auto loadB = [&](int c, int u, auto inside) {
         const long k0 = kb + (long)c * BK;
-        const char* src = baseB + (k0 + u * KB) * p.b_k * ES + offB[BX ? 0 : u];
-        lin_copy(kinB < ke - k0 - u * KB ? src : (const char*)lin_zeros, ringB + (c % NSB) * SB::BYTES + (wv + u * WAVES) * 1024);
+        if constexpr (decltype(inside)::value) {
+            lin_copy_from(baseB + (k0 + u * KB) * p.b_k * ES, offB[BX ? 0 : u], ringB + (c % NSB) * SB::BYTES + (wv + u * WAVES) * 1024);
+        } else {
+            const char* src = baseB + (k0 + u * KB) * p.b_k * ES + offB[BX ? 0 : u];
+            lin_copy(kinB < ke - k0 - u * KB ? src : (const char*)lin_zeros, ringB + (c % NSB) * SB::BYTES + (wv + u * WAVES) * 1024);
+        }
     };
 
     // ---- fragments
@@ -228,16 +242,20 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    // Chunks whose loads end inside the split go through a loop of their own, without the loads' comparisons, selections and 64-bit sums
+    // (1.7 vector instructions a matrix instruction else): 153,600 x 2,480 x 1,536 bf16 1,165 -> 1,140 us and its dx 1,111 -> 1,075, 8 bits 677 ->
+    // 669, 4,800 x 512 x 512 fp32 with its gradients 71 -> 67.  Small tiles of 16 and 8 bits have few chunks and lose by the longer code (29.8 -> 30.4).
+    constexpr bool FAST = ES == 4 || BM * BN >= 128 * 128;
     Frag f0, f1;
     if (chunks > 0) {
 #pragma unroll
         for (int c = 0; c < NSA; ++c) {
 #pragma unroll
             for (int u = 0; u < LA; ++u)
-                if (c < NSA - 1) loadA(c, u);
+                if (c < NSA - 1) loadA(c, u, Bool<false>());
 #pragma unroll
             for (int u = 0; u < LB; ++u)
-                if (c < NSB) loadB(c, u);
+                if (c < NSB) loadB(c, u, Bool<false>());
         }
         // chunk 0 has landed: what was issued behind it may be outstanding
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NSA - 2) * LA + (NSB - 1) * LB) : "memory");
@@ -245,19 +263,27 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int t = 0; t < READS; ++t) fetch(0, 0, f0, t);
-#pragma unroll 1
-        for (int c = 0; c < chunks; ++c) {
+        auto chunk = [&](int c, auto inside) {
 #pragma unroll
             for (int part = 0; part < PARTS - 1; ++part)
-                turn(part % 2 ? f1 : f0, c, part + 1, part % 2 ? f0 : f1, [&](int u) { loadA(c + NSA - 1, u); }, part * LA / (PARTS - 1),
+                turn(part % 2 ? f1 : f0, c, part + 1, part % 2 ? f0 : f1, [&](int u) { loadA(c + NSA - 1, u, inside); }, part * LA / (PARTS - 1),
                      (part + 1) * LA / (PARTS - 1));
             // this wave's loads of chunk c + 1 have landed, its reads of chunk c are done; behind the barrier that holds for every wave:
             // the stages of chunk c are free
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NSA - 2) * LA + (NSB - 2) * LB) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            turn(f1, c + 1, 0, f0, [&](int u) { loadB(c + NSB, u); }, 0, LB);
+            turn(f1, c + 1, 0, f0, [&](int u) { loadB(c + NSB, u, inside); }, 0, LB);
+        };
+        // as long as what is loaded is inside the split, and the last few
+        int c = 0;
+        if constexpr (FAST) {
+            const int last = (ke - kb) / BK - (NSB > NSA - 1 ? NSB : NSA - 1);
+#pragma unroll 1
+            for (; c < last; ++c) chunk(c, Bool<true>());
         }
+#pragma unroll 1
+        for (; c < chunks; ++c) chunk(c, Bool<false>());
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
