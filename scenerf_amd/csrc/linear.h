@@ -13,7 +13,7 @@ struct LinArgs {
     void* out; void* z;                  // dense [M][N]
     float* part;                         // not NULL: the raw sums of split s go to part[s][M][N] instead
     int act, tiles_i, tiles_j, splits, k_split;     // k_split: contraction elements per split
-    const void* A2; int half;            // half > 0: splits half .. 2 half - 1 are splits 0 .. half - 1 again, of A2
+    const void* A2;                      // not NULL (16 bits, backward): laid out like A, its products are added to A's
 };
 
 template <int W> __device__ static inline void act_any(int act, float (&v)[W]) {

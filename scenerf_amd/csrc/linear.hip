@@ -6,8 +6,9 @@
 // read along k), dx contracts the outputs (w is read across), dw contracts the rows (both are read across).
 //
 // Products of many rows run on staged tiles (linear_tile.h): bound by the chip's power where the contraction is long (153,600 x 2,480
-// x 1,536 bf16 1,044 us = 1.12 PFLOP/s; the library's product of that shape without an epilogue 1,054; 8 bits 635 us; 4,096 x 8,192 x 4,096 takes 256 us, and 162 if all of it is zeros), by the operands' and
-// results' bytes where it is short (153,600 x 512 x 512 bf16 with gelu, residual and kept sums 165 us for 629 MB).
+// x 1,536 bf16 999 us = 1.17 PFLOP/s; the library's product of that shape without an epilogue 1,054; 8 bits 630 us; 4,096 x 8,192 x 4,096 takes
+// 256 us, and 162 if all of it is zeros), by the operands' and results' bytes where it is short (153,600 x 512 x 512 bf16 with gelu,
+// residual and kept sums 165 us for 629 MB).
 #include "linear.h"
 
 typedef __attribute__((ext_vector_type(8))) __bf16 lin_bf16x8;
@@ -52,9 +53,8 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const long i0 = (long)(blockIdx.x / p.tiles_j) * ANY_TILE;
     const int j0 = (blockIdx.x % p.tiles_j) * ANY_TILE;
-    const bool again = p.half && (int)blockIdx.y >= p.half;
-    const void* A = again ? p.A2 : p.A;
-    const long kb = (long)(again ? blockIdx.y - p.half : blockIdx.y) * p.k_split, ke = min((long)p.K, kb + p.k_split);
+    const void* A = p.A;
+    const long kb = (long)blockIdx.y * p.k_split, ke = min((long)p.K, kb + p.k_split);
     lin_f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
@@ -85,6 +85,10 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
             } else {
                 acc = Mma<S>::run(*(const uint4*)(rb + k * 2), *(const uint4*)(ra + k * 2), acc);
             }
+        }
+        if (k0 + ANY_K >= ke && p.A2 && A == p.A) {        // once more, with A2
+            A = p.A2;
+            k0 = kb - ANY_K;
         }
     }
     const long i = i0 + (wv >> 1) * 32 + (lane & 31);
@@ -352,8 +356,8 @@ static const LinTileCost kLinCost32[] = {{LIN_128x128, 2, 4.7, {1.8, 3.6}}, {LIN
 #define LIN_MIN_CHUNKS 8            // a split keeps at least so many: its ends cost as much
 
 // `staged`: both operands are in 16-byte pieces
-// `like`: a tile whose product could share another one's launch, worth a tenth
-static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, long K, LinTile like = LIN_TILES) {
+// `like`: a tile whose product could share another one's launch, worth a tenth; `large`: 256 x 256 tiles are among them
+static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, long K, LinTile like = LIN_TILES, bool large = true) {
     LinPlan r = {0, 1, 0, LIN_128x128};
     // (bf16, this kernel against staged tiles: 1 row x 512 x 512 2.2 against 4.9 us, 8 rows 3.7 against 4.9, 8 x 2,480 x 1,536 5.5 against 9.7;
     // 16 rows 5.3 against 5.0.  It reads whole 16 bytes inside the row: a shorter row takes the element loads; a launch holds 2^32 threads)
@@ -381,6 +385,7 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
         double best = 1e300;
         for (int c = 0; c < kinds; ++c) {
             const LinTileCost& t = cost[c];
+            if (!large && t.tile == LIN_256x256) continue;
             const long tiles = tiles_of(kLinTileRows[t.tile], kLinTileCols[t.tile]), slots = 256L * t.per_cu;
             const long most = max(1L, min(slots / max(1L, tiles), chunks / LIN_MIN_CHUNKS));
             // 1, 2 or 3 workgroups a CU, or none of it split
@@ -404,11 +409,7 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
     r.k_split = (int)(((K + r.splits - 1) / r.splits + bk - 1) / bk * bk);
     return r;
 }
-// `twice`: with a second A (LinArgs.A2)
-static int64_t lin_part_bytes(const LinPlan& p, long M, int N, bool twice = false) {
-    const int splits = p.splits * (twice ? 2 : 1);
-    return splits > 1 ? align256((int64_t)splits * M * N * 4) : 0;
-}
+static int64_t lin_part_bytes(const LinPlan& p, long M, int N) { return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0; }
 
 template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, hipStream_t s) {
     // one piece a lane and row of w: one wave a group of columns; longer rows: four (bf16, 8 rows, 512 outputs, one wave against four: 512
@@ -417,8 +418,7 @@ template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, 
     else linear_few_kernel<T, O, MR, 4><<<cdiv(a.N, FEW_COLS), 256, 0, s>>>(a);
 }
 static void lin_fill(LinArgs& a, const LinPlan& plan, void* ws) {
-    a.half = a.A2 ? plan.splits : 0;
-    a.splits = plan.splits + a.half;
+    a.splits = plan.splits;
     a.k_split = plan.k_split;
     a.part = a.splits > 1 ? (float*)ws : nullptr;
     if (plan.kind == 2) {
@@ -471,17 +471,13 @@ static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPla
             return lin_run<TypeE4M3, TypeF16>(a, plan, ws, sums, s);
     }
 }
-static int lin_join_as(int type, const LinArgs& a, const ColumnSums& sums, hipStream_t s) {
-    return type == SCENERF_T_F32 ? lin_join<TypeF32>(a, sums, s) : type == SCENERF_T_BF16 ? lin_join<TypeBF16>(a, sums, s) : lin_join<TypeF16>(a, sums, s);
-}
-// dx and dw in one launch, then their joins
-static int lin_pair(int type, LinArgs dx, const LinPlan& plan_x, void* ws_x, LinArgs dw, const LinPlan& plan_w, void* ws_w, const ColumnSums& sums, hipStream_t s) {
-    lin_fill(dx, plan_x, ws_x);
-    lin_fill(dw, plan_w, ws_w);
+// dx and dw in one launch, then dw's join
+static int lin_pair(int type, LinArgs dx, const LinPlan& plan_x, LinArgs dw, const LinPlan& plan_w, void* ws, const ColumnSums& sums, hipStream_t s) {
+    lin_fill(dx, plan_x, nullptr);
+    lin_fill(dw, plan_w, ws);
     if (int e = type == SCENERF_T_F32 ? linear_pair_f32(dx, dw, plan_x.tile, s) : type == SCENERF_T_BF16 ? linear_pair_bf16(dx, dw, plan_x.tile, s) : linear_pair_f16(dx, dw, plan_x.tile, s)) return e;
-    if (dw.splits > 1)
-        if (int e = lin_join_as(type, dw, sums, s)) return e;
-    return dx.splits > 1 ? lin_join_as(type, dx, ColumnSums{}, s) : 0;
+    if (dw.splits == 1) return 0;
+    return type == SCENERF_T_F32 ? lin_join<TypeF32>(dw, sums, s) : type == SCENERF_T_BF16 ? lin_join<TypeBF16>(dw, sums, s) : lin_join<TypeF16>(dw, sums, s);
 }
 
 // A matrix whose rows the staged kernel can read in 16-byte pieces: aligned base and pitch, a length of whole pieces (or zeros up to one),
@@ -527,12 +523,12 @@ static int dz_strip(int64_t rows) {
 }
 struct BackwardPlan {
     bool make_dz;                   // dz is not dy itself
-    // Where few values share it, the rounding of dz to 16 bits is undone: its rest is a second operand of dx's (dw's) product, whose sums are
-    // joined.  With many values dx and dw are 1.45 times as far from exact as their own rounding makes them, whatever the inputs; of few, now
-    // and then twice as far, and the second product costs little.
+    // Where few values share it, the rounding of dz to 16 bits is undone: its rest is a second operand of dx's (dw's) product.  With many
+    // values dx and dw are 1.45 times as far from exact as their own rounding makes them, whatever the inputs; of few, now and then twice as
+    // far, and going over the contraction again costs little.
     bool rest_x, rest_w;
     int strip, strips, dz_pitch;
-    int64_t part, dz, rest, sums_x, sums_w;     // offsets of the column sums' parts, of dz, of its rest and of the split sums
+    int64_t part, dz, rest, sums;     // offsets of the column sums' parts, of dz, of its rest and of the split sums
     int64_t bytes;
     LinPlan dx, dw;
     // One launch for both where they are on tiles of one shape, two workgroups or more a CU: dw's start first, dx's fill the CUs behind them.
@@ -550,22 +546,20 @@ static BackwardPlan lin_backward_plan(const scenerf_linear* p) {
     b.make_dz = products && (p->activation != SCENERF_ACT_NONE || (dz_fits && !lin_pieces(p->dy, p->ld_dy, p->n, es, false)));
     b.strip = dz_strip(p->rows);
     b.strips = (int)((p->rows + b.strip - 1) / b.strip);
-    b.dx = lin_plan(p->in_type, false, true, dz_fits && lin_pieces(p->w, p->ldw, p->k, es, p->padded), p->rows, p->k, p->n);
-    b.dw = lin_plan(p->in_type, true, true, dz_fits && lin_pieces(p->x, p->ldx, p->k, es, p->padded), p->n, p->k, p->rows,
-                    p->dx && b.dx.kind == 2 && b.dx.splits == 1 && b.dx.tile != LIN_256x256 ? b.dx.tile : LIN_TILES);
-    b.pair = p->dx && p->dw && p->rows > 0 && b.dx.kind == 2 && b.dw.kind == 2 && b.dx.tile == b.dw.tile && b.dx.tile != LIN_256x256 && b.dx.splits == 1;
     const bool few = (int64_t)p->rows * p->n < 32768, rounds = products && es == 2 && p->activation != SCENERF_ACT_NONE;
     b.rest_x = rounds && p->dx && (few || (int64_t)p->rows * p->k < 16384);
     b.rest_w = rounds && p->dw && (few || (int64_t)p->n * p->k < 16384);
+    b.dx = lin_plan(p->in_type, false, true, dz_fits && lin_pieces(p->w, p->ldw, p->k, es, p->padded), p->rows, p->k, p->n, LIN_TILES, !b.rest_x);
+    b.dw = lin_plan(p->in_type, true, true, dz_fits && lin_pieces(p->x, p->ldx, p->k, es, p->padded), p->n, p->k, p->rows,
+                    p->dx && b.dx.kind == 2 && b.dx.splits == 1 && b.dx.tile != LIN_256x256 ? b.dx.tile : LIN_TILES, !b.rest_w);
+    b.pair = p->dx && p->dw && p->rows > 0 && b.dx.kind == 2 && b.dw.kind == 2 && b.dx.tile == b.dw.tile && b.dx.tile != LIN_256x256 && b.dx.splits == 1;
     int64_t at = 0;
     if (p->db) { b.part = at; at += align256((int64_t)b.strips * p->n * 4); }
     if (b.make_dz) { b.dz = at; at += align256(p->rows * b.dz_pitch * es); }
     if (b.rest_x || b.rest_w) { b.rest = at; at += align256(p->rows * b.dz_pitch * es); }
-    b.sums_x = at;
-    if (p->dx) at += lin_part_bytes(b.dx, p->rows, p->k, b.rest_x);
-    b.sums_w = at;
-    if (p->dw) at += lin_part_bytes(b.dw, p->n, p->k, b.rest_w);
-    b.bytes = at;
+    b.sums = at;
+    const int64_t sx = p->dx ? lin_part_bytes(b.dx, p->rows, p->k) : 0, sw = p->dw ? lin_part_bytes(b.dw, p->n, p->k) : 0;
+    b.bytes = at + (sx > sw ? sx : sw);
     return b;
 }
 static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
@@ -671,7 +665,7 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         if (e) return e;
     }
     ColumnSums sums = {};
-    if (p->db && p->dw && (b.dw.splits > 1 || b.rest_w)) sums = {part, p->db, b.strips, p->n, cdiv(p->n, 16)};
+    if (p->db && p->dw && b.dw.splits > 1) sums = {part, p->db, b.strips, p->n, cdiv(p->n, 16)};
     else if (p->db) {
         if (int e = launch_sum_parts(p->out_type, part, b.strips, p->n, p->db, s)) return e;
     }
@@ -693,11 +687,11 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         aw.out = p->dw;
         aw.A2 = b.rest_w ? rest : nullptr;
     }
-    if (b.pair) return lin_pair(p->in_type, ax, b.dx, ws + b.sums_x, aw, b.dw, ws + b.sums_w, sums, s);
+    if (b.pair) return lin_pair(p->in_type, ax, b.dx, aw, b.dw, ws + b.sums, sums, s);
     if (ax.out)
-        if (int e = lin_product(p->in_type, p->out_type, ax, b.dx, ws + b.sums_x, ColumnSums{}, s)) return e;
+        if (int e = lin_product(p->in_type, p->out_type, ax, b.dx, ws + b.sums, ColumnSums{}, s)) return e;
     if (aw.out)
-        if (int e = lin_product(p->in_type, p->out_type, aw, b.dw, ws + b.sums_w, sums, s)) return e;
+        if (int e = lin_product(p->in_type, p->out_type, aw, b.dw, ws + b.sums, sums, s)) return e;
     return 0;
 }
 

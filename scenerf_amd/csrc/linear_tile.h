@@ -91,12 +91,11 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
     const int split = id / tiles, tile = id - split * tiles;
     const long i0 = (long)(tile / p.tiles_j) * BM;
     const int j0 = (tile % p.tiles_j) * BN;
-    const bool again = p.half && split >= p.half;
-    const int kb = (int)min((long)p.K, (long)(again ? split - p.half : split) * p.k_split), ke = (int)min((long)p.K, (long)kb + p.k_split);
+    const int kb = (int)min((long)p.K, (long)split * p.k_split), ke = (int)min((long)p.K, (long)kb + p.k_split);
     const int chunks = ke > kb ? (ke - kb + BK - 1) / BK : 0;
 
     // ---- loads: of each side wave w moves pieces w, w + WAVES, ...  A's ring has NSA stages, B's behind it NSB.
-    const char* baseA = (const char*)(again ? p.A2 : p.A) + i0 * p.a_i * ES;
+    const char* baseA = (const char*)p.A + i0 * p.a_i * ES;
     const char* baseB = (const char*)p.B + (long)j0 * p.b_j * ES;
     const unsigned ringB = lds0 + NSA * SA::BYTES;
     // (the k of a wave's loads inside a chunk: the same for all of a side read along, equal steps apart for one read across)
@@ -246,8 +245,11 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
     // (1.7 vector instructions a matrix instruction else): 153,600 x 2,480 x 1,536 bf16 1,165 -> 1,140 us and its dx 1,111 -> 1,075, 8 bits 677 ->
     // 669, 4,800 x 512 x 512 fp32 with its gradients 71 -> 67.  Small tiles of 16 and 8 bits have few chunks and lose by the longer code (29.8 -> 30.4).
     constexpr bool FAST = ES == 4 || BM * BN >= 128 * 128;
+    constexpr bool TWICE = ES == 2 && BX && BM * BN < 256 * 256;       // (LinArgs.A2; the large tiles have no registers for it)
     Frag f0, f1;
-    if (chunks > 0) {
+    bool again = TWICE && p.A2;
+#pragma unroll 1
+    while (chunks > 0) {
 #pragma unroll
         for (int c = 0; c < NSA; ++c) {
 #pragma unroll
@@ -284,6 +286,14 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
         }
 #pragma unroll 1
         for (; c < chunks; ++c) chunk(c, Bool<false>());
+        if (!TWICE || !again) break;
+        if constexpr (TWICE) {
+            again = false;
+            baseA = (const char*)p.A2 + i0 * p.a_i * ES;
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();           // the rings are free again
+            asm volatile("" ::: "memory");
+        }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
