@@ -573,8 +573,8 @@ static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
     SRF_CHECK(p->ldx >= 0 && p->ldw >= 0 && p->ld_residual >= 0 && p->ld_dy >= 0, "%s: negative leading dimension", what);
     if (backward) {
         SRF_CHECK(p->in_type != SCENERF_T_E4M3, "%s: the 8-bit form has no gradients", what);
+        if (p->rows == 0) return 0;         // (an empty dx has no address)
         SRF_CHECK(p->dx || p->dw || p->db, "%s: nothing to compute", what);
-        if (p->rows == 0) return 0;
         SRF_CHECK(p->dy && (p->w || !p->dx) && (p->x || !p->dw), "%s: NULL dy, w or x", what);
         SRF_CHECK(p->activation == SCENERF_ACT_NONE || p->z, "%s: z is NULL", what);
     } else if (p->rows > 0) {

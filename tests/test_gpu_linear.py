@@ -495,3 +495,16 @@ def test_few_gradients_are_made_from_the_whole_dz(m, k, n, dtype):
     dy[0, 0] = float("inf")
     dx, dw, db = torch.autograd.grad(linear(*leaves, activation="silu"), leaves, dy)
     assert not bool(torch.isfinite(db[0])) and bool(torch.isfinite(db[1:]).all()) and bool(torch.isfinite(dx[1:]).all()) and bool(torch.isfinite(dw[1:]).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_no_rows_through_frozen_parameters(dtype):
+    from scenerf_amd.linear import linear
+    from scenerf_amd.norm import rms_norm
+    g = gen("frozen", dtype)
+    w, b = normal(g, 9, 12, dtype=dtype), normal(g, 9, dtype=dtype)
+    for act in ACTS:
+        x = normal(g, 0, 12, dtype=dtype).requires_grad_(True)
+        assert torch.autograd.grad(linear(x, w, b, activation=act).sum(), x)[0].shape == (0, 12)
+    x = normal(g, 0, 12, dtype=dtype).requires_grad_(True)
+    assert torch.autograd.grad(rms_norm(x, normal(g, 12, dtype=dtype)).sum(), x)[0].shape == (0, 12)

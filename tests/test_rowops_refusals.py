@@ -129,3 +129,15 @@ def test_a_call_without_its_workspace_says_so():
     r = _capi.Rms(type=0, width=8, rows=3, eps=1e-6)
     r.x, r.weight, r.rstd, r.dy, r.dweight = 16, 16, 16, 16, 16
     assert lib.scenerf_hip_rms_backward(C.byref(r), None) == _capi.NEEDS_WORKSPACE
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_a_step_back_of_no_rows_has_nothing_to_write(kind):
+    """Frozen parameters and no rows: the one gradient asked for, x's, is empty and its pointer NULL."""
+    lib = _capi.load()
+    p = _linear(in_type=kind, out_type=kind, rows=0, x=None, y=None, activation=2)
+    assert lib.scenerf_hip_linear_workspace(C.byref(p), 1) == 0
+    assert lib.scenerf_hip_linear_backward(C.byref(p), None) == 0
+    r = _rms(type=kind, rows=0, x=None, y=None)
+    assert lib.scenerf_hip_rms_workspace(C.byref(r), 1) == 0
+    assert lib.scenerf_hip_rms_backward(C.byref(r), None) == 0
