@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .rowops import LINEAR, MAX_ROWS, TYPE_CODES, check_float, check_tensors, no_gradient, rows_forward, rows_of, run_on, run_rows, together
+from .rowops import LINEAR, MAX_ROWS, TYPE_CODES, check_float, check_tensors, no_gradient, no_tangent, rows_forward, rows_of, run_on, run_rows, together
 
 
 def _activation(name: str) -> int:
@@ -89,6 +89,7 @@ def linear_step(x: torch.Tensor, weight: torch.Tensor, bias, residual, act: int,
 
 def linear_step_back(saved, dy: torch.Tensor, x_shape, need_x: bool, need_w: bool, need_b: bool):
     """(dx, dweight, dbias), None where not needed."""
+    no_tangent("linear's step back", dy)
     x2, w2, z, rows, n, k, pitch, padded, act = saved
     dev = dy.device
     # (dy is of x's type: autograd sees to it; new_empty takes less of the host's time than empty)
@@ -130,10 +131,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """``act(x @ weight.T + bias) + residual``: x (..., k), weight (n, k), bias (n,), residual (..., n), all of one type -> (..., n).
 
     ``activation``: "none", "relu", "gelu" (the exact one, by erf) or "silu".  Sums, bias, activation and addition are in 32 bits; the
-    result is rounded once.  Differentiable once in x, weight, bias and residual; where an activation is asked for and a gradient will
+    result is rounded once.  Differentiable once, in reverse, in x, weight, bias and residual; where an activation is asked for and a gradient will
     be, the sums in front of it are kept in the operands' type."""
     act = _activation(activation)
     dtype = x.dtype
+    no_tangent("linear", x, weight, bias, residual)
     if not together(x, weight, bias, residual):
         check_tensors("linear", x.device, dtype, ("weight", weight), ("bias", bias), ("residual", residual))
     code = check_float("linear", "x", dtype)
@@ -153,6 +155,7 @@ def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     bias, residual and the result are of ``out_dtype``.  Forward only."""
     act = _activation(activation)
     dev = x.device
+    no_tangent("linear_8bit", x_scale, weight_scale, bias, residual)
     check_tensors("linear_8bit", dev, torch.float8_e4m3fn, ("x", x), ("weight", weight))
     check_float("linear_8bit", "out_dtype", out_dtype)
     check_tensors("linear_8bit", dev, torch.float32, ("x_scale", x_scale), ("weight_scale", weight_scale))
@@ -172,6 +175,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows in 8 bits: x (..., width) float32 / bfloat16 / float16 -> (q (..., width) float8_e4m3fn, scale (...) float32) with
     scale = max(max|row| / 448, 2^-126) and q = x / scale rounded to nearest even: x is q * scale up to half a step of e4m3.  A row that
     holds a NaN or an infinity gets a scale that is not finite, and stands for no number."""
+    no_tangent("quantize_rows", x)
     check_tensors("quantize_rows", x.device, x.dtype)
     check_float("quantize_rows", "x", x.dtype)
     if x.dim() < 1 or x.shape[-1] < 1:

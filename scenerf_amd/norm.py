@@ -18,11 +18,12 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from .rowops import MAX_ROWS, RMS, TYPE_CODES, check_float, check_tensors, no_gradient, rows_forward, rows_of, run_rows, together
+from .rowops import MAX_ROWS, RMS, TYPE_CODES, check_float, check_tensors, no_gradient, no_tangent, rows_forward, rows_of, run_rows, together
 
 
 def _check(what, x, weight, residual, eps) -> None:
     shape = x.shape
+    no_tangent(what, x, weight, residual)
     if not together(x, weight, residual):
         check_tensors(what, x.device, x.dtype, ("weight", weight), ("residual", residual))
     check_float(what, "x", x.dtype)
@@ -42,6 +43,7 @@ def rms_step_back(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, eps
                   need_x: bool, need_w: bool, residual: Optional[torch.Tensor] = None):
     """(gradient of h, gradient of weight), None where not needed; h as the forward stored it (or its x, with its ``residual``), ``dh`` what
     else flows into it."""
+    no_tangent("rms_norm's step back", dy, dh)
     width, dev = h.shape[-1], h.device
     h2, dy2, w = rows_of(h, width), rows_of(dy, width), weight.contiguous()
     dh2 = rows_of(dh, width) if dh is not None else None
@@ -88,8 +90,8 @@ class _RmsNorm(torch.autograd.Function):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
              eps: float = 1e-6) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, h = x (+ residual): x and residual (..., width), weight
-    (width,), all of one type.  Returns y, or ``(y, h)`` where a residual is added: h is the next residual stream.  Differentiable once in
-    x, weight and residual (one gradient serves x and residual); none of x, residual and h may change before the backward pass."""
+    (width,), all of one type.  Returns y, or ``(y, h)`` where a residual is added: h is the next residual stream.  Differentiable once,
+    in reverse, in x, weight and residual (one gradient serves x and residual); none of x, residual and h may change before the backward pass."""
     _check("rms_norm", x, weight, residual, eps)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         return _RmsNorm.apply(x, weight, residual, float(eps))

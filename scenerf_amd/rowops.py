@@ -6,6 +6,7 @@ import struct
 from typing import Any, Dict
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _capi
 
@@ -98,6 +99,14 @@ def run_rows(name: str, backward: bool, args: bytes, dev: torch.device, what: st
         rc = run(args, stream)
     if rc:
         _capi.check(rc, what)
+
+
+def no_tangent(what: str, *tensors) -> None:
+    """Refuses dual tensors: nothing else about them says that a derivative is asked for, and grad mode does not concern them."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("%s has no forward-mode derivative (got a dual tensor)" % what)
 
 
 def no_gradient(what: str, *tensors) -> None:

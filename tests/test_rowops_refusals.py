@@ -141,3 +141,40 @@ def test_a_step_back_of_no_rows_has_nothing_to_write(kind):
     r = _rms(type=kind, rows=0, x=None, y=None)
     assert lib.scenerf_hip_rms_workspace(C.byref(r), 1) == 0
     assert lib.scenerf_hip_rms_backward(C.byref(r), None) == 0
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor asks for no gradient and has an address like any: without a refusal its tangent would be lost without a word."""
+    import torch.autograd.forward_ad as fwd
+    x, w, b = torch.ones(3, 4), torch.ones(5, 4), torch.ones(5)
+    q, s, wq = x.to(torch.float8_e4m3fn), torch.ones(3), w.to(torch.float8_e4m3fn)
+    one = torch.ones(4)
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+        for call in (lambda: linear(dual(x), w), lambda: linear(x, dual(w), b), lambda: linear(x, w, dual(b)), lambda: linear(x, w, residual=dual(torch.ones(3, 5))),
+                     lambda: linear_8bit(q, dual(s), wq, b), lambda: linear_8bit(q, s, wq, dual(b)), lambda: linear_8bit(q, s, wq, b, dual(b)),
+                     lambda: linear_8bit(q, s, wq, b, residual=dual(torch.ones(3, 5))), lambda: quantize_rows(dual(x)),
+                     lambda: rms_norm(dual(x), one), lambda: rms_norm(x, dual(one)), lambda: rms_norm(x, one, residual=dual(x)),
+                     lambda: rms_norm_8bit(dual(x), one), lambda: rms_norm_8bit(x, dual(one)), lambda: rms_norm_8bit(x, one, residual=dual(x))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="GPU only"):         # inside a level, but without a tangent
+            linear(x, w)
+
+
+@pytest.mark.parametrize("back", ["linear", "rms_norm"])
+def test_a_step_back_of_a_dual_tensor_is_refused(back):
+    """Forward mode over a step back: the incoming gradient alone has a tangent."""
+    import torch.autograd.forward_ad as fwd
+    from scenerf_amd.linear import linear_step_back
+    from scenerf_amd.norm import rms_step_back
+    with fwd.dual_level():
+        dy = fwd.make_dual(torch.ones(3, 4), torch.ones(3, 4))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            if back == "linear":
+                linear_step_back((torch.ones(3, 4), torch.ones(4, 4), None, 3, 4, 4, 4, 0, 0), dy, (3, 4), True, True, True)
+            else:
+                rms_step_back(torch.ones(3, 4), torch.ones(4), torch.ones(3), 1e-6, dy, None, True, True)
