@@ -508,3 +508,37 @@ def test_no_rows_through_frozen_parameters(dtype):
         assert torch.autograd.grad(linear(x, w, b, activation=act).sum(), x)[0].shape == (0, 12)
     x = normal(g, 0, 12, dtype=dtype).requires_grad_(True)
     assert torch.autograd.grad(rms_norm(x, normal(g, 12, dtype=dtype)).sum(), x)[0].shape == (0, 12)
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("m,n", [(3, 24), (70, 72), (300, 520), (5, 33)])
+def test_sums_past_the_range_of_their_type(m, n, dtype, act):
+    """Sums that are finite in 32 bits and not in the operands' type: the activation is at its limit there and so is its slope, 0 or 1."""
+    from scenerf_amd.linear import linear
+    g = gen("past", m, n, dtype, act)
+    k = 16
+    x, w, dy = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5), normal(g, m, n, dtype=dtype)
+    # three features alone reach the far columns: fp16 256 * 300 = 76,800; bf16 (1 + 127 / 128 + 3 / 512) 2^127, between the largest
+    # bf16, (1 + 127 / 128) 2^127, and the largest of 32 bits
+    big, weights = (2.0 ** 8, (300.0, 0.0, 0.0)) if dtype == torch.float16 else (2.0 ** 64, (2.0 ** 63, 2.0 ** 63 * 127 / 128, 2.0 ** 63 * 3 / 512))
+    x[:, :3], w[:, :3] = big, 0
+    low, high = list(range(0, n, 3)), list(range(1, n, 3))
+    near = [j for j in range(n) if j % 3 == 2]
+    w[low, :], w[high, :] = 0, 0
+    for f, v in enumerate(weights):
+        w[low, f], w[high, f] = -v, v
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    y = linear(x, w, activation=act)
+    z = x.detach().double() @ w.detach().double().t()
+    top = torch.finfo(dtype).max
+    assert bool((z[:, low] < -top).all()) and bool((z[:, high] > top).all()) and float(z.abs().max()) < torch.finfo(torch.float32).max
+    assert not bool(y.detach()[:, low].any())
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    # the far columns' slopes are 0 and 1 exactly; of dx the products with the three features' weights cancel or overflow: the others are held
+    part = linear64(x.detach()[:, 3:], w.detach()[near, 3:], None, act, None, dy[:, near])
+    hold(dx[:, 3:], part["dx"], "dx")
+    hold(dw[near, 3:], part["dw"], "dw of the near columns")
+    assert not bool(dw[low].any())
+    far = linear64(x.detach()[:, 3:], w.detach()[high, 3:], None, "none", None, dy[:, high])
+    hold(dw[high, 3:], far["dw"], "dw of the columns whose slope is 1")
