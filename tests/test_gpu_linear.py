@@ -542,3 +542,17 @@ def test_sums_past_the_range_of_their_type(m, n, dtype, act):
     assert not bool(dw[low].any())
     far = linear64(x.detach()[:, 3:], w.detach()[high, 3:], None, "none", None, dy[:, high])
     hold(dw[high, 3:], far["dw"], "dw of the columns whose slope is 1")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,d", [(1000, 512), (70, 515), (300, 2480), (40, 2481), (257, 4096), (33, 5000), (9, 4101)])
+def test_quantize_rows_to_the_bit(m, d, dtype):
+    """q is x / scale rounded once: values of 16 bits lie on e4m3's ties often, where the last bit of the quotient decides."""
+    from scenerf_amd.linear import quantize_rows
+    g = gen("ties", m, d, dtype)
+    x = normal(g, m, d, dtype=dtype)
+    q, s = quantize_rows(x)
+    x, q, s = x.cpu().float(), q.cpu(), s.cpu()
+    assert torch.equal(s, (x.abs().amax(1) / 448).clamp(min=2.0 ** -126))
+    want = (x / s[:, None]).to(torch.float8_e4m3fn)
+    assert torch.equal(q.view(torch.uint8), want.view(torch.uint8)), int((q.float() != want.float()).sum())
