@@ -172,7 +172,7 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
                                                  : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
     };
     // a chunk's contraction in PARTS, each one fragment of FR registers a lane per 32 rows: 16 (16-bit), 64 (8-bit), 8 (fp32) of it
-    constexpr bool WIDEN = ES == 1 && O::code == SCENERF_T_F32;
+    constexpr bool WIDEN = ES == 1 && O::code != SCENERF_T_BF16;
     constexpr int PARTS = ES == 1 ? 2 : 4, FR = ES == 1 ? 8 : 4;
     struct Frag { unsigned a[I][FR], b[J][FR]; };
     // item t of the READS that fetch a part: 16 bytes of the lane's for 32 rows of one side
@@ -202,8 +202,10 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
         auto eight = [](const unsigned (&r)[FR]) {
             return lin_i32x8{(int)r[0], (int)r[1], (int)r[2], (int)r[3], (int)r[4], (int)r[5], (int)r[6], (int)r[7]};
         };
-        // 8-bit operands of a result in 32 bits: the 8-bit matrix instruction adds 8 neighbouring products to 2^-13 of the largest of them
-        // (measured: linear.hip), not enough.  e4m3 is exact in bf16: widened here, at half the rate
+        // 8-bit operands of a result in fp32 or fp16: the 8-bit matrix instruction adds 8 neighbouring products to 2^-13 of the largest of them
+        // (measured: linear.hip), which is more than those types' own rounding (2^-24, 2^-11) where a group's 7 others lose it each.  e4m3 is exact
+        // in bf16: widened here, at half the rate.  A result in bf16, whose rounding is 2^-8 of it, takes the 8-bit instruction: what it
+        // leaves out shows where sums cancel to less than about 2^-3 of their terms' magnitudes
         auto wide = [&](const unsigned (&r)[FR]) {
             return __builtin_bit_cast(lin_bf16x8, make_uint4(widen2(r[2 * s], false), widen2(r[2 * s], true), widen2(r[2 * s + 1], false),
                                                              widen2(r[2 * s + 1], true)));

@@ -7,7 +7,7 @@ Here one call is one product with all of that behind its sums::
     q, s = quantize_rows(x)                                           # rows in e4m3 with one fp32 scale each
     y = linear_8bit(q, s, wq, ws, bias, activation="gelu", residual=h)
 
-float32 (fp32 matrix instructions), bfloat16 and float16 operands, 32-bit sums, every output rounded once.  Rows are whatever precedes
+float32 (fp32 matrix instructions), bfloat16 and float16 operands, 32-bit sums (``linear_8bit`` with a bfloat16 result: see there), every output rounded once.  Rows are whatever precedes
 the last dimension, zero rows included; a row's elements must be neighbours in memory (other layouts are copied first), its pitch is
 free.  CUDA tensors only: anything else raises, there is no fallback.
 """
@@ -152,7 +152,11 @@ def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
                 *, activation: str = "none", residual: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``linear`` on rows in 8 bits: x (..., k) and weight (n, k) float8_e4m3fn, x_scale (...) and weight_scale (n,) float32 as
     ``quantize_rows`` makes them; the sums of the 8-bit products are scaled by ``x_scale[row] * weight_scale[col]`` in front of the bias.
-    bias, residual and the result are of ``out_dtype``.  Forward only."""
+    bias, residual and the result are of ``out_dtype``.  Forward only.
+
+    Sums are in 32 bits where ``out_dtype`` is float32 or float16 (products at half the 8-bit rate) and for up to 8 rows.  For more rows with
+    a bfloat16 result the 8-bit matrix instructions add groups of 8 neighbouring products to 2^-13 of the group's largest: a sum may be off by 7 * 2^-13 of
+    its terms' magnitudes, which shows where it cancels, and a row computed alone may differ by that much from the same row among others."""
     act = _activation(activation)
     dev = x.device
     no_tangent("linear_8bit", x_scale, weight_scale, bias, residual)

@@ -556,3 +556,26 @@ def test_quantize_rows_to_the_bit(m, d, dtype):
     assert torch.equal(s, (x.abs().amax(1) / 448).clamp(min=2.0 ** -126))
     want = (x / s[:, None]).to(torch.float8_e4m3fn)
     assert torch.equal(q.view(torch.uint8), want.view(torch.uint8)), int((q.float() != want.float()).sum())
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.float16], ids=str)
+@pytest.mark.parametrize("m,k,n", [(1, 64, 16), (8, 512, 72), (9, 512, 72), (64, 40, 33), (300, 1024, 520), (5003, 1024, 130), (20011, 264, 48)])
+def test_8bit_sums_that_cancel(m, k, n, out):
+    """Large products that cancel beside small ones 2^-16 of their size.  Every partial sum, in any order, is a whole number of 2^-6 below 2^17, so
+    exact in 32 bits, and the result below 2^4, exact in fp16 too: the same bits whatever number of rows a call has."""
+    from scenerf_amd.linear import linear_8bit
+    g = gen("cancel", m, k, n)
+    small = torch.randint(-1, 2, (m, k), generator=g, device=DEV) * 2.0 ** -6
+    sign = 1 - 2 * torch.randint(0, 2, (n, k), generator=g, device=DEV).float()
+    at = torch.arange(0, k // 16 * 16, 8, device=DEV)          # one of each 8 neighbours, the next one's of the other sign
+    small[:, at] = 256.0
+    sign[:, at] = torch.where(at // 8 % 2 == 0, 4.0, -4.0)
+    x, w = small.to(torch.float8_e4m3fn), sign.to(torch.float8_e4m3fn)
+    assert torch.equal(x.float(), small) and torch.equal(w.float(), sign)
+    sx, sw = torch.ones(m, device=DEV), torch.ones(n, device=DEV)
+    want = small.double() @ sign.double().t()
+    assert float(want.abs().max()) < 16
+    got = linear_8bit(x, sx, w, sw, out_dtype=out)
+    assert torch.equal(got.double(), want), float((got.double() - want).abs().max())
+    alone = linear_8bit(x[m - 1:], sx[:1], w, sw, out_dtype=out)
+    assert torch.equal(alone[0], got[m - 1])
