@@ -14,6 +14,7 @@ struct LinArgs {
     float* part;                         // not NULL: the raw sums of split s go to part[s][M][N] instead
     int act, tiles_i, tiles_j, splits, k_split;     // k_split: contraction elements per split
     const void* A2;                      // not NULL (16 bits, backward): laid out like A, its products are added to A's
+    const float* unscale;                // not NULL (fp16, backward): A and A2 hold their values times 1 / *unscale, a power of two
 };
 
 template <int W> __device__ static inline void act_any(int act, float (&v)[W]) {
@@ -33,6 +34,7 @@ template <typename O> __device__ static inline float keep_z(float v) {
 template <typename O> __device__ static inline void epilogue_one(const LinArgs& p, long i, int j, float v) {
     typedef typename O::raw raw;
     if (p.row_scale) v = v * p.row_scale[i] * p.col_scale[j];
+    if (p.unscale) v *= *p.unscale;
     if (p.bias) v += O::to_f32(((const raw*)p.bias)[j]);
     if (p.z) ((raw*)p.z)[i * p.N + j] = O::from_f32(keep_z<O>(v));
     float one[1] = {v};
@@ -68,6 +70,11 @@ __device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<
         const float s = p.row_scale[i];
 #pragma unroll
         for (int e = 0; e < W; ++e) v[e] = v[e] * s * ec.scale[e];
+    }
+    if (p.unscale) {
+        const float s = *p.unscale;
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] *= s;
     }
 #pragma unroll
     for (int e = 0; e < W; ++e) v[e] += ec.bias[e];

@@ -274,14 +274,59 @@ template <int ACT> __device__ static inline void slopes(float (&g)[8], float (&z
 #pragma unroll
     for (int e = 0; e < 8; ++e) g[e] = e < valid ? g[e] * z[e] : 0.f;
 }
+// fp16's dz with a slope that is no whole number: dy times up to 1.13 may pass 65,504, and a dy of few bits (2^-20, say) times a slope would keep
+// fewer still.  So dz is held times the power of two that brings the largest finite |dy| into [2^14, 2^15), and the products' results are
+// divided by it, exactly: what is left below the largest dy's 2^-39 is all that fp16 does not hold.  This is that maximum, by strips of rows (157
+// MB of dy once more at 153,600 x 512: 541 -> 595 us there and back); a dy of bf16 or fp32 has its dz's range, and relu's slopes, 0 and 1, leave dy as it is.
+template <bool WHOLE>
+__global__ __launch_bounds__(256) void linear_dy_max_kernel(const void* dy_, long ld_dy, float* most, int M, int N, int strip) {
+    __shared__ float red[4];
+    const int per = (N + 7) / 8;
+    const long r0 = (long)blockIdx.x * strip, pieces = (min((long)M, r0 + strip) - r0) * per;
+    float m = 0.f;
+#pragma unroll 4
+    for (long t = threadIdx.x; t < pieces; t += 256) {
+        const long r = t / per;
+        const int j = (int)(t - r * per) * 8;
+        float v[8];
+        load_some<TypeF16, 8, WHOLE>((const uint16_t*)dy_ + (r0 + r) * ld_dy + j, N - j, N % 8, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fabsf(v[e]) < __builtin_inff() ? fmaxf(m, fabsf(v[e])) : m;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, WAVE));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) most[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+// the power of two from the strips' maxima, by every workgroup for itself; `red` is used before and may be used behind it
+__device__ static inline float dz_scale(const float* most, int count, float* red) {
+    float m = 0.f;
+    for (int t = threadIdx.x; t < count; t += 256) m = fmaxf(m, most[t]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, WAVE));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    __syncthreads();
+    return m > 0.f ? __uint_as_float((127u + 14u + 127u - (__float_as_uint(m) >> 23)) << 23) : 1.f;
+}
 // A workgroup's 256 threads stand as 2^lx columns of 8 by 256 / 2^lx rows (2^lx: 64, a wave a row, or what a narrower matrix needs: at 128
 // columns a fixed 32 left half the threads idle, 150 us for 262,144 x 128 fp32 instead of 78; 32 at 512 columns took 111 us for 153,600 rows
 // of bf16, 64 100); two rows a thread are in flight.  Bound by HBM: 4.7 and 5.2 TB/s.
+// `most`, not NULL (fp16): the strips' largest |dy|; dz is held scaled, and `unscale` says by what to multiply its products
 template <typename O, bool WHOLE>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld_dy, const void* z_, void* dz_, void* rest_, int pitch, float* part,
-                                                        int M, int N, int act, int strip, int lx) {
+                                                        const float* most, float* unscale, int M, int N, int act, int strip, int lx) {
     typedef typename O::raw raw;
     __shared__ float red[256 * 9];
+    float scale = 1.f;
+    if constexpr (O::code == SCENERF_T_F16) {
+        if (most) {
+            scale = dz_scale(most, gridDim.x, red);
+            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *unscale = 1.f / scale;
+        }
+    }
     const int tx = threadIdx.x & ((1 << lx) - 1), ty = threadIdx.x >> lx, rows = 256 >> lx;
     const int j0 = ((blockIdx.y << lx) + tx) * 8;           // (a pitch above N: zeros in the columns between)
     const long r0 = (long)blockIdx.x * strip, r1 = min((long)M, r0 + strip);
@@ -305,9 +350,13 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld
                 if (act == SCENERF_ACT_GELU) slopes<SCENERF_ACT_GELU>(g[q], z[q], N - j0);
                 else if (act == SCENERF_ACT_SILU) slopes<SCENERF_ACT_SILU>(g[q], z[q], N - j0);
                 else if (act == SCENERF_ACT_RELU) slopes<SCENERF_ACT_RELU>(g[q], z[q], N - j0);
-                if (dz_) store_vec<O, 8>((raw*)dz_ + (r + q * rows) * pitch + j0, g[q]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum[e] += g[q][e];
+                if constexpr (O::code == SCENERF_T_F16) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) g[q][e] *= scale;
+                }
+                if (dz_) store_vec<O, 8>((raw*)dz_ + (r + q * rows) * pitch + j0, g[q]);
                 if (rest_) {            // what dz's rounding left out
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -528,7 +577,8 @@ struct BackwardPlan {
     // far, and going over the contraction again costs little.
     bool rest_x, rest_w;
     int strip, strips, dz_pitch;
-    int64_t part, dz, rest, sums;     // offsets of the column sums' parts, of dz, of its rest and of the split sums
+    bool scaled;                    // dz is held times a power of two (linear_dy_max_kernel)
+    int64_t part, dz, rest, most, sums;     // offsets of the column sums' parts, of dz, of its rest, of the strips' largest |dy| and of the split sums
     int64_t bytes;
     LinPlan dx, dw;
     // One launch for both where they are on tiles of one shape, two workgroups or more a CU: dw's start first, dx's fill the CUs behind them.
@@ -553,10 +603,12 @@ static BackwardPlan lin_backward_plan(const scenerf_linear* p) {
     b.dw = lin_plan(p->in_type, true, true, dz_fits && lin_pieces(p->x, p->ldx, p->k, es, p->padded), p->n, p->k, p->rows,
                     p->dx && b.dx.kind == 2 && b.dx.splits == 1 && b.dx.tile != LIN_256x256 ? b.dx.tile : LIN_TILES, !b.rest_w);
     b.pair = p->dx && p->dw && p->rows > 0 && b.dx.kind == 2 && b.dw.kind == 2 && b.dx.tile == b.dw.tile && b.dx.tile != LIN_256x256 && b.dx.splits == 1;
+    b.scaled = b.make_dz && p->in_type == SCENERF_T_F16 && (p->activation == SCENERF_ACT_GELU || p->activation == SCENERF_ACT_SILU);
     int64_t at = 0;
     if (p->db) { b.part = at; at += align256((int64_t)b.strips * p->n * 4); }
     if (b.make_dz) { b.dz = at; at += align256(p->rows * b.dz_pitch * es); }
     if (b.rest_x || b.rest_w) { b.rest = at; at += align256(p->rows * b.dz_pitch * es); }
+    if (b.scaled) { b.most = at; at += align256((b.strips + 1) * 4LL); }        // (the last one: the products' factor)
     b.sums = at;
     const int64_t sx = p->dx ? lin_part_bytes(b.dx, p->rows, p->k) : 0, sw = p->dw ? lin_part_bytes(b.dw, p->n, p->k) : 0;
     b.bytes = at + (sx > sw ? sx : sw);
@@ -583,13 +635,21 @@ static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
     }
     return 0;
 }
-template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardPlan& b, void* dz, void* rest, float* part, hipStream_t s) {
+template <typename O> static int lin_dz(const scenerf_linear* p, const BackwardPlan& b, void* dz, void* rest, float* part, float* most, hipStream_t s) {
+    float* unscale = most ? most + b.strips : nullptr;
+    if (most) {
+        if (p->n % 8 == 0) linear_dy_max_kernel<true><<<b.strips, 256, 0, s>>>(p->dy, p->ld_dy, most, (int)p->rows, p->n, b.strip);
+        else linear_dy_max_kernel<false><<<b.strips, 256, 0, s>>>(p->dy, p->ld_dy, most, (int)p->rows, p->n, b.strip);
+        SRF_LAUNCH_CHECK("linear_dy_max_kernel");
+    }
     int lx = 2;
     while (lx < 6 && (8 << lx) < p->n) ++lx;
     const dim3 grid(b.strips, cdiv(p->n, 8 << lx));
     SRF_CHECK(grid.y <= 65535, "linear_backward: n is too large");
-    if (p->n % 8 == 0) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, rest, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
-    else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, rest, b.dz_pitch, part, (int)p->rows, p->n, p->activation, b.strip, lx);
+    if (p->n % 8 == 0) linear_dz_kernel<O, true><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, rest, b.dz_pitch, part, most, unscale, (int)p->rows, p->n, p->activation,
+                                                                         b.strip, lx);
+    else linear_dz_kernel<O, false><<<grid, 256, 0, s>>>(p->dy, p->ld_dy, p->z, dz, rest, b.dz_pitch, part, most, unscale, (int)p->rows, p->n, p->activation,
+                                                                         b.strip, lx);
     SRF_LAUNCH_CHECK("linear_dz_kernel");
     return 0;
 }
@@ -657,11 +717,13 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
     const void* dz = b.make_dz ? ws + b.dz : p->dy;
     const long ld_dz = b.make_dz ? b.dz_pitch : p->ld_dy;
     void* rest = b.rest_x || b.rest_w ? ws + b.rest : nullptr;
+    const float* unscale = b.scaled ? (const float*)(ws + b.most) + b.strips : nullptr;
     if (p->rows > 0 && (b.make_dz || p->db)) {
         float* sums = p->db ? part : nullptr;
         void* to = b.make_dz ? (void*)dz : nullptr;
-        int e = p->out_type == SCENERF_T_F32 ? lin_dz<TypeF32>(p, b, to, nullptr, sums, s)
-                : p->out_type == SCENERF_T_BF16 ? lin_dz<TypeBF16>(p, b, to, rest, sums, s) : lin_dz<TypeF16>(p, b, to, rest, sums, s);
+        int e = p->out_type == SCENERF_T_F32 ? lin_dz<TypeF32>(p, b, to, nullptr, sums, nullptr, s)
+                : p->out_type == SCENERF_T_BF16 ? lin_dz<TypeBF16>(p, b, to, rest, sums, nullptr, s)
+                : lin_dz<TypeF16>(p, b, to, rest, sums, b.scaled ? (float*)(ws + b.most) : nullptr, s);
         if (e) return e;
     }
     ColumnSums sums = {};
@@ -678,6 +740,7 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         ax.b_ext = pitch;
         ax.out = p->dx;
         ax.A2 = b.rest_x ? rest : nullptr;
+        ax.unscale = unscale;
     }
     if (p->dw) {     // rows == 0: an empty sum, zeros
         aw.A = dz; aw.a_i = 1; aw.a_k = ld_dz;
@@ -686,6 +749,7 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         aw.a_ext = b.make_dz ? b.dz_pitch : p->n; aw.b_ext = pitch;
         aw.out = p->dw;
         aw.A2 = b.rest_w ? rest : nullptr;
+        aw.unscale = unscale;
     }
     if (b.pair) return lin_pair(p->in_type, ax, b.dx, aw, b.dw, ws + b.sums, sums, s);
     if (ax.out)

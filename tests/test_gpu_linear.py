@@ -579,3 +579,78 @@ def test_8bit_sums_that_cancel(m, k, n, out):
     assert torch.equal(got.double(), want), float((got.double() - want).abs().max())
     alone = linear_8bit(x[m - 1:], sx[:1], w, sw, out_dtype=out)
     assert torch.equal(alone[0], got[m - 1])
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("m,k,n", [(4, 24, 40), (300, 64, 136), (5003, 72, 130), (20011, 264, 264)])
+def test_fp16_gradients_of_large_dy(m, k, n, act):
+    """dy near the type's largest value and a slope above 1: dz is past it, dx and db are not."""
+    from scenerf_amd.linear import linear
+    g = gen("large dy", m, k, n, act)
+    h = torch.float16
+    # sums around where the slope is largest: gelu 1.129 at 1.41, silu 1.0998 at 2.4
+    x, w, b = normal(g, m, k, dtype=h, scale=0.1), normal(g, n, k, dtype=h, scale=0.01), torch.full((n,), 1.41 if act == "gelu" else 2.4, dtype=h, device=DEV)
+    dy = torch.zeros(m, n, dtype=h, device=DEV)
+    rows = torch.arange(m, device=DEV)
+    dy[rows, rows % n] = torch.where(rows % 2 == 0, 65000.0, -64000.0).to(h)       # one a row
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(linear(*leaves, activation=act), leaves, dy)
+    want = linear64(*(t.detach() for t in leaves), act, None, dy)
+    assert float((dy.double() * 1.09).abs().max()) > 65504 * 1.05
+    for name, got in (("dx", dx), ("dw", dw), ("db", db)):
+        hold(got, want[name], name)
+    assert bool(torch.isfinite(dx).all())
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("m,k,n", [(300, 64, 136), (5003, 72, 130), (20011, 264, 264), (9001, 42, 1541)])
+def test_fp16_gradients_of_small_dy(m, k, n, act):
+    """dy around 2^-18, 60 times the smallest fp16: dz in fp16 itself would keep five bits.  Roundings are independent and add in squares: of dz, of z
+    in the slope and of the results together they are less than two half steps in the 2-norm."""
+    from scenerf_amd.linear import linear
+    g = gen("small dy", m, k, n, act)
+    h = torch.float16
+    # (w large, so that dx is not small itself; x small, so that z is of size 1)
+    x, w, b = normal(g, m, k, dtype=h, scale=2.0 ** -10), normal(g, n, k, dtype=h, scale=2.0 ** 9 * k ** -0.5), normal(g, n, dtype=h)
+    x[:, 0] = 0
+    x[:, 0] += 1
+    w[:, 0] = 0
+    dy = (normal(g, m, n) * 2.0 ** -18).to(h)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(linear(*leaves, activation=act), leaves, dy)
+    want = linear64(*(t.detach() for t in leaves), act, None, dy)
+    assert float(want["dx"][0][:, 1:].abs().mean()) > 2.0 ** -13
+    for name, got, v in (("dx", dx[:, 1:], want["dx"][0][:, 1:]), ("dw", dw[:, 0], want["dw"][0][:, 0])):
+        rounded = v.to(h).double()
+        lim = 2 * 2.0 ** -11 * float(v.norm()) + float((rounded - v).norm())
+        assert float((got.double() - v).norm()) <= lim, (name, float((got.double() - v).norm()) / float(v.norm()))
+
+
+@pytest.mark.parametrize("m,k,n", [(40, 72, 24), (5003, 72, 520)])
+def test_an_fp16_step_replays_with_dy_of_any_size(m, k, n):
+    """The power of two that dz is held by is found anew in every replay: dy of sizes 2^-18 to 2^14 in turn, each replay equal to the eager step."""
+    from scenerf_amd.linear import linear
+    g = gen("fp16 graph", m, k, n)
+    h = torch.float16
+    x, w, b = (t.requires_grad_(True) for t in (normal(g, m, k, dtype=h), normal(g, n, k, dtype=h, scale=k ** -0.5), normal(g, n, dtype=h)))
+    dy = normal(g, m, n, dtype=h)
+
+    def step():
+        return torch.autograd.grad(linear(x, w, b, activation="silu"), (x, w, b), dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = [t.detach() for t in step()]
+    for size in (-18, 0, 13, -10, 14):
+        dy.copy_((normal(g, m, n) * 2.0 ** size).clamp(-65504, 65504).to(h))
+        gr.replay()
+        eager = [t.detach() for t in step()]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) if bool(torch.isfinite(e).all()) else torch.equal(a.nan_to_num(), e.nan_to_num()) for a, e in zip(out, eager)), size
+    dy.zero_()
+    gr.replay()
+    assert all(not bool(t.any()) for t in out)
