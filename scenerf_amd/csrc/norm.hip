@@ -200,7 +200,8 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_rows_wide_kernel(RmsArgs p) 
             // max |h rstd w| = rstd max |h w|: the last bit may differ from the largest value's own, the scale's rounding
             m = block_max_u32(m, (uint32_t*)red);
             float top = __uint_as_float(m) * rstd;
-            if (m == 0x7f800000u && p.weight) {        // h w alone overflows: once more, in the order that y has
+            // h w alone overflows, or is too small to hold its bits (and its scale is not at its floor): once more, in the order that y has
+            if (p.weight && (m == 0x7f800000u || (m < 0x00800000u && rstd > 448.f))) {
                 m = 0;
                 for (long col = threadIdx.x; col < D; col += WIDE_THREADS) {
                     float h = E::to_f32(((const raw*)p.x)[row * p.ldx + col]);

@@ -270,3 +270,20 @@ def test_gradients_are_made_from_the_unrounded_sum(m, d, dtype):
         else:
             size = (dy.double() * h64 * rstd).abs().sum(0) * (1 + m)
         hold(got, (value, u * value.abs() + e * size + tiny), name)
+
+
+@pytest.mark.parametrize("m,d", [(3, 1030), (3, 5000), (300, 4096), (5, 512)])
+def test_8bit_rows_whose_weighted_values_underflow(m, d):
+    """h w below the smallest fp32, h rstd w well above it: the scale comes from y."""
+    from scenerf_amd.norm import rms_norm_8bit
+    g = gen("underflow", m, d)
+    x, w = normal(g, m, d) * 1e-18, (1 + 0.1 * normal(g, d)) * 1e-25
+    for rows in (slice(None), slice(0, 1)):
+        q, s = rms_norm_8bit(x[rows], w, eps=0.0)
+        y = rms64(x[rows], w, 0.0)["y"][0]
+        assert bool(((s.double() / (y.abs().amax(1) / 448) - 1).abs() <= (d + 32) * 2.0 ** -23).all())
+        back = q.double() * s.double()[:, None]
+        assert bool(((back - y).abs() <= (2.0 ** -4 + 2.0 ** -10) * y.abs() + s.double()[:, None] * 2.0 ** -9).all())
+    x[1] = 0                                        # (and a row of zeros stays one)
+    q, s = rms_norm_8bit(x, w, eps=1e-30)
+    assert not bool(q[1].float().any()) and float(s[1]) == 2.0 ** -126
