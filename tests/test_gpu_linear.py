@@ -654,3 +654,49 @@ def test_an_fp16_step_replays_with_dy_of_any_size(m, k, n):
     dy.zero_()
     gr.replay()
     assert all(not bool(t.any()) for t in out)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", TILES)
+def test_every_tile_on_whole_numbers(m, k, n, dtype):
+    """Sums that are exact in 32 bits, so that one product too few, or one twice, at the end of a tile, a split or a strip changes the result."""
+    from scenerf_amd.linear import linear
+    g = gen("whole tiles", m, k, n, dtype)
+    x, w, dy = whole(g, m, k, dtype=dtype), whole(g, n, k, dtype=dtype), whole(g, m, n, dtype=dtype)
+    b = whole(g, n, dtype=dtype) + 0.5
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    z = x.detach().double() @ w.detach().double().t() + b.detach().double()
+    for act in ("none", "relu"):
+        on = (z > 0).double() if act == "relu" else torch.ones_like(z)
+        dz = dy.double() * on
+        want = {"y": z * on, "dx": dz @ w.detach().double(), "dw": dz.t() @ x.detach().double(), "db": dz.sum(0)}
+        y = linear(*leaves, activation=act)
+        for name, got in zip(("y", "dx", "dw", "db"), (y.detach(),) + torch.autograd.grad(y, leaves, dy)):
+            assert float(want[name].abs().max()) < 2 ** 22
+            assert torch.equal(got, want[name].float().to(dtype)), (act, name, int((got.double() != want[name].float().to(dtype).double()).sum()))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", TILES)
+def test_every_tile_on_a_dy_of_few_rows(m, k, n, dtype):
+    """dy is not 0 in the last rows and around every 256th alone: a row of these that a split or strip drops is most of a sum, not one of thousands."""
+    from scenerf_amd.linear import linear
+    g = gen("few dy", m, k, n, dtype)
+    x, w, dy = whole(g, m, k, dtype=dtype), whole(g, n, k, dtype=dtype), torch.zeros(m, n, dtype=dtype, device=DEV)
+    rows = torch.tensor(sorted({r for c in range(0, m + 256, 256) for r in (c - 1, c) if 0 <= r < m} | set(range(max(0, m - 9), m))), device=DEV)
+    dy[rows] = whole(g, len(rows), n, dtype=dtype)
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    dx, dw = torch.autograd.grad(linear(*leaves), leaves, dy)
+    assert torch.equal(dx, (dy.double() @ w.detach().double()).float().to(dtype))
+    assert torch.equal(dw, (dy[rows].double().t() @ x.detach()[rows].double()).float().to(dtype))
+
+
+@pytest.mark.parametrize("out", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(20011, 42, 263), (300, 16392, 1544), (9001, 42, 1541), (9001, 16392, 130), (20011, 1544, 520), (300, 4104, 48), (5, 2480, 96)])
+def test_every_tile_in_8_bits_on_whole_numbers(m, k, n, out):
+    from scenerf_amd.linear import linear_8bit
+    g = gen("whole 8", m, k, n)
+    x, w = whole(g, m, k, dtype=torch.float32), whole(g, n, k, dtype=torch.float32)
+    x[:, k - 17:], w[:, k - 17:] = 2, 2         # (the end of the contraction weighs most)
+    got = linear_8bit(x.to(torch.float8_e4m3fn), torch.ones(m, device=DEV), w.to(torch.float8_e4m3fn), torch.ones(n, device=DEV), out_dtype=out)
+    assert torch.equal(got, (x.double() @ w.double().t()).float().to(out))

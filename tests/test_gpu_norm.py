@@ -287,3 +287,37 @@ def test_8bit_rows_whose_weighted_values_underflow(m, d):
     x[1] = 0                                        # (and a row of zeros stays one)
     q, s = rms_norm_8bit(x, w, eps=1e-30)
     assert not bool(q[1].float().any()) and float(s[1]) == 2.0 ** -126
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("m,d", [(1, 5000), (3, 515), (32, 272), (120, 512), (4801, 515), (700, 4100)])
+def test_gradients_do_not_know_the_rounded_sum(m, d, dtype):
+    """16 bits, in the 2-norm: the gradients are off by their own rounding and 32-bit sums, and an oracle made from h as it is stored is not."""
+    from scenerf_amd.norm import rms_norm
+    g = gen("unrounded norm", m, d, dtype)
+    x, r = normal(g, m, d, dtype=dtype), normal(g, m, d, dtype=dtype)
+    w = (1 + 0.2 * normal(g, d)).to(dtype)
+    h64 = x.double() + r.double()
+    leaves = [t.requires_grad_(True) for t in (x, r, w)]
+    # for dx a dy along h, so that the mean term weighs as much as the first; for dw one across it, so that its sum does not outgrow h's roundings
+    noise = normal(g, m, d)
+    along, across = (h64 + 0.5 * noise.double()).to(dtype), noise.to(dtype)
+    dx, dr = torch.autograd.grad(rms_norm(x, w, residual=r)[0], leaves[:2], along)
+    dw, = torch.autograd.grad(rms_norm(x, w, residual=r)[0], leaves[2:], across)
+    assert torch.equal(dx, dr)
+
+    def oracle(h, dy):
+        rstd = 1 / torch.sqrt((h64 * h64).mean(1, keepdim=True) + 1e-6)
+        a, xhat = dy.double() * w.detach().double(), h * rstd
+        terms = dy.double() * xhat
+        return {"dx": (rstd * (a - xhat * (a * xhat).mean(1, keepdim=True)), rstd * (a.abs() + xhat.abs() * (a * xhat).abs().mean(1, keepdim=True))),
+                "dw": (terms.sum(0), (terms * terms).sum(0).sqrt())}
+    for name, got, dy in (("dx", dx, along), ("dw", dw, across)):
+        value, size = oracle(h64, dy)[name]
+        stored, _ = oracle(h64.to(dtype).double(), dy)[name]
+        own = float((value.to(dtype).double() - value).norm())
+        # a value off by e before it is rounded is off by at most 2 e more behind it; the errors of 32-bit sums of m and d terms add in squares
+        lim = own + 2 * 4 * (m ** 0.5 + d ** 0.5) * 2.0 ** -24 * float(size.norm())
+        assert float((got.double() - value).norm()) <= lim, (name, float((got.double() - value).norm()), own, lim)
+        worse = float((stored.to(dtype).double() - value).norm())
+        assert worse > 1.1 * lim, (name, worse, lim)
