@@ -121,8 +121,12 @@ class PackedNormedMLP:
         return linear(rms_norm(h, n.norm_out, eps=eps).float(), n.w_out, n.b_out), None
 
     def _norm(self, x, weight, residual):
+        """y, h and what ``_norm_back`` needs: in 16 bits x and residual, whose sum h is rounded as it is stored."""
         y, _, h, rstd, x2 = rows_forward("rms_norm", x, weight, residual, self.spec.eps, keep_rstd=True)
-        return y, h, (x2 if h is None else h, weight, rstd)
+        return y, h, (x2, weight, rstd, residual) if h is None or self.dtype != torch.float32 else (h, weight, rstd, None)
+
+    def _norm_back(self, saved, dy, dh):
+        return rms_step_back(*saved[:3], self.spec.eps, dy, dh, True, True, saved[3])
 
     def _forward_kept(self, xenc, Z):
         n, nb, H, dt = self.net, self.n_blocks, self.d_hidden, self.dtype
@@ -144,18 +148,18 @@ class PackedNormedMLP:
     # ---- backward: parameter gradients into the sink; returns the gradient of zs (M, n_blocks * d_hidden)
     def backward(self, saved, d_logits: torch.Tensor) -> torch.Tensor:
         s_in, s_z, blocks, s_norm, s_out = saved
-        nb, H, dt, eps = self.n_blocks, self.d_hidden, self.dtype, self.spec.eps
+        nb, H, dt = self.n_blocks, self.d_hidden, self.dtype
         M = d_logits.shape[0]
         grads: List[Optional[torch.Tensor]] = [None] * len(self.shapes)
         dzs = torch.empty((M, nb, H), dtype=dt, device=d_logits.device)
         da, grads[2], grads[3] = linear_step_back(s_out, d_logits.contiguous(), (M, H), True, True, True)
-        dh, grads[4 + 7 * nb] = rms_step_back(*s_norm, eps, da.to(dt), None, True, True)
+        dh, grads[4 + 7 * nb] = self._norm_back(s_norm, da.to(dt), None)
         for b in range(nb - 1, -1, -1):
             s_n, s_0, s_1 = blocks[b]
             at = 4 + 6 * b
             dt_, grads[at + 2], grads[at + 3] = linear_step_back(s_1, dh, (M, H), True, True, True)
             da, grads[at], grads[at + 1] = linear_step_back(s_0, dt_, (M, H), True, True, True)
-            dh, grads[4 + 6 * nb + b] = rms_step_back(*s_n, eps, da, dh, True, True)
+            dh, grads[4 + 6 * nb + b] = self._norm_back(s_n, da, dh)
             dzs[:, b] = dh
         dzs = dzs.view(M, nb * H)
         _, dwz, dbz = linear_step_back(s_z, dzs, None, False, True, True)

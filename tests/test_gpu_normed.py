@@ -289,3 +289,26 @@ def test_one_reduction_of_the_gradients_per_net():
     assert sorted(seen) == sorted(sum(p.numel() for p in n.parameters()) for n in (m.mlp, m.mlp_gaussian))
     for a, b in zip(whole, half):
         assert off(2 * b, a) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,n_blocks,d_hidden", [(33, 1, 16), (257, 2, 144), (1000, 3, 512)])
+def test_a_session_trains_as_the_net_on_its_own_does(rows, n_blocks, d_hidden, dtype):
+    """The same operators on the same rows: every gradient behind lin_in (whose rows are padded in a session) has the same bits, in the type that
+    the net's own step rounds it to."""
+    m = net(11, 4, n_blocks, d_hidden)
+    pk = packed(m, "fp32" if dtype == torch.float32 else "bf16", True)
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    Z, dy = torch.randn(rows, 2480, generator=g, device=DEV).to(dtype), torch.randn(rows, 4, generator=g, device=DEV).to(dtype)
+    xenc = torch.zeros(rows, 48, device=DEV)
+    xenc[:, :42] = torch.randn(rows, 42, generator=g, device=DEV).to(dtype).float()
+    y, saved = pk.forward(xenc, Z, True)
+    own = m(torch.cat([Z, xenc[:, :42].to(dtype)], 1))
+    assert torch.equal(y.to(dtype), own.detach())
+    want = torch.autograd.grad(own, m.ordered_params(), dy)
+    pk.backward(saved, dy.float())
+    names = {id(v): k for k, v in m.named_parameters()}
+    for p, a, b in zip(m.ordered_params(), pk.unpack_grads(), want):
+        kind = torch.float32 if names[id(p)].startswith("lin_out") else dtype
+        if not names[id(p)].startswith("lin_in"):
+            assert torch.equal(a.to(kind), b.to(kind)), (names[id(p)], off(a, b))
