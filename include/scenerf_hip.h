@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define SCENERF_HIP_ABI_VERSION 11
+#define SCENERF_HIP_ABI_VERSION 12
 #define SCENERF_N_SCALES 5          /* feature maps "1_1","1_2","1_4","1_8","1_16" */
 #define SCENERF_D_LATENT 2480       /* 80+160+320+640+1280 (resnetfc d_latent, scenerf.py:100-114) */
 #define SCENERF_D_HIDDEN 512
@@ -594,8 +594,9 @@ int scenerf_hip_sphere_resample_backward_nhwc(const float* dout, int64_t planes,
  * that much on whether it is computed alone.
  * backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = the column sums of dz (the residual's gradient is dy itself). */
 typedef struct scenerf_linear {
-    int32_t in_type;                /* x, w (and dx, dw) */
-    int32_t out_type;               /* bias, residual, y, z, dy, db: equal to in_type unless that is E4M3 */
+    int32_t in_type;                /* x, w (and dx) */
+    int32_t out_type;               /* forward: bias, residual, y, z; equal to in_type unless that is E4M3.  backward (z and dy are of in_type):
+                                     * dw and db; in_type, or F32 for their sums as they are, to be added to others before they are rounded */
     int32_t activation;
     int32_t n, k;                   /* >= 1 */
     int32_t padded;                 /* 1: x and w are scenerf_hip_linear_pad's copies, zeros behind each row up to a whole number of 16 bytes */
@@ -633,6 +634,7 @@ typedef struct scenerf_rms {
     int32_t width;                  /* >= 1 */
     int64_t rows;                   /* >= 0, < 2^31 - 1024 */
     float eps;
+    int32_t dweight_f32;            /* backward: 1 for dweight in F32, its sum as it is; else 0 */
     const void* x; int64_t ldx;
     const void* residual; int64_t ld_residual;
     const void* weight;             /* [width] */
@@ -645,7 +647,7 @@ typedef struct scenerf_rms {
     const void* dy; int64_t ld_dy;
     const void* dh; int64_t ld_dh;  /* gradient of h, or NULL */
     void* dx;                       /* [rows][width], dense: the gradient of x and of residual */
-    void* dweight;                  /* [width], or NULL */
+    void* dweight;                  /* [width] of `type` or F32, or NULL */
     void* workspace; int64_t workspace_bytes;
 } scenerf_rms;
 int64_t scenerf_hip_rms_workspace(const scenerf_rms* p, int backward);

@@ -23,7 +23,7 @@ D_HIDDEN = 512
 D_XENC = 48
 TILE_ROWS = 128
 W_STREAM_BLOCKS = (3 * D_XENC + D_LATENT) // 16 + 2 * ((512 + D_LATENT) // 16) + 10 * (512 // 16)   # scenerf_hip.h
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 vp = C.c_void_p
 
@@ -121,7 +121,7 @@ class Linear(C.Structure):
 
 class Rms(C.Structure):
     """scenerf_rms (scenerf_hip.h)."""
-    _fields_ = [("type", C.c_int32), ("width", C.c_int32), ("rows", C.c_int64), ("eps", C.c_float),
+    _fields_ = [("type", C.c_int32), ("width", C.c_int32), ("rows", C.c_int64), ("eps", C.c_float), ("dweight_f32", C.c_int32),
                 ("x", vp), ("ldx", C.c_int64), ("residual", vp), ("ld_residual", C.c_int64), ("weight", vp), ("h", vp), ("y", vp),
                 ("q", vp), ("scale", vp), ("rstd", vp), ("dy", vp), ("ld_dy", C.c_int64), ("dh", vp), ("ld_dh", C.c_int64),
                 ("dx", vp), ("dweight", vp), ("workspace", vp), ("workspace_bytes", C.c_int64)]

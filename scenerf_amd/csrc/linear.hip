@@ -458,7 +458,8 @@ static LinPlan lin_plan(int type, bool ax, bool bx, bool staged, long M, int N, 
     r.k_split = (int)(((K + r.splits - 1) / r.splits + bk - 1) / bk * bk);
     return r;
 }
-static int64_t lin_part_bytes(const LinPlan& p, long M, int N) { return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0; }
+// `sums`: a result in fp32 of 16-bit operands (dw as it is summed), which the join alone writes
+static int64_t lin_part_bytes(const LinPlan& p, long M, int N, bool sums = false) { return p.splits > 1 || sums ? align256((int64_t)p.splits * M * N * 4) : 0; }
 
 template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, hipStream_t s) {
     // one piece a lane and row of w: one wave a group of columns; longer rows: four (bf16, 8 rows, 512 outputs, one wave against four: 512
@@ -466,25 +467,26 @@ template <typename T, typename O, int MR> static void lin_few(const LinArgs& a, 
     if (a.K <= 64 * (16 / (int)sizeof(typename T::raw))) linear_few_kernel<T, O, MR, 1><<<cdiv(a.N, 4 * FEW_COLS), 256, 0, s>>>(a);
     else linear_few_kernel<T, O, MR, 4><<<cdiv(a.N, FEW_COLS), 256, 0, s>>>(a);
 }
-static void lin_fill(LinArgs& a, const LinPlan& plan, void* ws) {
+static void lin_fill(LinArgs& a, const LinPlan& plan, void* ws, bool sums = false) {
     a.splits = plan.splits;
     a.k_split = plan.k_split;
-    a.part = a.splits > 1 ? (float*)ws : nullptr;
+    a.part = a.splits > 1 || sums ? (float*)ws : nullptr;
     if (plan.kind == 2) {
         a.tiles_i = (int)((a.M + (long)kLinTileRows[plan.tile] - 1) / kLinTileRows[plan.tile]);
         a.tiles_j = (int)((a.N + (long)kLinTileCols[plan.tile] - 1) / kLinTileCols[plan.tile]);
     }
 }
 template <typename O> static int lin_join(const LinArgs& a, const ColumnSums& sums, hipStream_t s) {
+    if (!a.part) return 0;
     constexpr int W = 16 / (int)sizeof(typename O::raw);
     const long work = ((long)a.M * ((a.N + W - 1) / W) + 31) / 32;
     linear_join_kernel<O><<<(unsigned)(work < 16384 ? work : 16384) + sums.blocks, 256, 0, s>>>(a, sums);
     SRF_LAUNCH_CHECK("linear_join_kernel");
     return 0;
 }
-// `sums`: column sums that ride along where the product is joined
-template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& plan, void* ws, const ColumnSums& sums, hipStream_t s) {
-    lin_fill(a, plan, ws);
+// `sums`: column sums that ride along where the product is joined; `in_sums`: lin_part_bytes
+template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& plan, void* ws, bool in_sums, const ColumnSums& sums, hipStream_t s) {
+    lin_fill(a, plan, ws, in_sums);
     if (plan.kind == 1) {
         if (a.M == 1) lin_few<T, O, 1>(a, s);
         else if (a.M == 2) lin_few<T, O, 2>(a, s);
@@ -507,26 +509,26 @@ template <typename T, typename O> static int lin_run(LinArgs a, const LinPlan& p
         linear_any_kernel<T, O><<<dim3((unsigned)blocks, a.splits), 256, 0, s>>>(a);
         SRF_LAUNCH_CHECK("linear_any_kernel");
     }
-    return a.splits > 1 ? lin_join<O>(a, sums, s) : 0;
+    return in_sums ? lin_join<TypeF32>(a, sums, s) : lin_join<O>(a, sums, s);
 }
 static int lin_product(int in_type, int out_type, const LinArgs& a, const LinPlan& plan, void* ws, const ColumnSums& sums, hipStream_t s) {
+    const bool in_sums = in_type != SCENERF_T_E4M3 && out_type != in_type;
     switch (in_type) {
-        case SCENERF_T_F32: return lin_run<TypeF32, TypeF32>(a, plan, ws, sums, s);
-        case SCENERF_T_BF16: return lin_run<TypeBF16, TypeBF16>(a, plan, ws, sums, s);
-        case SCENERF_T_F16: return lin_run<TypeF16, TypeF16>(a, plan, ws, sums, s);
+        case SCENERF_T_F32: return lin_run<TypeF32, TypeF32>(a, plan, ws, false, sums, s);
+        case SCENERF_T_BF16: return lin_run<TypeBF16, TypeBF16>(a, plan, ws, in_sums, sums, s);
+        case SCENERF_T_F16: return lin_run<TypeF16, TypeF16>(a, plan, ws, in_sums, sums, s);
         default:
-            if (out_type == SCENERF_T_F32) return lin_run<TypeE4M3, TypeF32>(a, plan, ws, sums, s);
-            if (out_type == SCENERF_T_BF16) return lin_run<TypeE4M3, TypeBF16>(a, plan, ws, sums, s);
-            return lin_run<TypeE4M3, TypeF16>(a, plan, ws, sums, s);
+            if (out_type == SCENERF_T_F32) return lin_run<TypeE4M3, TypeF32>(a, plan, ws, false, sums, s);
+            if (out_type == SCENERF_T_BF16) return lin_run<TypeE4M3, TypeBF16>(a, plan, ws, false, sums, s);
+            return lin_run<TypeE4M3, TypeF16>(a, plan, ws, false, sums, s);
     }
 }
 // dx and dw in one launch, then dw's join
-static int lin_pair(int type, LinArgs dx, const LinPlan& plan_x, LinArgs dw, const LinPlan& plan_w, void* ws, const ColumnSums& sums, hipStream_t s) {
+static int lin_pair(int type, int dw_type, LinArgs dx, const LinPlan& plan_x, LinArgs dw, const LinPlan& plan_w, void* ws, const ColumnSums& sums, hipStream_t s) {
     lin_fill(dx, plan_x, nullptr);
-    lin_fill(dw, plan_w, ws);
+    lin_fill(dw, plan_w, ws, dw_type != type);
     if (int e = type == SCENERF_T_F32 ? linear_pair_f32(dx, dw, plan_x.tile, s) : type == SCENERF_T_BF16 ? linear_pair_bf16(dx, dw, plan_x.tile, s) : linear_pair_f16(dx, dw, plan_x.tile, s)) return e;
-    if (dw.splits == 1) return 0;
-    return type == SCENERF_T_F32 ? lin_join<TypeF32>(dw, sums, s) : type == SCENERF_T_BF16 ? lin_join<TypeBF16>(dw, sums, s) : lin_join<TypeF16>(dw, sums, s);
+    return dw_type == SCENERF_T_F32 ? lin_join<TypeF32>(dw, sums, s) : dw_type == SCENERF_T_BF16 ? lin_join<TypeBF16>(dw, sums, s) : lin_join<TypeF16>(dw, sums, s);
 }
 
 // A matrix whose rows the staged kernel can read in 16-byte pieces: aligned base and pitch, a length of whole pieces (or zeros up to one),
@@ -610,7 +612,7 @@ static BackwardPlan lin_backward_plan(const scenerf_linear* p) {
     if (b.rest_x || b.rest_w) { b.rest = at; at += align256(p->rows * b.dz_pitch * es); }
     if (b.scaled) { b.most = at; at += align256((b.strips + 1) * 4LL); }        // (the last one: the products' factor)
     b.sums = at;
-    const int64_t sx = p->dx ? lin_part_bytes(b.dx, p->rows, p->k) : 0, sw = p->dw ? lin_part_bytes(b.dw, p->n, p->k) : 0;
+    const int64_t sx = p->dx ? lin_part_bytes(b.dx, p->rows, p->k) : 0, sw = p->dw ? lin_part_bytes(b.dw, p->n, p->k, p->out_type != p->in_type) : 0;
     b.bytes = at + (sx > sw ? sx : sw);
     return b;
 }
@@ -618,7 +620,7 @@ static int lin_check(const scenerf_linear* p, const char* what, bool backward) {
     SRF_CHECK(p, "%s: NULL argument", what);
     SRF_CHECK(p->in_type >= SCENERF_T_F32 && p->in_type <= SCENERF_T_E4M3 && p->out_type >= SCENERF_T_F32 && p->out_type <= SCENERF_T_F16,
               "%s: types must be F32, BF16, F16 or (x and w) E4M3", what);
-    SRF_CHECK(p->in_type == SCENERF_T_E4M3 || p->in_type == p->out_type, "%s: in_type and out_type differ", what);
+    SRF_CHECK(p->in_type == SCENERF_T_E4M3 || p->in_type == p->out_type || (backward && p->out_type == SCENERF_T_F32), "%s: in_type and out_type differ", what);
     SRF_CHECK(p->activation >= SCENERF_ACT_NONE && p->activation <= SCENERF_ACT_SILU, "%s: unknown activation %d", what, p->activation);
     SRF_CHECK(p->n >= 1 && p->k >= 1 && p->n < ROWOPS_GRID_MAX - 1024 && p->k < ROWOPS_GRID_MAX - 1024, "%s: n and k must be in [1, 2^31 - 1024)", what);
     SRF_CHECK(p->rows >= 0 && p->rows < ROWOPS_GRID_MAX - 1024, "%s: rows must be in [0, 2^31 - 1024)", what);
@@ -721,8 +723,8 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
     if (p->rows > 0 && (b.make_dz || p->db)) {
         float* sums = p->db ? part : nullptr;
         void* to = b.make_dz ? (void*)dz : nullptr;
-        int e = p->out_type == SCENERF_T_F32 ? lin_dz<TypeF32>(p, b, to, nullptr, sums, nullptr, s)
-                : p->out_type == SCENERF_T_BF16 ? lin_dz<TypeBF16>(p, b, to, rest, sums, nullptr, s)
+        int e = p->in_type == SCENERF_T_F32 ? lin_dz<TypeF32>(p, b, to, nullptr, sums, nullptr, s)
+                : p->in_type == SCENERF_T_BF16 ? lin_dz<TypeBF16>(p, b, to, rest, sums, nullptr, s)
                 : lin_dz<TypeF16>(p, b, to, rest, sums, b.scaled ? (float*)(ws + b.most) : nullptr, s);
         if (e) return e;
     }
@@ -751,9 +753,9 @@ int scenerf_hip_linear_backward(const scenerf_linear* p, scenerf_stream_t stream
         aw.A2 = b.rest_w ? rest : nullptr;
         aw.unscale = unscale;
     }
-    if (b.pair) return lin_pair(p->in_type, ax, b.dx, aw, b.dw, ws + b.sums, sums, s);
+    if (b.pair) return lin_pair(p->in_type, p->out_type, ax, b.dx, aw, b.dw, ws + b.sums, sums, s);
     if (ax.out)
-        if (int e = lin_product(p->in_type, p->out_type, ax, b.dx, ws + b.sums, ColumnSums{}, s)) return e;
+        if (int e = lin_product(p->in_type, p->in_type, ax, b.dx, ws + b.sums, ColumnSums{}, s)) return e;
     if (aw.out)
         if (int e = lin_product(p->in_type, p->out_type, aw, b.dw, ws + b.sums, sums, s)) return e;
     return 0;

@@ -446,6 +446,7 @@ static int rms_check(const scenerf_rms* p, const char* what, bool backward) {
     SRF_CHECK(p->type >= SCENERF_T_F32 && p->type <= SCENERF_T_F16, "%s: type must be F32, BF16 or F16", what);
     SRF_CHECK(p->width >= 1 && p->rows >= 0 && p->rows < ROWOPS_GRID_MAX - 1024, "%s: width >= 1 and 0 <= rows < 2^31 - 1024", what);
     SRF_CHECK(p->eps >= 0.f, "%s: eps must not be negative", what);
+    SRF_CHECK(p->dweight_f32 == 0 || p->dweight_f32 == 1, "%s: dweight_f32 is 0 or 1", what);
     SRF_CHECK(p->ldx >= 0 && p->ld_residual >= 0 && p->ld_dy >= 0 && p->ld_dh >= 0, "%s: negative leading dimension", what);
     if (p->rows == 0 && !(backward && p->dweight)) return 0;
     if (backward) {
@@ -509,7 +510,7 @@ template <typename E, bool WHOLE> static int rms_dispatch(const scenerf_rms* p, 
                 SRF_LAUNCH_CHECK("rms_dweight_cols_kernel");
             }
         }
-        if (p->dweight) return launch_sum_parts(E::code, a.partial, parts, p->width, p->dweight, s);
+        if (p->dweight) return launch_sum_parts(p->dweight_f32 ? SCENERF_T_F32 : E::code, a.partial, parts, p->width, p->dweight, s);
         return 0;
     }
     // (few and wide rows: a workgroup a row is done sooner than a wave -- 64 x 4,096 bf16 4.1 against 7.5 us, 256 x 2,048 4.1 against 5.0, but

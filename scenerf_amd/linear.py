@@ -87,15 +87,16 @@ def linear_step(x: torch.Tensor, weight: torch.Tensor, bias, residual, act: int,
     return y, (*pieces[5], z, rows, n, k, pieces[1], pieces[4], act)
 
 
-def linear_step_back(saved, dy: torch.Tensor, x_shape, need_x: bool, need_w: bool, need_b: bool):
-    """(dx, dweight, dbias), None where not needed."""
+def linear_step_back(saved, dy: torch.Tensor, x_shape, need_x: bool, need_w: bool, need_b: bool, sums: bool = False):
+    """(dx, dweight, dbias), None where not needed.  ``sums``: dweight and dbias in fp32, not rounded to their type."""
     no_tangent("linear's step back", dy)
     x2, w2, z, rows, n, k, pitch, padded, act = saved
     dev = dy.device
     # (dy is of x's type: autograd sees to it; new_empty takes less of the host's time than empty)
     dx = dy.new_empty(x_shape) if need_x else None
-    dw = dy.new_empty((n, k)) if need_w else None
-    db = dy.new_empty(n) if need_b else None
+    kind = torch.float32 if sums else dy.dtype
+    dw = dy.new_empty((n, k), dtype=kind) if need_w else None
+    db = dy.new_empty(n, dtype=kind) if need_b else None
     dy2 = rows_of(dy, n)
     code, xp = TYPE_CODES[x2.dtype], x2.data_ptr()
     if padded:
@@ -103,7 +104,7 @@ def linear_step_back(saved, dy: torch.Tensor, x_shape, need_x: bool, need_w: boo
     else:       # (where a hook on saved tensors has moved them, their pitch may be another)
         ldx, wp, ldw = x2.stride(0), w2.data_ptr(), w2.stride(0)
     run_rows("linear", True, LINEAR.pack(
-        code, code, act, n, k, padded, rows, xp, ldx, wp, ldw, 0, 0, 0, 0, 0, 0, 0 if z is None else z.data_ptr(), dy2.data_ptr(), dy2.stride(0),
+        code, _capi.T_F32 if sums else code, act, n, k, padded, rows, xp, ldx, wp, ldw, 0, 0, 0, 0, 0, 0, 0 if z is None else z.data_ptr(), dy2.data_ptr(), dy2.stride(0),
         0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), 0, 0), dev, "linear backward")
     return dx, dw, db
 

@@ -40,18 +40,18 @@ def _check(what, x, weight, residual, eps) -> None:
 
 
 def rms_step_back(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, eps: float, dy: torch.Tensor, dh: Optional[torch.Tensor],
-                  need_x: bool, need_w: bool, residual: Optional[torch.Tensor] = None):
+                  need_x: bool, need_w: bool, residual: Optional[torch.Tensor] = None, sums: bool = False):
     """(gradient of h, gradient of weight), None where not needed; h as the forward stored it (or its x, with its ``residual``), ``dh`` what
-    else flows into it."""
+    else flows into it.  ``sums``: the weight's in fp32, not rounded to its type."""
     no_tangent("rms_norm's step back", dy, dh)
     width, dev = h.shape[-1], h.device
     h2, dy2, w = rows_of(h, width), rows_of(dy, width), weight.contiguous()
     dh2 = rows_of(dh, width) if dh is not None else None
     r2 = rows_of(residual, width) if residual is not None else None
     dx = dy.new_empty(dy.shape) if need_x else None
-    dw = dy.new_empty(width) if need_w else None
+    dw = torch.empty(width, dtype=torch.float32 if sums else dy.dtype, device=dev) if need_w else None
     run_rows("rms", True, RMS.pack(
-        TYPE_CODES[h.dtype], width, h2.shape[0], eps, h2.data_ptr(), h2.stride(0), 0 if r2 is None else r2.data_ptr(),
+        TYPE_CODES[h.dtype], width, h2.shape[0], eps, int(sums), h2.data_ptr(), h2.stride(0), 0 if r2 is None else r2.data_ptr(),
         0 if r2 is None else r2.stride(0), w.data_ptr(), 0, 0, 0, 0, rstd.data_ptr(),
         dy2.data_ptr(), dy2.stride(0), 0 if dh2 is None else dh2.data_ptr(), 0 if dh2 is None else dh2.stride(0),
         0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0, 0), dev, "rms_norm backward")

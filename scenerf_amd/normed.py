@@ -62,8 +62,8 @@ def evaluate(params: NetParams, z: torch.Tensor, x: torch.Tensor) -> torch.Tenso
 
 
 class PackedNormedMLP:
-    """Such a net inside a render session: what ``PackedMLP`` is for the fused kernels' nets, where the chunk touches it.  Gradients are
-    summed over the session's chunks in one flat fp32 buffer (one all-reduce per net), laid out like the parameters."""
+    """Such a net inside a render session: what ``PackedMLP`` is for the fused kernels' nets, where the chunk touches it.  Gradients leave
+    their kernels in fp32 and are summed over the session's chunks in one flat buffer of it (one all-reduce per net), laid out like the parameters."""
     normed = True
 
     def __init__(self, params: List[torch.Tensor], spec: NetParams, d_out: int, cfg, trainable: bool):
@@ -126,7 +126,7 @@ class PackedNormedMLP:
         return y, h, (x2, weight, rstd, residual) if h is None or self.dtype != torch.float32 else (h, weight, rstd, None)
 
     def _norm_back(self, saved, dy, dh):
-        return rms_step_back(*saved[:3], self.spec.eps, dy, dh, True, True, saved[3])
+        return rms_step_back(*saved[:3], self.spec.eps, dy, dh, True, True, saved[3], sums=True)
 
     def _forward_kept(self, xenc, Z):
         n, nb, H, dt = self.net, self.n_blocks, self.d_hidden, self.dtype
@@ -152,23 +152,23 @@ class PackedNormedMLP:
         M = d_logits.shape[0]
         grads: List[Optional[torch.Tensor]] = [None] * len(self.shapes)
         dzs = torch.empty((M, nb, H), dtype=dt, device=d_logits.device)
-        da, grads[2], grads[3] = linear_step_back(s_out, d_logits.contiguous(), (M, H), True, True, True)
+        da, grads[2], grads[3] = linear_step_back(s_out, d_logits.contiguous(), (M, H), True, True, True, sums=True)
         dh, grads[4 + 7 * nb] = self._norm_back(s_norm, da.to(dt), None)
         for b in range(nb - 1, -1, -1):
             s_n, s_0, s_1 = blocks[b]
             at = 4 + 6 * b
-            dt_, grads[at + 2], grads[at + 3] = linear_step_back(s_1, dh, (M, H), True, True, True)
-            da, grads[at], grads[at + 1] = linear_step_back(s_0, dt_, (M, H), True, True, True)
+            dt_, grads[at + 2], grads[at + 3] = linear_step_back(s_1, dh, (M, H), True, True, True, sums=True)
+            da, grads[at], grads[at + 1] = linear_step_back(s_0, dt_, (M, H), True, True, True, sums=True)
             dh, grads[4 + 6 * nb + b] = self._norm_back(s_n, da, dh)
             dzs[:, b] = dh
         dzs = dzs.view(M, nb * H)
-        _, dwz, dbz = linear_step_back(s_z, dzs, None, False, True, True)
+        _, dwz, dbz = linear_step_back(s_z, dzs, None, False, True, True, sums=True)
         for b in range(nb):
             grads[8 + 6 * b], grads[9 + 6 * b] = dwz[b * H:(b + 1) * H], dbz[b * H:(b + 1) * H]
-        _, dwi, grads[1] = linear_step_back(s_in, dh.float(), None, False, True, True)
+        _, dwi, grads[1] = linear_step_back(s_in, dh.float(), None, False, True, True, sums=True)
         grads[0] = dwi[:, :42]
         self.grad_sink()
-        torch._foreach_add_(self.gviews["all"], [g.float() for g in grads])
+        torch._foreach_add_(self.gviews["all"], grads)
         return dzs
 
     def grad_sink(self):

@@ -52,7 +52,7 @@ def together(x: torch.Tensor, *others) -> bool:
 # The arguments of one call, laid out as scenerf_linear / scenerf_rms: packed bytes cost a small call half of what the structures do
 # (tests/test_rowops_refusals.py holds them to the structures' offsets).  The last two fields are the workspace and its bytes.
 LINEAR = struct.Struct("@6i19q")
-RMS = struct.Struct("@2iqf18q")
+RMS = struct.Struct("@2iqfi18q")
 _WORKSPACE = struct.Struct("@2q")
 _entries: Dict[str, Any] = {}
 
@@ -130,7 +130,7 @@ def rows_forward(what, x, weight, residual, eps, *, quantize=False, keep_rstd=Fa
     scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if quantize else None
     rstd = torch.empty((rows,), dtype=torch.float32, device=dev) if keep_rstd else None
     run_rows("rms", False, RMS.pack(
-        TYPE_CODES[dtype], width, rows, eps, x2.data_ptr(), x2.stride(0), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0),
+        TYPE_CODES[dtype], width, rows, eps, 0, x2.data_ptr(), x2.stride(0), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0),
         0 if weight is None else weight.data_ptr(), 0 if h is None else h.data_ptr(), 0 if quantize else out.data_ptr(),
         out.data_ptr() if quantize else 0, 0 if scale is None else scale.data_ptr(), 0 if rstd is None else rstd.data_ptr(),
         0, 0, 0, 0, 0, 0, 0, 0), dev, what)

@@ -700,3 +700,33 @@ def test_every_tile_in_8_bits_on_whole_numbers(m, k, n, out):
     x[:, k - 17:], w[:, k - 17:] = 2, 2         # (the end of the contraction weighs most)
     got = linear_8bit(x.to(torch.float8_e4m3fn), torch.ones(m, device=DEV), w.to(torch.float8_e4m3fn), torch.ones(n, device=DEV), out_dtype=out)
     assert torch.equal(got, (x.double() @ w.double().t()).float().to(out))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", [(0, 24, 40), (1, 16, 16), (40, 72, 24), (300, 42, 515), (1001, 1032, 264), (20011, 264, 48), (9001, 42, 1541), (2049, 2056, 520)])
+def test_weight_gradients_as_they_are_summed(m, k, n, dtype):
+    """``sums``: dweight and dbias in fp32.  Whole numbers: exact, where 16 bits would round them; otherwise 32-bit sums' bounds, and the rounded ones'
+    own bits."""
+    from scenerf_amd import _capi
+    from scenerf_amd.linear import linear_step, linear_step_back
+    g = gen("sums", m, k, n, dtype)
+
+    def back(x, w, b, dy, act, sums):
+        y, saved = linear_step(x, w, b, None, _capi.ACTIVATIONS[act], (m, n), act != "none")
+        return linear_step_back(saved, dy, (m, k), True, True, True, sums=sums)
+    x, w, dy, b = whole(g, m, k, dtype=dtype), whole(g, n, k, dtype=dtype), whole(g, m, n, dtype=dtype), whole(g, n, dtype=dtype) + 0.5
+    on = (x.double() @ w.double().t() + b.double() > 0).double()
+    for act, dz in (("none", dy.double()), ("relu", dy.double() * on)):
+        dx, dw, db = back(x, w, b, dy, act, True)
+        assert dx.dtype == dtype and dw.dtype == db.dtype == torch.float32
+        assert torch.equal(dw.double(), dz.t() @ x.double()) and torch.equal(db.double(), dz.sum(0))
+        assert torch.equal(dx, (dz @ w.double()).float().to(dtype))
+    x, w, b, dy = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5), normal(g, n, dtype=dtype), normal(g, m, n, dtype=dtype)
+    for act in ("gelu", "silu"):
+        dx, dw, db = back(x, w, b, dy, act, True)
+        rounded = back(x, w, b, dy, act, False)
+        assert torch.equal(dx, rounded[0]) and torch.equal(dw.to(dtype), rounded[1]) and torch.equal(db.to(dtype), rounded[2])
+        if m:
+            want = linear64(x, w, b, act, None, dy)
+            hold(dw, want["dw"], act + " dw")
+            hold(db, want["db"], act + " db")

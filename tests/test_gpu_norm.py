@@ -321,3 +321,22 @@ def test_gradients_do_not_know_the_rounded_sum(m, d, dtype):
         assert float((got.double() - value).norm()) <= lim, (name, float((got.double() - value).norm()), own, lim)
         worse = float((stored.to(dtype).double() - value).norm())
         assert worse > 1.1 * lim, (name, worse, lim)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,d", [(0, 24), (1, 16), (33, 515), (4801, 130), (700, 4100)])
+def test_the_weights_gradient_as_it_is_summed(m, d, dtype):
+    """``sums``: dweight in fp32, whose rounding is the gradient that autograd gets.  Against 64 bits: 32-bit sums' errors of m and d terms, in squares."""
+    from scenerf_amd.norm import rms_step_back
+    from scenerf_amd.rowops import rows_forward
+    g = gen("norm sums", m, d, dtype)
+    x, r, dy = (normal(g, m, d, dtype=dtype) for _ in range(3))
+    w = (1 + 0.2 * normal(g, d)).to(dtype)
+    _, _, h, rstd, x2 = rows_forward("rms_norm", x, w, r, 1e-6, keep_rstd=True)
+    dx, dw = rms_step_back(x2, w, rstd, 1e-6, dy, None, True, True, r, sums=True)
+    dx2, rounded = rms_step_back(x2, w, rstd, 1e-6, dy, None, True, True, r)
+    assert dw.dtype == torch.float32 and rounded.dtype == dtype and torch.equal(dw.to(dtype), rounded) and torch.equal(dx, dx2)
+    h64 = x.double() + r.double()
+    terms = dy.double() * h64 / torch.sqrt((h64 * h64).mean(1, keepdim=True) + 1e-6)
+    lim = 4 * (m ** 0.5 + d ** 0.5) * 2.0 ** -24 * float((terms * terms).sum(0).sqrt().norm())
+    assert float((dw.double() - terms.sum(0)).norm()) <= lim

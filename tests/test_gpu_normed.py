@@ -312,3 +312,32 @@ def test_a_session_trains_as_the_net_on_its_own_does(rows, n_blocks, d_hidden, d
         kind = torch.float32 if names[id(p)].startswith("lin_out") else dtype
         if not names[id(p)].startswith("lin_in"):
             assert torch.equal(a.to(kind), b.to(kind)), (names[id(p)], off(a, b))
+
+
+@pytest.mark.parametrize("chunks", [1, 6])
+def test_a_session_sums_its_chunks_in_32_bits(chunks):
+    """bf16: lin_z's gradients are sums over every chunk's rows of dzs and Z, both in hand here; a rounding to bf16 a chunk would put them 2^-9 off.
+    Errors of 32-bit sums of n terms add in squares: sqrt(n) 2^-24 of the terms' norm, four times over."""
+    rows, nb, H = 700, 2, 144
+    m = net(13, 4, nb, H)
+    pk = packed(m, "bf16", True)
+    g = torch.Generator(device=DEV).manual_seed(chunks)
+    dw, db = torch.zeros(nb * H, 2480, dtype=torch.float64, device=DEV), torch.zeros(nb * H, dtype=torch.float64, device=DEV)
+    size_w, size_b = torch.zeros_like(dw), torch.zeros_like(db)
+    for _ in range(chunks):
+        Z = torch.randn(rows, 2480, generator=g, device=DEV).to(pk.dtype)
+        xenc = torch.zeros(rows, 48, device=DEV)
+        xenc[:, :42] = torch.randn(rows, 42, generator=g, device=DEV)
+        _, saved = pk.forward(xenc, Z, True)
+        dzs = pk.backward(saved, torch.randn(rows, 4, generator=g, device=DEV)).double()
+        dw, db = dw + dzs.t() @ Z.double(), db + dzs.sum(0)
+        size_w, size_b = size_w + (dzs ** 2).t() @ Z.double() ** 2, size_b + (dzs ** 2).sum(0)
+    order = {id(t): i for i, t in enumerate(m.ordered_params())}
+    got = pk.unpack_grads()
+    for b in range(nb):
+        for p, want, size in ((m.lin_z[b].weight, dw, size_w), (m.lin_z[b].bias, db, size_b)):
+            a = got[order[id(p)]]
+            want, size = want[b * H:(b + 1) * H], size[b * H:(b + 1) * H]
+            assert a.dtype == torch.float32
+            lim = 4 * (chunks * rows) ** 0.5 * 2.0 ** -24 * float(size.sqrt().norm())
+            assert float((a.double() - want).norm()) <= lim, (float((a.double() - want).norm()), lim)

@@ -178,3 +178,13 @@ def test_a_step_back_of_a_dual_tensor_is_refused(back):
                 linear_step_back((torch.ones(3, 4), torch.ones(4, 4), None, 3, 4, 4, 4, 0, 0), dy, (3, 4), True, True, True)
             else:
                 rms_step_back(torch.ones(3, 4), torch.ones(4), torch.ones(3), 1e-6, dy, None, True, True)
+
+
+def test_gradients_in_32_bits_are_asked_for_by_their_type():
+    lib = _capi.load()
+    back = dict(dx=4096, dw=4096, dy=4096, ld_dy=4)
+    assert lib.scenerf_hip_linear_workspace(C.byref(_linear(in_type=1, out_type=0, **back)), 1) >= 4 * 8 * 4
+    assert "differ" in _said(lib.scenerf_hip_linear_backward(C.byref(_linear(in_type=1, out_type=2, **back)), None))
+    assert "differ" in _said(lib.scenerf_hip_linear_backward(C.byref(_linear(in_type=0, out_type=1, **back)), None))
+    assert "differ" in _said(lib.scenerf_hip_linear_forward(C.byref(_linear(in_type=2, out_type=0)), None))
+    assert "dweight_f32" in _said(lib.scenerf_hip_rms_backward(C.byref(_rms(dweight=4096, dy=4096, rstd=4096, dweight_f32=2)), None))
