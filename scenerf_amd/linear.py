@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .rowops import LINEAR, MAX_ROWS, TYPE_CODES, check_float, check_tensors, no_gradient, no_tangent, rows_forward, rows_of, run_on, run_rows, together
+from .rowops import LINEAR, MAX_ROWS, TYPE_CODES, check_float, check_tensors, no_gradient, no_tangent, rows_forward, rows_of, run_on, run_rows, together, vector_of
 
 
 def _activation(name: str) -> int:
@@ -65,8 +65,8 @@ def _in_pieces(x2: torch.Tensor, w2: torch.Tensor, back: bool = False):
 def _forward(what, pieces, rows, n, k, bias, residual, shape, in_type, out_dtype, dev, act, keep_z, scales=None):
     y = torch.empty(shape, dtype=out_dtype, device=dev)
     z = y.new_empty((rows, n)) if keep_z else None
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
+    if bias is not None:
+        bias = vector_of(bias)
     r = rows_of(residual, n) if residual is not None else None
     xp, ldx, wp, ldw, padded, _ = pieces
     run_rows("linear", False, LINEAR.pack(
@@ -173,7 +173,7 @@ def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     n, k = weight.shape
     x2 = rows_of(x, k)
     return _forward("linear_8bit", _in_pieces(x2, rows_of(weight, k)), x2.shape[0], n, k, bias, residual, shape, _capi.T_E4M3, out_dtype, dev, act,
-                    False, (x_scale.contiguous(), weight_scale.contiguous()))[0]
+                    False, (vector_of(x_scale), vector_of(weight_scale)))[0]
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -18,7 +18,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from .rowops import MAX_ROWS, RMS, TYPE_CODES, check_float, check_tensors, no_gradient, no_tangent, rows_forward, rows_of, run_rows, together
+from .rowops import MAX_ROWS, RMS, TYPE_CODES, check_float, check_tensors, no_gradient, no_tangent, rows_forward, rows_of, run_rows, together, vector_of
 
 
 def _check(what, x, weight, residual, eps) -> None:
@@ -45,7 +45,7 @@ def rms_step_back(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, eps
     else flows into it.  ``sums``: the weight's in fp32, not rounded to its type."""
     no_tangent("rms_norm's step back", dy, dh)
     width, dev = h.shape[-1], h.device
-    h2, dy2, w = rows_of(h, width), rows_of(dy, width), weight.contiguous()
+    h2, dy2, w = rows_of(h, width), rows_of(dy, width), vector_of(weight)
     dh2 = rows_of(dh, width) if dh is not None else None
     r2 = rows_of(residual, width) if residual is not None else None
     dx = dy.new_empty(dy.shape) if need_x else None

@@ -16,9 +16,16 @@ MAX_ROWS = 2 ** 31 - 1025
 
 def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
     """``t`` as (rows, width) with neighbouring elements inside a row: a view where the layout allows it."""
+    if t.is_neg():          # (the imaginary part of a conjugate: its memory holds the other sign)
+        t = t.resolve_neg()
     if t.dim() != 2:
         t = t.reshape(-1, width)
     return t if width == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def vector_of(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with neighbouring elements, as it is where the layout allows it."""
+    return t if t.is_contiguous() and not t.is_neg() else t.resolve_neg().contiguous()
 
 
 def check_tensors(what: str, dev: torch.device, dtype: torch.dtype, *named) -> None:
@@ -122,8 +129,8 @@ def rows_forward(what, x, weight, residual, eps, *, quantize=False, keep_rstd=Fa
     width = shape[-1]
     x2 = rows_of(x, width)
     rows = x2.shape[0]
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
+    if weight is not None:
+        weight = vector_of(weight)
     r2 = rows_of(residual, width) if residual is not None else None
     h = x.new_empty(shape) if residual is not None else None
     out = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev) if quantize else x.new_empty(shape)

@@ -188,3 +188,18 @@ def test_gradients_in_32_bits_are_asked_for_by_their_type():
     assert "differ" in _said(lib.scenerf_hip_linear_backward(C.byref(_linear(in_type=0, out_type=1, **back)), None))
     assert "differ" in _said(lib.scenerf_hip_linear_forward(C.byref(_linear(in_type=2, out_type=0)), None))
     assert "dweight_f32" in _said(lib.scenerf_hip_rms_backward(C.byref(_rms(dweight=4096, dy=4096, rstd=4096, dweight_f32=2)), None))
+
+
+def test_a_lazily_negated_tensor_is_read_as_it_reads():
+    """The imaginary part of a conjugate holds its numbers with the other sign and a flag: what the kernels are given an address of has none."""
+    from scenerf_amd.rowops import rows_of, vector_of
+    c = torch.complex(torch.ones(5, 1), torch.full((5, 1), 3.0)).conj()
+    assert c.imag.is_neg()
+    got = rows_of(c.imag, 1)
+    assert not got.is_neg() and torch.equal(got, torch.full((5, 1), -3.0))
+    wide = torch.complex(torch.ones(4, 8), torch.full((4, 8), 3.0)).conj().imag
+    assert not rows_of(wide, 8).is_neg() and rows_of(wide, 8).stride(1) == 1 and torch.equal(rows_of(wide, 8), wide)
+    one = c.imag[0]
+    assert one.is_neg() and one.is_contiguous() and not vector_of(one).is_neg() and torch.equal(vector_of(one), torch.full((1,), -3.0))
+    plain = torch.ones(7)
+    assert vector_of(plain) is plain and vector_of(torch.ones(7, 2)[:, 0]).is_contiguous()
