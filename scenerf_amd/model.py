@@ -201,11 +201,11 @@ class ResnetFC(nn.Module):
             return normed.NetParams([p[n] for n in names], self.n_blocks, self.activation, self.norm_eps, self.eight_bit)
         return [p[n] for n in names]
 
-    def forward(self, zx, *a, **k):
+    def forward(self, zx=None, *a, **k):
         """resnetfc.py:133-164 for a net with ``norm="rms"``: zx (..., d_latent + d_in), latent first -> (..., d_out), differentiable.
         The nets without a norm are evaluated inside the render pass only."""
         if self.norm == "rms":
-            if a or k:
+            if zx is None or a or k:
                 raise TypeError("ResnetFC.forward takes the rows alone")
             return normed.evaluate(self.ordered_params(), zx[..., :self.d_latent], zx[..., self.d_latent:])
         raise RuntimeError("ResnetFC is evaluated by the HIP MLP pass; call SceneRF.render_rays_batch")

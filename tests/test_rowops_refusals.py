@@ -203,3 +203,13 @@ def test_a_lazily_negated_tensor_is_read_as_it_reads():
     assert one.is_neg() and one.is_contiguous() and not vector_of(one).is_neg() and torch.equal(vector_of(one), torch.full((1,), -3.0))
     plain = torch.ones(7)
     assert vector_of(plain) is plain and vector_of(torch.ones(7, 2)[:, 0]).is_contiguous()
+
+
+def test_a_net_without_norms_says_where_it_is_evaluated():
+    from scenerf_amd.model import ResnetFC
+    for call in (lambda m: m(), lambda m: m(torch.zeros(1, 2522)), lambda m: m(zx=torch.zeros(1, 2522)), lambda m: m(points=1, views=2)):
+        with pytest.raises(RuntimeError, match="render_rays_batch"):
+            call(ResnetFC(d_hidden=16, n_blocks=1))
+    for call in (lambda m: m(), lambda m: m(torch.zeros(1, 2522), 1), lambda m: m(points=1)):
+        with pytest.raises(TypeError):
+            call(ResnetFC(d_hidden=16, n_blocks=1, norm="rms"))
