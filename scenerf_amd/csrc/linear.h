@@ -23,13 +23,10 @@ template <int W> __device__ static inline void act_any(int act, float (&v)[W]) {
     else if (act == SCENERF_ACT_SILU) act_fwd<SCENERF_ACT_SILU, W>(v);
 }
 // z as it is kept for the backward pass, in O.  A positive z that rounds to zero (fp16) is kept as the smallest positive value: relu's
-// slope there is 1, and the other slopes do not notice.  A finite z past O's range is kept as O's largest value: every slope has its limit,
-// 0 or 1, long before, and would be NaN (infinity times 0) at the infinity it rounds to.
+// slope there is 1, and the other slopes do not notice.  (A finite z past O's range is kept as an infinity: act_slope.)
 template <typename O> __device__ static inline float keep_z(float v) {
-    if constexpr (O::code == SCENERF_T_F32) return v;
-    constexpr float top = O::code == SCENERF_T_F16 ? 65504.f : 3.3895313892515355e38f;
-    if constexpr (O::code == SCENERF_T_F16) v = v > 0.f && v < 5.9604645e-8f ? 5.9604645e-8f : v;
-    return fabsf(v) > top && fabsf(v) < __builtin_inff() ? copysignf(top, v) : v;
+    if constexpr (O::code == SCENERF_T_F16) return v > 0.f && v < 5.9604645e-8f ? 5.9604645e-8f : v;
+    return v;
 }
 template <typename O> __device__ static inline void epilogue_one(const LinArgs& p, long i, int j, float v) {
     typedef typename O::raw raw;

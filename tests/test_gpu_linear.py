@@ -730,3 +730,28 @@ def test_weight_gradients_as_they_are_summed(m, k, n, dtype):
             want = linear64(x, w, b, act, None, dy)
             hold(dw, want["dw"], act + " dw")
             hold(db, want["db"], act + " db")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+def test_slopes_of_kept_values_that_are_not_finite(dtype, act):
+    """The step back from a z of infinities, NaN and the type's ends: 0 and 1 at the infinities, NaN at NaN, and no other column knows."""
+    from scenerf_amd import _capi
+    from scenerf_amd.linear import linear_step_back
+    g = gen("slopes", dtype, act)
+    m, k, n = 40, 24, 16
+    x, w, dy = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype), normal(g, m, n, dtype=dtype)
+    z = normal(g, m, n, dtype=dtype)
+    top = torch.finfo(dtype).max
+    for j, v in enumerate((float("inf"), float("-inf"), top, -top, float("nan"))):
+        z[:, j] = v
+    dx, dw, db = linear_step_back((x, w, z, m, n, k, k, 0, _capi.ACTIVATIONS[act]), dy, (m, k), True, True, True)
+    ones = linear64(x, w[[0, 2]], torch.zeros(2, dtype=dtype, device=DEV), "none", None, dy[:, [0, 2]])
+    hold(dw[[0, 2]], ones["dw"], "slope 1")
+    hold(db[[0, 2]], ones["db"], "slope 1")
+    assert not bool(dw[[1, 3]].any()) and not bool(db[[1, 3]].any())
+    if act == "relu":                                # (a comparison: NaN is not above 0)
+        assert not bool(dw[4].any()) and bool(torch.isfinite(dx).all())
+    else:
+        assert bool(torch.isnan(dw[4]).all()) and bool(torch.isnan(db[4])) and bool(torch.isnan(dx).all())
+    assert bool(torch.isfinite(dw[5:]).all()) and bool(torch.isfinite(db[5:]).all())
