@@ -32,21 +32,22 @@ __device__ static inline float row_scale(uint32_t max_bits) {
     return m < 1.1754943508222875e-38f ? 1.1754943508222875e-38f : m;   // NaN stays
 }
 // v / s of a row's values.  Values of 16 bits lie on e4m3's ties often, so the quotient has to be a rounded one: a product with 1 / s put one of
-// 80 bf16 values a whole step off.  s = m 2^e, m in [1, 2): q0 = v 2^-e (1 / m) is off by 1.5 units at most, its remainder against m brings it to
-// the quotient but for 2^-23 of a unit, rounded once (Markstein's correction).  Nothing underflows whose quotient e4m3 could tell from 0.  The
-// compiler's full division instead: 70 us for 40,001 x 2,480 fp16 rows, 61 so.  s not finite: 0 or NaN.
+// 80 bf16 values a whole step off.  v (1 / s) is off by 1.5 units at most, its remainder against s brings it to the quotient but for 2^-23 of a
+// unit, rounded once (Markstein's correction).  The remainder of a row under 2^-80 would underflow: such a row is `small`, and its
+// values come times 2^64, as s does here.  The compiler's full division took 70 us for 40,001 x 2,480 fp16 rows, this 62, the product
+// alone 60.  s not finite: 0 or NaN.
 struct RowQuotient {
-    float k, m, inv;
-    __device__ inline RowQuotient(float s) {
-        const uint32_t b = __float_as_uint(s);
-        const bool fine = b < 0x7f800000u;
-        k = fine ? __uint_as_float((254u - (b >> 23)) << 23) : 1.f / s;
-        m = fine ? __uint_as_float((b & 0x007fffffu) | 0x3f800000u) : 1.f;
-        inv = 1.f / m;
+    float inv, s;
+    bool small;
+    __device__ inline RowQuotient(float scale) {
+        small = scale < 0x1p-88f;
+        s = small ? scale * 0x1p64f : scale;
+        inv = 1.f / s;
+        if (!(s < __builtin_inff())) s = 0.f;
     }
     __device__ inline float operator()(float v) const {
-        const float t = v * k, q = t * inv;
-        return fmaf(fmaf(-q, m, t), inv, q);
+        const float q = v * inv;
+        return fmaf(-fmaf(q, s, -v), inv, q);       // (in this order -0 stays -0)
     }
 };
 
@@ -130,6 +131,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void rms_rows_kernel(RmsArgs p) {
             const float s = row_scale(wave_max_u32(m));
             if (lane == 0) p.scale[row] = s;
             const RowQuotient over(s);
+            if (over.small)
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int e = 0; e < VW; ++e) h[c][e] *= 0x1p64f;
 #pragma unroll
             for (int c = 0; c < C; ++c)
                 if (in[c] > 0) {
@@ -233,7 +239,7 @@ __global__ __launch_bounds__(WIDE_THREADS) void rms_rows_wide_kernel(RmsArgs p) 
             if (p.y) store_some<E, VW, WHOLE>((raw*)p.y + row * D + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
             if (p.q) {
 #pragma unroll
-                for (int e = 0; e < VW; ++e) h[e] = over(h[e]);
+                for (int e = 0; e < VW; ++e) h[e] = over(over.small ? h[e] * 0x1p64f : h[e]);
                 store_some<TypeE4M3, VW, WHOLE>(p.q + row * D + col, (int)min(D - col, (long)VW), (int)(D % VW), h);
             }
         }

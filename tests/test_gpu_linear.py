@@ -755,3 +755,16 @@ def test_slopes_of_kept_values_that_are_not_finite(dtype, act):
     else:
         assert bool(torch.isnan(dw[4]).all()) and bool(torch.isnan(db[4])) and bool(torch.isnan(dx).all())
     assert bool(torch.isfinite(dw[5:]).all()) and bool(torch.isfinite(db[5:]).all())
+
+
+@pytest.mark.parametrize("m,d", [(40, 512), (9, 4101), (300, 515)])
+def test_quantize_rows_of_any_size_to_the_bit(m, d):
+    """Rows from the smallest fp32 numbers to the largest, each row of one size."""
+    from scenerf_amd.linear import quantize_rows
+    g = gen("sizes", m, d)
+    x = normal(g, m, d) * torch.exp2(torch.linspace(-140, 120, m, device=DEV))[:, None]
+    q, s = quantize_rows(x)
+    x, q, s = x.cpu(), q.cpu(), s.cpu()
+    assert torch.equal(s, (x.abs().amax(1) / 448).clamp(min=2.0 ** -126))
+    want = (x / s[:, None]).to(torch.float8_e4m3fn)
+    assert torch.equal(q.view(torch.uint8), want.view(torch.uint8)), int((q.float() != want.float()).sum())
