@@ -17,10 +17,11 @@ struct LinArgs {
     const float* unscale;                // not NULL (fp16, backward): A and A2 hold their values times 1 / *unscale, a power of two
 };
 
-template <int W> __device__ static inline void act_any(int act, float (&v)[W]) {
-    if (act == SCENERF_ACT_RELU) act_fwd<SCENERF_ACT_RELU, W>(v);
-    else if (act == SCENERF_ACT_GELU) act_fwd<SCENERF_ACT_GELU, W>(v);
-    else if (act == SCENERF_ACT_SILU) act_fwd<SCENERF_ACT_SILU, W>(v);
+template <typename O, int W> __device__ static inline void act_any(int act, float (&v)[W]) {
+    constexpr bool FINE = O::code == SCENERF_T_F32;
+    if (act == SCENERF_ACT_RELU) act_fwd<SCENERF_ACT_RELU, W, FINE>(v);
+    else if (act == SCENERF_ACT_GELU) act_fwd<SCENERF_ACT_GELU, W, FINE>(v);
+    else if (act == SCENERF_ACT_SILU) act_fwd<SCENERF_ACT_SILU, W, FINE>(v);
 }
 // z as it is kept for the backward pass, in O.  A positive z that rounds to zero (fp16) is kept as the smallest positive value: relu's
 // slope there is 1, and the other slopes do not notice.  (A finite z past O's range is kept as an infinity: act_slope.)
@@ -35,7 +36,7 @@ template <typename O> __device__ static inline void epilogue_one(const LinArgs& 
     if (p.bias) v += O::to_f32(((const raw*)p.bias)[j]);
     if (p.z) ((raw*)p.z)[i * p.N + j] = O::from_f32(keep_z<O>(v));
     float one[1] = {v};
-    act_any<1>(p.act, one);
+    act_any<O, 1>(p.act, one);
     v = one[0];
     if (p.residual) v += O::to_f32(((const raw*)p.residual)[i * p.ld_residual + j]);
     ((raw*)p.out)[i * p.N + j] = O::from_f32(v);
@@ -81,7 +82,7 @@ __device__ static inline void epilogue_vec(const LinArgs& p, const EpilogueCols<
         for (int e = 0; e < W; ++e) t[e] = keep_z<O>(v[e]);
         store_some<O, W, WHOLE>((raw*)p.z + i * p.N + j, n, p.N % W, t);
     }
-    act_any<W>(p.act, v);
+    act_any<O, W>(p.act, v);
     if (p.residual) {
         float t[W];
         unpack16<O>(res, t);

@@ -269,8 +269,8 @@ __global__ __launch_bounds__(256) void linear_pad_kernel(PadSide x, PadSide w, i
 }
 
 // ---- dz = dy act'(z), and the column sums of dz by strips of rows ------------------------------------------------------------------
-template <int ACT> __device__ static inline void slopes(float (&g)[8], float (&z)[8], int valid) {
-    act_slope<ACT, 8>(z);
+template <int ACT, typename O> __device__ static inline void slopes(float (&g)[8], float (&z)[8], int valid) {
+    act_slope<ACT, 8, O::code == SCENERF_T_F32>(z);
 #pragma unroll
     for (int e = 0; e < 8; ++e) g[e] = e < valid ? g[e] * z[e] : 0.f;
 }
@@ -347,9 +347,9 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const void* dy_, long ld
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 if (q == 1 && !two) continue;
-                if (act == SCENERF_ACT_GELU) slopes<SCENERF_ACT_GELU>(g[q], z[q], N - j0);
-                else if (act == SCENERF_ACT_SILU) slopes<SCENERF_ACT_SILU>(g[q], z[q], N - j0);
-                else if (act == SCENERF_ACT_RELU) slopes<SCENERF_ACT_RELU>(g[q], z[q], N - j0);
+                if (act == SCENERF_ACT_GELU) slopes<SCENERF_ACT_GELU, O>(g[q], z[q], N - j0);
+                else if (act == SCENERF_ACT_SILU) slopes<SCENERF_ACT_SILU, O>(g[q], z[q], N - j0);
+                else if (act == SCENERF_ACT_RELU) slopes<SCENERF_ACT_RELU, O>(g[q], z[q], N - j0);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum[e] += g[q][e];
                 if constexpr (O::code == SCENERF_T_F16) {

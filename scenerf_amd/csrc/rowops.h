@@ -183,45 +183,50 @@ template <typename E, int W, bool WHOLE = false> __device__ static inline void s
 }
 
 // Activations and their slopes.  relu keeps NaN (a comparison, not fmaxf, which would drop it) and its slope at 0 is 0.
-// gelu's normal distribution function by Abramowitz & Stegun 7.1.26, erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by
-// at most 1.5e-7: one exponential and one reciprocal (1 ulp each) serve the value and the slope, whose density is the same exponential.
+// gelu's normal distribution function: Phi(-x) = t P(t) exp(-x^2 / 2), t = 1 / (1 + p x), x >= 0: one exponential and one reciprocal (1 ulp each) serve
+// the value and the slope, whose density is the same exponential.  For results in 16 bits P is of degree 4, Abramowitz & Stegun 7.1.26 with the
+// constants of z / sqrt 2 and of the half folded in: off by at most 0.75e-7.  For results in 32 bits (FINE) that is more than their own rounding: in the
+// 2-norm over normal z gelu was 8.8e-8 off and its slope 1.1e-7, with a correctly rounded erf 3.7e-8 and 3.9e-8.  There P is of degree 6, fitted here
+// to the smallest largest error (least squares, weights moved to where it was largest), 2.1e-9: 4.0e-8 and 5.9e-8.  Everywhere, it would cost
+// 4 us of 187 at 153,600 x 512 x 512 bf16.
 // The library's erff and expf took 145 us of a step's 153,600 x 512 slopes, bound by the vector units; this takes what the bytes take.
 __device__ static inline float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
-#define CDF_STEP() __builtin_amdgcn_sched_barrier(0)
+#define CDF_STEP(expression)                      \
+    _Pragma("unroll") for (int i = 0; i < W; ++i) expression; \
+    __builtin_amdgcn_sched_barrier(0)
 // Phi(z), and the exponential exp(-z^2 / 2) in e, of W values a step at a time: one after the other they are a chain of 16 dependent
-// instructions each, which the compiler leaves as they are (153,600 x 512 x 512 bf16 with its sums kept 199 us so, 196 by steps; the constants of z / sqrt 2 and of the half are folded in)
-template <int W> __device__ static inline void normal_cdf(const float (&z)[W], float (&c)[W], float (&e)[W]) {
+// instructions each, which the compiler leaves as they are (153,600 x 512 x 512 bf16 with its sums kept 199 us so, 196 by steps)
+template <int W, bool FINE> __device__ static inline void normal_cdf(const float (&z)[W], float (&c)[W], float (&e)[W]) {
     float t[W];
 #pragma unroll
-    for (int i = 0; i < W; ++i) t[i] = fmaf(0.23164189f, fabsf(z[i]), 1.f);
+    for (int i = 0; i < W; ++i) t[i] = fmaf(FINE ? 0.45f : 0.23164189f, fabsf(z[i]), 1.f);
 #pragma unroll
     for (int i = 0; i < W; ++i) e[i] = z[i] * z[i] * -0.72134752f;
 #pragma unroll
     for (int i = 0; i < W; ++i) t[i] = __builtin_amdgcn_rcpf(t[i]);
-#pragma unroll
-    for (int i = 0; i < W; ++i) e[i] = __builtin_amdgcn_exp2f(e[i]);
-    CDF_STEP();
-#pragma unroll
-    for (int i = 0; i < W; ++i) c[i] = fmaf(0.53070271f, t[i], -0.72657601f);
-    CDF_STEP();
-#pragma unroll
-    for (int i = 0; i < W; ++i) c[i] = fmaf(c[i], t[i], 0.71070687f);
-    CDF_STEP();
-#pragma unroll
-    for (int i = 0; i < W; ++i) c[i] = fmaf(c[i], t[i], -0.14224837f);
-    CDF_STEP();
-#pragma unroll
-    for (int i = 0; i < W; ++i) c[i] = fmaf(c[i], t[i], 0.12741480f) * t[i];
-    CDF_STEP();
+    CDF_STEP(e[i] = __builtin_amdgcn_exp2f(e[i]));
+    if constexpr (FINE) {
+        CDF_STEP(c[i] = fmaf(-0.0378535874f, t[i], 0.217445642f));
+        CDF_STEP(c[i] = fmaf(c[i], t[i], -0.474038959f));
+        CDF_STEP(c[i] = fmaf(c[i], t[i], 0.393637121f));
+        CDF_STEP(c[i] = fmaf(c[i], t[i], 0.0181375835f));
+        CDF_STEP(c[i] = fmaf(c[i], t[i], 0.205400571f));
+        CDF_STEP(c[i] = fmaf(c[i], t[i], 0.177271649f) * t[i]);
+    } else {
+        CDF_STEP(c[i] = fmaf(0.53070271f, t[i], -0.72657601f));
+        CDF_STEP(c[i] = fmaf(c[i], t[i], 0.71070687f));
+        CDF_STEP(c[i] = fmaf(c[i], t[i], -0.14224837f));
+        CDF_STEP(c[i] = fmaf(c[i], t[i], 0.12741480f) * t[i]);
+    }
 #pragma unroll
     for (int i = 0; i < W; ++i) c[i] *= e[i];
 #pragma unroll
     for (int i = 0; i < W; ++i) c[i] = z[i] < 0.f ? c[i] : 1.f - c[i];
 }
-// W values of the activation, or of its slope, in place
-template <int ACT, int W> __device__ static inline void act_fwd(float (&z)[W]) {
+// W values of the activation, or of its slope, in place; FINE: for results in 32 bits
+template <int ACT, int W, bool FINE> __device__ static inline void act_fwd(float (&z)[W]) {
     float c[W], e[W];
-    if constexpr (ACT == SCENERF_ACT_GELU) normal_cdf<W>(z, c, e);
+    if constexpr (ACT == SCENERF_ACT_GELU) normal_cdf<W, FINE>(z, c, e);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
         if constexpr (ACT == SCENERF_ACT_RELU) z[i] = z[i] < 0.f ? 0.f : z[i];
@@ -232,10 +237,10 @@ template <int ACT, int W> __device__ static inline void act_fwd(float (&z)[W]) {
 // (A z kept in 16 bits may be the infinity that a finite sum past the type's range rounds to.  The slopes have their limits there, 0 and 1: z's
 // factor is held to finite numbers, or it would be infinity times 0.  NaN comes through e, c and p.  Clamping z where it is kept instead cost the
 // forward pass 8 us of 185 at 153,600 x 512 x 512 bf16; here HBM hides it.)
-template <int ACT, int W> __device__ static inline void act_slope(float (&z)[W]) {
+template <int ACT, int W, bool FINE> __device__ static inline void act_slope(float (&z)[W]) {
     constexpr float top = 3.4028234663852886e38f;
     float c[W], e[W];
-    if constexpr (ACT == SCENERF_ACT_GELU) normal_cdf<W>(z, c, e);
+    if constexpr (ACT == SCENERF_ACT_GELU) normal_cdf<W, FINE>(z, c, e);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
         if constexpr (ACT == SCENERF_ACT_RELU) z[i] = z[i] > 0.f ? 1.f : 0.f;
