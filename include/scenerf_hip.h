@@ -592,7 +592,9 @@ int scenerf_hip_sphere_resample_backward_nhwc(const float* dout, int64_t planes,
  * or a call has up to 8 rows; with a result in BF16 and more rows the 8-bit matrix instructions add them in groups of 8 neighbours, each group
  * with what lies below 2^-13 of its largest product cut off: a sum may be off by 7 2^-13 of its terms' magnitudes, and a row's result depends
  * that much on whether it is computed alone.
- * backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = the column sums of dz (the residual's gradient is dy itself). */
+ * backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = the column sums of dz (the residual's gradient is dy itself).  In 16 bits z is
+ * what the forward kept of it, and where there is an activation dz is rounded to in_type in front of the two products (F16: times a power of two
+ * found from dy, so that neither end of its range is met); db is made from the unrounded dz. */
 typedef struct scenerf_linear {
     int32_t in_type;                /* x, w (and dx) */
     int32_t out_type;               /* forward: bias, residual, y, z; equal to in_type unless that is E4M3.  backward (z and dy are of in_type):

@@ -6,9 +6,9 @@
 // read along k), dx contracts the outputs (w is read across), dw contracts the rows (both are read across).
 //
 // Products of many rows run on staged tiles (linear_tile.h): bound by the chip's power where the contraction is long (153,600 x 2,480
-// x 1,536 bf16 999 us = 1.17 PFLOP/s; the library's product of that shape without an epilogue 1,054; 8 bits 630 us; 4,096 x 8,192 x 4,096 takes
-// 256 us, and 162 if all of it is zeros), by the operands' and results' bytes where it is short (153,600 x 512 x 512 bf16 with gelu,
-// residual and kept sums 165 us for 629 MB).
+// x 1,536 bf16 1,000 to 1,060 us from card to card, 1.10 to 1.17 PFLOP/s; the library's product of that shape without an epilogue takes the same;
+// 8 bits 615 to 646; 4,096 x 8,192 x 4,096 takes 256 us, and 162 if all of it is zeros), by the operands' and results' bytes where it is short
+// (153,600 x 512 x 512 bf16 with gelu, residual and kept sums 169 to 188 us for 629 MB).
 #include "linear.h"
 
 typedef __attribute__((ext_vector_type(8))) __bf16 lin_bf16x8;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p) {
     }
 }
 // the splits' sums, added in a fixed order, then the epilogue: a workgroup owns 32 pieces of W results, 8 threads each, thread y of them
-// adds splits y, y + 8, ..  Bound by the sums' bytes: 64 splits of 512 x 512 13.7 us, 4.9 TB/s
+// adds splits y, y + 8, ..  Bound by the sums' bytes: 64 splits of 512 x 512 (67 MB) 16.7 us, 4.0 TB/s
 // db's column sums ride along in front of dw's join, a launch less: each of `sums.blocks` workgroups adds 16 columns in 16 chains
 struct ColumnSums { const float* part; void* out; int count, width, blocks; };
 template <typename O> __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs p, ColumnSums sums) {
@@ -394,8 +394,9 @@ struct LinPlan {
 };
 // What a tile costs, in us: a workgroup's start and end, and a chunk of 128 bytes of the contraction with 1, 2, 3 workgroups on a CU (as many as
 // their LDS lets in).  Fitted to products of 1,024 to 153,600 rows by 48 to 2,480 features, forward and both gradients: on 364 of 366 of them
-// (bf16 and fp32) what the plan chooses took no more than 7 percent or 2 us above the fastest of all tiles and splits.  Where the tiles
-// differ most: 153,600 x 2,480 x 1,536 bf16 256^2 1,034 us and 128^2 1,521; 262,144 x 128 x 128 50 and 32; 1,024 x 512 x 512 20, 9.8 and 64^2
+// (bf16 and fp32) what the plan chooses took no more than 7 percent or 2 us above the fastest of all tiles and splits.  fp16, whose
+// instructions have bf16's rates, and e4m3, which has half its chunks (where it is widened, each of twice the matrix time), take bf16's
+// costs, and were not gone through like that.  Where the tiles differ most (on one box): 153,600 x 2,480 x 1,536 bf16 256^2 1,034 us and 128^2 1,521; 262,144 x 128 x 128 50 and 32; 1,024 x 512 x 512 20, 9.8 and 64^2
 // 6.1; dw of 12,288 rows x 512 x 2,480 54, 52 (6 splits) and 64^2 unsplit 108.
 struct LinTileCost { LinTile tile; int per_cu; double ends, chunk[3]; };
 static const LinTileCost kLinCost16[] = {{LIN_256x256, 1, 9.0, {1.7}}, {LIN_128x128, 2, 4.7, {0.61, 1.1}}, {LIN_64x64, 3, 1.8, {0.35, 0.55, 0.78}}};
@@ -574,9 +575,11 @@ static int dz_strip(int64_t rows) {
 }
 struct BackwardPlan {
     bool make_dz;                   // dz is not dy itself
-    // Where few values share it, the rounding of dz to 16 bits is undone: its rest is a second operand of dx's (dw's) product.  With many
-    // values dx and dw are 1.45 times as far from exact as their own rounding makes them, whatever the inputs; of few, now and then twice as
-    // far, and going over the contraction again costs little.
+    // dz of 16 bits is rounded in front of its products (z, in its slopes, as it was kept): dx and dw are 1.45 times as far from exact, in the
+    // 2-norm, as their own rounding makes them, whatever the inputs and sizes.  Where dz, or dx or dw, has few values the rounding is undone: its
+    // rest is a second operand of the product, 1.05 times.  The counts are not a caller's accuracy, they are where that is worth its cost: of
+    // few values the worst is now and then twice as far, which a mean over many hides, and going over a short contraction again costs
+    // little (a layer above them is less exact than one below, at 1.45).
     bool rest_x, rest_w;
     int strip, strips, dz_pitch;
     bool scaled;                    // dz is held times a power of two (linear_dy_max_kernel)

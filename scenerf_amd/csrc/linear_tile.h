@@ -244,7 +244,7 @@ __device__ static inline void linear_tile(const LinArgs& p, int block, int block
         }
     };
     // Chunks whose loads end inside the split go through a loop of their own, without the loads' comparisons, selections and 64-bit sums
-    // (1.7 vector instructions a matrix instruction else): 153,600 x 2,480 x 1,536 bf16 1,165 -> 1,140 us and its dx 1,111 -> 1,075, 8 bits 677 ->
+    // (1.7 vector instructions a matrix instruction else; before and behind it on one box): 153,600 x 2,480 x 1,536 bf16 1,165 -> 1,140 us and its dx 1,111 -> 1,075, 8 bits 677 ->
     // 669, 4,800 x 512 x 512 fp32 with its gradients 71 -> 67.  Small tiles of 16 and 8 bits have few chunks and lose by the longer code (29.8 -> 30.4).
     constexpr bool FAST = ES == 4 || BM * BN >= 128 * 128;
     constexpr bool TWICE = ES == 2 && BX && BM * BN < 256 * 256;       // (LinArgs.A2; the large tiles have no registers for it)

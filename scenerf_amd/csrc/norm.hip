@@ -9,8 +9,10 @@
 // wide ones, go through a workgroup that reads the row twice (the second time from L2).  The weight's gradient is summed per lane over the wave's rows, then over the workgroup's waves in
 // LDS, then over the workgroups by a second kernel in a fixed order: no atomics, the same bits every time.  Rows of any length and
 // alignment move 16 bytes at a time, but for a last piece that the row does not fill.
-// 153,600 x 512 bf16: forward with residual 109 to 116 us for 629 MB (5.4 to 5.8 TB/s; a large copy reaches 5.2), gradients with residual 130 for 786 MB, 8
-// bits 102 us for 551 MB; 40,001 x 2,480 fp16 to 8 bits 60 us for 298 MB; 4,801 x 515 fp32 out of wider rows 9 us.
+// 153,600 x 512 bf16: forward with residual 107 us for 629 MB (5.9 TB/s; a large copy reaches 5.2), gradients with residual 159 + 5 for 786 MB (5.0), 8
+// bits 101 to 108 us for 551 MB; 40,001 x 2,480 fp16 to 8 bits 62 to 66 us for 298 MB; 4,801 x 515 fp32 out of wider rows 8.6 us.  20,000 x 8,192
+// bf16, wider than a wave holds: forward 251 us for 1,311 MB, dx 331 for 1,638 MB at dh with it, dweight 525 (x, residual and dy once more,
+// two bytes a lane: 1.9 TB/s, the slowest pass here by its bytes).
 #include "rowops.h"
 
 #define ROW_WAVES 4

@@ -133,7 +133,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
     ``activation``: "none", "relu", "gelu" (the exact one, by erf) or "silu".  Sums, bias, activation and addition are in 32 bits; the
     result is rounded once.  Differentiable once, in reverse, in x, weight, bias and residual; where an activation is asked for and a gradient will
-    be, the sums in front of it are kept in the operands' type."""
+    be, the sums in front of it are kept in the operands' type; in 16 bits the gradient behind the activation is rounded to it as well in front
+    of the two products that x's and weight's gradients are."""
     act = _activation(activation)
     dtype = x.dtype
     no_tangent("linear", x, weight, bias, residual)
