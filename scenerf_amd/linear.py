@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -66,7 +67,7 @@ def _forward(what, pieces, rows, n, k, bias, residual, shape, in_type, out_dtype
     y = torch.empty(shape, dtype=out_dtype, device=dev)
     z = y.new_empty((rows, n)) if keep_z else None
     if bias is not None:
-        bias = vector_of(bias)
+        bias = vector_of(bias, n)
     r = rows_of(residual, n) if residual is not None else None
     xp, ldx, wp, ldw, padded, _ = pieces
     run_rows("linear", False, LINEAR.pack(
@@ -89,7 +90,8 @@ def linear_step(x: torch.Tensor, weight: torch.Tensor, bias, residual, act: int,
 
 def linear_step_back(saved, dy: torch.Tensor, x_shape, need_x: bool, need_w: bool, need_b: bool, sums: bool = False):
     """(dx, dweight, dbias), None where not needed.  ``sums``: dweight and dbias in fp32, not rounded to their type."""
-    no_tangent("linear's step back", dy)
+    if forward_ad._current_level >= 0:
+        no_tangent("linear's step back", dy)
     x2, w2, z, rows, n, k, pitch, padded, act = saved
     dev = dy.device
     # (dy is of x's type: autograd sees to it; new_empty takes less of the host's time than empty)
@@ -137,7 +139,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     of the two products that x's and weight's gradients are."""
     act = _activation(activation)
     dtype = x.dtype
-    no_tangent("linear", x, weight, bias, residual)
+    if forward_ad._current_level >= 0:
+        no_tangent("linear", x, weight, bias, residual)
     if not together(x, weight, bias, residual):
         check_tensors("linear", x.device, dtype, ("weight", weight), ("bias", bias), ("residual", residual))
     code = check_float("linear", "x", dtype)
@@ -161,7 +164,8 @@ def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     its terms' magnitudes, which shows where it cancels, and a row computed alone may differ by that much from the same row among others."""
     act = _activation(activation)
     dev = x.device
-    no_tangent("linear_8bit", x_scale, weight_scale, bias, residual)
+    if forward_ad._current_level >= 0:
+        no_tangent("linear_8bit", x_scale, weight_scale, bias, residual)
     check_tensors("linear_8bit", dev, torch.float8_e4m3fn, ("x", x), ("weight", weight))
     check_float("linear_8bit", "out_dtype", out_dtype)
     check_tensors("linear_8bit", dev, torch.float32, ("x_scale", x_scale), ("weight_scale", weight_scale))
@@ -174,14 +178,15 @@ def linear_8bit(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     n, k = weight.shape
     x2 = rows_of(x, k)
     return _forward("linear_8bit", _in_pieces(x2, rows_of(weight, k)), x2.shape[0], n, k, bias, residual, shape, _capi.T_E4M3, out_dtype, dev, act,
-                    False, (vector_of(x_scale), vector_of(weight_scale)))[0]
+                    False, (vector_of(x_scale, x2.shape[0]), vector_of(weight_scale, n)))[0]
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows in 8 bits: x (..., width) float32 / bfloat16 / float16 -> (q (..., width) float8_e4m3fn, scale (...) float32) with
     scale = max(max|row| / 448, 2^-126) and q = x / scale rounded to nearest even: x is q * scale up to half a step of e4m3.  A row that
     holds a NaN or an infinity gets a scale that is not finite, and stands for no number."""
-    no_tangent("quantize_rows", x)
+    if forward_ad._current_level >= 0:
+        no_tangent("quantize_rows", x)
     check_tensors("quantize_rows", x.device, x.dtype)
     check_float("quantize_rows", "x", x.dtype)
     if x.dim() < 1 or x.shape[-1] < 1:

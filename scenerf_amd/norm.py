@@ -15,6 +15,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
@@ -23,7 +24,8 @@ from .rowops import MAX_ROWS, RMS, TYPE_CODES, check_float, check_tensors, no_gr
 
 def _check(what, x, weight, residual, eps) -> None:
     shape = x.shape
-    no_tangent(what, x, weight, residual)
+    if forward_ad._current_level >= 0:
+        no_tangent(what, x, weight, residual)
     if not together(x, weight, residual):
         check_tensors(what, x.device, x.dtype, ("weight", weight), ("residual", residual))
     check_float(what, "x", x.dtype)
@@ -43,9 +45,10 @@ def rms_step_back(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, eps
                   need_x: bool, need_w: bool, residual: Optional[torch.Tensor] = None, sums: bool = False):
     """(gradient of h, gradient of weight), None where not needed; h as the forward stored it (or its x, with its ``residual``), ``dh`` what
     else flows into it.  ``sums``: the weight's in fp32, not rounded to its type."""
-    no_tangent("rms_norm's step back", dy, dh)
+    if forward_ad._current_level >= 0:
+        no_tangent("rms_norm's step back", dy, dh)
     width, dev = h.shape[-1], h.device
-    h2, dy2, w = rows_of(h, width), rows_of(dy, width), vector_of(weight)
+    h2, dy2, w = rows_of(h, width), rows_of(dy, width), vector_of(weight, width)
     dh2 = rows_of(dh, width) if dh is not None else None
     r2 = rows_of(residual, width) if residual is not None else None
     dx = dy.new_empty(dy.shape) if need_x else None

@@ -16,16 +16,16 @@ MAX_ROWS = 2 ** 31 - 1025
 
 def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
     """``t`` as (rows, width) with neighbouring elements inside a row: a view where the layout allows it."""
-    if t.is_neg():          # (the imaginary part of a conjugate: its memory holds the other sign)
-        t = t.resolve_neg()
     if t.dim() != 2:
         t = t.reshape(-1, width)
-    return t if width == 1 or t.stride(1) == 1 else t.contiguous()
+    if width == 1:          # (the imaginary part of a conjugate holds the other sign in its memory: every second element, so wider rows are copied)
+        return t.resolve_neg()
+    return t if t.stride(1) == 1 else t.contiguous()
 
 
-def vector_of(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with neighbouring elements, as it is where the layout allows it."""
-    return t if t.is_contiguous() and not t.is_neg() else t.resolve_neg().contiguous()
+def vector_of(t: torch.Tensor, n: int = 1) -> torch.Tensor:
+    """``t`` of ``n`` elements as neighbours, as it is where the layout allows it (``rows_of`` says why one alone is looked at)."""
+    return (t.resolve_neg() if n == 1 else t).contiguous()
 
 
 def check_tensors(what: str, dev: torch.device, dtype: torch.dtype, *named) -> None:
@@ -109,11 +109,11 @@ def run_rows(name: str, backward: bool, args: bytes, dev: torch.device, what: st
 
 
 def no_tangent(what: str, *tensors) -> None:
-    """Refuses dual tensors: nothing else about them says that a derivative is asked for, and grad mode does not concern them."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError("%s has no forward-mode derivative (got a dual tensor)" % what)
+    """Refuses dual tensors: nothing else about them says that a derivative is asked for, and grad mode does not concern them.  Called where
+    ``forward_ad._current_level`` is not negative: there are none outside a level, and a small call feels the function."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("%s has no forward-mode derivative (got a dual tensor)" % what)
 
 
 def no_gradient(what: str, *tensors) -> None:
@@ -130,7 +130,7 @@ def rows_forward(what, x, weight, residual, eps, *, quantize=False, keep_rstd=Fa
     x2 = rows_of(x, width)
     rows = x2.shape[0]
     if weight is not None:
-        weight = vector_of(weight)
+        weight = vector_of(weight, width)
     r2 = rows_of(residual, width) if residual is not None else None
     h = x.new_empty(shape) if residual is not None else None
     out = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev) if quantize else x.new_empty(shape)
